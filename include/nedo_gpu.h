@@ -354,6 +354,116 @@ NEDO_GPU_API int nedo_gpu_decoder_reset(nedo_gpu_decoder* d);
 /* Free the decoder's device memory and graphs (NULL is a no-op). */
 NEDO_GPU_API void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d);
 
+/* ---- Paged key/value cache of many sequences ----------------------------
+ *
+ * Device entry points for serving a batch of sequences: a cache of pages that a
+ * page table deals out to the sequences, the append that fills it, and the
+ * attention that reads it.  They stand next to nedo_gpu_matvec_dev (batch > 1)
+ * as its single-sequence counterparts inside nedo_gpu_decoder stand next to the
+ * matvec: q|k|v of a batch comes from one nedo_gpu_matvec_dev, goes through
+ * nedo_gpu_kv_append_dev, and the attention output goes into the output
+ * projection.  The arithmetic is that of src/model.cpp:218-247 and
+ * src/kernels.cpp:93-105 per sequence; pages, ragged batches, shared prefixes and
+ * page selection have no reference counterpart.
+ *
+ * All of them are asynchronous on `stream`, allocate nothing and keep nothing
+ * between calls, so they can be captured in CUDA graphs and may run at the same
+ * time on several streams (each call with a workspace of its own).  Buffers are
+ * 16-byte aligned device memory.  Results repeat bit for bit.
+ *
+ * Token row t of sequence s (q_start[s] <= t < q_start[s+1]) stands at position
+ * kv_len[s] - (q_start[s+1] - t).  A row whose position is negative -- its
+ * sequence has fewer cached tokens than rows, e.g. an unused slot of a padded
+ * batch with kv_len 0 -- is padding: append writes nothing for it, attention
+ * gives it zeros.  Rows from q_start[seqs] on belong to no sequence; their
+ * outputs are left as they were.
+ *
+ * Lengths and page ids are read from device memory.  A sequence whose values are
+ * out of range (rows beyond `tokens` or `max_q_len`, more than `max_kv_len`
+ * cached tokens, decreasing q_start) is left out, a page id of num_pages or more
+ * counts as a page without keys, and either is reported by nedo_gpu_status as
+ * NEDO_GPU_ERR_DEVICE. */
+typedef struct {
+    uint32_t type;       /* 0 (F32) or NEDO_GPU_F16                                       */
+    uint32_t kv_heads;
+    uint32_t head_dim;   /* a multiple of 8, at most 256                                 */
+    uint32_t page_size;  /* tokens per page: 16, 32, 64, 128 or 256                      */
+    uint64_t num_pages;
+    void* k;             /* [num_pages][kv_heads][page_size][head_dim]                   */
+    void* v;             /* [num_pages][kv_heads][page_size][head_dim]                   */
+    void* bounds;        /* [num_pages][kv_heads][2][head_dim], in `type`: the smallest and
+                            the largest value of each channel of the page's keys (NULL: not
+                            kept; nedo_gpu_block_select_dev needs it)                      */
+} nedo_gpu_kv_cache;
+
+typedef struct {
+    uint32_t seqs;               /* sequences                                            */
+    uint32_t tokens;             /* rows of the q, qkv and output buffers                */
+    uint32_t max_q_len;          /* no sequence has more rows (a bound; shapes the launch) */
+    uint32_t max_kv_len;         /* no sequence has more cached tokens (a bound)          */
+    uint32_t max_pages;          /* row length of page_table                             */
+    uint32_t shared_pages;       /* paged attention: the first shared_pages entries of every
+                                    row of page_table are the same pages (0: none shared) */
+    const uint32_t* q_start;     /* device, [seqs + 1]: first token row of each sequence  */
+    const uint32_t* kv_len;      /* device, [seqs]: cached tokens, this call's included   */
+    const uint32_t* page_table;  /* device, [seqs][max_pages]; entries behind a sequence's
+                                    last page, or in front of its window, are not read    */
+} nedo_gpu_kv_batch;
+
+/* The new tokens of a batch: rotates queries and keys to their positions and
+ * writes keys and values into the cache.  qkv_dev holds `tokens` rows of
+ * heads * head_dim query, kv_heads * head_dim key and as many value elements (the
+ * decoder's q|k|v layout); the rotated queries go to q_out_dev
+ * [tokens][heads][head_dim], which must not overlap qkv_dev.  Channels i and
+ * i + head_dim/2 turn by position * rope_theta^(-2i/head_dim), the angle in 64
+ * bits; rope_theta 0: no rotation.  With cache->bounds, the channel bounds of every
+ * page written are brought up to date: the range of the keys stored since the
+ * page's first slot was last written (NaN keys left out). */
+NEDO_GPU_API int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                        uint32_t heads, const float* qkv_dev, float rope_theta, float* q_out_dev,
+                                        void* stream);
+
+/* Bytes of workspace that nedo_gpu_paged_attention_dev needs for these sizes
+ * (possibly 0).  Reads no device memory and needs no device. */
+NEDO_GPU_API int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                                    uint32_t heads, uint32_t window, uint64_t* bytes);
+
+/* Attention of every query row over its sequence's cached tokens, itself
+ * included: q_dev and out_dev [tokens][heads][head_dim] (not overlapping),
+ *   out = sum_j softmax_j(scale * q.k_j) v_j,  max(0, p - window + 1) <= j <= p
+ * for a row at position p (window 0: all).  With shared_pages > 0 the keys of the
+ * shared prefix are read once for the whole batch.  Sums and softmax statistics
+ * are kept in 32 bits. */
+NEDO_GPU_API int nedo_gpu_paged_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                              uint32_t heads, const float* q_dev, float* out_dev, float scale,
+                                              uint32_t window, void* workspace_dev, uint64_t workspace_bytes,
+                                              void* stream);
+
+/* For every query row and KV head, the `picks` (1..1024) pages whose keys can
+ * score highest: blocks_dev [tokens][kv_heads][picks] receives logical page
+ * numbers (indexes into the sequence's row of page_table) in ascending order,
+ * 0xFFFFFFFF behind the last.  The page of the row's own position is always among
+ * them; the others, of those before it, by
+ *   score = sum_d (hi_d * sum_g max(q_gd, 0) + lo_d * sum_g min(q_gd, 0))
+ * with the page's bounds lo, hi and the KV head's query heads g, summed in 64 bits
+ * (equal scores: the lower page; NaN last).  At most 16384 pages per sequence. */
+NEDO_GPU_API int nedo_gpu_block_select_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                           uint32_t heads, const float* q_dev, uint32_t picks, uint32_t* blocks_dev,
+                                           void* stream);
+
+/* Bytes of workspace that nedo_gpu_block_attention_dev needs for these sizes. */
+NEDO_GPU_API int nedo_gpu_block_attention_workspace(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                                    uint32_t heads, uint32_t picks, uint64_t* bytes);
+
+/* Attention of every query row over the cached tokens, up to itself, of the pages
+ * listed for it and the KV head (blocks_dev as nedo_gpu_block_select_dev writes
+ * it; shared_pages is not used).  An entry counts when it is above every entry
+ * before it and not beyond the row's own page; others are passed over. */
+NEDO_GPU_API int nedo_gpu_block_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
+                                              uint32_t heads, const float* q_dev, const uint32_t* blocks_dev,
+                                              uint32_t picks, float* out_dev, float scale, void* workspace_dev,
+                                              uint64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -251,6 +251,50 @@ cudaError_t launch_advance(DecodeIo* io, const int64_t* pick, uint32_t* ids, uin
 cudaError_t launch_silu_mul(float* gu, uint32_t f, const float* route, const DecodeIo* io, uint32_t shared_w,
                             uint32_t root_w, uint32_t suffix_w, cudaStream_t stream, bool pdl);
 
+// ---- paged KV cache (kv_append.cu, paged_attention.cu, block_select.cu) ----
+// Kernel-side views of nedo_gpu_kv_cache and nedo_gpu_kv_batch, checked by the host.
+constexpr uint32_t kF32 = 0;
+struct PagedKv {
+    uint32_t type = 0;       // kF32 or kF16
+    uint32_t kv_heads = 0, head_dim = 0;
+    uint32_t page_size = 0, page_shift = 0;
+    uint32_t num_pages = 0;
+    void* k = nullptr;       // [num_pages][kv_heads][page_size][head_dim]
+    void* v = nullptr;
+    void* bounds = nullptr;  // [num_pages][kv_heads][2][head_dim] or null
+};
+struct PagedBatch {
+    uint32_t seqs = 0, tokens = 0, max_q_len = 0, max_kv_len = 0, max_pages = 0;
+    const uint32_t* q_start = nullptr;  // [seqs + 1]
+    const uint32_t* kv_len = nullptr;   // [seqs]
+    const uint32_t* table = nullptr;    // [seqs][max_pages]
+};
+cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
+                             float* q_out, DeviceStatus* st, cudaStream_t stream);
+
+// One attention call: the plan (sizes of its launches and of its workspace) and its run.
+struct PagedAttention {
+    PagedKv kv;
+    PagedBatch b;
+    uint32_t heads = 0, window = 0;
+    uint32_t shared_pages = 0;       // dense: leading pages common to all sequences
+    const uint32_t* blocks = nullptr;  // sparse: [tokens][kv_heads][picks] logical pages
+    uint32_t picks = 0;              // sparse: entries per list (0: dense)
+    // plan: keys per work item and work items per row tile of each part
+    uint32_t own_chunk = 0, own_chunks = 0, prefix_chunk = 0, prefix_chunks = 0;
+    uint64_t workspace = 0;          // bytes
+};
+// false: more work items than one launch holds.  Plans for the 148 SMs of a B200, so
+// that a workspace can be sized without a device.
+bool plan_paged_attention(PagedAttention* a);
+cudaError_t launch_paged_attention(const PagedAttention& a, const float* q, float* out, float scale, void* workspace,
+                                   DeviceStatus* st, cudaStream_t stream);
+
+constexpr uint32_t kMaxPicks = 1024;       // pages a selection holds
+constexpr uint32_t kMaxSelectPages = 16384;  // pages a sequence may have for a selection
+cudaError_t launch_block_select(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* q, uint32_t picks,
+                                uint32_t* blocks, DeviceStatus* st, cudaStream_t stream);
+
 // cuTensorMapEncodeTiled reached through the runtime's driver entry point
 // (null when the driver does not provide it).
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

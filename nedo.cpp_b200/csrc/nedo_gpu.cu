@@ -1646,3 +1646,184 @@ void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d) {
 }
 
 }  // extern "C"
+
+// ---- paged KV cache: append, attention, page selection ----------------------
+namespace {
+
+// Checks the two descriptors (everything the host can see) and fills the kernels'
+// views.  Lengths and page ids live in device memory: the kernels check those.
+int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_batch* b, uint32_t heads, PagedKv* kv,
+                PagedBatch* pb) {
+    const std::string w = std::string(what) + ": ";
+    if (!c || !b) return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    if (c->type != kF32 && c->type != kF16) return fail(NEDO_GPU_ERR_TYPE, w + "KV cache type not supported");
+    if (!heads || !c->kv_heads || heads % c->kv_heads) return fail(NEDO_GPU_ERR_ARG, w + "invalid GQA dimensions");
+    if (heads > 4096u) return fail(NEDO_GPU_ERR_ARG, w + "more than 4096 heads");
+    if (c->head_dim == 0 || c->head_dim > 256u || c->head_dim % 8u)
+        return fail(NEDO_GPU_ERR_ARG, w + "head_dim must be a multiple of 8 in 8..256");
+    if (c->page_size < 16u || c->page_size > 256u || (c->page_size & (c->page_size - 1u)))
+        return fail(NEDO_GPU_ERR_ARG, w + "page_size must be 16, 32, 64, 128 or 256");
+    if (c->num_pages == 0 || c->num_pages >= 0xFFFFFFFFull)
+        return fail(NEDO_GPU_ERR_ARG, w + "num_pages must be in 1..2^32-2");
+    if (!c->k || !c->v) return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->bounds))
+        return fail(NEDO_GPU_ERR_ARG, w + "cache buffers must be 16-byte aligned");
+    if (b->tokens > 0x7FFFFFFFu || b->seqs > 0xFFFFFFu || b->max_kv_len > 0x7FFFFFFFu)
+        return fail(NEDO_GPU_ERR_ARG, w + "batch too large");
+    if (b->max_kv_len > static_cast<uint64_t>(b->max_pages) * c->page_size)
+        return fail(NEDO_GPU_ERR_ARG, w + "max_kv_len exceeds max_pages pages");
+    if (b->shared_pages > b->max_pages || static_cast<uint64_t>(b->shared_pages) * c->page_size > 0x7FFFFFFFull)
+        return fail(NEDO_GPU_ERR_ARG, w + "shared_pages exceeds max_pages");
+    if (b->seqs && b->tokens && (!b->q_start || !b->kv_len || (b->max_pages && !b->page_table)))
+        return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    uint32_t shift = 0;
+    while ((1u << shift) < c->page_size) ++shift;
+    kv->type = c->type;
+    kv->kv_heads = c->kv_heads;
+    kv->head_dim = c->head_dim;
+    kv->page_size = c->page_size;
+    kv->page_shift = shift;
+    kv->num_pages = static_cast<uint32_t>(c->num_pages);
+    kv->k = c->k;
+    kv->v = c->v;
+    kv->bounds = c->bounds;
+    pb->seqs = b->seqs;
+    pb->tokens = b->tokens;
+    pb->max_q_len = std::min(b->max_q_len, b->tokens);
+    pb->max_kv_len = b->max_kv_len;
+    pb->max_pages = b->max_pages;
+    pb->q_start = b->q_start;
+    pb->kv_len = b->kv_len;
+    pb->table = b->page_table;
+    return 0;
+}
+
+bool overlap(const void* a, uint64_t na, const void* b, uint64_t nb) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + nb && y < x + na;
+}
+
+int check_picks(const char* what, uint32_t picks) {
+    if (picks == 0 || picks > kMaxPicks)
+        return fail(NEDO_GPU_ERR_ARG, std::string(what) + ": picks must be in 1.." + std::to_string(kMaxPicks));
+    return 0;
+}
+
+// The plan of an attention call (dense: picks 0).
+int plan_attention(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_batch* b, uint32_t heads,
+                   uint32_t window, const uint32_t* blocks, uint32_t picks, PagedAttention* a) {
+    if (int rc = check_paged(what, c, b, heads, &a->kv, &a->b)) return rc;
+    a->heads = heads;
+    a->window = window;
+    a->shared_pages = picks ? 0u : b->shared_pages;
+    a->blocks = blocks;
+    a->picks = picks;
+    if (!a->b.seqs || !a->b.tokens) return 0;
+    if (!plan_paged_attention(a)) return fail(NEDO_GPU_ERR_ARG, std::string(what) + ": batch too large");
+    return 0;
+}
+
+int run_attention(const char* what, const PagedAttention& a, const float* q, float* out, float scale, void* workspace,
+                  uint64_t workspace_bytes, void* stream) {
+    const std::string w = std::string(what) + ": ";
+    if (!a.b.seqs || !a.b.tokens) return 0;
+    if (!q || !out) return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(workspace))
+        return fail(NEDO_GPU_ERR_ARG, w + "buffers must be 16-byte aligned");
+    const uint64_t bytes = static_cast<uint64_t>(a.b.tokens) * a.heads * a.kv.head_dim * sizeof(float);
+    if (overlap(q, bytes, out, bytes)) return fail(NEDO_GPU_ERR_ARG, w + "q and out overlap");
+    if (a.workspace && (!workspace || workspace_bytes < a.workspace))
+        return fail(NEDO_GPU_ERR_ARG, w + "workspace smaller than " + std::to_string(a.workspace) + " bytes");
+    DeviceState* s = nullptr;
+    if (int rc = get_state(&s)) return rc;
+    cudaError_t e = launch_paged_attention(a, q, out, scale, workspace, s->status, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, what);
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                           const float* qkv_dev, float rope_theta, float* q_out_dev, void* stream) {
+    PagedKv kv;
+    PagedBatch b;
+    if (int rc = check_paged("kv_append", cache, batch, heads, &kv, &b)) return rc;
+    if (!(rope_theta >= 0.f) || !std::isfinite(rope_theta))
+        return fail(NEDO_GPU_ERR_ARG, "kv_append: rope_theta must be positive, or 0 for no rotation");
+    if (!b.seqs || !b.tokens) return 0;
+    if (!qkv_dev || !q_out_dev) return fail(NEDO_GPU_ERR_ARG, "kv_append: null pointer");
+    if (!aligned16(qkv_dev) || !aligned16(q_out_dev))
+        return fail(NEDO_GPU_ERR_ARG, "kv_append: buffers must be 16-byte aligned");
+    const uint64_t row = static_cast<uint64_t>(b.tokens) * kv.head_dim * sizeof(float);
+    if (overlap(qkv_dev, row * (heads + 2ull * kv.kv_heads), q_out_dev, row * heads))
+        return fail(NEDO_GPU_ERR_ARG, "kv_append: qkv and q_out overlap");
+    DeviceState* s = nullptr;
+    if (int rc = get_state(&s)) return rc;
+    cudaError_t e = launch_kv_append(kv, b, heads, qkv_dev, rope_theta, q_out_dev, s->status,
+                                     static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv_append launch");
+    return 0;
+}
+
+int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                                       uint32_t window, uint64_t* bytes) {
+    if (!bytes) return fail(NEDO_GPU_ERR_ARG, "paged_attention: null pointer");
+    PagedAttention a;
+    if (int rc = plan_attention("paged_attention", cache, batch, heads, window, nullptr, 0, &a)) return rc;
+    *bytes = a.workspace;
+    return 0;
+}
+
+int nedo_gpu_paged_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                                 const float* q_dev, float* out_dev, float scale, uint32_t window,
+                                 void* workspace_dev, uint64_t workspace_bytes, void* stream) {
+    PagedAttention a;
+    if (int rc = plan_attention("paged_attention", cache, batch, heads, window, nullptr, 0, &a)) return rc;
+    return run_attention("paged_attention", a, q_dev, out_dev, scale, workspace_dev, workspace_bytes, stream);
+}
+
+int nedo_gpu_block_select_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                              const float* q_dev, uint32_t picks, uint32_t* blocks_dev, void* stream) {
+    PagedKv kv;
+    PagedBatch b;
+    if (int rc = check_paged("block_select", cache, batch, heads, &kv, &b)) return rc;
+    if (int rc = check_picks("block_select", picks)) return rc;
+    if (!kv.bounds) return fail(NEDO_GPU_ERR_ARG, "block_select: the cache has no key bounds");
+    if ((static_cast<uint64_t>(b.max_kv_len) + kv.page_size - 1u) / kv.page_size > kMaxSelectPages)
+        return fail(NEDO_GPU_ERR_ARG, "block_select: more than " + std::to_string(kMaxSelectPages) + " pages per sequence");
+    if (!b.seqs || !b.tokens) return 0;
+    if (!q_dev || !blocks_dev) return fail(NEDO_GPU_ERR_ARG, "block_select: null pointer");
+    if (!aligned16(q_dev)) return fail(NEDO_GPU_ERR_ARG, "block_select: q must be 16-byte aligned");
+    if (static_cast<uint64_t>(b.tokens) * kv.kv_heads > 0x0FFFFFFFull)
+        return fail(NEDO_GPU_ERR_ARG, "block_select: batch too large");
+    DeviceState* s = nullptr;
+    if (int rc = get_state(&s)) return rc;
+    cudaError_t e = launch_block_select(kv, b, heads, q_dev, picks, blocks_dev, s->status,
+                                        static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "block_select launch");
+    return 0;
+}
+
+int nedo_gpu_block_attention_workspace(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                                       uint32_t picks, uint64_t* bytes) {
+    if (!bytes) return fail(NEDO_GPU_ERR_ARG, "block_attention: null pointer");
+    if (int rc = check_picks("block_attention", picks)) return rc;
+    PagedAttention a;
+    if (int rc = plan_attention("block_attention", cache, batch, heads, 0, nullptr, picks, &a)) return rc;
+    *bytes = a.workspace;
+    return 0;
+}
+
+int nedo_gpu_block_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
+                                 const float* q_dev, const uint32_t* blocks_dev, uint32_t picks, float* out_dev,
+                                 float scale, void* workspace_dev, uint64_t workspace_bytes, void* stream) {
+    if (int rc = check_picks("block_attention", picks)) return rc;
+    PagedAttention a;
+    if (int rc = plan_attention("block_attention", cache, batch, heads, 0, blocks_dev, picks, &a)) return rc;
+    if (a.b.seqs && a.b.tokens && !blocks_dev) return fail(NEDO_GPU_ERR_ARG, "block_attention: null pointer");
+    return run_attention("block_attention", a, q_dev, out_dev, scale, workspace_dev, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -22,7 +22,8 @@ import numpy as np
 from . import blocks
 from .blocks import F16, Q4_0, Q8_0, row_bytes
 
-__all__ = ["F16", "Q4_0", "Q8_0", "row_bytes", "blocks", "Library", "load", "NedoGpuError", "LIB_PATH"]
+__all__ = ["F16", "Q4_0", "Q8_0", "row_bytes", "blocks", "Library", "load", "NedoGpuError", "LIB_PATH",
+           "KvCache", "KvBatch"]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(os.path.dirname(HERE), "lib")
@@ -63,6 +64,12 @@ EXPORTS = (
     "nedo_gpu_decoder_logits_dev",
     "nedo_gpu_decoder_reset",
     "nedo_gpu_decoder_destroy",
+    "nedo_gpu_kv_append_dev",
+    "nedo_gpu_paged_attention_workspace",
+    "nedo_gpu_paged_attention_dev",
+    "nedo_gpu_block_select_dev",
+    "nedo_gpu_block_attention_workspace",
+    "nedo_gpu_block_attention_dev",
 )
 
 
@@ -91,6 +98,22 @@ class TensorView(ctypes.Structure):
     _fields_ = [("type", ctypes.c_uint32), ("ndims", ctypes.c_uint32), ("shape", ctypes.c_uint64 * 2),
                 ("data", ctypes.c_void_p), ("nbytes", ctypes.c_uint64)]
 
+
+class KvCache(ctypes.Structure):
+    """nedo_gpu_kv_cache: a paged key/value cache (device addresses; `bounds` may be None)."""
+    _fields_ = [("type", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("num_pages", ctypes.c_uint64), ("k", ctypes.c_void_p),
+                ("v", ctypes.c_void_p), ("bounds", ctypes.c_void_p)]
+
+
+class KvBatch(ctypes.Structure):
+    """nedo_gpu_kv_batch: a ragged batch over a KvCache (device addresses of its uint32 lists)."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("seqs", "tokens", "max_q_len", "max_kv_len", "max_pages",
+                                                "shared_pages")] + [(n, ctypes.c_void_p) for n in
+                                                                    ("q_start", "kv_len", "page_table")]
+
+
+_cachep, _batchp = ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch)
 
 _SIGNATURES = {
     "nedo_gpu_version": ([], _i32),
@@ -125,6 +148,13 @@ _SIGNATURES = {
     "nedo_gpu_decoder_logits_dev": ([_vp, ctypes.POINTER(_vp)], _i32),
     "nedo_gpu_decoder_reset": ([_vp], _i32),
     "nedo_gpu_decoder_destroy": ([_vp], None),
+    "nedo_gpu_kv_append_dev": ([_cachep, _batchp, _u32, _vp, ctypes.c_float, _vp, _vp], _i32),
+    "nedo_gpu_paged_attention_workspace": ([_cachep, _batchp, _u32, _u32, _u64p], _i32),
+    "nedo_gpu_paged_attention_dev": ([_cachep, _batchp, _u32, _vp, _vp, ctypes.c_float, _u32, _vp, _u64, _vp], _i32),
+    "nedo_gpu_block_select_dev": ([_cachep, _batchp, _u32, _vp, _u32, _vp, _vp], _i32),
+    "nedo_gpu_block_attention_workspace": ([_cachep, _batchp, _u32, _u32, _u64p], _i32),
+    "nedo_gpu_block_attention_dev": ([_cachep, _batchp, _u32, _vp, _vp, _u32, _vp, ctypes.c_float, _vp, _u64, _vp],
+                                     _i32),
 }
 
 
@@ -269,6 +299,39 @@ class Library:
     def dequant_rows_dev(self, type_, rows, cols, w_ptr, row_begin, row_count, out_ptr, stream=0) -> None:
         self._check(self.lib.nedo_gpu_dequant_rows_dev(type_, rows, cols, w_ptr, row_begin, row_count, out_ptr,
                                                        stream))
+
+    # ------------------------------------------------------ paged KV cache
+    def kv_append_dev(self, cache: KvCache, batch: KvBatch, heads, qkv_ptr, rope_theta, q_out_ptr, stream=0) -> None:
+        """Rotate the q|k|v rows of a batch to their positions; keys and values into the cache."""
+        self._check(self.lib.nedo_gpu_kv_append_dev(cache, batch, heads, qkv_ptr, rope_theta, q_out_ptr, stream))
+
+    def paged_attention_workspace(self, cache: KvCache, batch: KvBatch, heads, window=0) -> int:
+        """Bytes of device workspace that paged_attention_dev needs for these sizes."""
+        n = _u64(0)
+        self._check(self.lib.nedo_gpu_paged_attention_workspace(cache, batch, heads, window, n))
+        return n.value
+
+    def paged_attention_dev(self, cache: KvCache, batch: KvBatch, heads, q_ptr, out_ptr, scale, window=0,
+                            workspace_ptr=None, workspace_bytes=0, stream=0) -> None:
+        """Causal attention of every query row over its sequence's pages (window 0: no limit)."""
+        self._check(self.lib.nedo_gpu_paged_attention_dev(cache, batch, heads, q_ptr, out_ptr, scale, window,
+                                                          workspace_ptr, workspace_bytes, stream))
+
+    def block_select_dev(self, cache: KvCache, batch: KvBatch, heads, q_ptr, picks, blocks_ptr, stream=0) -> None:
+        """The `picks` pages per query row and KV head whose key bounds allow the largest scores."""
+        self._check(self.lib.nedo_gpu_block_select_dev(cache, batch, heads, q_ptr, picks, blocks_ptr, stream))
+
+    def block_attention_workspace(self, cache: KvCache, batch: KvBatch, heads, picks) -> int:
+        """Bytes of device workspace that block_attention_dev needs for these sizes."""
+        n = _u64(0)
+        self._check(self.lib.nedo_gpu_block_attention_workspace(cache, batch, heads, picks, n))
+        return n.value
+
+    def block_attention_dev(self, cache: KvCache, batch: KvBatch, heads, q_ptr, blocks_ptr, picks, out_ptr, scale,
+                            workspace_ptr=None, workspace_bytes=0, stream=0) -> None:
+        """Attention of every query row over the pages listed for it (block_select_dev's layout)."""
+        self._check(self.lib.nedo_gpu_block_attention_dev(cache, batch, heads, q_ptr, blocks_ptr, picks, out_ptr,
+                                                          scale, workspace_ptr, workspace_bytes, stream))
 
     def status(self, stream=0) -> None:
         self._check(self.lib.nedo_gpu_status(stream))
