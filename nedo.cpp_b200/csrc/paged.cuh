@@ -40,6 +40,8 @@ __device__ __forceinline__ PagedSeq load_seq(const PagedBatch& b, uint32_t s, De
 // The sequence that holds token row t (the last one starting at or before it), or
 // kNone for a row behind the last sequence or before the first.
 __device__ __forceinline__ uint32_t seq_of_token(const PagedBatch& b, uint32_t t) {
+    // one row per sequence, as in decoding: no search
+    if (t < b.seqs && b.q_start[t] == t && b.q_start[t + 1u] == t + 1u) return t;
     uint32_t lo = 0, hi = b.seqs + 1u;  // first index in [0, seqs] whose start is above t
     while (lo < hi) {
         const uint32_t mid = (lo + hi) >> 1;

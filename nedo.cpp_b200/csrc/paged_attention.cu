@@ -15,38 +15,10 @@
 // once for the whole batch.
 #include <algorithm>
 
-#include "paged.cuh"
+#include "paged_attention.cuh"
 
 namespace nedo_gpu {
 namespace {
-
-enum : uint32_t { kPartOwn = 0, kPartPrefix = 1, kPartBlocks = 2 };
-
-struct AttnArgs {
-    PagedKv kv;
-    PagedBatch b;
-    const float* q;
-    float* out;
-    float scale_log2;
-    uint32_t heads, group, window;
-    uint32_t part;
-    uint32_t shared_len;     // keys of the shared prefix
-    uint32_t chunk, chunks;  // keys per item, items per row tile
-    uint32_t slot0;          // first partial slot of this part
-    uint32_t direct;         // one item per row: write out
-    float* part_o;           // [slots][tokens * heads][head_dim]
-    float2* part_ml;         // [slots][tokens * heads]
-    const uint32_t* blocks;
-    uint32_t picks, row_blocks;
-    DeviceStatus* st;
-};
-
-// First chunk of sequence `sq` that any of its rows sees (own part).
-__device__ __forceinline__ uint32_t own_first_chunk(const PagedSeq& sq, uint32_t window, uint32_t base, uint32_t chunk) {
-    const int p0 = sq.pos(0) > 0 ? sq.pos(0) : 0;
-    const uint32_t lo = first_key(p0, window);
-    return lo > base ? (lo - base) / chunk : 0u;
-}
 
 // ---- the general kernel: any type, any head size, CUDA cores ----------------
 constexpr uint32_t kRows = 8;   // query rows per tile
@@ -80,24 +52,8 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
     PagedSeq sq{0u, 0u, 0u};
     if (a.part == kPartOwn) {
         if (warp == 0) {
-            uint32_t seq = kNone, tile = 0, before = 0;
-            for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-                uint32_t cnt = 0;
-                if (s0 + lane < a.b.seqs) cnt = (load_seq(a.b, s0 + lane, a.st).n * a.group + kRows - 1u) / kRows;
-                uint32_t inc = cnt;
-                for (uint32_t o = 1; o < 32u; o <<= 1) {
-                    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                    if (lane >= o) inc += v;
-                }
-                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > rest);
-                if (hit != 0u) {
-                    const uint32_t w = __ffs(hit) - 1u;
-                    seq = s0 + w;
-                    tile = rest - before - __shfl_sync(0xFFFFFFFFu, inc - cnt, w);
-                    break;
-                }
-                before += __shfl_sync(0xFFFFFFFFu, inc, 31);
-            }
+            uint32_t tile;
+            const uint32_t seq = find_tile(a, rest, kRows, &tile);
             if (lane == 0) {
                 found[0] = seq;
                 found[1] = tile;
@@ -128,15 +84,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
         if (tid < nrows) {
             tok = t0 + (r0 + tid) / a.group;
             head = kh * a.group + (r0 + tid) % a.group;
-            if (a.part == kPartPrefix) {
-                const uint32_t ss = seq_of_token(a.b, tok);
-                if (ss != kNone) {
-                    const PagedSeq q2 = load_seq(a.b, ss, a.st);
-                    if (q2.n != 0u) p = max(-1, q2.pos(tok - q2.t0));
-                }
-            } else {
-                p = max(-1, sq.pos(tok - sq.t0));
-            }
+            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
         }
         row_tok[tid] = tok;
         row_head[tid] = head;
@@ -149,25 +97,7 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
     uint32_t kb = kNone, ke = 0;
     if (a.part == kPartBlocks) {
         const uint32_t* l = a.blocks + (static_cast<size_t>(t0) * a.kv.kv_heads + kh) * a.picks;
-        const int p = row_pos[0];
-        // an entry counts when it is above all entries before it and at or below the query's page
-        if (warp == 0) {
-            int best = -1;
-            for (uint32_t i0 = 0; i0 < a.picks; i0 += 32u) {
-                const uint32_t v = i0 + lane < a.picks ? l[i0 + lane] : kNone;
-                const bool in = p >= 0 && v <= (static_cast<uint32_t>(max(p, 0)) >> a.kv.page_shift);
-                int run = in ? static_cast<int>(v) : -1;
-                for (uint32_t o = 1; o < 32u; o <<= 1) {
-                    const int u = __shfl_up_sync(0xFFFFFFFFu, run, o);
-                    if (lane >= o) run = max(run, u);
-                }
-                int prev = __shfl_up_sync(0xFFFFFFFFu, run, 1);
-                if (lane == 0) prev = -1;
-                prev = max(prev, best);
-                if (i0 + lane < a.picks) list[i0 + lane] = in && static_cast<int>(v) > prev ? v : kNone;
-                best = max(best, __shfl_sync(0xFFFFFFFFu, run, 31));
-            }
-        }
+        if (warp == 0) checked_list(l, a.picks, row_pos[0], a.kv.page_shift, list);
         __syncthreads();
         kb = c * a.chunk;
         ke = min(kb + a.chunk, a.picks << a.kv.page_shift);
@@ -296,6 +226,15 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
     }
 }
 
+cudaError_t launch_simt(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    const size_t smem = simt_smem(a.kv.head_dim);
+    auto* kernel = a.kv.type == kF16 ? attention_simt_kernel<__half> : attention_simt_kernel<float>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    kernel<<<static_cast<uint32_t>(items), kThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+}
+
 // ---- adding a row's chunks ---------------------------------------------------
 struct CombineArgs {
     PagedKv kv;
@@ -305,23 +244,31 @@ struct CombineArgs {
     const float2* part_ml;
     uint32_t heads, window, shared_len;
     uint32_t own_chunk, own_chunks, prefix_chunk, prefix_chunks;
+    uint32_t few_rows, few_chunk;        // sequences of at most few_rows rows have chunks of their own
+    uint32_t own_direct, few_direct;     // written out already
+    uint32_t group;
     uint32_t blocks;  // the sparse call: every slot is written
 };
 
-// One warp per (token, head): first the maximum over the row's chunks, then their
-// sum in chunk order.  A chunk in which the row sees nothing has weight sum 0.
-constexpr uint32_t kCombineWarps = 4;
-__global__ void __launch_bounds__(32 * kCombineWarps) attention_combine_kernel(CombineArgs a) {
-    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-    const size_t row = static_cast<size_t>(blockIdx.x) * kCombineWarps + (threadIdx.x >> 5);
-    const uint32_t lane = threadIdx.x & 31u;
-    if (row >= rows_all) return;
+// One CTA per (token, head).  The maximum over the row's chunks first, then in blocks of
+// kCombineThreads chunks their weights 2^(m_i - m) into shared memory, and the weighted
+// sum with head_dim / 4 threads to a chunk and as many chunks at once as the CTA holds,
+// four loads in flight each; the groups' sums meet in group order.  A chunk in which the
+// row sees nothing has weight sum 0 and may hold anything.  Launched so that it comes up
+// while the last work items run; it waits for their sums before it reads them.
+constexpr uint32_t kCombineThreads = 128;
+__global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(CombineArgs a) {
+    __shared__ float wt[kCombineThreads], red[kCombineThreads / 32u];
+    __shared__ float4 sums[kCombineThreads];
+    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads, row = blockIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t t = static_cast<uint32_t>(row / a.heads);
     const uint32_t s = seq_of_token(a.b, t);
-    if (s == kNone) return;
-    const PagedSeq sq = load_seq(a.b, s, nullptr);
-    if (sq.n == 0u) return;
-    const int p = sq.pos(t - sq.t0);
+    PagedSeq sq{0u, 0u, 0u};
+    if (s != kNone) sq = load_seq(a.b, s, nullptr);
+    const int p = sq.n != 0u ? sq.pos(t - sq.t0) : -1;
+    const bool few = sq.n * a.group <= a.few_rows;
+    const uint32_t chunk = few ? a.few_chunk : a.own_chunk;
     // the row's slots: [b0, e0) of the prefix, [b1, e1) of its own keys
     uint32_t b0 = 0, e0 = 0, b1 = 0, e1 = 0;
     if (a.blocks) {
@@ -333,55 +280,182 @@ __global__ void __launch_bounds__(32 * kCombineWarps) attention_combine_kernel(C
             e0 = (min(hi, a.shared_len) + a.prefix_chunk - 1u) / a.prefix_chunk;
         }
         if (hi > a.shared_len) {
-            const uint32_t first = own_first_chunk(sq, a.window, a.shared_len, a.own_chunk);
-            b1 = a.prefix_chunks + (max(lo, a.shared_len) - a.shared_len) / a.own_chunk - first;
-            e1 = a.prefix_chunks + (hi - 1u - a.shared_len) / a.own_chunk + 1u - first;
+            const uint32_t first = own_first_chunk(sq, a.window, a.shared_len, chunk);
+            b1 = a.prefix_chunks + (max(lo, a.shared_len) - a.shared_len) / chunk - first;
+            e1 = a.prefix_chunks + (hi - 1u - a.shared_len) / chunk + 1u - first;
         }
     }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (sq.n == 0u || (few ? a.few_direct : a.own_direct)) return;  // no row of any sequence, or done
     const uint32_t n0 = e0 - b0, n = n0 + (e1 - b1);
+    const float2* ml = a.part_ml + row;
+    auto slot = [&](uint32_t i) -> size_t { return i < n0 ? b0 + i : b1 + (i - n0); };
     float m = -INFINITY;
-    for (uint32_t i = lane; i < n; i += 32u) {
-        const uint32_t slot = i < n0 ? b0 + i : b1 + (i - n0);
-        m = fmaxf(m, a.part_ml[slot * rows_all + row].x);
-    }
+    for (uint32_t i = tid; i < n; i += kCombineThreads) m = fmaxf(m, ml[slot(i) * rows_all].x);
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const uint32_t hd = a.kv.head_dim;
-    float l = 0.f, acc[8];
-#pragma unroll
-    for (uint32_t u = 0; u < 8u; ++u) acc[u] = 0.f;
-    for (uint32_t i = 0; i < n; ++i) {
-        const size_t slot = i < n0 ? b0 + i : b1 + (i - n0);
-        const float2 ml = a.part_ml[slot * rows_all + row];
-        if (ml.y == 0.f) continue;  // the row sees nothing there, or every weight underflowed
-        const float w = exp2f(ml.x - m);
-        l = fmaf(ml.y, w, l);
-        const float* o = a.part_o + (slot * rows_all + row) * hd;
-#pragma unroll
-        for (uint32_t u = 0; u < 8u; ++u)
-            if (lane + 32u * u < hd) acc[u] = fmaf(o[lane + 32u * u], w, acc[u]);
+    if (lane == 0u) red[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    const uint32_t hd = a.kv.head_dim, hd4 = hd / 4u, groups = kCombineThreads / hd4;
+    const uint32_t grp = tid / hd4, d = tid - grp * hd4;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t i0 = 0; i0 < n; i0 += kCombineThreads) {
+        const uint32_t cnt = min(kCombineThreads, n - i0);
+        __syncthreads();
+        float w = 0.f;
+        if (tid < cnt) {
+            const float2 x = ml[slot(i0 + tid) * rows_all];
+            if (x.y != 0.f) {
+                w = exp2f(x.x - m);
+                l = fmaf(x.y, w, l);
+            }
+        }
+        wt[tid] = w;
+        __syncthreads();
+        if (grp < groups) {
+#pragma unroll 4
+            for (uint32_t i = grp; i < cnt; i += groups) {
+                const float f = wt[i];
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f != 0.f) x = *reinterpret_cast<const float4*>(a.part_o + (slot(i0 + i) * rows_all + row) * hd + 4u * d);
+                acc.x = fmaf(x.x, f, acc.x);
+                acc.y = fmaf(x.y, f, acc.y);
+                acc.z = fmaf(x.z, f, acc.z);
+                acc.w = fmaf(x.w, f, acc.w);
+            }
+        }
     }
-#pragma unroll
-    for (uint32_t u = 0; u < 8u; ++u)
-        if (lane + 32u * u < hd) a.out[row * hd + lane + 32u * u] = l == 0.f ? 0.f : acc[u] / l;
+    l = warp_sum(l);
+    __syncthreads();
+    if (lane == 0u) red[warp] = l;
+    sums[tid] = acc;
+    __syncthreads();
+    if (tid >= hd4) return;
+    l = (red[0] + red[1]) + (red[2] + red[3]);
+    for (uint32_t k = 1; k < groups; ++k) {
+        const float4 x = sums[k * hd4 + tid];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+    }
+    const bool none = l == 0.f;
+    *reinterpret_cast<float4*>(a.out + row * hd + 4u * tid) =
+        none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
+}
+
+// Which kernel takes a part, and what its work items cost (for the plan).
+enum class Kernel { kFew, kMany, kSimt };
+struct Cost {
+    uint32_t rows;       // query rows per tile
+    uint32_t slots;      // work items that run at once on 148 SMs
+    uint32_t max_chunk;  // keys an item can take (0: any number)
+    double ns_per_key, ns_fixed;
+};
+Cost cost_of(Kernel k, const PagedKv& kv) {
+    const uint32_t hd = kv.head_dim;
+    switch (k) {
+        case Kernel::kFew: {  // reads 4 hd bytes per key of the SMs' common 6.5 TB/s
+            const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
+            return {kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0};
+        }
+        case Kernel::kMany: {  // 64 rows through the tensor cores, two items to an SM
+            const uint32_t slots = 148u * (hd <= 128u ? 2u : 1u);
+            return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0};
+        }
+        default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0};
+    }
+}
+
+// Keys per work item, a multiple of 64 and of the page size: of the chunkings that fill
+// one, two, ... rounds of items the one with the least estimated time, the fixed cost of an
+// item and the bytes of the chunks' sums counted.
+uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c) {
+    const uint64_t step = std::max(64u, kv.page_size);
+    if (keys <= step) return static_cast<uint32_t>(step);
+    auto rounded = [&](uint64_t n) { return ((keys + n - 1u) / n + step - 1u) / step * step; };
+    uint64_t best = 0;
+    double best_ns = 0.0;
+    auto consider = [&](uint64_t n) {
+        uint64_t chunk = rounded(n);
+        if (c.max_chunk != 0u && chunk > c.max_chunk) chunk = c.max_chunk / step * step;
+        n = (keys + chunk - 1u) / chunk;
+        const double rounds = static_cast<double>((units * n + c.slots - 1u) / c.slots);
+        // a chunk's sums are written once and read once at about half the copy rate
+        const double ns = rounds * (static_cast<double>(chunk) * c.ns_per_key + c.ns_fixed) +
+                          (n > 1u ? 2000.0 + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0 : 0.0);
+        if (best == 0u || ns < best_ns) {
+            best = chunk;
+            best_ns = ns;
+        }
+    };
+    consider(1);
+    for (uint64_t rounds = 1; rounds <= 12u; ++rounds) {
+        const uint64_t n = rounds * c.slots / units;
+        if (n > 1u) consider(std::min<uint64_t>(n, (keys + step - 1u) / step));
+    }
+    return static_cast<uint32_t>(best);
+}
+
+uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1u) / b; }
+
+// Row tiles of the own part: every sequence has whole tiles.
+uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
+    const uint64_t group = a.heads / a.kv.kv_heads;
+    return std::min<uint64_t>(a.b.tokens * group / rows + a.b.seqs, a.b.seqs * ceil_div(a.b.max_q_len * group, rows));
+}
+
+Kernel prefix_kernel(const PagedAttention& a) {
+    if (a.kv.type != kF16) return Kernel::kSimt;
+    return static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads) <= kFewRows ? Kernel::kFew : Kernel::kMany;
+}
+Kernel own_kernel(const PagedAttention& a) {
+    if (a.kv.type != kF16) return Kernel::kSimt;
+    if (a.picks) return Kernel::kFew;
+    return static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads) <= kFewRows ? Kernel::kFew : Kernel::kMany;
 }
 
 }  // namespace
 
 bool plan_paged_attention(PagedAttention* a) {
-    const uint64_t hd = a->kv.head_dim, rows = static_cast<uint64_t>(a->b.tokens) * a->heads;
-    const uint32_t shared = a->picks ? 0u : a->shared_pages << a->kv.page_shift;
-    a->prefix_chunk = 1024;
-    a->own_chunk = 1024;
-    a->prefix_chunks = (shared + a->prefix_chunk - 1u) / a->prefix_chunk;
-    uint64_t keys = a->picks ? static_cast<uint64_t>(a->picks) << a->kv.page_shift
-                             : (a->b.max_kv_len > shared ? a->b.max_kv_len - shared : 0u);
-    uint64_t n = (keys + a->own_chunk - 1u) / a->own_chunk;
-    if (!a->picks && a->window != 0u)
-        n = std::min<uint64_t>(n, (static_cast<uint64_t>(a->window) + a->b.max_q_len + a->own_chunk - 2u) / a->own_chunk + 1u);
-    a->own_chunks = static_cast<uint32_t>(std::max<uint64_t>(n, 1u));
-    const uint64_t slots = static_cast<uint64_t>(a->own_chunks) + a->prefix_chunks;
-    a->workspace = slots == 1u ? 0u : slots * rows * (hd * sizeof(float) + sizeof(float2));
-    return true;
+    const uint64_t rows = static_cast<uint64_t>(a->b.tokens) * a->heads;
+    const uint64_t group = a->heads / a->kv.kv_heads, all = a->b.tokens * group;
+    const uint64_t sums = rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));  // bytes of one chunk of every row
+    const uint64_t shared = a->picks ? 0u : static_cast<uint64_t>(a->shared_pages) << a->kv.page_shift;
+    uint64_t units = 0, prefix_units = 0;
+    if (shared != 0u) {
+        const Cost c = cost_of(prefix_kernel(*a), a->kv);
+        prefix_units = ceil_div(all, c.rows) * a->kv.kv_heads;
+        a->prefix_chunk = chunk_keys(shared, prefix_units, sums, a->kv, c);
+        a->prefix_chunks = static_cast<uint32_t>(ceil_div(shared, a->prefix_chunk));
+    }
+    const uint64_t most = a->picks ? static_cast<uint64_t>(a->picks) << a->kv.page_shift
+                                   : (a->b.max_kv_len > shared ? a->b.max_kv_len - shared : 0u);
+    uint64_t keys = most;
+    if (!a->picks && a->window != 0u) keys = std::min<uint64_t>(keys, static_cast<uint64_t>(a->window) + a->b.max_q_len - 1u);
+    // chunks of at most `chunk` keys that a row tile's keys touch: a window that starts
+    // inside a chunk reaches one chunk further
+    auto chunks = [&](uint64_t chunk) {
+        const uint64_t n = ceil_div(keys, chunk);
+        return static_cast<uint32_t>(std::max<uint64_t>(n * chunk < most ? n + 1u : n, 1u));
+    };
+    const Cost c = cost_of(own_kernel(*a), a->kv);
+    units = (a->picks ? a->b.tokens * ceil_div(group, c.rows) : own_tiles(*a, c.rows)) * a->kv.kv_heads;
+    a->own_chunk = chunk_keys(keys, units, sums, a->kv, c);
+    a->own_chunks = chunks(a->own_chunk);
+    uint64_t grid = units * a->own_chunks, slots = a->own_chunks;
+    if (own_kernel(*a) == Kernel::kMany && a->b.seqs > 1u) {
+        const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads;
+        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(Kernel::kFew, a->kv));
+        a->few_chunks = chunks(a->few_chunk);
+        grid = std::max(grid, u * a->few_chunks);
+        slots = std::max<uint64_t>(slots, a->few_chunks);
+    }
+    slots += a->prefix_chunks;
+    a->workspace = slots == 1u ? 0u : slots * sums;
+    // the launches' grids
+    return grid <= 0x7FFFFFFFull && prefix_units * a->prefix_chunks <= 0x7FFFFFFFull && rows <= 0x7FFFFFFFull;
 }
 
 cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, float* out, float scale, void* workspace,
@@ -399,40 +473,61 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     a.blocks = p.blocks;
     a.picks = p.picks;
     a.st = st;
-    const uint64_t slots = static_cast<uint64_t>(p.own_chunks) + p.prefix_chunks;
+    a.rows_to = kNone;
+    const uint64_t slots = static_cast<uint64_t>(std::max(p.own_chunks, p.few_chunks)) + p.prefix_chunks;
     const uint64_t rows = static_cast<uint64_t>(p.b.tokens) * p.heads;
-    a.direct = slots == 1u;
+    const bool own_direct = p.prefix_chunks == 0u && p.own_chunks == 1u;
+    const bool few_direct = p.prefix_chunks == 0u && p.few_chunks <= 1u;
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * rows * p.kv.head_dim);
-    const size_t smem = simt_smem(p.kv.head_dim);
-    auto* kernel = p.kv.type == kF16 ? attention_simt_kernel<__half> : attention_simt_kernel<float>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
+    cudaError_t e = cudaSuccess;
     if (p.prefix_chunks != 0u) {
         a.part = kPartPrefix;
         a.chunk = p.prefix_chunk;
         a.chunks = p.prefix_chunks;
         a.slot0 = 0;
-        const uint64_t tiles = (static_cast<uint64_t>(p.b.tokens) * a.group + kRows - 1u) / kRows;
-        kernel<<<static_cast<uint32_t>(tiles * p.kv.kv_heads * a.chunks), kThreads, smem, stream>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+        const Kernel k = prefix_kernel(p);
+        const uint64_t tiles = ceil_div(static_cast<uint64_t>(p.b.tokens) * a.group, cost_of(k, p.kv).rows);
+        e = k == Kernel::kFew    ? launch_attention_few(a, tiles * p.kv.kv_heads * a.chunks, stream)
+            : k == Kernel::kMany ? launch_attention_many(a, tiles, stream)
+                                 : launch_simt(a, tiles * p.kv.kv_heads * a.chunks, stream);
+        if (e != cudaSuccess) return e;
     }
     a.chunk = p.own_chunk;
     a.chunks = p.own_chunks;
     a.slot0 = p.prefix_chunks;
-    uint64_t tiles;
+    a.direct = own_direct;
+    const Kernel k = own_kernel(p);
+    const uint32_t tile = cost_of(k, p.kv).rows;
     if (p.picks) {
         a.part = kPartBlocks;
-        a.row_blocks = (a.group + kRows - 1u) / kRows;
-        tiles = static_cast<uint64_t>(p.b.tokens) * a.row_blocks;
+        a.row_blocks = static_cast<uint32_t>(ceil_div(a.group, tile));
+        const uint64_t items = static_cast<uint64_t>(p.b.tokens) * a.row_blocks * p.kv.kv_heads * a.chunks;
+        e = k == Kernel::kFew ? launch_attention_few(a, items, stream) : launch_simt(a, items, stream);
     } else {
         a.part = kPartOwn;
-        tiles = std::min<uint64_t>(static_cast<uint64_t>(p.b.tokens) * a.group / kRows + p.b.seqs,
-                                   static_cast<uint64_t>(p.b.seqs) * ((static_cast<uint64_t>(p.b.max_q_len) * a.group + kRows - 1u) / kRows));
+        const uint64_t pairs = static_cast<uint64_t>(p.b.seqs) * p.kv.kv_heads;
+        if (k == Kernel::kSimt) {
+            e = launch_simt(a, own_tiles(p, tile) * p.kv.kv_heads * a.chunks, stream);
+        } else if (k == Kernel::kFew) {
+            e = launch_attention_few(a, pairs * a.chunks, stream);
+        } else {
+            // sequences with few rows among others go to the few-rows kernel: a 64-row tile
+            // would do eight times their work
+            const bool mixed = p.few_chunks != 0u;
+            a.rows_from = mixed ? kFewRows + 1u : 0u;
+            e = launch_attention_many(a, own_tiles(p, tile), stream);
+            if (e == cudaSuccess && mixed) {
+                a.rows_from = 0u;
+                a.rows_to = kFewRows;
+                a.chunk = p.few_chunk;
+                a.chunks = p.few_chunks;
+                a.direct = few_direct;
+                e = launch_attention_few(a, pairs * a.chunks, stream);
+            }
+        }
     }
-    kernel<<<static_cast<uint32_t>(tiles * p.kv.kv_heads * a.chunks), kThreads, smem, stream>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    if (a.direct) return cudaSuccess;
+    if (e != cudaSuccess || (own_direct && few_direct)) return e;
     CombineArgs c = {};
     c.kv = p.kv;
     c.b = p.b;
@@ -446,10 +541,22 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     c.own_chunks = p.own_chunks;
     c.prefix_chunk = p.prefix_chunk;
     c.prefix_chunks = p.prefix_chunks;
+    c.few_rows = p.few_chunks != 0u ? kFewRows : 0u;
+    c.few_chunk = p.few_chunk;
+    c.own_direct = own_direct;
+    c.few_direct = few_direct;
+    c.group = a.group;
     c.blocks = p.picks != 0u;
-    attention_combine_kernel<<<static_cast<uint32_t>((rows + kCombineWarps - 1u) / kCombineWarps), 32 * kCombineWarps, 0,
-                               stream>>>(c);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<uint32_t>(rows));
+    cfg.blockDim = dim3(kCombineThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_combine_kernel, c);
 }
 
 }  // namespace nedo_gpu

@@ -1,0 +1,365 @@
+// paged_attention_few.cu -- attention over a paged F16 cache for tiles of at most
+// eight query rows (single tokens with their group of heads, a few tokens of small
+// groups, the rows of a page list): the shape of decoding, bound by reading the cache.
+//
+// Mathematics.  Queries and weights are fp32 and the cache is fp16, so every product
+// runs on the fp16 tensor cores with the fp32 side split in two halves,
+// x = hi + lo, that keep 22 bits of it: q is scaled by a power of two per row (its
+// largest channel to [2^13, 2^14), so that the low half stays a normal number), and the
+// weights p = 2^(s - m + 14) are taken up by the same factor in numerator and sum.  The
+// two halves ride in one m16n8k16 operand, rows 0-7 the high and rows 8-15 the low half
+// of the same eight query rows, so the split costs no extra instruction: both parts of a
+// row's sum land in the same thread, which adds them.
+//
+// Work.  A CTA of four warps takes one row tile and one chunk of keys; each warp streams
+// every fourth 16-key tile through a ring of its own (cp.async, three stages), with its
+// own running maximum and sums, so the warps meet only at the end.  A 16-key tile lies
+// within one page.  Two CTAs share an SM.
+#include "paged_attention.cuh"
+#include "paged_mma.cuh"
+
+namespace nedo_gpu {
+namespace {
+
+constexpr uint32_t kWarps = 4;
+constexpr uint32_t kThreads = 32 * kWarps;
+constexpr uint32_t kKeys = 16;         // keys per tile
+
+template <uint32_t HD>
+struct Few {
+    static constexpr uint32_t kStages = HD == 256 ? 2 : 3;
+    static constexpr uint32_t kRowBytes = HD * 2u;
+    static constexpr uint32_t kTileBytes = kKeys * kRowBytes;      // keys or values of one tile
+    static constexpr uint32_t kStageBytes = 2u * kTileBytes;
+    static constexpr uint32_t kSmem = kWarps * kStages * kStageBytes;
+};
+
+// Byte offset of 16-byte chunk `c` of row `r` in a tile: chunks swapped by the row's
+// number so that eight rows' same chunk falls into eight different bank groups.
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
+    return r * Few<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(AttnArgs a) {
+    using F = Few<HD>;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ uint32_t row_tok[kFewRows], row_head[kFewRows];
+    __shared__ int row_pos[kFewRows];
+    __shared__ float wm[kWarps][kFewRows], wl[kWarps][kFewRows];
+    __shared__ uint32_t list[kMaxPicks];
+    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t c = blockIdx.x % a.chunks;
+    uint32_t rest = blockIdx.x / a.chunks;
+    const uint32_t kh = rest % a.kv.kv_heads;
+    rest /= a.kv.kv_heads;
+
+    // rows
+    uint32_t s = 0, r0 = 0, nrows, t0 = 0;
+    PagedSeq sq{0u, 0u, 0u};
+    if (a.part == kPartPrefix) {
+        nrows = a.b.tokens * a.group;
+    } else {
+        if (a.part == kPartOwn) {
+            s = rest;
+        } else {
+            t0 = rest / a.row_blocks;
+            r0 = (rest % a.row_blocks) * kFewRows;
+            s = seq_of_token(a.b, t0);
+            if (s == kNone) return;
+        }
+        sq = load_seq(a.b, s, a.st);
+        if (sq.n == 0u) return;
+        if (a.part == kPartOwn) t0 = sq.t0;
+        if (a.part == kPartOwn && sq.n * a.group > a.rows_to) return;  // the many-rows kernel's
+        nrows = a.part == kPartOwn ? sq.n * a.group : min(kFewRows, a.group - r0);
+    }
+    if (tid < kFewRows) {
+        int p = -2;
+        uint32_t tok = 0, head = 0;
+        if (tid < nrows) {
+            tok = t0 + (r0 + tid) / a.group;
+            head = kh * a.group + (r0 + tid) % a.group;
+            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
+        }
+        row_tok[tid] = tok;
+        row_head[tid] = head;
+        row_pos[tid] = p;
+    }
+    __syncthreads();
+    // keys [kb, ke): positions, or places in the page list; [all_b, all_e): seen by every row
+    uint32_t kb = kNone, ke = 0, all_b = 0, all_e = kNone;
+    for (uint32_t r = 0; r < kFewRows; ++r) {
+        if (row_pos[r] < 0) continue;
+        const uint32_t lo = first_key(row_pos[r], a.window), hi = static_cast<uint32_t>(row_pos[r]) + 1u;
+        kb = min(kb, lo);
+        ke = max(ke, hi);
+        all_b = max(all_b, lo);
+        all_e = min(all_e, hi);
+    }
+    if (a.part == kPartBlocks) {
+        const uint32_t e0 = (c * a.chunk) >> a.kv.page_shift;
+        const uint32_t e1 = min(e0 + (a.chunk >> a.kv.page_shift), a.picks);
+        if (warp == 0)
+            checked_list(a.blocks + (static_cast<size_t>(t0) * a.kv.kv_heads + kh) * a.picks, e1, row_pos[0],
+                         a.kv.page_shift, list);
+        __syncthreads();
+        kb = e0 << a.kv.page_shift;
+        ke = e1 << a.kv.page_shift;
+    } else {
+        uint32_t base = 0, first = 0;
+        if (a.part == kPartOwn) {
+            base = a.shared_len;
+            first = own_first_chunk(sq, a.window, base, a.chunk);
+        } else {
+            ke = min(ke, a.shared_len);
+        }
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
+        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
+        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
+    }
+    // this warp's tiles: tile i starts at key j0 + 16 (4 i + warp); lane i holds its page and
+    // the position of its first key
+    const uint32_t j0 = kb & ~(kKeys - 1u);
+    const uint32_t ntiles_all = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
+    const uint32_t ntiles = ntiles_all > warp ? (ntiles_all - warp + kWarps - 1u) / kWarps : 0u;
+    uint32_t my_page = kNone, my_pos = 0;
+    if (lane < ntiles) {
+        const uint32_t j = j0 + kKeys * (kWarps * lane + warp);
+        const uint32_t lp = a.part == kPartBlocks ? list[j >> a.kv.page_shift] : j >> a.kv.page_shift;
+        if (lp != kNone) {
+            my_pos = (lp << a.kv.page_shift) + (j & (a.kv.page_size - 1u));
+            // a list's last page may reach beyond the sequence
+            if (a.part != kPartBlocks || my_pos <= static_cast<uint32_t>(row_pos[0]))
+                my_page = load_page(a.b, a.kv, s, lp, a.st);
+        }
+    }
+    uint8_t* my_ring = ring + warp * F::kStages * F::kStageBytes;
+    const uint32_t ring_addr = smem_addr(my_ring);
+    if (hd < HD) {  // channels beyond the head stay zero
+        for (uint32_t i = lane; i < F::kStages * F::kStageBytes / 16u; i += 32u)
+            reinterpret_cast<uint4*>(my_ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncwarp();
+    }
+    const uint32_t chunks16 = hd >> 3;  // 16-byte chunks of a row
+    const __half* kbase = static_cast<const __half*>(a.kv.k);
+    const __half* vbase = static_cast<const __half*>(a.kv.v);
+    // the keys of a tile that some row may see are copied, the others are zero
+    auto fetch = [&](uint32_t i) {
+        if (i < ntiles) {
+            const uint32_t page = __shfl_sync(0xFFFFFFFFu, my_page, i), pos = __shfl_sync(0xFFFFFFFFu, my_pos, i);
+            const uint32_t dst = ring_addr + (i % F::kStages) * F::kStageBytes;
+            const size_t off = ((static_cast<size_t>(page == kNone ? 0u : page) * a.kv.kv_heads + kh) * a.kv.page_size +
+                                (pos & (a.kv.page_size - 1u))) * hd;
+            const uint32_t lo = a.part == kPartBlocks ? 0u : kb;
+            const uint32_t hi = page == kNone ? 0u : a.part == kPartBlocks ? static_cast<uint32_t>(row_pos[0]) + 1u : ke;
+#pragma unroll
+            for (uint32_t x = lane; x < kKeys * (HD / 8u); x += 32u) {
+                const uint32_t r = x / (HD / 8u), ch = x % (HD / 8u);
+                if (ch >= chunks16) continue;
+                const uint32_t bytes = pos + r >= lo && pos + r < hi ? 16u : 0u;
+                const size_t o = off + static_cast<size_t>(bytes ? r : 0u) * hd + ch * 8u;
+                cp_async16(dst + at<HD>(r, ch), kbase + o, bytes);
+                cp_async16(dst + F::kTileBytes + at<HD>(r, ch), vbase + o, bytes);
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1u < F::kStages; ++i) fetch(i);
+
+    // this thread's query row: g, channels 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
+    const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u;
+    const int p = row_pos[g];
+    uint32_t qf[HD / 16][4];
+    float unscale;
+    {
+        const float* q = a.q + (static_cast<size_t>(row_tok[g]) * a.heads + row_head[g]) * hd;
+        float2 x[HD / 8];
+        float big = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 8; ++i) {
+            x[i] = make_float2(0.f, 0.f);
+            if (p >= 0 && i * 8u < hd) x[i] = *reinterpret_cast<const float2*>(q + i * 8u + t2);
+            x[i].x *= a.scale_log2;
+            x[i].y *= a.scale_log2;
+            big = fmaxf(big, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));
+        }
+        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+        const int e = up_exponent(big);
+        const float up = power_of_two(e);
+        unscale = power_of_two(-e);
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 16; ++i) {
+            split(x[2 * i].x * up, x[2 * i].y * up, &qf[i][0], &qf[i][1]);
+            split(x[2 * i + 1].x * up, x[2 * i + 1].y * up, &qf[i][2], &qf[i][3]);
+        }
+    }
+    const uint32_t p_lo = p >= 0 ? first_key(p, a.window) : kNone, p_hi = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+    float m = -INFINITY, l = 0.f;
+    float acc[HD / 8][4];
+#pragma unroll
+    for (uint32_t n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+
+    const uint32_t mi = lane >> 3, mr = lane & 7u;  // ldmatrix: this lane's matrix and row
+    for (uint32_t i = 0; i < ntiles; ++i) {
+        fetch(i + F::kStages - 1u);
+        cp_wait<F::kStages - 1>();
+        __syncwarp();
+        const uint32_t ks = ring_addr + (i % F::kStages) * F::kStageBytes, vs = ks + F::kTileBytes;
+        float sc[2][4];
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+        for (uint32_t k = 0; k < HD / 16; ++k) {
+            uint32_t b[4];
+            ldsm4(b, ks + at<HD>((mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
+            mma(sc[0], qf[k], b[0], b[1]);
+            mma(sc[1], qf[k], b[2], b[3]);
+        }
+        const uint32_t page = __shfl_sync(0xFFFFFFFFu, my_page, i), pos = __shfl_sync(0xFFFFFFFFu, my_pos, i);
+        float v[4];  // keys pos + 2t, 2t + 1, 2t + 8, 2t + 9
+        v[0] = (sc[0][0] + sc[0][2]) * unscale;
+        v[1] = (sc[0][1] + sc[0][3]) * unscale;
+        v[2] = (sc[1][0] + sc[1][2]) * unscale;
+        v[3] = (sc[1][1] + sc[1][3]) * unscale;
+        const bool whole = page != kNone && pos >= all_b && pos + kKeys <= all_e;
+        if (!whole) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t at_key = pos + t2 + (j & 1u) + (j >> 1) * 8u;
+                if (page == kNone || at_key < p_lo || at_key >= p_hi) v[j] = -INFINITY;
+            }
+        }
+        float mt = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
+        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
+        if (__any_sync(0xFFFFFFFFu, mt > m)) {
+            const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : exp2f(m - mn);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (uint32_t n = 0; n < HD / 8; ++n) {
+                acc[n][0] *= al;
+                acc[n][1] *= al;
+                acc[n][2] *= al;
+                acc[n][3] *= al;
+            }
+        }
+        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) v[j] = exp2_fast(v[j] - ref);
+        l += (v[0] + v[1]) + (v[2] + v[3]);
+        uint32_t pf[4];
+        split(v[0], v[1], &pf[0], &pf[1]);
+        split(v[2], v[3], &pf[2], &pf[3]);
+        // a value that is not finite must not reach the rows that do not see it (0 * inf):
+        // only tiles that some row sees in part can hold one, and those are few
+        bool odd = false;
+        if (!whole) {
+#pragma unroll
+            for (uint32_t n = 0; n < HD / 16; ++n) {
+                uint32_t b[4];
+                ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+                odd |= not_finite(b[0]) || not_finite(b[1]) || not_finite(b[2]) || not_finite(b[3]);
+            }
+            odd = __any_sync(0xFFFFFFFFu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+            for (uint32_t n = 0; n < HD / 16; ++n) {
+                uint32_t b[4];
+                ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+                mma(acc[2 * n], pf, b[0], b[1]);
+                mma(acc[2 * n + 1], pf, b[2], b[3]);
+            }
+        } else {
+            for (uint32_t j = 0; j < kKeys; ++j) {
+                const uint32_t from = (lane & ~3u) | ((j & 7u) >> 1);
+                const float w0 = __shfl_sync(0xFFFFFFFFu, v[0], from), w1 = __shfl_sync(0xFFFFFFFFu, v[1], from);
+                const float w2 = __shfl_sync(0xFFFFFFFFu, v[2], from), w3 = __shfl_sync(0xFFFFFFFFu, v[3], from);
+                const float w = j < 8u ? (j & 1u ? w1 : w0) : (j & 1u ? w3 : w2);
+                if (pos + j < p_lo || pos + j >= p_hi || page == kNone) continue;
+#pragma unroll
+                for (uint32_t n = 0; n < HD / 8; ++n) {
+                    const uint8_t* row = my_ring + (vs - ring_addr) + at<HD>(j, n) + t2 * 2u;
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(row));
+                    acc[n][0] = fmaf(w, f.x, acc[n][0]);
+                    acc[n][1] = fmaf(w, f.y, acc[n][1]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+    cp_wait<0>();
+    asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
+    // the warps' sums, in warp order
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+    if ((lane & 3u) == 0u) {
+        wm[warp][g] = (m == -INFINITY ? 0.f : m) - kUp;
+        wl[warp][g] = p >= 0 ? l : 0.f;  // padding sees nothing
+    }
+    __syncthreads();
+    float* part = reinterpret_cast<float*>(ring);  // [warp][row][HD + 4]
+    constexpr uint32_t kPitch = HD + 4u;
+#pragma unroll
+    for (uint32_t n = 0; n < HD / 8; ++n)
+        *reinterpret_cast<float2*>(part + (warp * kFewRows + g) * kPitch + n * 8u + t2) =
+            make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+    __syncthreads();
+    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+    const uint32_t hd4 = hd / 4u;
+    for (uint32_t i = tid; i < kFewRows * hd4; i += kThreads) {
+        const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
+        if (row_pos[r] == -2) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w)
+            if (wl[w][r] != 0.f) top = fmaxf(top, wm[w][r]);
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t w = 0; w < kWarps; ++w) {
+            if (wl[w][r] == 0.f) continue;  // nothing seen there
+            const float f = exp2f(wm[w][r] - top);
+            const float4 x = *reinterpret_cast<const float4*>(part + (w * kFewRows + r) * kPitch + d);
+            sum = fmaf(wl[w][r], f, sum);
+            o.x = fmaf(x.x, f, o.x);
+            o.y = fmaf(x.y, f, o.y);
+            o.z = fmaf(x.z, f, o.z);
+            o.w = fmaf(x.w, f, o.w);
+        }
+        const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
+        if (a.direct) {
+            const bool none = sum == 0.f;
+            *reinterpret_cast<float4*>(a.out + row * hd + d) =
+                none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
+        } else {
+            *reinterpret_cast<float4*>(a.part_o + ((a.slot0 + c) * rows_all + row) * hd + d) = o;
+            if (d == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(top, sum);
+        }
+    }
+}
+
+template <uint32_t HD>
+cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(Few<HD>::kSmem));
+    if (e != cudaSuccess) return e;
+    attention_few_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Few<HD>::kSmem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_few(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    if (a.kv.head_dim <= 64u) return launch<64>(a, items, stream);
+    if (a.kv.head_dim <= 128u) return launch<128>(a, items, stream);
+    return launch<256>(a, items, stream);
+}
+
+}  // namespace nedo_gpu

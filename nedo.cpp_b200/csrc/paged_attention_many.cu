@@ -1,0 +1,417 @@
+// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 64 query rows
+// (prompts, and the tokens of a whole batch over their shared prefix): bound by the
+// tensor cores.
+//
+// Mathematics.  As in paged_attention_few.cu the fp32 factors are split in two fp16
+// halves; here each half is an operand of its own, the low one first, so that the sums
+// grow in few steps (the tensor core cuts its fp32 sums instead of rounding them; a
+// tile's weighted values are therefore summed from zero in 8 steps and added to the
+// running sums in fp32 with the rescaling by 2^(m_old - m_new)).
+//
+// Work.  A CTA of four warps, 16 rows each, takes the 64 rows through its keys in tiles of
+// 64 (32 for heads above 128); the tiles of keys and values are shared by the warps, brought in by cp.async two
+// tiles deep.  Tiles that none of a warp's rows sees are skipped by it, and only tiles
+// seen in part are masked.  Two CTAs share an SM (one for heads above 128).
+#include "paged_attention.cuh"
+#include "paged_mma.cuh"
+
+namespace nedo_gpu {
+namespace {
+
+constexpr uint32_t kWarps = 4;
+constexpr uint32_t kThreads = 32 * kWarps;
+constexpr uint32_t kStages = 2;
+
+template <uint32_t HD>
+struct Many {
+    static constexpr uint32_t kKeys = HD <= 128 ? 64u : 32u;    // keys per tile
+    static constexpr uint32_t kRowBytes = HD * 2u;
+    static constexpr uint32_t kQBytes = kManyRows * kRowBytes;  // one half of the queries
+    static constexpr uint32_t kTileBytes = kKeys * kRowBytes;   // keys or values of a tile
+    static constexpr uint32_t kStageBytes = 2u * kTileBytes;
+    static constexpr uint32_t kSmem = 2u * kQBytes + kStages * kStageBytes;
+};
+
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
+    return r * Many<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many_kernel(AttnArgs a) {
+    using M = Many<HD>;
+    constexpr uint32_t kKeys = M::kKeys, kGroups = kKeys / 16u, kCols = kKeys / 8u;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t row_tok[kManyRows], row_head[kManyRows];
+    __shared__ int row_pos[kManyRows];
+    __shared__ float row_unscale[kManyRows];
+    __shared__ uint32_t found[2];
+    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t kh = blockIdx.x % a.kv.kv_heads;
+    uint32_t rest = blockIdx.x / a.kv.kv_heads;
+    const uint32_t c = rest % a.chunks;
+    rest /= a.chunks;
+
+    // rows
+    uint32_t s = 0, r0 = 0, nrows, t0 = 0;
+    PagedSeq sq{0u, 0u, 0u};
+    if (a.part == kPartPrefix) {
+        r0 = rest * kManyRows;
+        nrows = min(kManyRows, a.b.tokens * a.group - r0);
+    } else {
+        // the last tiles first: with causal rows they have the most keys
+        if (warp == 0) {
+            uint32_t tile;
+            const uint32_t seq = find_tile(a, a.tiles - 1u - rest, kManyRows, &tile);
+            if (lane == 0u) {
+                found[0] = seq;
+                found[1] = tile;
+            }
+        }
+        __syncthreads();
+        s = found[0];
+        if (s == kNone) return;
+        sq = load_seq(a.b, s, a.st);
+        t0 = sq.t0;
+        r0 = found[1] * kManyRows;
+        nrows = min(kManyRows, sq.n * a.group - r0);
+    }
+    if (tid < kManyRows) {
+        int p = -2;
+        uint32_t tok = 0, head = 0;
+        if (tid < nrows) {
+            tok = t0 + (r0 + tid) / a.group;
+            head = kh * a.group + (r0 + tid) % a.group;
+            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
+        }
+        row_tok[tid] = tok;
+        row_head[tid] = head;
+        row_pos[tid] = p;
+    }
+    __syncthreads();
+    // keys [kb, ke) of the tile and [wb, we) of this warp; [all_b, all_e): seen by all its rows
+    uint32_t kb = kNone, ke = 0, wb = kNone, we = 0, all_b = 0, all_e = kNone;
+    {
+        uint32_t lo[2], hi[2];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const int p = row_pos[lane + 32u * u];
+            lo[u] = p >= 0 ? first_key(p, a.window) : kNone;
+            hi[u] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        }
+        kb = __reduce_min_sync(0xFFFFFFFFu, min(lo[0], lo[1]));
+        ke = __reduce_max_sync(0xFFFFFFFFu, max(hi[0], hi[1]));
+        const int p = row_pos[warp * 16u + (lane & 15u)];
+        const uint32_t l1 = p >= 0 ? first_key(p, a.window) : kNone, h1 = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        wb = __reduce_min_sync(0xFFFFFFFFu, l1);
+        we = __reduce_max_sync(0xFFFFFFFFu, h1);
+        all_b = __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? l1 : 0u);
+        all_e = __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? h1 : kNone);
+    }
+    {
+        uint32_t base = 0, first = 0;
+        if (a.part == kPartOwn) {
+            base = a.shared_len;
+            first = own_first_chunk(sq, a.window, base, a.chunk);
+        } else {
+            ke = min(ke, a.shared_len);
+        }
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
+        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
+        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
+    }
+    const uint32_t j0 = kb & ~(kKeys - 1u), ntiles = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
+
+    const uint32_t q_addr = smem_addr(sm), ring = q_addr + 2u * M::kQBytes;
+    if (hd < HD) {  // channels beyond the head stay zero
+        for (uint32_t i = tid; i < M::kSmem / 16u; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+    }
+    const uint32_t chunks16 = hd >> 3;
+    const __half* kbase = static_cast<const __half*>(a.kv.k);
+    const __half* vbase = static_cast<const __half*>(a.kv.v);
+    // pages of the next tile's groups of 16 keys (a group lies within one page)
+    uint32_t pages[kGroups];
+    auto look_up = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t u = 0; u < kGroups; ++u) {
+            const uint32_t j = j0 + i * kKeys + u * 16u;
+            pages[u] = i < ntiles && j < ke && j + 16u > kb ? load_page(a.b, a.kv, s, j >> a.kv.page_shift, a.st) : kNone;
+        }
+    };
+    __shared__ uint32_t tile_gap[kStages];  // a page of the tile is no page
+    auto fetch = [&](uint32_t i) {
+        if (i < ntiles) {
+            const uint32_t dst = ring + (i % kStages) * M::kStageBytes;
+            constexpr uint32_t kPer = kKeys * (HD / 8u) / kThreads;       // copies of 16 bytes per thread, keys and values each
+            constexpr uint32_t kRowsAtOnce = kThreads / (HD / 8u);
+            const uint32_t ch = tid % (HD / 8u);
+            bool gap = false;
+#pragma unroll
+            for (uint32_t u = 0; u < kGroups; ++u) {
+                const uint32_t j = j0 + i * kKeys + u * 16u;
+                gap |= pages[u] == kNone && j < ke && j + 16u > kb;
+            }
+            if (tid == 0) tile_gap[i % kStages] = gap;
+            if (ch < chunks16) {
+#pragma unroll
+                for (uint32_t x = 0; x < kPer; ++x) {
+                    const uint32_t r = tid / (HD / 8u) + x * kRowsAtOnce;
+                    const uint32_t j = j0 + i * kKeys + r;
+                    const uint32_t page = pages[x * kRowsAtOnce / 16u];  // r stays within the group
+                    const bool there = page != kNone && j >= kb && j < ke;
+                    const size_t o = (((there ? static_cast<size_t>(page) : 0u) * a.kv.kv_heads + kh) * a.kv.page_size +
+                                      (there ? j & (a.kv.page_size - 1u) : 0u)) * hd + ch * 8u;
+                    cp_async16(dst + at<HD>(r, ch), kbase + o, there ? 16u : 0u);
+                    cp_async16(dst + M::kTileBytes + at<HD>(r, ch), vbase + o, there ? 16u : 0u);
+                }
+            }
+        }
+        cp_commit();
+    };
+    look_up(0);
+    fetch(0);
+    look_up(1);
+
+    // queries: scaled, split and stored; a row per two threads
+    {
+        const uint32_t r = tid >> 1;
+        const int p = row_pos[r];
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+        float big = 0.f;
+        if (p >= 0)
+            for (uint32_t d = (tid & 1u) * 8u; d < hd; d += 16u)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(q + d + e);
+                    big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
+                                           fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
+                }
+        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+        const int e2 = up_exponent(big);
+        const float up = power_of_two(e2);
+        if ((tid & 1u) == 0u) row_unscale[r] = power_of_two(-e2);
+        for (uint32_t d = (tid & 1u) * 8u; d < HD; d += 16u) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                float2 x = make_float2(0.f, 0.f);
+                if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
+                split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
+            }
+            *reinterpret_cast<uint4*>(sm + at<HD>(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(sm + M::kQBytes + at<HD>(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+    __syncthreads();
+
+    // this thread's rows g and g + 8 of the warp's 16
+    const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u, mi = lane >> 3, mr = lane & 7u;
+    float unscale[2], m[2], l[2];
+    uint32_t lo_key[2], hi_key[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t r = warp * 16u + g + 8u * h;
+        const int p = row_pos[r];
+        unscale[h] = row_unscale[r];
+        lo_key[h] = p >= 0 ? first_key(p, a.window) : kNone;
+        hi_key[h] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+    }
+    float acc[HD / 8][4];
+#pragma unroll
+    for (uint32_t n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+
+    for (uint32_t i = 0; i < ntiles; ++i) {
+        fetch(i + 1u);
+        look_up(i + 2u);
+        cp_wait<1>();
+        __syncthreads();
+        const uint32_t j = j0 + i * kKeys;
+        if (j < we && j + kKeys > wb) {
+            const uint32_t ks = ring + (i % kStages) * M::kStageBytes, vs = ks + M::kTileBytes;
+            float sc[kCols][4];
+#pragma unroll
+            for (uint32_t n = 0; n < kCols; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (uint32_t half = 0; half < 2; ++half) {  // low halves first
+#pragma unroll
+                for (uint32_t k = 0; k < HD / 16; ++k) {
+                    uint32_t qf[4];
+                    ldsm4(qf, q_addr + (half ? 0u : M::kQBytes) + at<HD>(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1)));
+#pragma unroll
+                    for (uint32_t n = 0; n < kGroups; ++n) {
+                        uint32_t b[4];
+                        ldsm4(b, ks + at<HD>(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
+                        mma(sc[2 * n], qf, b[0], b[1]);
+                        mma(sc[2 * n + 1], qf, b[2], b[3]);
+                    }
+                }
+            }
+            const bool gap = tile_gap[i % kStages] != 0u;
+            const bool whole = !gap && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
+            if (!whole) {
+                uint32_t there = ~0u;  // groups of 16 keys whose page is a page
+                if (gap) {
+                    there = 0u;
+#pragma unroll
+                    for (uint32_t u = 0; u < kGroups; ++u) {
+                        const uint32_t jj = j + u * 16u;
+                        if (jj < ke && jj + 16u > kb && load_page(a.b, a.kv, s, jj >> a.kv.page_shift, a.st) != kNone)
+                            there |= 1u << u;
+                    }
+                }
+#pragma unroll
+                for (uint32_t n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const uint32_t key = j + n * 8u + t2 + (e & 1u), h = e >> 1;
+                        if (key < lo_key[h] || key >= hi_key[h] || key < kb || key >= ke || !(there >> (n >> 1) & 1u))
+                            sc[n][e] = -INFINITY;
+                    }
+            }
+            float alpha[2], ref[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                float mt = sc[0][2 * h];
+#pragma unroll
+                for (uint32_t n = 0; n < kCols; ++n) mt = fmaxf(mt, fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
+                mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
+                mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
+                const float mn = fmaxf(m[h], mt * unscale[h]);
+                alpha[h] = mn == -INFINITY ? 1.f : exp2_fast(m[h] - mn);
+                m[h] = mn;
+                ref[h] = (mn == -INFINITY ? 0.f : mn) - kUp;
+                l[h] *= alpha[h];
+            }
+            uint32_t phi[kGroups][4], plo[kGroups][4];
+#pragma unroll
+            for (uint32_t n = 0; n < kCols; ++n) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    sc[n][e] = exp2_fast(fmaf(sc[n][e], unscale[e >> 1], -ref[e >> 1]));
+                    l[e >> 1] += sc[n][e];
+                }
+                split(sc[n][0], sc[n][1], &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
+                split(sc[n][2], sc[n][3], &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
+            }
+            bool odd = false;
+            if (!whole) {
+                // a value that is not finite must not reach the rows that do not see it (0 * inf)
+                for (uint32_t x = lane; x < kKeys * (HD / 8u); x += 32u) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(sm + (vs - q_addr) + x * 16u);
+                    odd |= not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
+                }
+                odd = __any_sync(0xFFFFFFFFu, odd);
+            }
+            if (!odd) {
+#pragma unroll
+                for (uint32_t n = 0; n < HD / 16; ++n) {
+                    float o[2][4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+                    uint32_t b[kGroups][4];
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k)
+                        ldsm4t(b[k], vs + at<HD>(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k) {
+                        mma(o[0], plo[k], b[k][0], b[k][1]);
+                        mma(o[1], plo[k], b[k][2], b[k][3]);
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k) {
+                        mma(o[0], phi[k], b[k][0], b[k][1]);
+                        mma(o[1], phi[k], b[k][2], b[k][3]);
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        acc[2 * n][e] = fmaf(acc[2 * n][e], alpha[e >> 1], o[0][e]);
+                        acc[2 * n + 1][e] = fmaf(acc[2 * n + 1][e], alpha[e >> 1], o[1][e]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (uint32_t n = 0; n < HD / 8; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) acc[n][e] *= alpha[e >> 1];
+#pragma unroll
+                for (uint32_t n8 = 0; n8 < kCols; ++n8) {
+                    for (uint32_t jj = 0; jj < 8; ++jj) {
+                        const uint32_t from = (lane & ~3u) | (jj >> 1), key = j + n8 * 8u + jj;
+                        float w[2];
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const float w0 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h], from);
+                            const float w1 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h + 1], from);
+                            w[h] = jj & 1u ? w1 : w0;
+                        }
+                        const bool see0 = key >= lo_key[0] && key < hi_key[0], see1 = key >= lo_key[1] && key < hi_key[1];
+#pragma unroll
+                        for (uint32_t n = 0; n < HD / 8; ++n) {
+                            const uint8_t* at_v = sm + (vs - q_addr) + at<HD>(n8 * 8u + jj, n) + t2 * 2u;
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(at_v));
+                            if (see0) {
+                                acc[n][0] = fmaf(w[0], f.x, acc[n][0]);
+                                acc[n][1] = fmaf(w[0], f.y, acc[n][1]);
+                            }
+                            if (see1) {
+                                acc[n][2] = fmaf(w[1], f.x, acc[n][2]);
+                                acc[n][3] = fmaf(w[1], f.y, acc[n][3]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+    cp_wait<0>();
+    asm volatile("griddepcontrol.launch_dependents;");
+    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+        const uint32_t r = warp * 16u + g + 8u * h;
+        const int p = row_pos[r];
+        if (p == -2) continue;
+        if (p < 0) l[h] = 0.f;  // padding sees nothing
+        const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
+        float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
+        const float f = !a.direct ? 1.f : l[h] == 0.f ? 0.f : 1.f / l[h];
+        const bool none = l[h] == 0.f;
+#pragma unroll
+        for (uint32_t n = 0; n < HD / 8; ++n) {
+            if (n * 8u >= hd) continue;
+            *reinterpret_cast<float2*>(o + n * 8u + t2) =
+                none ? make_float2(0.f, 0.f) : make_float2(acc[n][2 * h] * f, acc[n][2 * h + 1] * f);
+        }
+        if (!a.direct && (lane & 3u) == 0u)
+            a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2((m[h] == -INFINITY ? 0.f : m[h]) - kUp, l[h]);
+    }
+}
+
+template <uint32_t HD>
+cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(attention_many_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(Many<HD>::kSmem));
+    if (e != cudaSuccess) return e;
+    attention_many_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Many<HD>::kSmem, stream>>>(a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_many(const AttnArgs& args, uint64_t tiles, cudaStream_t stream) {
+    AttnArgs a = args;
+    a.tiles = static_cast<uint32_t>(tiles);
+    const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
+    if (a.kv.head_dim <= 64u) return launch<64>(a, items, stream);
+    if (a.kv.head_dim <= 128u) return launch<128>(a, items, stream);
+    return launch<256>(a, items, stream);
+}
+
+}  // namespace nedo_gpu

@@ -1,0 +1,64 @@
+// paged_mma.cuh -- fp16 tensor-core pieces of the attention kernels: asynchronous
+// copies, fragment loads, the split of an fp32 factor into two fp16 halves.
+#pragma once
+
+#include "common.cuh"
+
+namespace nedo_gpu {
+
+constexpr float kUp = 14.f;  // exponent by which the softmax weights are taken up before they are split
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+// x, y as two fp16 halves each: {hi, lo}
+__device__ __forceinline__ void split(float x, float y, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    *hi = pack(h);
+    *lo = pack(__floats2half2_rn(x - f.x, y - f.y));
+}
+__device__ __forceinline__ bool not_finite(uint32_t two_halves) {
+    return (two_halves & 0x7C00u) == 0x7C00u || (two_halves & 0x7C000000u) == 0x7C000000u;
+}
+
+// The power of two that takes a row's largest magnitude to [2^13, 2^14), where the low
+// half of its fp16 split is a normal number (0 for zero, infinite and NaN rows).
+__device__ __forceinline__ int up_exponent(float big) {
+    return big > 0.f && big < INFINITY ? min(126, 13 - static_cast<int>(ilogbf(big))) : 0;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
+
+// 2^x; results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace nedo_gpu

@@ -73,7 +73,10 @@ class Setup:
         The tolerance counts fp32 roundings as independent: a dot of hd terms is off
         by about u (sqrt(hd) + 4) S with S = scale sum |q k|, the weights by twice that
         (numerator and normaliser), the weighted sum of n keys by u (sqrt(n) + 16) of
-        sum p |v|; twice the total is allowed."""
+        sum p |v|; twice the total is allowed.  In the weighted sum an F16 value below 2^-14
+        counts as 2^-14: the tensor core takes the exponent of a subnormal operand as -14 when it
+        lines products up, so what it cuts off is u of p 2^-14, not of p |v| (found with values
+        of one or two smallest steps, 2^-24, whose sums were 1e-12 off)."""
         out = np.zeros((self.tokens, self.heads, self.hd))
         tol = np.zeros_like(out)
         inside = np.zeros(self.tokens, bool)
@@ -101,8 +104,9 @@ class Setup:
                 w /= w.sum(1, keepdims=True)
                 out[t, kh * g:(kh + 1) * g] = w @ v
                 big = (np.abs(q) @ np.abs(k).T * abs(self.scale)).max(1, keepdims=True)
-                rel = 2 * U * (math.sqrt(self.hd) + 4) * big + U * (math.sqrt(pos.size) + 16)
-                tol[t, kh * g:(kh + 1) * g] = 2 * rel * (w @ np.abs(v))
+                least = 2.0 ** -14 if self.type == F16 else 0.0
+                tol[t, kh * g:(kh + 1) * g] = (4 * U * (math.sqrt(self.hd) + 4) * big * (w @ np.abs(v)) +
+                                               2 * U * (math.sqrt(pos.size) + 16) * (w @ np.maximum(np.abs(v), least)))
         return out, tol, inside
 
     def select(self, picks):
