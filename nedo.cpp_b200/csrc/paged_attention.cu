@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kMany, kSimt };
+enum class Kernel { kFew, kFew32, kMany, kSimt };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -363,6 +363,10 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
         case Kernel::kMany: {  // 64 rows through the tensor cores, two items to an SM
             const uint32_t slots = 148u * (hd <= 128u ? 2u : 1u);
             return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0};
+        }
+        case Kernel::kFew32: {
+            const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
+            return {kFewRows, slots, 1024u, 8.0 * hd * slots / 6500.0, 4000.0};
         }
         default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0};
     }
@@ -407,13 +411,23 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 }
 
 Kernel prefix_kernel(const PagedAttention& a) {
-    if (a.kv.type != kF16) return Kernel::kSimt;
-    return static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads) <= kFewRows ? Kernel::kFew : Kernel::kMany;
+    const bool few = static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads) <= kFewRows;
+    return a.kv.type == kF16 ? (few ? Kernel::kFew : Kernel::kMany) : few ? Kernel::kFew32 : Kernel::kSimt;
 }
 Kernel own_kernel(const PagedAttention& a) {
-    if (a.kv.type != kF16) return Kernel::kSimt;
-    if (a.picks) return Kernel::kFew;
-    return static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads) <= kFewRows ? Kernel::kFew : Kernel::kMany;
+    const bool few = a.picks != 0u || static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads) <= kFewRows;
+    return a.kv.type == kF16 ? (few ? Kernel::kFew : Kernel::kMany) : few ? Kernel::kFew32 : Kernel::kSimt;
+}
+
+// A part on its kernel: `tiles` row tiles of up to max_rows rows, times KV heads and chunks.
+cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t max_rows, cudaStream_t stream) {
+    const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
+    switch (k) {
+        case Kernel::kFew: return launch_attention_few(a, items, stream);
+        case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
+        case Kernel::kMany: return launch_attention_many(a, tiles, stream);
+        default: return launch_simt(a, items, stream);
+    }
 }
 
 }  // namespace
@@ -445,9 +459,9 @@ bool plan_paged_attention(PagedAttention* a) {
     a->own_chunk = chunk_keys(keys, units, sums, a->kv, c);
     a->own_chunks = chunks(a->own_chunk);
     uint64_t grid = units * a->own_chunks, slots = a->own_chunks;
-    if (own_kernel(*a) == Kernel::kMany && a->b.seqs > 1u) {
+    if ((own_kernel(*a) == Kernel::kMany || own_kernel(*a) == Kernel::kSimt) && a->b.seqs > 1u) {
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads;
-        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(Kernel::kFew, a->kv));
+        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv));
         a->few_chunks = chunks(a->few_chunk);
         grid = std::max(grid, u * a->few_chunks);
         slots = std::max<uint64_t>(slots, a->few_chunks);
@@ -487,10 +501,8 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         a.chunks = p.prefix_chunks;
         a.slot0 = 0;
         const Kernel k = prefix_kernel(p);
-        const uint64_t tiles = ceil_div(static_cast<uint64_t>(p.b.tokens) * a.group, cost_of(k, p.kv).rows);
-        e = k == Kernel::kFew    ? launch_attention_few(a, tiles * p.kv.kv_heads * a.chunks, stream)
-            : k == Kernel::kMany ? launch_attention_many(a, tiles, stream)
-                                 : launch_simt(a, tiles * p.kv.kv_heads * a.chunks, stream);
+        const uint64_t all = static_cast<uint64_t>(p.b.tokens) * a.group;
+        e = launch_part(k, a, ceil_div(all, cost_of(k, p.kv).rows), all, stream);
         if (e != cudaSuccess) return e;
     }
     a.chunk = p.own_chunk;
@@ -502,29 +514,22 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     if (p.picks) {
         a.part = kPartBlocks;
         a.row_blocks = static_cast<uint32_t>(ceil_div(a.group, tile));
-        const uint64_t items = static_cast<uint64_t>(p.b.tokens) * a.row_blocks * p.kv.kv_heads * a.chunks;
-        e = k == Kernel::kFew ? launch_attention_few(a, items, stream) : launch_simt(a, items, stream);
+        e = launch_part(k, a, static_cast<uint64_t>(p.b.tokens) * a.row_blocks, a.group, stream);
     } else {
+        // sequences with few rows among others go to the few-rows kernel: a tile of many rows
+        // would do eight times their work
+        const bool mixed = p.few_chunks != 0u;
+        const uint64_t max_rows = static_cast<uint64_t>(p.b.max_q_len) * a.group;
         a.part = kPartOwn;
-        const uint64_t pairs = static_cast<uint64_t>(p.b.seqs) * p.kv.kv_heads;
-        if (k == Kernel::kSimt) {
-            e = launch_simt(a, own_tiles(p, tile) * p.kv.kv_heads * a.chunks, stream);
-        } else if (k == Kernel::kFew) {
-            e = launch_attention_few(a, pairs * a.chunks, stream);
-        } else {
-            // sequences with few rows among others go to the few-rows kernel: a 64-row tile
-            // would do eight times their work
-            const bool mixed = p.few_chunks != 0u;
-            a.rows_from = mixed ? kFewRows + 1u : 0u;
-            e = launch_attention_many(a, own_tiles(p, tile), stream);
-            if (e == cudaSuccess && mixed) {
-                a.rows_from = 0u;
-                a.rows_to = kFewRows;
-                a.chunk = p.few_chunk;
-                a.chunks = p.few_chunks;
-                a.direct = few_direct;
-                e = launch_attention_few(a, pairs * a.chunks, stream);
-            }
+        a.rows_from = mixed ? kFewRows + 1u : 0u;
+        e = launch_part(k, a, k == Kernel::kFew || k == Kernel::kFew32 ? p.b.seqs : own_tiles(p, tile), max_rows, stream);
+        if (e == cudaSuccess && mixed) {
+            a.rows_from = 0u;
+            a.rows_to = kFewRows;
+            a.chunk = p.few_chunk;
+            a.chunks = p.few_chunks;
+            a.direct = few_direct;
+            e = launch_part(p.kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a, p.b.seqs, kFewRows, stream);
         }
     }
     if (e != cudaSuccess || (own_direct && few_direct)) return e;

@@ -50,76 +50,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(AttnArgs a) 
     __shared__ float wm[kWarps][kFewRows], wl[kWarps][kFewRows];
     __shared__ uint32_t list[kMaxPicks];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    const uint32_t c = blockIdx.x % a.chunks;
-    uint32_t rest = blockIdx.x / a.chunks;
-    const uint32_t kh = rest % a.kv.kv_heads;
-    rest /= a.kv.kv_heads;
-
-    // rows
-    uint32_t s = 0, r0 = 0, nrows, t0 = 0;
-    PagedSeq sq{0u, 0u, 0u};
-    if (a.part == kPartPrefix) {
-        nrows = a.b.tokens * a.group;
-    } else {
-        if (a.part == kPartOwn) {
-            s = rest;
-        } else {
-            t0 = rest / a.row_blocks;
-            r0 = (rest % a.row_blocks) * kFewRows;
-            s = seq_of_token(a.b, t0);
-            if (s == kNone) return;
-        }
-        sq = load_seq(a.b, s, a.st);
-        if (sq.n == 0u) return;
-        if (a.part == kPartOwn) t0 = sq.t0;
-        if (a.part == kPartOwn && sq.n * a.group > a.rows_to) return;  // the many-rows kernel's
-        nrows = a.part == kPartOwn ? sq.n * a.group : min(kFewRows, a.group - r0);
-    }
-    if (tid < kFewRows) {
-        int p = -2;
-        uint32_t tok = 0, head = 0;
-        if (tid < nrows) {
-            tok = t0 + (r0 + tid) / a.group;
-            head = kh * a.group + (r0 + tid) % a.group;
-            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
-        }
-        row_tok[tid] = tok;
-        row_head[tid] = head;
-        row_pos[tid] = p;
-    }
-    __syncthreads();
-    // keys [kb, ke): positions, or places in the page list; [all_b, all_e): seen by every row
-    uint32_t kb = kNone, ke = 0, all_b = 0, all_e = kNone;
-    for (uint32_t r = 0; r < kFewRows; ++r) {
-        if (row_pos[r] < 0) continue;
-        const uint32_t lo = first_key(row_pos[r], a.window), hi = static_cast<uint32_t>(row_pos[r]) + 1u;
-        kb = min(kb, lo);
-        ke = max(ke, hi);
-        all_b = max(all_b, lo);
-        all_e = min(all_e, hi);
-    }
-    if (a.part == kPartBlocks) {
-        const uint32_t e0 = (c * a.chunk) >> a.kv.page_shift;
-        const uint32_t e1 = min(e0 + (a.chunk >> a.kv.page_shift), a.picks);
-        if (warp == 0)
-            checked_list(a.blocks + (static_cast<size_t>(t0) * a.kv.kv_heads + kh) * a.picks, e1, row_pos[0],
-                         a.kv.page_shift, list);
-        __syncthreads();
-        kb = e0 << a.kv.page_shift;
-        ke = e1 << a.kv.page_shift;
-    } else {
-        uint32_t base = 0, first = 0;
-        if (a.part == kPartOwn) {
-            base = a.shared_len;
-            first = own_first_chunk(sq, a.window, base, a.chunk);
-        } else {
-            ke = min(ke, a.shared_len);
-        }
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
-        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
-        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
-        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
-    }
+    FewItem it;
+    if (!few_setup(a, row_tok, row_head, row_pos, list, &it)) return;
+    const uint32_t c = it.c, kh = it.kh, s = it.s, kb = it.kb, ke = it.ke, all_b = it.all_b, all_e = it.all_e;
     // this warp's tiles: tile i starts at key j0 + 16 (4 i + warp); lane i holds its page and
     // the position of its first key
     const uint32_t j0 = kb & ~(kKeys - 1u);
@@ -311,38 +244,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(AttnArgs a) 
         *reinterpret_cast<float2*>(part + (warp * kFewRows + g) * kPitch + n * 8u + t2) =
             make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
     __syncthreads();
-    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-    const uint32_t hd4 = hd / 4u;
-    for (uint32_t i = tid; i < kFewRows * hd4; i += kThreads) {
-        const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
-        if (row_pos[r] == -2) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w)
-            if (wl[w][r] != 0.f) top = fmaxf(top, wm[w][r]);
-        float sum = 0.f;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) {
-            if (wl[w][r] == 0.f) continue;  // nothing seen there
-            const float f = exp2f(wm[w][r] - top);
-            const float4 x = *reinterpret_cast<const float4*>(part + (w * kFewRows + r) * kPitch + d);
-            sum = fmaf(wl[w][r], f, sum);
-            o.x = fmaf(x.x, f, o.x);
-            o.y = fmaf(x.y, f, o.y);
-            o.z = fmaf(x.z, f, o.z);
-            o.w = fmaf(x.w, f, o.w);
-        }
-        const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
-        if (a.direct) {
-            const bool none = sum == 0.f;
-            *reinterpret_cast<float4*>(a.out + row * hd + d) =
-                none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
-        } else {
-            *reinterpret_cast<float4*>(a.part_o + ((a.slot0 + c) * rows_all + row) * hd + d) = o;
-            if (d == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(top, sum);
-        }
-    }
+    few_finish<kWarps>(a, c, row_tok, row_head, row_pos, wm, wl, part, kPitch);
 }
 
 template <uint32_t HD>
