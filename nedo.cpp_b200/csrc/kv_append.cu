@@ -8,113 +8,235 @@
 // The angle is formed in 64 bits, as a fraction of a turn: p * frequency loses
 // nothing that matters at any position (32 bits are 1e-3 of a turn off at position
 // 10^5), and the sine and cosine of the remaining fraction are taken in 32 bits.
+//
+// One launch with two kinds of CTAs.  The first take one page that the call writes and
+// one KV head: keys, and the page's channel bounds, whose minimum and maximum over the new
+// tokens need them in one place (16 bytes of a token per thread, the tokens of the page
+// spread over the thread groups, one round of loads for a page of 64).  The others take
+// one or four token rows: all query heads and the values, with the rows' sines and
+// cosines computed once for all heads.  Bound by the copies, and for single tokens by the
+// launch and three dependent loads.
 #include "paged.cuh"
 
 namespace nedo_gpu {
 namespace {
 
-constexpr uint32_t kAppendThreads = 128;
+constexpr uint32_t kMaxRows = 4;  // token rows of a query CTA
 
+struct AppendArgs {
+    PagedKv kv;
+    PagedBatch b;
+    const float* qkv;
+    float* q_out;
+    double log2_theta;
+    uint32_t heads, rotate;
+    uint32_t segs;      // pages that a sequence's new tokens can touch
+    uint32_t key_ctas;  // CTAs of the first kind
+    uint32_t rows;      // token rows of a CTA of the second kind
+    DeviceStatus* st;
+};
+
+// Turns per position of channel pair i.
+__device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
+    return exp2(-2.0 * i / a.kv.head_dim * a.log2_theta) * 0.15915494309189535;  // 1 / (2 pi)
+}
+// Cosine and sine of position p's rotation.
+__device__ __forceinline__ float2 rotation(int p, double turns) {
+    double turn = static_cast<double>(p) * turns;
+    turn -= rint(turn);
+    float2 c;
+    sincospif(2.f * static_cast<float>(turn), &c.y, &c.x);
+    return c;
+}
+__device__ __forceinline__ void rotate4(float4& x, float4& y, const float2* c) {
+    const float4 u = x, w = y;
+    x = make_float4(u.x * c[0].x - w.x * c[0].y, u.y * c[1].x - w.y * c[1].y, u.z * c[2].x - w.z * c[2].y,
+                    u.w * c[3].x - w.w * c[3].y);
+    y = make_float4(u.x * c[0].y + w.x * c[0].x, u.y * c[1].y + w.y * c[1].x, u.z * c[2].y + w.z * c[2].x,
+                    u.w * c[3].y + w.w * c[3].x);
+}
+// Four values into the cache, and what they are there.
+__device__ __forceinline__ void store4(float* dst, float4& x) { *reinterpret_cast<float4*>(dst) = x; }
+__device__ __forceinline__ void store4(__half* dst, float4& x) {
+    __half2 h[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
+    *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(h);
+    const float2 lo = __half22float2(h[0]), hi = __half22float2(h[1]);
+    x = make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+__device__ __forceinline__ float4 min4(const float4& a, const float4& b) {
+    return make_float4(fminf(a.x, b.x), fminf(a.y, b.y), fminf(a.z, b.z), fminf(a.w, b.w));
+}
+__device__ __forceinline__ float4 max4(const float4& a, const float4& b) {
+    return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
+}
+
+// The keys of one page and KV head, and its bounds (fminf / fmaxf leave NaN out).  A page
+// whose first slot is written begins anew.
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(PagedKv kv, PagedBatch b, uint32_t heads,
-                                                                   const float* __restrict__ qkv, bool rotate, double log2_theta,
-                                                                   float* __restrict__ q_out, DeviceStatus* st) {
-    __shared__ float2 cs[128];
-    const uint32_t t = blockIdx.x;
-    const uint32_t s = seq_of_token(b, t);
-    if (s == kNone) return;
-    const PagedSeq sq = load_seq(b, s, st);
-    if (sq.n == 0u) return;
-    const int p = sq.pos(t - sq.t0);
-    if (p < 0) return;
-    const uint32_t page = load_page(b, kv, s, static_cast<uint32_t>(p) >> kv.page_shift, st);
+__device__ void append_keys(const AppendArgs& a, float4* sums) {
+    const uint32_t h = blockIdx.x % a.kv.kv_heads, i = blockIdx.x / a.kv.kv_heads, s = i / a.segs, seg = i % a.segs;
+    const PagedSeq sq = load_seq(a.b, s, a.st);
+    const uint32_t fresh = min(sq.n, sq.kv);  // rows that are tokens
+    if (fresh == 0u) return;
+    const uint32_t begin = sq.kv - fresh, lp = (begin >> a.kv.page_shift) + seg, first = lp << a.kv.page_shift;
+    if (first >= sq.kv) return;
+    const uint32_t page = load_page(a.b, a.kv, s, lp, a.st);
     if (page == kNone) return;
-    const uint32_t hd = kv.head_dim, half = hd / 2u;
-    for (uint32_t i = threadIdx.x; i < half; i += kAppendThreads) {
-        float2 c = make_float2(1.f, 0.f);
-        if (rotate) {
-            double turn = static_cast<double>(p) * exp2(-2.0 * i / hd * log2_theta) * 0.15915494309189535;
-            turn -= rint(turn);
-            sincospif(2.f * static_cast<float>(turn), &c.y, &c.x);
+    const uint32_t j0 = first < begin ? begin - first : 0u, j1 = min(sq.kv - first, a.kv.page_size);
+    const uint32_t hd = a.kv.head_dim, half = hd / 2u, quads = half / 4u, width = (a.heads + 2u * a.kv.kv_heads) * hd;
+    const uint32_t groups = blockDim.x / quads, g = threadIdx.x / quads, d = (threadIdx.x - g * quads) * 4u;
+    const float* src = a.qkv + static_cast<size_t>(a.heads + h) * hd + d;
+    const size_t head = static_cast<size_t>(page) * a.kv.kv_heads + h;
+    T* dst = static_cast<T*>(a.kv.k) + head * a.kv.page_size * hd + d;
+    float4 lo[2], hi[2];
+    lo[0] = lo[1] = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
+    hi[0] = hi[1] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (g < groups) {
+        double turns[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) turns[e] = a.rotate ? turns_of(a, d + e) : 0.0;
+#pragma unroll 4
+        for (uint32_t j = j0 + g; j < j1; j += groups) {
+            const uint32_t p = first + j;
+            const float* row = src + static_cast<size_t>(sq.t0 + sq.n - (sq.kv - p)) * width;
+            float4 x = *reinterpret_cast<const float4*>(row), y = *reinterpret_cast<const float4*>(row + half);
+            if (a.rotate) {
+                float2 c[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) c[e] = rotation(static_cast<int>(p), turns[e]);
+                rotate4(x, y, c);
+            }
+            store4(dst + static_cast<size_t>(j) * hd, x);
+            store4(dst + static_cast<size_t>(j) * hd + half, y);
+            lo[0] = min4(lo[0], x);
+            lo[1] = min4(lo[1], y);
+            hi[0] = max4(hi[0], x);
+            hi[1] = max4(hi[1], y);
         }
-        cs[i] = c;
+    }
+    if (a.kv.bounds == nullptr) return;
+    // the groups' extremes meet, by halves
+    float4* mine = sums + threadIdx.x * 4u;
+    mine[0] = lo[0];
+    mine[1] = lo[1];
+    mine[2] = hi[0];
+    mine[3] = hi[1];
+    for (uint32_t n = min(groups, j1 - j0); n > 1u; n = (n + 1u) / 2u) {
+        __syncthreads();
+        const uint32_t from = g + (n + 1u) / 2u;
+        if (from < n) {
+            const float4* other = sums + (threadIdx.x + (from - g) * quads) * 4u;
+            mine[0] = lo[0] = min4(lo[0], other[0]);
+            mine[1] = lo[1] = min4(lo[1], other[1]);
+            mine[2] = hi[0] = max4(hi[0], other[2]);
+            mine[3] = hi[1] = max4(hi[1], other[3]);
+        }
+    }
+    if (g != 0u) return;
+    T* bo = static_cast<T*>(a.kv.bounds) + head * 2u * hd + d;
+    if (j0 != 0u) {
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+            const T* o = bo + k * half;
+            lo[k] = min4(lo[k], make_float4(kv_float(o[0]), kv_float(o[1]), kv_float(o[2]), kv_float(o[3])));
+            hi[k] = max4(hi[k], make_float4(kv_float(o[hd]), kv_float(o[hd + 1]), kv_float(o[hd + 2]), kv_float(o[hd + 3])));
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+        store4(bo + k * half, lo[k]);
+        store4(bo + hd + k * half, hi[k]);
+    }
+}
+
+// The query heads and the values of a.rows token rows.
+template <typename T>
+__device__ void append_rows(const AppendArgs& a, float2 (*cs)[128]) {
+    __shared__ int row_pos[kMaxRows];
+    __shared__ uint32_t row_page[kMaxRows];
+    const uint32_t t0 = (blockIdx.x - a.key_ctas) * a.rows, tid = threadIdx.x, nt = blockDim.x;
+    const uint32_t hd = a.kv.head_dim, half = hd / 2u, kvh = a.kv.kv_heads;
+    if (tid < a.rows) {
+        int p = -1;
+        uint32_t page = kNone;
+        if (t0 + tid < a.b.tokens) {
+            const uint32_t s = seq_of_token(a.b, t0 + tid);
+            if (s != kNone) {
+                const PagedSeq sq = load_seq(a.b, s, a.st);
+                if (sq.n != 0u) p = sq.pos(t0 + tid - sq.t0);
+                if (p >= 0) page = load_page(a.b, a.kv, s, static_cast<uint32_t>(p) >> a.kv.page_shift, a.st);
+            }
+        }
+        row_pos[tid] = p;
+        row_page[tid] = page;
     }
     __syncthreads();
-    const float* row = qkv + static_cast<size_t>(t) * (heads + 2u * kv.kv_heads) * hd;
-    const uint32_t slot = static_cast<uint32_t>(p) & (kv.page_size - 1u);
-    for (uint32_t i = threadIdx.x; i < (heads + kv.kv_heads) * half; i += kAppendThreads) {
-        const uint32_t h = i / half, d = i - h * half;
-        const float x = row[h * hd + d], y = row[h * hd + d + half];
-        const float2 c = cs[d];
-        const float x1 = x * c.x - y * c.y, y1 = x * c.y + y * c.x;
-        if (h < heads) {
-            float* o = q_out + (static_cast<size_t>(t) * heads + h) * hd + d;
-            o[0] = x1;
-            o[half] = y1;
-        } else {
-            T* o = static_cast<T*>(kv.k) +
-                   ((static_cast<size_t>(page) * kv.kv_heads + (h - heads)) * kv.page_size + slot) * hd + d;
-            o[0] = to_kv<T>(x1);
-            o[half] = to_kv<T>(y1);
+    if (a.rotate) {
+        // rows innermost: a thread's pairs, and with them the frequencies, stay the same
+        for (uint32_t i = tid; i < half; i += nt) {
+            const double turns = turns_of(a, i);
+            for (uint32_t r = 0; r < a.rows; ++r)
+                if (row_pos[r] >= 0) cs[r][i] = rotation(row_pos[r], turns);
         }
+        __syncthreads();
     }
-    for (uint32_t i = threadIdx.x; i < kv.kv_heads * hd; i += kAppendThreads) {
-        const uint32_t h = i / hd, d = i - h * hd;
-        static_cast<T*>(kv.v)[((static_cast<size_t>(page) * kv.kv_heads + h) * kv.page_size + slot) * hd + d] =
-            to_kv<T>(row[(heads + kv.kv_heads) * hd + i]);
-    }
-}
-
-// Channel-wise minimum and maximum of a page's stored keys, per KV head: one CTA
-// for each page that this call writes and each KV head.  A page whose first slot
-// is written begins anew.  fminf / fmaxf leave NaN keys out.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) kv_bounds_kernel(PagedKv kv, PagedBatch b, uint32_t segs) {
-    const uint32_t h = blockIdx.x % kv.kv_heads, i = blockIdx.x / kv.kv_heads, s = i / segs, seg = i % segs;
-    const PagedSeq sq = load_seq(b, s, nullptr);
-    const uint32_t fresh = sq.n < sq.kv ? sq.n : sq.kv;  // rows that are tokens
-    if (fresh == 0u) return;
-    const uint32_t begin = sq.kv - fresh, lp = (begin >> kv.page_shift) + seg;
-    const uint32_t first = lp << kv.page_shift;
-    if (first >= sq.kv) return;
-    const uint32_t page = load_page(b, kv, s, lp, nullptr);
-    if (page == kNone) return;
-    const uint32_t j0 = first < begin ? begin - first : 0u;
-    const uint32_t j1 = sq.kv - first < kv.page_size ? sq.kv - first : kv.page_size;
-    const uint32_t hd = kv.head_dim;
-    const T* k = static_cast<const T*>(kv.k) + (static_cast<size_t>(page) * kv.kv_heads + h) * kv.page_size * hd;
-    T* bo = static_cast<T*>(kv.bounds) + (static_cast<size_t>(page) * kv.kv_heads + h) * 2u * hd;
-    for (uint32_t d = threadIdx.x; d < hd; d += kAppendThreads) {
-        float lo = j0 == 0u ? INFINITY : kv_float(bo[d]), hi = j0 == 0u ? -INFINITY : kv_float(bo[hd + d]);
-        for (uint32_t j = j0; j < j1; ++j) {
-            const float v = kv_float(k[static_cast<size_t>(j) * hd + d]);
-            lo = fminf(lo, v);
-            hi = fmaxf(hi, v);
+    const uint32_t quads = half / 4u, qn = a.heads * quads, vn = kvh * hd / 4u;
+    const size_t width = static_cast<size_t>(a.heads + 2u * kvh) * hd;
+    for (uint32_t i = tid; i < a.rows * (qn + vn); i += nt) {
+        const uint32_t r = i / (qn + vn), k = i - r * (qn + vn);
+        const int p = row_pos[r];
+        if (p < 0) continue;
+        const float* row = a.qkv + (t0 + r) * width;
+        if (k < qn) {
+            const uint32_t h = k / quads, d = (k - h * quads) * 4u;
+            float4 x = *reinterpret_cast<const float4*>(row + h * hd + d);
+            float4 y = *reinterpret_cast<const float4*>(row + h * hd + d + half);
+            if (a.rotate) rotate4(x, y, &cs[r][d]);
+            float* o = a.q_out + (static_cast<size_t>(t0 + r) * a.heads + h) * hd + d;
+            *reinterpret_cast<float4*>(o) = x;
+            *reinterpret_cast<float4*>(o + half) = y;
+        } else if (row_page[r] != kNone) {
+            const uint32_t e = (k - qn) * 4u, h = e / hd, d = e - h * hd;
+            float4 x = *reinterpret_cast<const float4*>(row + (a.heads + kvh) * hd + e);
+            store4(static_cast<T*>(a.kv.v) +
+                       ((static_cast<size_t>(row_page[r]) * kvh + h) * a.kv.page_size +
+                        (static_cast<uint32_t>(p) & (a.kv.page_size - 1u))) * hd + d,
+                   x);
         }
-        bo[d] = to_kv<T>(lo);
-        bo[hd + d] = to_kv<T>(hi);
     }
 }
 
 template <typename T>
-cudaError_t append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, bool rotate,
-                   double log2_theta, float* q_out, DeviceStatus* st, cudaStream_t stream) {
-    kv_append_kernel<T><<<b.tokens, kAppendThreads, 0, stream>>>(kv, b, heads, qkv, rotate, log2_theta, q_out, st);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess || kv.bounds == nullptr) return e;
-    const uint32_t segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
-    kv_bounds_kernel<T><<<b.seqs * segs * kv.kv_heads, kAppendThreads, 0, stream>>>(kv, b, segs);
-    return cudaGetLastError();
+__global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
+    __shared__ __align__(16) uint8_t sm[256 * 4 * sizeof(float4)];
+    if (blockIdx.x < a.key_ctas) append_keys<T>(a, reinterpret_cast<float4*>(sm));
+    else append_rows<T>(a, reinterpret_cast<float2(*)[128]>(sm));
 }
 
 }  // namespace
 
 cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
                              float* q_out, DeviceStatus* st, cudaStream_t stream) {
-    const bool rotate = theta > 0.0;
-    const double l = rotate ? log2(theta) : 0.0;
-    return kv.type == kF16 ? append<__half>(kv, b, heads, qkv, rotate, l, q_out, st, stream)
-                           : append<float>(kv, b, heads, qkv, rotate, l, q_out, st, stream);
+    AppendArgs a = {};
+    a.kv = kv;
+    a.b = b;
+    a.qkv = qkv;
+    a.q_out = q_out;
+    a.rotate = theta > 0.0;
+    a.log2_theta = a.rotate ? log2(theta) : 0.0;
+    a.heads = heads;
+    a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
+    a.rows = b.tokens >= 8u * 148u ? kMaxRows : 1u;
+    a.st = st;
+    const uint64_t keys = static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
+    const uint64_t grid = keys + (b.tokens + a.rows - 1u) / a.rows;
+    if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    a.key_ctas = static_cast<uint32_t>(keys);
+    // a page's tokens want more thread groups than one token per sequence does
+    const uint32_t threads = b.max_q_len > 4u ? 256u : 128u;
+    if (kv.type == kF16) kv_append_kernel<__half><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
+    else kv_append_kernel<float><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace nedo_gpu
