@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kFew32, kMany, kSimt };
+enum class Kernel { kFew, kFew32, kMany, kTc, kSimt };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -364,6 +364,8 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t slots = 148u * (hd <= 128u ? 2u : 1u);
             return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0};
         }
+        case Kernel::kTc:  // 128 rows through 32 MMAs per 128 keys, an item to an SM
+            return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 5000.0};
         case Kernel::kFew32: {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {kFewRows, slots, 1024u, 8.0 * hd * slots / 6500.0, 4000.0};
@@ -410,14 +412,20 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
     return std::min<uint64_t>(a.b.tokens * group / rows + a.b.seqs, a.b.seqs * ceil_div(a.b.max_q_len * group, rows));
 }
 
+// The kernel of a part whose row tiles have up to `rows` rows.
+Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
+    if (kv.type != kF16) return rows <= kFewRows ? Kernel::kFew32 : Kernel::kSimt;
+    if (rows <= kFewRows) return Kernel::kFew;
+    const bool tc = kv.head_dim <= 128u && static_cast<uint64_t>(kv.num_pages) * kv.kv_heads < (1ull << 31);
+    return tc ? Kernel::kTc : Kernel::kMany;
+}
 Kernel prefix_kernel(const PagedAttention& a) {
-    const bool few = static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads) <= kFewRows;
-    return a.kv.type == kF16 ? (few ? Kernel::kFew : Kernel::kMany) : few ? Kernel::kFew32 : Kernel::kSimt;
+    return kernel_for(a.kv, static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads));
 }
 Kernel own_kernel(const PagedAttention& a) {
-    const bool few = a.picks != 0u || static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads) <= kFewRows;
-    return a.kv.type == kF16 ? (few ? Kernel::kFew : Kernel::kMany) : few ? Kernel::kFew32 : Kernel::kSimt;
+    return kernel_for(a.kv, a.picks ? 1u : static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads));
 }
+bool takes_few(Kernel k) { return k == Kernel::kFew || k == Kernel::kFew32; }
 
 // A part on its kernel: `tiles` row tiles of up to max_rows rows, times KV heads and chunks.
 cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t max_rows, cudaStream_t stream) {
@@ -426,6 +434,7 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
         case Kernel::kFew: return launch_attention_few(a, items, stream);
         case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
         case Kernel::kMany: return launch_attention_many(a, tiles, stream);
+        case Kernel::kTc: return launch_attention_tc(a, tiles, stream);
         default: return launch_simt(a, items, stream);
     }
 }
@@ -459,7 +468,7 @@ bool plan_paged_attention(PagedAttention* a) {
     a->own_chunk = chunk_keys(keys, units, sums, a->kv, c);
     a->own_chunks = chunks(a->own_chunk);
     uint64_t grid = units * a->own_chunks, slots = a->own_chunks;
-    if ((own_kernel(*a) == Kernel::kMany || own_kernel(*a) == Kernel::kSimt) && a->b.seqs > 1u) {
+    if (!takes_few(own_kernel(*a)) && a->b.seqs > 1u) {
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads;
         a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv));
         a->few_chunks = chunks(a->few_chunk);
@@ -522,7 +531,7 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         const uint64_t max_rows = static_cast<uint64_t>(p.b.max_q_len) * a.group;
         a.part = kPartOwn;
         a.rows_from = mixed ? kFewRows + 1u : 0u;
-        e = launch_part(k, a, k == Kernel::kFew || k == Kernel::kFew32 ? p.b.seqs : own_tiles(p, tile), max_rows, stream);
+        e = launch_part(k, a, takes_few(k) ? p.b.seqs : own_tiles(p, tile), max_rows, stream);
         if (e == cudaSuccess && mixed) {
             a.rows_from = 0u;
             a.rows_to = kFewRows;

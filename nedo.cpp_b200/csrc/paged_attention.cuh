@@ -232,5 +232,9 @@ cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_
 // tiles of kManyRows.
 constexpr uint32_t kManyRows = 64;
 cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
+// Tiles of kTcRows rows on the 5th-generation tensor cores (paged_attention_tc.cu): F16
+// caches, heads of up to 128 channels, num_pages * kv_heads below 2^31.
+constexpr uint32_t kTcRows = 128;
+cudaError_t launch_attention_tc(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
 
 }  // namespace nedo_gpu

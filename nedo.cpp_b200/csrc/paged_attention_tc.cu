@@ -1,0 +1,597 @@
+// paged_attention_tc.cu -- attention over a paged F16 cache for tiles of 128 query rows on
+// the 5th-generation tensor cores (prompts, the tokens of a whole batch over their shared
+// prefix, groups of more than eight rows), heads of up to 128 channels.
+//
+// Mathematics.  As in the other tensor-core kernels the fp32 factors are split in two fp16
+// halves, low halves first: S = q_lo K^T + q_hi K^T, O = p_lo V + p_hi V, so every 128 x 128
+// tile is 32 MMAs of 128 x 128 x 16.  The tensor core cuts its fp32 sums instead of rounding
+// them, so a tile's O starts from zero in TMEM and is added to the running sums in fp32
+// registers, together with the rescaling by 2^(m_old - m_new).
+//
+// Work.  A CTA (one per SM, 384 threads) takes 128 rows through their keys in tiles of 128:
+//   * warp 8 brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
+//     swizzle), in the order of their use, four half-tile slots deep.  Of a tile that the
+//     item's key range cuts it zeroes the values outside, whatever the pages hold there;
+//   * one thread of warp 9 issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so the
+//     tensor core works while a softmax runs;
+//   * warps 0-3 take the even and warps 4-7 the odd tiles, a row per thread: they read S from
+//     TMEM, write the split weights over it (the A operand of P V), and add O to their own
+//     running sums.  The two halves' sums meet at the end in shared memory.
+// TMEM: two S/P and two O tiles of 128 columns each.  Registers: the softmax warps hold 128
+// sums each, so they take 208 registers and the other warps give theirs up.
+#include "paged_attention.cuh"
+#include "paged_mma.cuh"
+
+namespace nedo_gpu {
+namespace {
+
+constexpr uint32_t kRows = kTcRows;     // 128
+constexpr uint32_t kKeys = 128;         // keys per tile
+constexpr uint32_t kSlots = 4;          // ring slots: the keys or the values of one tile
+constexpr uint32_t kThreads = 384;
+constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
+constexpr uint32_t kLoadWarp = 8, kMmaWarp = 9;
+
+template <uint32_t HD>
+struct Tc {
+    static constexpr uint32_t kBlocks = HD / 64u;
+    static constexpr uint32_t kTile = kBlocks * kBlock;   // one half of the queries, or a ring slot
+    static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u;
+};
+
+struct TcMaps {
+    CUtensorMap k, v;  // [num_pages * kv_heads][page_size][head_dim], boxes of 64 channels x box_rows slots
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2,
+                                            uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_addr(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+// D (TMEM) = A (shared memory) * B (shared memory) [+ D]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// D (TMEM) = A (TMEM) * B (shared memory) [+ D]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes: a row per thread.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float tmem_load1(uint32_t addr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    return __uint_as_float(v);
+}
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
+        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
+        : "memory");
+}
+
+// Shared-memory matrix descriptors, 128-byte swizzle, 8-row atoms of 1024 bytes.
+// K-major (queries, keys: rows of 64 channels): the next 8 rows 1024 bytes on.
+// MN-major (values: N = channels contiguous, K = keys): 8 keys 1024 bytes on, the next 64
+// channels one block on.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+    uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(lbo >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;  // descriptor version of sm_100
+    d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
+    return d;
+}
+// kind::f16: fp16 operands, fp32 sums, M = 128, N = n; B K-major or MN-major.
+__host__ __device__ constexpr uint32_t idesc(uint32_t n, bool b_mn) {
+    return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Byte offset of 16-byte chunk c (of all the row's channels) of row r.
+__device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
+    return (c >> 3) * kBlock + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_rows) {
+    using T = Tc<HD>;
+    extern __shared__ uint8_t sm_raw[];
+    __shared__ uint32_t row_tok[kRows], row_head[kRows];
+    __shared__ int row_pos[kRows];
+    __shared__ float row_unscale[kRows], half_m[kRows], half_l[kRows];
+    __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[2], p_full[2], o_full[2], done;
+    __shared__ uint32_t found[2], tmem_slot, gaps[4];
+    const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
+    uint8_t* const sm = sm_raw + (s0 - smem_addr(sm_raw));
+    const uint32_t q_addr = s0, ring = s0 + 2u * T::kTile;
+    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t kh = blockIdx.x % a.kv.kv_heads;
+    uint32_t rest = blockIdx.x / a.kv.kv_heads;
+    const uint32_t c = rest % a.chunks;
+    rest /= a.chunks;
+
+    // ---- the item: rows and keys
+    uint32_t s = 0, r0 = 0, nrows, t0 = 0;
+    PagedSeq sq{0u, 0u, 0u};
+    if (a.part == kPartPrefix) {
+        r0 = rest * kRows;
+        nrows = min(kRows, a.b.tokens * a.group - r0);
+    } else {
+        // the last tiles first: with causal rows they have the most keys
+        if (warp == 0) {
+            uint32_t tile;
+            const uint32_t seq = find_tile(a, a.tiles - 1u - rest, kRows, &tile);
+            if (lane == 0u) {
+                found[0] = seq;
+                found[1] = tile;
+            }
+        }
+        __syncthreads();
+        s = found[0];
+        if (s == kNone) return;
+        sq = load_seq(a.b, s, a.st);
+        t0 = sq.t0;
+        r0 = found[1] * kRows;
+        nrows = min(kRows, sq.n * a.group - r0);
+    }
+    if (tid < kRows) {
+        int p = -2;
+        uint32_t tok = 0, head = 0;
+        if (tid < nrows) {
+            tok = t0 + (r0 + tid) / a.group;
+            head = kh * a.group + (r0 + tid) % a.group;
+            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
+        }
+        row_tok[tid] = tok;
+        row_head[tid] = head;
+        row_pos[tid] = p;
+    }
+    __syncthreads();
+    uint32_t kb = kNone, ke = 0;
+    {
+        uint32_t lo = kNone, hi = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < kRows / 32u; ++u) {
+            const int p = row_pos[lane + 32u * u];
+            if (p >= 0) {
+                lo = min(lo, first_key(p, a.window));
+                hi = max(hi, static_cast<uint32_t>(p) + 1u);
+            }
+        }
+        kb = __reduce_min_sync(0xFFFFFFFFu, lo);
+        ke = __reduce_max_sync(0xFFFFFFFFu, hi);
+        uint32_t base = 0, first = 0;
+        if (a.part == kPartOwn) {
+            base = a.shared_len;
+            first = own_first_chunk(sq, a.window, base, a.chunk);
+        } else {
+            ke = min(ke, a.shared_len);
+        }
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
+        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
+        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
+    }
+    const uint32_t j0 = kb & ~(kKeys - 1u), ntiles = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
+
+    // ---- barriers, TMEM, queries
+    if (tid == 0u) {
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&cut, 1);
+        for (uint32_t i = 0; i < 2u; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(&done, 1);
+        fence_barrier_init();
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
+                     "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid < 256u) {  // a row per two threads: scaled, split, stored
+        const uint32_t r = tid >> 1;
+        const int p = row_pos[r];
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+        float big = 0.f;
+        if (p >= 0)
+            for (uint32_t d = (tid & 1u) * 8u; d < hd; d += 16u)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; e += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(q + d + e);
+                    big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
+                                           fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
+                }
+        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+        const int e2 = up_exponent(big);
+        const float up = power_of_two(e2);
+        if ((tid & 1u) == 0u) row_unscale[r] = power_of_two(-e2);
+        for (uint32_t d = (tid & 1u) * 8u; d < HD; d += 16u) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                float2 x = make_float2(0.f, 0.f);
+                if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
+                split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
+            }
+            *reinterpret_cast<uint4*>(sm + at(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(sm + T::kTile + at(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    // Ring order: K0, K1, V0, K2, V1, ..., V(last): the order in which the MMAs use them.
+    auto k_at = [&](uint32_t i) { return i == 0u ? 0u : 2u * i - 1u; };
+    auto v_at = [&](uint32_t i) { return i + 1u < ntiles ? 2u * i + 2u : 2u * ntiles - 1u; };
+
+    if (warp >= kLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == kLoadWarp) {
+            // ---- loads
+            const uint32_t boxes = kKeys / box_rows, box_bytes = box_rows * 128u;
+            // lane b: page of box b of a tile (kNone: no keys of the item there, or no page)
+            auto look_up = [&](uint32_t i) {
+                const uint32_t j = j0 + i * kKeys + lane * box_rows;
+                return lane < boxes && i < ntiles && j < ke && j + box_rows > kb
+                           ? load_page(a.b, a.kv, s, j >> a.kv.page_shift, a.st)
+                           : kNone;
+            };
+            bool ok = true;
+            uint32_t issued = 0, cuts = 0;
+            auto load = [&](uint32_t n, uint32_t i, uint32_t pages, bool values) {
+                const uint32_t slot = n % kSlots, dst = ring + slot * T::kTile;
+                if (ok && n >= kSlots) ok = mbar_wait_bounded(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u);
+                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (!ok) return;
+                const uint32_t j = j0 + i * kKeys, there = __ballot_sync(0xFFFFFFFFu, pages != kNone);
+                const uint32_t want = __ballot_sync(
+                    0xFFFFFFFFu, lane < boxes && j + lane * box_rows < ke && j + (lane + 1u) * box_rows > kb);
+                const bool whole = there == (1u << boxes) - 1u && j >= kb && j + kKeys <= ke;
+                const bool patch = values && !whole;
+                uint64_t* bar = patch ? &cut : &full[slot];
+                if (lane == 0u) {
+                    if (!values) gaps[i & 3u] = want & ~there;
+                    const uint32_t bytes = __popc(there) * T::kBlocks * box_bytes;
+                    if (bytes != 0u) mbar_arrive_expect_tx(bar, bytes);
+                    else mbar_arrive(bar);
+                }
+                __syncwarp();
+                if (pages != kNone) {
+                    const int32_t slot_row = static_cast<int32_t>((j + lane * box_rows) & (a.kv.page_size - 1u));
+                    const int32_t head = static_cast<int32_t>(pages * a.kv.kv_heads + kh);
+#pragma unroll
+                    for (uint32_t b = 0; b < T::kBlocks; ++b)
+                        tma_load_3d(dst + b * kBlock + lane * box_bytes, values ? &maps.v : &maps.k,
+                                    static_cast<int32_t>(64u * b), slot_row, head, bar);
+                }
+                if (patch) {
+                    // values outside the item's keys count as zero
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&cut, cuts & 1u, a.st, 62u));
+                    ++cuts;
+                    if (!ok) return;
+                    for (uint32_t x = lane; x < kKeys * 8u * T::kBlocks; x += 32u) {
+                        const uint32_t r = x / (8u * T::kBlocks), ch = x % (8u * T::kBlocks);
+                        if (j + r < kb || j + r >= ke || !(there >> (r / box_rows) & 1u))
+                            *reinterpret_cast<uint4*>(sm + (dst - s0) + at(r, ch)) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0u) mbar_arrive(&full[slot]);
+                }
+                issued = n + 1u;
+            };
+            uint32_t before = kNone, now = look_up(0), next = look_up(1);
+            for (uint32_t i = 0; i < ntiles && ok; ++i) {
+                const uint32_t after = look_up(i + 2u);
+                load(k_at(i), i, now, false);
+                if (i > 0u && ok) load(v_at(i - 1u), i - 1u, before, true);
+                before = now;
+                now = next;
+                next = after;
+            }
+            if (ntiles != 0u && ok) load(v_at(ntiles - 1u), ntiles - 1u, before, true);
+            // the last copies into every slot have landed before the CTA ends
+            for (uint32_t n = issued > kSlots ? issued - kSlots : 0u; n < issued; ++n)
+                mbar_wait_bounded(&full[n % kSlots], (n / kSlots) & 1u, a.st, 63u);
+        } else if (warp == kMmaWarp) {
+            if (lane == 0u) {
+                // ---- MMAs
+                bool ok = true;
+                constexpr uint32_t kS = idesc(kKeys, false), kO = idesc(HD, true);
+                auto qk = [&](uint32_t i) {
+                    const uint32_t n = k_at(i), slot = n % kSlots;
+                    ok = mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 64u);
+                    if (!ok) return;
+                    tc_fence_after();
+                    const uint32_t d = tmem + (i & 1u) * 128u;
+#pragma unroll
+                    for (uint32_t half = 0; half < 2u; ++half)  // low halves first
+#pragma unroll
+                        for (uint32_t k = 0; k < HD / 16u; ++k) {
+                            const uint32_t off = (k >> 2) * kBlock + (k & 3u) * 32u;
+                            mma_ss(d, desc(q_addr + (half ? 0u : T::kTile) + off, 16u), desc(ring + slot * T::kTile + off, 16u),
+                                   kS, half + k != 0u);
+                        }
+                    tc_commit(&s_full[i & 1u]);
+                    tc_commit(&empty[slot]);
+                };
+                if (ntiles != 0u) qk(0);
+                for (uint32_t i = 0; i < ntiles && ok; ++i) {
+                    if (i + 1u < ntiles) qk(i + 1u);
+                    const uint32_t n = v_at(i), slot = n % kSlots;
+                    ok = ok && mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 65u);
+                    ok = ok && mbar_wait_bounded(&p_full[i & 1u], (i >> 1) & 1u, a.st, 66u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t d = tmem + 256u + (i & 1u) * 128u, p = tmem + (i & 1u) * 128u;
+#pragma unroll
+                    for (uint32_t half = 0; half < 2u; ++half)
+#pragma unroll
+                        for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 columns of weights, 2048 bytes of values
+                            mma_ts(d, p + (k >> 1) * 32u + (half ? 0u : 16u) + (k & 1u) * 8u,
+                                   desc(ring + slot * T::kTile + k * 2048u, kBlock), kO, half + k != 0u);
+                    tc_commit(&o_full[i & 1u]);
+                    tc_commit(&empty[slot]);
+                }
+                tc_commit(&done);  // every MMA issued above has completed when this arrives
+                mbar_wait_bounded(&done, 0u, a.st, 67u);
+            }
+            __syncwarp();
+        }
+    } else {
+        // ---- softmax: a row per thread, tiles half, half + 2, ...
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const uint32_t half = warp >> 2, r = tid & 127u;
+        const uint32_t lanes = tmem + ((warp & 3u) << 21);  // the warp's 32 TMEM lanes
+        const uint32_t st_addr = lanes + half * 128u, o_addr = lanes + 256u + half * 128u;
+        const int p = row_pos[r];
+        const float unscale = row_unscale[r];
+        const uint32_t lo_key = p >= 0 ? first_key(p, a.window) : kNone, hi_key = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        // keys that some / every row of the warp sees
+        const uint32_t wb = __reduce_min_sync(0xFFFFFFFFu, lo_key), we = __reduce_max_sync(0xFFFFFFFFu, hi_key);
+        const uint32_t all_b = __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? lo_key : 0u);
+        const uint32_t all_e = __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? hi_key : kNone);
+        float acc[HD];
+#pragma unroll
+        for (uint32_t d = 0; d < HD; ++d) acc[d] = 0.f;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (uint32_t i = half; i < ntiles && ok; i += 2u) {
+            const uint32_t ph = (i >> 1) & 1u, j = j0 + i * kKeys;
+            ok = mbar_wait_bounded(&s_full[half], ph, a.st, 68u);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const bool mine = j < we && j + kKeys > wb;  // a tile that none of the warp's rows sees is passed over
+            float alpha = 1.f;
+            bool odd = false;
+            if (mine) {
+                const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 3u]);
+                const bool whole = gap == 0u && j >= max(all_b, kb) && j + kKeys <= min(all_e, ke);
+                // first and last key of the tile that this row sees
+                const uint32_t from = max(max(lo_key, kb), j), to = min(min(hi_key, ke), j + kKeys);
+                auto unseen = [&](uint32_t x) {  // x: key in the tile
+                    return j + x < from || j + x >= to || (gap >> (x / box_rows) & 1u);
+                };
+                uint32_t x[32];
+                float mt = -INFINITY;
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q) {
+                    tmem_load(st_addr + 32u * q, x);
+                    if (!whole) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 32u; ++e)
+                            if (unseen(32u * q + e)) x[e] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; ++e) mt = fmaxf(mt, __uint_as_float(x[e]));
+                }
+                const float mn = fmaxf(m, mt * unscale);
+                alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+                m = mn;
+                const float ref = (mn == -INFINITY ? 0.f : mn) - kUp;
+                if (!whole) {
+                    // a value that is not finite must not reach the rows that do not see it (0 * inf)
+                    const uint32_t n = v_at(i);
+                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&full[n % kSlots], (n / kSlots) & 1u, a.st, 69u));
+                    if (!ok) break;
+                    const uint8_t* v = sm + (ring - s0) + (n % kSlots) * T::kTile;
+                    for (uint32_t y = lane; y < T::kTile / 16u; y += 32u) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(v + y * 16u);
+                        odd |= not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w);
+                    }
+                    odd = __any_sync(0xFFFFFFFFu, odd);
+                    if (odd) {  // key by key, for the rows that see it; the tensor core's sums are left out
+#pragma unroll
+                        for (uint32_t d = 0; d < HD; ++d) acc[d] *= alpha;
+                        for (uint32_t k = 0; k < kKeys; ++k) {
+                            const float w = exp2_fast(fmaf(tmem_load1(st_addr + k), unscale, -ref));
+                            if (!unseen(k)) {
+#pragma unroll
+                                for (uint32_t ch = 0; ch < HD / 8u; ++ch) {
+                                    const uint4 y = *reinterpret_cast<const uint4*>(v + at(k, ch));
+                                    const uint32_t h[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                                    for (uint32_t e = 0; e < 4u; ++e) {
+                                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
+                                        acc[8u * ch + 2u * e] = fmaf(w, f.x, acc[8u * ch + 2u * e]);
+                                        acc[8u * ch + 2u * e + 1u] = fmaf(w, f.y, acc[8u * ch + 2u * e + 1u]);
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+                float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t q = 0; q < 4u; ++q) {
+                    tmem_load(st_addr + 32u * q, x);
+                    if (!whole) {
+#pragma unroll
+                        for (uint32_t e = 0; e < 32u; ++e)
+                            if (unseen(32u * q + e)) x[e] = 0xFF800000u;
+                    }
+                    uint32_t w[32];  // 16 columns of high halves, 16 of low halves
+#pragma unroll
+                    for (uint32_t e = 0; e < 16u; ++e) {
+                        const float a0 = exp2_fast(fmaf(__uint_as_float(x[2 * e]), unscale, -ref));
+                        const float a1 = exp2_fast(fmaf(__uint_as_float(x[2 * e + 1]), unscale, -ref));
+                        part[(2 * e) & 3u] += a0;
+                        part[(2 * e + 1) & 3u] += a1;
+                        split(a0, a1, &w[e], &w[16 + e]);
+                    }
+                    tmem_store(st_addr + 32u * q, w);
+                }
+                l = fmaf(l, alpha, (part[0] + part[1]) + (part[2] + part[3]));
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            }
+            tc_fence_before();
+            mbar_arrive(&p_full[half]);
+            ok = mbar_wait_bounded(&o_full[half], ph, a.st, 70u);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (mine && !odd) {
+#pragma unroll
+                for (uint32_t q = 0; q < HD / 32u; ++q) {
+                    uint32_t x[32];
+                    tmem_load(o_addr + 32u * q, x);
+#pragma unroll
+                    for (uint32_t e = 0; e < 32u; ++e) acc[32u * q + e] = fmaf(acc[32u * q + e], alpha, __uint_as_float(x[e]));
+                }
+            }
+        }
+        // the halves meet: the odd tiles' sums through shared memory (the ring is done with)
+        asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
+        named_barrier_sync(1, 256);
+        constexpr uint32_t kPitch = HD + 4u;
+        float* sums = reinterpret_cast<float*>(sm + (ring - s0));
+        const float mine_m = m == -INFINITY ? 0.f : m;
+        if (half == 1u) {
+            half_m[r] = mine_m;
+            half_l[r] = p >= 0 ? l : 0.f;
+#pragma unroll
+            for (uint32_t d = 0; d < HD; d += 4u)
+                *reinterpret_cast<float4*>(sums + r * kPitch + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+        }
+        named_barrier_sync(1, 256);
+        if (half == 0u) {
+            const float l0 = p >= 0 ? l : 0.f, l1 = half_l[r], m1 = half_m[r];  // padding sees nothing
+            const float top = l0 == 0.f ? m1 : l1 == 0.f ? mine_m : fmaxf(mine_m, m1);
+            const float f0 = l0 == 0.f ? 0.f : exp2_fast(mine_m - top), f1 = l1 == 0.f ? 0.f : exp2_fast(m1 - top);
+            const float sum = l0 * f0 + l1 * f1;
+            const float scale = a.direct && sum != 0.f ? 1.f / sum : 1.f;
+#pragma unroll
+            for (uint32_t d = 0; d < HD; d += 4u) {
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (l1 != 0.f) x = *reinterpret_cast<const float4*>(sums + r * kPitch + d);
+                if (l1 != 0.f) x = make_float4(x.x * f1, x.y * f1, x.z * f1, x.w * f1);
+                if (l0 != 0.f)
+                    x = make_float4(fmaf(acc[d], f0, x.x), fmaf(acc[d + 1], f0, x.y), fmaf(acc[d + 2], f0, x.z),
+                                    fmaf(acc[d + 3], f0, x.w));
+                *reinterpret_cast<float4*>(sums + r * kPitch + d) =
+                    make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+            }
+            half_m[r] = top - kUp;
+            half_l[r] = sum;
+        }
+        named_barrier_sync(1, 256);
+        if (ok) {
+            const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+            const uint32_t hd4 = hd / 4u;
+            for (uint32_t x = tid; x < kRows * hd4; x += 256u) {
+                const uint32_t rr = x / hd4, d = (x - rr * hd4) * 4u;
+                if (row_pos[rr] == -2) continue;
+                const size_t row = static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr];
+                float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
+                *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(sums + rr * kPitch + d);
+                if (!a.direct && d == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(half_m[rr], half_l[rr]);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows) {
+    EncodeTiled encode = encode_tiled_fn();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {kv.head_dim, kv.page_size, static_cast<cuuint64_t>(kv.num_pages) * kv.kv_heads};
+    const cuuint64_t strides[2] = {kv.head_dim * 2ull, static_cast<cuuint64_t>(kv.page_size) * kv.head_dim * 2ull};
+    const cuuint32_t box[3] = {64u, box_rows, 1u}, step[3] = {1u, 1u, 1u};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <uint32_t HD>
+cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    TcMaps maps;
+    const uint32_t box_rows = a.kv.page_size < kKeys ? a.kv.page_size : kKeys;
+    if (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows))
+        return cudaErrorInvalidValue;
+    cudaError_t e = cudaFuncSetAttribute(attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(Tc<HD>::kSmem));
+    if (e != cudaSuccess) return e;
+    attention_tc_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Tc<HD>::kSmem, stream>>>(maps, a, box_rows);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_tc(const AttnArgs& args, uint64_t tiles, cudaStream_t stream) {
+    AttnArgs a = args;
+    a.tiles = static_cast<uint32_t>(tiles);
+    const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
+    return a.kv.head_dim <= 64u ? launch<64>(a, items, stream) : launch<128>(a, items, stream);
+}
+
+}  // namespace nedo_gpu
