@@ -19,6 +19,8 @@
 //     running sums.  The two halves' sums meet at the end in shared memory.
 // TMEM: two S/P and two O tiles of 128 columns each.  Registers: the softmax warps hold 128
 // sums each, so they take 208 registers and the other warps give theirs up.
+#include <algorithm>
+
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
@@ -73,32 +75,28 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
-// 32 columns of this warp's 32 lanes: a row per thread.
-__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[32]) {
+// 16 columns of this warp's 32 lanes, a row per thread: the load is under way until
+// tmem_ready, which takes the registers so that nothing reads them before it.
+__device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float tmem_load1(uint32_t addr) {
-    uint32_t v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-    return __uint_as_float(v);
+__device__ __forceinline__ void tmem_ready(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                   "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::
+                     "memory");
 }
-__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(v[0]),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15};" ::"r"(v[0]),
         "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
-        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]),
-        "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
-        "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(addr)
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
         : "memory");
 }
 
@@ -125,7 +123,7 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
 
 template <uint32_t HD>
 __global__ void __launch_bounds__(kThreads, 1)
-    attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_rows) {
+    attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_shift) {
     using T = Tc<HD>;
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
@@ -270,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == kLoadWarp) {
             // ---- loads
-            const uint32_t boxes = kKeys / box_rows, box_bytes = box_rows * 128u;
+            const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
             // lane b: page of box b of a tile (kNone: no keys of the item there, or no page)
             auto look_up = [&](uint32_t i) {
                 const uint32_t j = j0 + i * kKeys + lane * box_rows;
@@ -313,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) return;
                     for (uint32_t x = lane; x < kKeys * 8u * T::kBlocks; x += 32u) {
                         const uint32_t r = x / (8u * T::kBlocks), ch = x % (8u * T::kBlocks);
-                        if (j + r < kb || j + r >= ke || !(there >> (r / box_rows) & 1u))
+                        if (j + r < kb || j + r >= ke || !(there >> (r >> box_shift) & 1u))
                             *reinterpret_cast<uint4*>(sm + (dst - s0) + at(r, ch)) = make_uint4(0u, 0u, 0u, 0u);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -369,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (uint32_t half = 0; half < 2u; ++half)
 #pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 columns of weights, 2048 bytes of values
-                            mma_ts(d, p + (k >> 1) * 32u + (half ? 0u : 16u) + (k & 1u) * 8u,
+                        for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 + 8 columns of weights, 2048 bytes of values
+                            mma_ts(d, p + k * 16u + (half ? 0u : 8u),
                                    desc(ring + slot * T::kTile + k * 2048u, kBlock), kO, half + k != 0u);
                     tc_commit(&o_full[i & 1u]);
                     tc_commit(&empty[slot]);
@@ -405,85 +403,57 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             tc_fence_after();
             const bool mine = j < we && j + kKeys > wb;  // a tile that none of the warp's rows sees is passed over
-            float alpha = 1.f;
-            bool odd = false;
+            float alpha = 1.f, ref = 0.f;
+            bool whole = true;
+            uint32_t gap = 0u;
+            // keys of the tile that this row sees: bits of 16 keys from key 16 k on
+            const uint32_t from = max(max(lo_key, kb), j) - j, to = min(min(hi_key, ke), j + kKeys) - min(j, min(hi_key, ke));
+            auto seen = [&](uint32_t k) -> uint32_t {
+                const uint32_t b = min(max(from, 16u * k) - 16u * k, 16u), e = min(max(to, 16u * k) - 16u * k, 16u);
+                return gap >> ((16u * k) >> box_shift) & 1u ? 0u : (0xFFFFu << b) & ((1u << e) - 1u);
+            };
             if (mine) {
-                const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 3u]);
-                const bool whole = gap == 0u && j >= max(all_b, kb) && j + kKeys <= min(all_e, ke);
-                // first and last key of the tile that this row sees
-                const uint32_t from = max(max(lo_key, kb), j), to = min(min(hi_key, ke), j + kKeys);
-                auto unseen = [&](uint32_t x) {  // x: key in the tile
-                    return j + x < from || j + x >= to || (gap >> (x / box_rows) & 1u);
+                gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 3u]);
+                whole = gap == 0u && j >= max(all_b, kb) && j + kKeys <= min(all_e, ke);
+                auto mask = [&](uint32_t (&x)[16], uint32_t k) {
+                    const uint32_t bits = seen(k);
+#pragma unroll
+                    for (uint32_t e = 0; e < 16u; ++e)
+                        if (!(bits >> e & 1u)) x[e] = 0xFF800000u;
                 };
-                uint32_t x[32];
-                float mt = -INFINITY;
+                uint32_t x[2][16];
+                float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                tmem_load(st_addr, x[0]);
 #pragma unroll
-                for (uint32_t q = 0; q < 4u; ++q) {
-                    tmem_load(st_addr + 32u * q, x);
-                    if (!whole) {
+                for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+                    tmem_ready(x[k & 1u]);
+                    if (k + 1u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+                    if (!whole) mask(x[k & 1u], k);
 #pragma unroll
-                        for (uint32_t e = 0; e < 32u; ++e)
-                            if (unseen(32u * q + e)) x[e] = 0xFF800000u;
-                    }
-#pragma unroll
-                    for (uint32_t e = 0; e < 32u; ++e) mt = fmaxf(mt, __uint_as_float(x[e]));
+                    for (uint32_t e = 0; e < 16u; ++e) mt[e & 3u] = fmaxf(mt[e & 3u], __uint_as_float(x[k & 1u][e]));
                 }
-                const float mn = fmaxf(m, mt * unscale);
+                const float mn = fmaxf(m, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])) * unscale);
                 alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 m = mn;
-                const float ref = (mn == -INFINITY ? 0.f : mn) - kUp;
-                if (!whole) {
-                    // a value that is not finite must not reach the rows that do not see it (0 * inf)
-                    const uint32_t n = v_at(i);
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&full[n % kSlots], (n / kSlots) & 1u, a.st, 69u));
-                    if (!ok) break;
-                    const uint8_t* v = sm + (ring - s0) + (n % kSlots) * T::kTile;
-                    for (uint32_t y = lane; y < T::kTile / 16u; y += 32u) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(v + y * 16u);
-                        odd |= not_finite(w.x) || not_finite(w.y) || not_finite(w.z) || not_finite(w.w);
-                    }
-                    odd = __any_sync(0xFFFFFFFFu, odd);
-                    if (odd) {  // key by key, for the rows that see it; the tensor core's sums are left out
-#pragma unroll
-                        for (uint32_t d = 0; d < HD; ++d) acc[d] *= alpha;
-                        for (uint32_t k = 0; k < kKeys; ++k) {
-                            const float w = exp2_fast(fmaf(tmem_load1(st_addr + k), unscale, -ref));
-                            if (!unseen(k)) {
-#pragma unroll
-                                for (uint32_t ch = 0; ch < HD / 8u; ++ch) {
-                                    const uint4 y = *reinterpret_cast<const uint4*>(v + at(k, ch));
-                                    const uint32_t h[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                                    for (uint32_t e = 0; e < 4u; ++e) {
-                                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
-                                        acc[8u * ch + 2u * e] = fmaf(w, f.x, acc[8u * ch + 2u * e]);
-                                        acc[8u * ch + 2u * e + 1u] = fmaf(w, f.y, acc[8u * ch + 2u * e + 1u]);
-                                    }
-                                }
-                            }
-                            __syncwarp();
-                        }
-                    }
-                }
+                ref = (mn == -INFINITY ? 0.f : mn) - kUp;
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
+                tmem_load(st_addr, x[0]);
 #pragma unroll
-                for (uint32_t q = 0; q < 4u; ++q) {
-                    tmem_load(st_addr + 32u * q, x);
-                    if (!whole) {
+                for (uint32_t k = 0; k < kKeys / 16u; ++k) {
+                    uint32_t (&y)[16] = x[k & 1u];
+                    tmem_ready(y);
+                    if (k + 1u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+                    if (!whole) mask(y, k);
+                    uint32_t w[16];  // 8 columns of high halves, 8 of low halves
 #pragma unroll
-                        for (uint32_t e = 0; e < 32u; ++e)
-                            if (unseen(32u * q + e)) x[e] = 0xFF800000u;
-                    }
-                    uint32_t w[32];  // 16 columns of high halves, 16 of low halves
-#pragma unroll
-                    for (uint32_t e = 0; e < 16u; ++e) {
-                        const float a0 = exp2_fast(fmaf(__uint_as_float(x[2 * e]), unscale, -ref));
-                        const float a1 = exp2_fast(fmaf(__uint_as_float(x[2 * e + 1]), unscale, -ref));
+                    for (uint32_t e = 0; e < 8u; ++e) {
+                        const float a0 = exp2_fast(fmaf(__uint_as_float(y[2 * e]), unscale, -ref));
+                        const float a1 = exp2_fast(fmaf(__uint_as_float(y[2 * e + 1]), unscale, -ref));
                         part[(2 * e) & 3u] += a0;
                         part[(2 * e + 1) & 3u] += a1;
-                        split(a0, a1, &w[e], &w[16 + e]);
+                        split(a0, a1, &w[e], &w[8 + e]);
                     }
-                    tmem_store(st_addr + 32u * q, w);
+                    tmem_store(st_addr + 16u * k, w);
                 }
                 l = fmaf(l, alpha, (part[0] + part[1]) + (part[2] + part[3]));
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -494,13 +464,51 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
             tc_fence_after();
-            if (mine && !odd) {
+            if (mine) {
+                bool odd = false;
+                uint32_t x[2][16];
+                if (!whole) {
+                    // a value that is not finite must not reach the rows that do not see it, yet
+                    // 0 * inf is in their sums: then the tile is done key by key
+                    float t = 0.f;
+                    tmem_load(o_addr, x[0]);
 #pragma unroll
-                for (uint32_t q = 0; q < HD / 32u; ++q) {
-                    uint32_t x[32];
-                    tmem_load(o_addr + 32u * q, x);
+                    for (uint32_t k = 0; k < HD / 16u; ++k) {
+                        tmem_ready(x[k & 1u]);
+                        if (k + 1u < HD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
 #pragma unroll
-                    for (uint32_t e = 0; e < 32u; ++e) acc[32u * q + e] = fmaf(acc[32u * q + e], alpha, __uint_as_float(x[e]));
+                        for (uint32_t e = 0; e < 16u; ++e) t = fmaf(__uint_as_float(x[k & 1u][e]), 0.f, t);
+                    }
+                    odd = p >= 0 && t != 0.f;
+                }
+                if (!__any_sync(0xFFFFFFFFu, odd)) {
+                    tmem_load(o_addr, x[0]);
+#pragma unroll
+                    for (uint32_t k = 0; k < HD / 16u; ++k) {
+                        tmem_ready(x[k & 1u]);
+                        if (k + 1u < HD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+#pragma unroll
+                        for (uint32_t e = 0; e < 16u; ++e)
+                            acc[16u * k + e] = fmaf(acc[16u * k + e], alpha, __uint_as_float(x[k & 1u][e]));
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t d = 0; d < HD; ++d) acc[d] *= alpha;
+                    const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+                    for (uint32_t k = from; k < to; ++k) {
+                        if (!(seen(k >> 4) >> (k & 15u) & 1u)) continue;
+                        const uint32_t page = a.b.table[static_cast<size_t>(s) * a.b.max_pages + ((j + k) >> a.kv.page_shift)];
+                        const size_t off = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size +
+                                            ((j + k) & (a.kv.page_size - 1u))) * hd;
+                        const __half *kr = static_cast<const __half*>(a.kv.k) + off, *vr = static_cast<const __half*>(a.kv.v) + off;
+                        float sum = 0.f;
+                        for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, __half2float(kr[d]), sum);
+                        const float w = exp2_fast(sum - ref);
+#pragma unroll
+                        for (uint32_t d = 0; d < HD; ++d)
+                            if (d < hd) acc[d] = fmaf(w, __half2float(vr[d]), acc[d]);
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -575,13 +583,13 @@ bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows
 template <uint32_t HD>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
     TcMaps maps;
-    const uint32_t box_rows = a.kv.page_size < kKeys ? a.kv.page_size : kKeys;
+    const uint32_t box_rows = std::min(a.kv.page_size, kKeys);
     if (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows))
         return cudaErrorInvalidValue;
     cudaError_t e = cudaFuncSetAttribute(attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(Tc<HD>::kSmem));
     if (e != cudaSuccess) return e;
-    attention_tc_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Tc<HD>::kSmem, stream>>>(maps, a, box_rows);
+    attention_tc_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Tc<HD>::kSmem, stream>>>(maps, a, std::min(a.kv.page_shift, 7u));
     return cudaGetLastError();
 }
 
