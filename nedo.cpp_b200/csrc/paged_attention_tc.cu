@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto v_at = [&](uint32_t i) { return i + 1u < ntiles ? 2u * i + 2u : 2u * ntiles - 1u; };
 
     if (warp >= kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == kLoadWarp) {
             // ---- loads
             const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // ---- softmax: a row per thread, tiles half, half + 2, ...
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const uint32_t half = warp >> 2, r = tid & 127u;
         const uint32_t lanes = tmem + ((warp & 3u) << 21);  // the warp's 32 TMEM lanes
         const uint32_t st_addr = lanes + half * 128u, o_addr = lanes + 256u + half * 128u;
@@ -423,26 +423,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 uint32_t x[2][16];
                 float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto top = [&](uint32_t (&y)[16], uint32_t k) {
+                    if (!whole) mask(y, k);
+#pragma unroll
+                    for (uint32_t e = 0; e < 16u; ++e) mt[e & 3u] = fmaxf(mt[e & 3u], __uint_as_float(y[e]));
+                };
                 tmem_load(st_addr, x[0]);
-#pragma unroll
-                for (uint32_t k = 0; k < kKeys / 16u; ++k) {
-                    tmem_ready(x[k & 1u]);
-                    if (k + 1u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
-                    if (!whole) mask(x[k & 1u], k);
-#pragma unroll
-                    for (uint32_t e = 0; e < 16u; ++e) mt[e & 3u] = fmaxf(mt[e & 3u], __uint_as_float(x[k & 1u][e]));
+#pragma unroll 1
+                for (uint32_t k = 0; k < kKeys / 16u; k += 2u) {
+                    tmem_ready(x[0]);
+                    tmem_load(st_addr + 16u * (k + 1u), x[1]);
+                    top(x[0], k);
+                    tmem_ready(x[1]);
+                    tmem_load(st_addr + 16u * ((k + 2u) & 7u), x[0]);  // the last one is the next pass's first
+                    top(x[1], k + 1u);
                 }
                 const float mn = fmaxf(m, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])) * unscale);
                 alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 m = mn;
                 ref = (mn == -INFINITY ? 0.f : mn) - kUp;
                 float part[4] = {0.f, 0.f, 0.f, 0.f};
-                tmem_load(st_addr, x[0]);
-#pragma unroll
-                for (uint32_t k = 0; k < kKeys / 16u; ++k) {
-                    uint32_t (&y)[16] = x[k & 1u];
-                    tmem_ready(y);
-                    if (k + 1u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+                auto weigh = [&](uint32_t (&y)[16], uint32_t k) {
                     if (!whole) mask(y, k);
                     uint32_t w[16];  // 8 columns of high halves, 8 of low halves
 #pragma unroll
@@ -454,6 +455,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         split(a0, a1, &w[e], &w[8 + e]);
                     }
                     tmem_store(st_addr + 16u * k, w);
+                };
+#pragma unroll 1
+                for (uint32_t k = 0; k < kKeys / 16u; k += 2u) {
+                    tmem_ready(x[0]);
+                    tmem_load(st_addr + 16u * (k + 1u), x[1]);
+                    weigh(x[0], k);
+                    tmem_ready(x[1]);
+                    if (k + 2u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 2u), x[0]);
+                    weigh(x[1], k + 1u);
                 }
                 l = fmaf(l, alpha, (part[0] + part[1]) + (part[2] + part[3]));
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
