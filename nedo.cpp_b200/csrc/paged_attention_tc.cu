@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 auto top = [&](uint32_t (&y)[16], uint32_t k) {
                     if (!whole) mask(y, k);
 #pragma unroll
-                    for (uint32_t e = 0; e < 16u; ++e) mt[e & 3u] = fmaxf(mt[e & 3u], __uint_as_float(y[e]));
+                    for (uint32_t e = 0; e < 16u; e += 2u)
+                        mt[(e >> 1) & 3u] = fmaxf(fmaxf(mt[(e >> 1) & 3u], __uint_as_float(y[e])), __uint_as_float(y[e + 1]));
                 };
                 tmem_load(st_addr, x[0]);
 #pragma unroll 1
@@ -442,17 +443,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                 alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 m = mn;
                 ref = (mn == -INFINITY ? 0.f : mn) - kUp;
-                float part[4] = {0.f, 0.f, 0.f, 0.f};
+                float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                const float2 unscale2 = make_float2(unscale, unscale), ref2 = make_float2(-ref, -ref);
                 auto weigh = [&](uint32_t (&y)[16], uint32_t k) {
                     if (!whole) mask(y, k);
                     uint32_t w[16];  // 8 columns of high halves, 8 of low halves
 #pragma unroll
                     for (uint32_t e = 0; e < 8u; ++e) {
-                        const float a0 = exp2_fast(fmaf(__uint_as_float(y[2 * e]), unscale, -ref));
-                        const float a1 = exp2_fast(fmaf(__uint_as_float(y[2 * e + 1]), unscale, -ref));
-                        part[(2 * e) & 3u] += a0;
-                        part[(2 * e + 1) & 3u] += a1;
-                        split(a0, a1, &w[e], &w[8 + e]);
+                        float2 v = ffma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), unscale2, ref2);
+                        v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+                        part[e & 1u] = fadd2(part[e & 1u], v);
+                        split(v, &w[e], &w[8 + e]);
                     }
                     tmem_store(st_addr + 16u * k, w);
                 };
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (k + 2u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 2u), x[0]);
                     weigh(x[1], k + 1u);
                 }
-                l = fmaf(l, alpha, (part[0] + part[1]) + (part[2] + part[3]));
+                l = fmaf(l, alpha, (part[0].x + part[1].x) + (part[0].y + part[1].y));
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             }
             tc_fence_before();
@@ -498,8 +499,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_ready(x[k & 1u]);
                         if (k + 1u < HD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
 #pragma unroll
-                        for (uint32_t e = 0; e < 16u; ++e)
-                            acc[16u * k + e] = fmaf(acc[16u * k + e], alpha, __uint_as_float(x[k & 1u][e]));
+                        for (uint32_t e = 0; e < 16u; e += 2u) {
+                            const float2 y = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), make_float2(alpha, alpha),
+                                                   make_float2(__uint_as_float(x[k & 1u][e]), __uint_as_float(x[k & 1u][e + 1u])));
+                            acc[16u * k + e] = y.x;
+                            acc[16u * k + e + 1u] = y.y;
+                        }
                     }
                 } else {
 #pragma unroll

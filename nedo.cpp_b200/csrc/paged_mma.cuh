@@ -43,6 +43,13 @@ __device__ __forceinline__ void split(float x, float y, uint32_t* hi, uint32_t* 
     *hi = pack(h);
     *lo = pack(__floats2half2_rn(x - f.x, y - f.y));
 }
+// the same for a pair in packed arithmetic
+__device__ __forceinline__ void split(float2 x, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __float22half2_rn(x);
+    const float2 f = __half22float2(h);
+    *hi = pack(h);
+    *lo = pack(__float22half2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y))));
+}
 __device__ __forceinline__ bool not_finite(uint32_t two_halves) {
     return (two_halves & 0x7C00u) == 0x7C00u || (two_halves & 0x7C000000u) == 0x7C000000u;
 }
