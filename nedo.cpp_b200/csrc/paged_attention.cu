@@ -246,11 +246,11 @@ struct CombineArgs {
     uint32_t own_chunk, own_chunks, prefix_chunk, prefix_chunks;
     uint32_t few_rows, few_chunk;        // sequences of at most few_rows rows have chunks of their own
     uint32_t own_direct, few_direct;     // written out already
-    uint32_t group;
+    uint32_t group, heads_per_cta;
     uint32_t blocks;  // the sparse call: every slot is written
 };
 
-// One CTA per (token, head).  The maximum over the row's chunks first, then in blocks of
+// One CTA per token and head (per token where most rows are done already).  The maximum over the row's chunks first, then in blocks of
 // kCombineThreads chunks their weights 2^(m_i - m) into shared memory, and the weighted
 // sum with head_dim / 4 threads to a chunk and as many chunks at once as the CTA holds,
 // four loads in flight each; the groups' sums meet in group order.  A chunk in which the
@@ -260,9 +260,10 @@ constexpr uint32_t kCombineThreads = 128;
 __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(CombineArgs a) {
     __shared__ float wt[kCombineThreads], red[kCombineThreads / 32u];
     __shared__ float4 sums[kCombineThreads];
-    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads, row = blockIdx.x;
+    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    const uint32_t t = static_cast<uint32_t>(row / a.heads);
+    const uint32_t per_token = a.heads / a.heads_per_cta;  // CTAs
+    const uint32_t t = blockIdx.x / per_token;
     const uint32_t s = seq_of_token(a.b, t);
     PagedSeq sq{0u, 0u, 0u};
     if (s != kNone) sq = load_seq(a.b, s, nullptr);
@@ -288,61 +289,70 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (sq.n == 0u || (few ? a.few_direct : a.own_direct)) return;  // no row of any sequence, or done
     const uint32_t n0 = e0 - b0, n = n0 + (e1 - b1);
-    const float2* ml = a.part_ml + row;
-    auto slot = [&](uint32_t i) -> size_t { return i < n0 ? b0 + i : b1 + (i - n0); };
-    float m = -INFINITY;
-    for (uint32_t i = tid; i < n; i += kCombineThreads) m = fmaxf(m, ml[slot(i) * rows_all].x);
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (lane == 0u) red[warp] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const uint32_t hd = a.kv.head_dim, hd4 = hd / 4u, groups = kCombineThreads / hd4;
-    const uint32_t grp = tid / hd4, d = tid - grp * hd4;
-    float l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t i0 = 0; i0 < n; i0 += kCombineThreads) {
-        const uint32_t cnt = min(kCombineThreads, n - i0);
-        __syncthreads();
-        float w = 0.f;
-        if (tid < cnt) {
-            const float2 x = ml[slot(i0 + tid) * rows_all];
-            if (x.y != 0.f) {
-                w = exp2f(x.x - m);
-                l = fmaf(x.y, w, l);
-            }
+    for (uint32_t h = 0; h < a.heads_per_cta; ++h) {
+        const size_t row = static_cast<size_t>(t) * a.heads + (blockIdx.x % per_token) * a.heads_per_cta + h;
+        const float2* ml = a.part_ml + row;
+        auto slot = [&](uint32_t i) -> size_t { return i < n0 ? b0 + i : b1 + (i - n0); };
+        float m = -INFINITY;
+        for (uint32_t i = tid; i < n; i += kCombineThreads) {
+            const float2 x = ml[slot(i) * rows_all];
+            if (x.y != 0.f) m = fmaxf(m, x.x);
         }
-        wt[tid] = w;
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
         __syncthreads();
-        if (grp < groups) {
+        if (lane == 0u) red[warp] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const uint32_t hd = a.kv.head_dim, hd4 = hd / 4u, groups = kCombineThreads / hd4;
+        const uint32_t grp = tid / hd4, d = tid - grp * hd4;
+        float l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t i0 = 0; i0 < n; i0 += kCombineThreads) {
+            const uint32_t cnt = min(kCombineThreads, n - i0);
+            __syncthreads();
+            float w = 0.f;
+            if (tid < cnt) {
+                const float2 x = ml[slot(i0 + tid) * rows_all];
+                if (x.y != 0.f) {
+                    w = exp2f(x.x - m);
+                    l = fmaf(x.y, w, l);
+                }
+            }
+            wt[tid] = w;
+            __syncthreads();
+            if (grp < groups) {
 #pragma unroll 4
-            for (uint32_t i = grp; i < cnt; i += groups) {
-                const float f = wt[i];
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (f != 0.f) x = *reinterpret_cast<const float4*>(a.part_o + (slot(i0 + i) * rows_all + row) * hd + 4u * d);
-                acc.x = fmaf(x.x, f, acc.x);
-                acc.y = fmaf(x.y, f, acc.y);
-                acc.z = fmaf(x.z, f, acc.z);
-                acc.w = fmaf(x.w, f, acc.w);
+                for (uint32_t i = grp; i < cnt; i += groups) {
+                    const float f = wt[i];
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (f != 0.f)
+                        x = *reinterpret_cast<const float4*>(a.part_o + (slot(i0 + i) * rows_all + row) * hd + 4u * d);
+                    acc.x = fmaf(x.x, f, acc.x);
+                    acc.y = fmaf(x.y, f, acc.y);
+                    acc.z = fmaf(x.z, f, acc.z);
+                    acc.w = fmaf(x.w, f, acc.w);
+                }
             }
         }
+        l = warp_sum(l);
+        __syncthreads();
+        if (lane == 0u) red[warp] = l;
+        sums[tid] = acc;
+        __syncthreads();
+        if (tid < hd4) {
+            l = (red[0] + red[1]) + (red[2] + red[3]);
+            for (uint32_t k = 1; k < groups; ++k) {
+                const float4 x = sums[k * hd4 + tid];
+                acc.x += x.x;
+                acc.y += x.y;
+                acc.z += x.z;
+                acc.w += x.w;
+            }
+            const bool none = l == 0.f;
+            *reinterpret_cast<float4*>(a.out + row * hd + 4u * tid) =
+                none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
+        }
     }
-    l = warp_sum(l);
-    __syncthreads();
-    if (lane == 0u) red[warp] = l;
-    sums[tid] = acc;
-    __syncthreads();
-    if (tid >= hd4) return;
-    l = (red[0] + red[1]) + (red[2] + red[3]);
-    for (uint32_t k = 1; k < groups; ++k) {
-        const float4 x = sums[k * hd4 + tid];
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-    }
-    const bool none = l == 0.f;
-    *reinterpret_cast<float4*>(a.out + row * hd + 4u * tid) =
-        none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
@@ -560,9 +570,10 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     c.own_direct = own_direct;
     c.few_direct = few_direct;
     c.group = a.group;
+    c.heads_per_cta = own_direct ? p.heads : 1u;
     c.blocks = p.picks != 0u;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<uint32_t>(rows));
+    cfg.gridDim = dim3(static_cast<uint32_t>(rows / c.heads_per_cta));
     cfg.blockDim = dim3(kCombineThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

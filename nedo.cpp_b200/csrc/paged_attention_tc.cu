@@ -8,17 +8,18 @@
 // them, so a tile's O starts from zero in TMEM and is added to the running sums in fp32
 // registers, together with the rescaling by 2^(m_old - m_new).
 //
-// Work.  A CTA (one per SM, 384 threads) takes 128 rows through their keys in tiles of 128:
-//   * warp 8 brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
+// Work.  A CTA (one per SM, 640 threads) takes 128 rows through their keys in tiles of 128:
+//   * warp 16 brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
 //     swizzle), in the order of their use, four half-tile slots deep.  Of a tile that the
 //     item's key range cuts it zeroes the values outside, whatever the pages hold there;
-//   * one thread of warp 9 issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so the
+//   * one thread of warp 17 issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so the
 //     tensor core works while a softmax runs;
-//   * warps 0-3 take the even and warps 4-7 the odd tiles, a row per thread: they read S from
-//     TMEM, write the split weights over it (the A operand of P V), and add O to their own
-//     running sums.  The two halves' sums meet at the end in shared memory.
-// TMEM: two S/P and two O tiles of 128 columns each.  Registers: the softmax warps hold 128
-// sums each, so they take 208 registers and the other warps give theirs up.
+//   * warps 0-7 take the even and warps 8-15 the odd tiles, two threads to a row, each with
+//     half of the tile's keys and half of the channels: they read S from TMEM, agree on the
+//     row's maximum, write the split weights over S (the A operand of P V), and add O to their
+//     running sums.  The even and the odd sums meet at the end in shared memory.
+// TMEM: two S/P and two O tiles of 128 columns each.  Registers: the softmax threads hold 64
+// sums each, so they take 104 registers and the other warps give theirs up.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -30,9 +31,10 @@ namespace {
 constexpr uint32_t kRows = kTcRows;     // 128
 constexpr uint32_t kKeys = 128;         // keys per tile
 constexpr uint32_t kSlots = 4;          // ring slots: the keys or the values of one tile
-constexpr uint32_t kThreads = 384;
+constexpr uint32_t kSoftmax = 512;      // softmax threads: four to a row
+constexpr uint32_t kThreads = kSoftmax + 128;
 constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
-constexpr uint32_t kLoadWarp = 8, kMmaWarp = 9;
+constexpr uint32_t kLoadWarp = 16, kMmaWarp = 17;
 
 template <uint32_t HD>
 struct Tc {
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float row_unscale[kRows], half_m[kRows], half_l[kRows];
+    __shared__ float row_unscale[kRows], tile_max[4][kRows], sum_l[4][kRows], sum_m[2][kRows];
     __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[2], p_full[2], o_full[2], done;
     __shared__ uint32_t found[2], tmem_slot, gaps[4];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&cut, 1);
         for (uint32_t i = 0; i < 2u; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
+            mbar_init(&p_full[i], 256);
             mbar_init(&o_full[i], 1);
         }
         mbar_init(&done, 1);
@@ -265,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto v_at = [&](uint32_t i) { return i + 1u < ntiles ? 2u * i + 2u : 2u * ntiles - 1u; };
 
     if (warp >= kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp == kLoadWarp) {
             // ---- loads
             const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
@@ -379,11 +381,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
         }
     } else {
-        // ---- softmax: a row per thread, tiles half, half + 2, ...
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        const uint32_t half = warp >> 2, r = tid & 127u;
+        // ---- softmax: tiles half, half + 2, ...; keys and channels of this side
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        const uint32_t half = warp >> 3, side = (warp >> 2) & 1u, r = tid & 127u;
+        constexpr uint32_t kD = HD / 2u, kC = kKeys / 32u;  // channels and 16-key pieces of a side
         const uint32_t lanes = tmem + ((warp & 3u) << 21);  // the warp's 32 TMEM lanes
-        const uint32_t st_addr = lanes + half * 128u, o_addr = lanes + 256u + half * 128u;
+        const uint32_t st_addr = lanes + half * 128u + side * 64u, o_addr = lanes + 256u + half * 128u + side * kD;
         const int p = row_pos[r];
         const float unscale = row_unscale[r];
         const uint32_t lo_key = p >= 0 ? first_key(p, a.window) : kNone, hi_key = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
@@ -391,9 +394,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t wb = __reduce_min_sync(0xFFFFFFFFu, lo_key), we = __reduce_max_sync(0xFFFFFFFFu, hi_key);
         const uint32_t all_b = __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? lo_key : 0u);
         const uint32_t all_e = __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? hi_key : kNone);
-        float acc[HD];
+        float acc[kD];
 #pragma unroll
-        for (uint32_t d = 0; d < HD; ++d) acc[d] = 0.f;
+        for (uint32_t d = 0; d < kD; ++d) acc[d] = 0.f;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (uint32_t i = half; i < ntiles && ok; i += 2u) {
@@ -412,59 +415,57 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t b = min(max(from, 16u * k) - 16u * k, 16u), e = min(max(to, 16u * k) - 16u * k, 16u);
                 return gap >> ((16u * k) >> box_shift) & 1u ? 0u : (0xFFFFu << b) & ((1u << e) - 1u);
             };
+            auto mask = [&](uint32_t (&x)[16], uint32_t k) {
+                const uint32_t bits = seen(kC * side + k);
+#pragma unroll
+                for (uint32_t e = 0; e < 16u; ++e)
+                    if (!(bits >> e & 1u)) x[e] = 0xFF800000u;
+            };
             if (mine) {
                 gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 3u]);
                 whole = gap == 0u && j >= max(all_b, kb) && j + kKeys <= min(all_e, ke);
-                auto mask = [&](uint32_t (&x)[16], uint32_t k) {
-                    const uint32_t bits = seen(k);
-#pragma unroll
-                    for (uint32_t e = 0; e < 16u; ++e)
-                        if (!(bits >> e & 1u)) x[e] = 0xFF800000u;
-                };
-                uint32_t x[2][16];
-                float mt[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto top = [&](uint32_t (&y)[16], uint32_t k) {
-                    if (!whole) mask(y, k);
-#pragma unroll
-                    for (uint32_t e = 0; e < 16u; e += 2u)
-                        mt[(e >> 1) & 3u] = fmaxf(fmaxf(mt[(e >> 1) & 3u], __uint_as_float(y[e])), __uint_as_float(y[e + 1]));
-                };
-                tmem_load(st_addr, x[0]);
+                float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                for (uint32_t k = 0; k < kKeys / 16u; k += 2u) {
-                    tmem_ready(x[0]);
+                for (uint32_t k = 0; k < kC; k += 2u) {
+                    uint32_t x[2][16];
+                    tmem_load(st_addr + 16u * k, x[0]);
                     tmem_load(st_addr + 16u * (k + 1u), x[1]);
-                    top(x[0], k);
+                    tmem_ready(x[0]);
                     tmem_ready(x[1]);
-                    tmem_load(st_addr + 16u * ((k + 2u) & 7u), x[0]);  // the last one is the next pass's first
-                    top(x[1], k + 1u);
+#pragma unroll
+                    for (uint32_t u = 0; u < 2u; ++u) {
+                        if (!whole) mask(x[u], k + u);
+#pragma unroll
+                        for (uint32_t e = 0; e < 16u; e += 2u)
+                            mt[(e >> 1) & 1u] =
+                                fmaxf(fmaxf(mt[(e >> 1) & 1u], __uint_as_float(x[u][e])), __uint_as_float(x[u][e + 1]));
+                    }
                 }
-                const float mn = fmaxf(m, fmaxf(fmaxf(mt[0], mt[1]), fmaxf(mt[2], mt[3])) * unscale);
+                tile_max[half * 2u + side][r] = fmaxf(mt[0], mt[1]);
+            }
+            named_barrier_sync(1u + half, 256);
+            if (mine) {
+                const float mt = fmaxf(tile_max[half * 2u][r], tile_max[half * 2u + 1u][r]);
+                const float mn = fmaxf(m, mt * unscale);
                 alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
                 m = mn;
                 ref = (mn == -INFINITY ? 0.f : mn) - kUp;
                 float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                 const float2 unscale2 = make_float2(unscale, unscale), ref2 = make_float2(-ref, -ref);
-                auto weigh = [&](uint32_t (&y)[16], uint32_t k) {
-                    if (!whole) mask(y, k);
-                    uint32_t w[16];  // 8 columns of high halves, 8 of low halves
+#pragma unroll 1
+                for (uint32_t k = 0; k < kC; ++k) {
+                    uint32_t x[16], w[16];  // w: 8 columns of high halves, 8 of low halves
+                    tmem_load(st_addr + 16u * k, x);
+                    tmem_ready(x);
+                    if (!whole) mask(x, k);
 #pragma unroll
                     for (uint32_t e = 0; e < 8u; ++e) {
-                        float2 v = ffma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), unscale2, ref2);
+                        float2 v = ffma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), unscale2, ref2);
                         v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
                         part[e & 1u] = fadd2(part[e & 1u], v);
                         split(v, &w[e], &w[8 + e]);
                     }
                     tmem_store(st_addr + 16u * k, w);
-                };
-#pragma unroll 1
-                for (uint32_t k = 0; k < kKeys / 16u; k += 2u) {
-                    tmem_ready(x[0]);
-                    tmem_load(st_addr + 16u * (k + 1u), x[1]);
-                    weigh(x[0], k);
-                    tmem_ready(x[1]);
-                    if (k + 2u < kKeys / 16u) tmem_load(st_addr + 16u * (k + 2u), x[0]);
-                    weigh(x[1], k + 1u);
                 }
                 l = fmaf(l, alpha, (part[0].x + part[1].x) + (part[0].y + part[1].y));
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -484,9 +485,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float t = 0.f;
                     tmem_load(o_addr, x[0]);
 #pragma unroll
-                    for (uint32_t k = 0; k < HD / 16u; ++k) {
+                    for (uint32_t k = 0; k < kD / 16u; ++k) {
                         tmem_ready(x[k & 1u]);
-                        if (k + 1u < HD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+                        if (k + 1u < kD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
 #pragma unroll
                         for (uint32_t e = 0; e < 16u; ++e) t = fmaf(__uint_as_float(x[k & 1u][e]), 0.f, t);
                     }
@@ -495,9 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!__any_sync(0xFFFFFFFFu, odd)) {
                     tmem_load(o_addr, x[0]);
 #pragma unroll
-                    for (uint32_t k = 0; k < HD / 16u; ++k) {
+                    for (uint32_t k = 0; k < kD / 16u; ++k) {
                         tmem_ready(x[k & 1u]);
-                        if (k + 1u < HD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
+                        if (k + 1u < kD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
 #pragma unroll
                         for (uint32_t e = 0; e < 16u; e += 2u) {
                             const float2 y = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), make_float2(alpha, alpha),
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 } else {
 #pragma unroll
-                    for (uint32_t d = 0; d < HD; ++d) acc[d] *= alpha;
+                    for (uint32_t d = 0; d < kD; ++d) acc[d] *= alpha;
                     const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
                     for (uint32_t k = from; k < to; ++k) {
                         if (!(seen(k >> 4) >> (k & 15u) & 1u)) continue;
@@ -520,8 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, __half2float(kr[d]), sum);
                         const float w = exp2_fast(sum - ref);
 #pragma unroll
-                        for (uint32_t d = 0; d < HD; ++d)
-                            if (d < hd) acc[d] = fmaf(w, __half2float(vr[d]), acc[d]);
+                        for (uint32_t d = 0; d < kD; ++d)
+                            if (side * kD + d < hd) acc[d] = fmaf(w, __half2float(vr[side * kD + d]), acc[d]);
                     }
                     __syncwarp();
                 }
@@ -529,49 +530,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the halves meet: the odd tiles' sums through shared memory (the ring is done with)
         asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
-        named_barrier_sync(1, 256);
         constexpr uint32_t kPitch = HD + 4u;
-        float* sums = reinterpret_cast<float*>(sm + (ring - s0));
-        const float mine_m = m == -INFINITY ? 0.f : m;
+        float* sums = reinterpret_cast<float*>(sm + (ring - s0)) + r * kPitch + side * kD;
+        sum_l[half * 2u + side][r] = p >= 0 ? l : 0.f;  // padding sees nothing
+        if (side == 0u) sum_m[half][r] = m == -INFINITY ? 0.f : m;
+        named_barrier_sync(3, kSoftmax);
         if (half == 1u) {
-            half_m[r] = mine_m;
-            half_l[r] = p >= 0 ? l : 0.f;
 #pragma unroll
-            for (uint32_t d = 0; d < HD; d += 4u)
-                *reinterpret_cast<float4*>(sums + r * kPitch + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+            for (uint32_t d = 0; d < kD; d += 4u)
+                *reinterpret_cast<float4*>(sums + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
         }
-        named_barrier_sync(1, 256);
+        named_barrier_sync(3, kSoftmax);
+        const float l0 = sum_l[0][r] + sum_l[1][r], l1 = sum_l[2][r] + sum_l[3][r];
+        const float top = l0 == 0.f ? sum_m[1][r] : l1 == 0.f ? sum_m[0][r] : fmaxf(sum_m[0][r], sum_m[1][r]);
+        const float f0 = l0 == 0.f ? 0.f : exp2_fast(sum_m[0][r] - top), f1 = l1 == 0.f ? 0.f : exp2_fast(sum_m[1][r] - top);
+        const float sum = l0 * f0 + l1 * f1;
         if (half == 0u) {
-            const float l0 = p >= 0 ? l : 0.f, l1 = half_l[r], m1 = half_m[r];  // padding sees nothing
-            const float top = l0 == 0.f ? m1 : l1 == 0.f ? mine_m : fmaxf(mine_m, m1);
-            const float f0 = l0 == 0.f ? 0.f : exp2_fast(mine_m - top), f1 = l1 == 0.f ? 0.f : exp2_fast(m1 - top);
-            const float sum = l0 * f0 + l1 * f1;
             const float scale = a.direct && sum != 0.f ? 1.f / sum : 1.f;
 #pragma unroll
-            for (uint32_t d = 0; d < HD; d += 4u) {
+            for (uint32_t d = 0; d < kD; d += 4u) {
                 float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (l1 != 0.f) x = *reinterpret_cast<const float4*>(sums + r * kPitch + d);
+                if (l1 != 0.f) x = *reinterpret_cast<const float4*>(sums + d);
                 if (l1 != 0.f) x = make_float4(x.x * f1, x.y * f1, x.z * f1, x.w * f1);
                 if (l0 != 0.f)
                     x = make_float4(fmaf(acc[d], f0, x.x), fmaf(acc[d + 1], f0, x.y), fmaf(acc[d + 2], f0, x.z),
                                     fmaf(acc[d + 3], f0, x.w));
-                *reinterpret_cast<float4*>(sums + r * kPitch + d) =
-                    make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
+                *reinterpret_cast<float4*>(sums + d) = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
             }
-            half_m[r] = top - kUp;
-            half_l[r] = sum;
         }
-        named_barrier_sync(1, 256);
+        const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+        if (ok && half == 0u && side == 0u && !a.direct && p != -2)
+            a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]] =
+                make_float2(top - kUp, sum);
+        named_barrier_sync(3, kSoftmax);
         if (ok) {
-            const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+            const float* all = reinterpret_cast<const float*>(sm + (ring - s0));
             const uint32_t hd4 = hd / 4u;
-            for (uint32_t x = tid; x < kRows * hd4; x += 256u) {
+            for (uint32_t x = tid; x < kRows * hd4; x += kSoftmax) {
                 const uint32_t rr = x / hd4, d = (x - rr * hd4) * 4u;
                 if (row_pos[rr] == -2) continue;
                 const size_t row = static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr];
                 float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
-                *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(sums + rr * kPitch + d);
-                if (!a.direct && d == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(half_m[rr], half_l[rr]);
+                *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(all + rr * kPitch + d);
             }
         }
     }

@@ -112,6 +112,23 @@ def test_large_scores(lib, cuda, type_):
 
 
 @pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,kv_heads", [(6, 2), (2, 2), (48, 2)])
+def test_very_negative_scores(lib, cuda, type_, heads, kv_heads):
+    """Every score far below zero, in rows that see nothing of some chunks: a chunk without weight
+    has no say in the row's maximum."""
+    d = dev(lib, cuda, type_, heads, kv_heads, 64, 16, q=[1, 30, 1, 1], kv=[900, 2600, 33, 40], shared=64, seed=35)
+    d.s.queries = -np.abs(d.s.queries) - 1
+    d.q.copy_(cuda.from_numpy(d.s.queries))
+    for sq in range(4):
+        for i in range(-(-d.s.kv[sq] // 16)):
+            d.s.k[d.s.table[sq, i]] = np.abs(d.s.k[d.s.table[sq, i]]) + 1
+    d.k.copy_(cuda.from_numpy(d.s.k))
+    d.s.scale = 3.0
+    check_attention(d.s, d.attention(), d.s.attention())
+    check_attention(d.s, d.attention(500), d.s.attention(500))
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 3e4, 1e30])
 def test_query_sizes(lib, cuda, type_, size):
     """Queries far from 1 (the scale brings the scores back), and rows with one large channel."""
