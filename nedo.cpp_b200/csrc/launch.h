@@ -283,6 +283,7 @@ struct PagedAttention {
     // plan: keys per work item and work items per row tile of each part
     uint32_t own_chunk = 0, own_chunks = 0, prefix_chunk = 0, prefix_chunks = 0;
     uint32_t few_chunk = 0, few_chunks = 0;  // own part of sequences with few rows, where others have many
+    bool own_cluster = false, few_cluster = false;  // a row tile's chunks are added within a cluster
     uint64_t workspace = 0;          // bytes
 };
 // false: more work items than one launch holds.  Plans for the 148 SMs of a B200, so

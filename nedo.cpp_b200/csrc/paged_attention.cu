@@ -28,7 +28,7 @@ constexpr uint32_t kThreads = 128;
 size_t simt_smem(uint32_t hd) { return (kRows + 2u * kTile) * static_cast<size_t>(hd + 4u) * sizeof(float); }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
+__device__ __forceinline__ void attention_simt(const AttnArgs& a) {
     extern __shared__ __align__(16) float sm[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
@@ -226,13 +226,15 @@ __global__ void __launch_bounds__(kThreads) attention_simt_kernel(AttnArgs a) {
     }
 }
 
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_constant__ AttnArgs a) {
+    attention_simt<T>(a);
+    end_after_previous(a);
+}
+
 cudaError_t launch_simt(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    const size_t smem = simt_smem(a.kv.head_dim);
-    auto* kernel = a.kv.type == kF16 ? attention_simt_kernel<__half> : attention_simt_kernel<float>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-    kernel<<<static_cast<uint32_t>(items), kThreads, smem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_items(a, a.kv.type == kF16 ? attention_simt_kernel<__half> : attention_simt_kernel<float>, items, kThreads,
+                        simt_smem(a.kv.head_dim), stream, a);
 }
 
 // ---- adding a row's chunks ---------------------------------------------------
@@ -362,32 +364,35 @@ struct Cost {
     uint32_t slots;      // work items that run at once on 148 SMs
     uint32_t max_chunk;  // keys an item can take (0: any number)
     double ns_per_key, ns_fixed;
+    double least;        // share of ns_per_key that an item takes on its own
 };
 Cost cost_of(Kernel k, const PagedKv& kv) {
     const uint32_t hd = kv.head_dim;
     switch (k) {
         case Kernel::kFew: {  // reads 4 hd bytes per key of the SMs' common 6.5 TB/s
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
-            return {kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0};
+            return {kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
         case Kernel::kMany: {  // 64 rows through the tensor cores, two items to an SM
             const uint32_t slots = 148u * (hd <= 128u ? 2u : 1u);
-            return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0};
+            return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0, 1.0};
         }
         case Kernel::kTc:  // 128 rows through 32 MMAs per 128 keys, an item to an SM
-            return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 5000.0};
+            return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 5000.0, 1.0};
         case Kernel::kFew32: {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
-            return {kFewRows, slots, 1024u, 8.0 * hd * slots / 6500.0, 4000.0};
+            return {kFewRows, slots, 1024u, 8.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
-        default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0};
+        default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0, 1.0};
     }
 }
 
 // Keys per work item, a multiple of 64 and of the page size: of the chunkings that fill
 // one, two, ... rounds of items the one with the least estimated time, the fixed cost of an
 // item and the bytes of the chunks' sums counted.
-uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c) {
+// `cluster`: up to kMaxCluster chunks of a row tile can be added within a cluster, without the
+// combining kernel.
+uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c, bool cluster) {
     const uint64_t step = std::max(64u, kv.page_size);
     if (keys <= step) return static_cast<uint32_t>(step);
     auto rounded = [&](uint64_t n) { return ((keys + n - 1u) / n + step - 1u) / step * step; };
@@ -399,14 +404,18 @@ uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const Pag
         n = (keys + chunk - 1u) / chunk;
         const double rounds = static_cast<double>((units * n + c.slots - 1u) / c.slots);
         // a chunk's sums are written once and read once at about half the copy rate
-        const double ns = rounds * (static_cast<double>(chunk) * c.ns_per_key + c.ns_fixed) +
-                          (n > 1u ? 2000.0 + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0 : 0.0);
+        // few items do not share the memory's rate, but one alone has only its own copies in flight
+        const double busy = std::min(1.0, static_cast<double>(units * n) / c.slots);
+        const double ns = rounds * (static_cast<double>(chunk) * c.ns_per_key * std::max(busy, c.least) + c.ns_fixed) +
+                          (n == 1u                          ? 0.0
+                           : cluster && n <= kMaxCluster ? 1000.0
+                                                         : 4000.0 + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0);
         if (best == 0u || ns < best_ns) {
             best = chunk;
             best_ns = ns;
         }
     };
-    consider(1);
+    for (uint64_t n = 1; n <= (cluster ? kMaxCluster : 1u); ++n) consider(n);
     for (uint64_t rounds = 1; rounds <= 12u; ++rounds) {
         const uint64_t n = rounds * c.slots / units;
         if (n > 1u) consider(std::min<uint64_t>(n, (keys + step - 1u) / step));
@@ -460,7 +469,7 @@ bool plan_paged_attention(PagedAttention* a) {
     if (shared != 0u) {
         const Cost c = cost_of(prefix_kernel(*a), a->kv);
         prefix_units = ceil_div(all, c.rows) * a->kv.kv_heads;
-        a->prefix_chunk = chunk_keys(shared, prefix_units, sums, a->kv, c);
+        a->prefix_chunk = chunk_keys(shared, prefix_units, sums, a->kv, c, false);
         a->prefix_chunks = static_cast<uint32_t>(ceil_div(shared, a->prefix_chunk));
     }
     const uint64_t most = a->picks ? static_cast<uint64_t>(a->picks) << a->kv.page_shift
@@ -473,17 +482,21 @@ bool plan_paged_attention(PagedAttention* a) {
         const uint64_t n = ceil_div(keys, chunk);
         return static_cast<uint32_t>(std::max<uint64_t>(n * chunk < most ? n + 1u : n, 1u));
     };
-    const Cost c = cost_of(own_kernel(*a), a->kv);
+    const Kernel own = own_kernel(*a);
+    const Cost c = cost_of(own, a->kv);
     units = (a->picks ? a->b.tokens * ceil_div(group, c.rows) : own_tiles(*a, c.rows)) * a->kv.kv_heads;
-    a->own_chunk = chunk_keys(keys, units, sums, a->kv, c);
+    const bool alone = shared == 0u;
+    a->own_chunk = chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(own));
     a->own_chunks = chunks(a->own_chunk);
-    uint64_t grid = units * a->own_chunks, slots = a->own_chunks;
-    if (!takes_few(own_kernel(*a)) && a->b.seqs > 1u) {
+    a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
+    uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
+    if (!takes_few(own) && a->b.seqs > 1u) {
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads;
-        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv));
+        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv), alone);
         a->few_chunks = chunks(a->few_chunk);
+        a->few_cluster = alone && a->few_chunks > 1u && a->few_chunks <= kMaxCluster;
         grid = std::max(grid, u * a->few_chunks);
-        slots = std::max<uint64_t>(slots, a->few_chunks);
+        if (!a->few_cluster) slots = std::max<uint64_t>(slots, a->few_chunks);
     }
     slots += a->prefix_chunks;
     a->workspace = slots == 1u ? 0u : slots * sums;
@@ -507,10 +520,11 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     a.picks = p.picks;
     a.st = st;
     a.rows_to = kNone;
-    const uint64_t slots = static_cast<uint64_t>(std::max(p.own_chunks, p.few_chunks)) + p.prefix_chunks;
+    const uint64_t slots = std::max(p.own_cluster ? 1u : p.own_chunks, p.few_cluster ? 1u : p.few_chunks) +
+                           static_cast<uint64_t>(p.prefix_chunks);
     const uint64_t rows = static_cast<uint64_t>(p.b.tokens) * p.heads;
-    const bool own_direct = p.prefix_chunks == 0u && p.own_chunks == 1u;
-    const bool few_direct = p.prefix_chunks == 0u && p.few_chunks <= 1u;
+    const bool own_direct = p.prefix_chunks == 0u && (p.own_chunks == 1u || p.own_cluster);
+    const bool few_direct = p.prefix_chunks == 0u && (p.few_chunks <= 1u || p.few_cluster);
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = reinterpret_cast<float2*>(a.part_o + slots * rows * p.kv.head_dim);
     cudaError_t e = cudaSuccess;
@@ -523,11 +537,13 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         const uint64_t all = static_cast<uint64_t>(p.b.tokens) * a.group;
         e = launch_part(k, a, ceil_div(all, cost_of(k, p.kv).rows), all, stream);
         if (e != cudaSuccess) return e;
+        a.late = 1u;
     }
     a.chunk = p.own_chunk;
     a.chunks = p.own_chunks;
     a.slot0 = p.prefix_chunks;
     a.direct = own_direct;
+    a.cluster = p.own_cluster;
     const Kernel k = own_kernel(p);
     const uint32_t tile = cost_of(k, p.kv).rows;
     if (p.picks) {
@@ -548,6 +564,8 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
             a.chunk = p.few_chunk;
             a.chunks = p.few_chunks;
             a.direct = few_direct;
+            a.cluster = p.few_cluster;
+            a.late = 1u;
             e = launch_part(p.kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a, p.b.seqs, kFewRows, stream);
         }
     }

@@ -19,7 +19,9 @@ struct AttnArgs {
     uint32_t shared_len;     // keys of the shared prefix
     uint32_t chunk, chunks;  // keys per item, items per row tile
     uint32_t slot0;          // first partial slot of this part
-    uint32_t direct;         // one item per row: write out
+    uint32_t direct;         // one item, or one cluster of items, per row: write out
+    uint32_t cluster;        // few-rows kernels: a row tile's chunks are the CTAs of a cluster
+    uint32_t late;           // launched while another part's kernel may still run
     float* part_o;           // [slots][tokens * heads][head_dim]
     float2* part_ml;         // [slots][tokens * heads]
     uint32_t tiles;          // many-rows kernel: row tiles of the launch
@@ -98,6 +100,7 @@ __device__ __forceinline__ void checked_list(const uint32_t* __restrict__ l, uin
 }
 
 constexpr uint32_t kFewRows = 8;
+constexpr uint32_t kMaxCluster = 8;  // chunks that a cluster can hold
 // The work item of a few-rows CTA: its row tile (into shared memory: token, head and
 // position of each row, position -2 where there is none) and its keys.
 struct FewItem {
@@ -183,15 +186,47 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     return true;
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// This CTA's shared address in CTA `rank` of the cluster, and loads from there.
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 load2_cluster(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load4_cluster(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
 // The warps' sums of a few-rows CTA (part [warp][row][pitch], maxima wm and weight sums wl
-// in shared memory) added in warp order and written out, or to the chunk's place.
+// in shared memory) added in warp order and written out, or to the chunk's place, or, where
+// the row tile's chunks are a cluster, into shared memory behind `part`: there every CTA adds
+// a share of the rows' channels over the chunks, in chunk order, and writes it out.
 template <uint32_t WARPS>
 __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const uint32_t* row_tok, const uint32_t* row_head,
                                            const int* row_pos, const float (*wm)[kFewRows], const float (*wl)[kFewRows],
-                                           const float* part, uint32_t pitch) {
-    const uint32_t tid = threadIdx.x, hd = a.kv.head_dim;
+                                           float* part, uint32_t pitch) {
+    __shared__ float2 chunk_ml[kFewRows];
+    const uint32_t tid = threadIdx.x, hd = a.kv.head_dim, hd4 = hd / 4u;
     const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-    const uint32_t hd4 = hd / 4u;
+    float* const mine = part + WARPS * kFewRows * pitch;  // cluster: [row][hd]
     for (uint32_t i = tid; i < kFewRows * hd4; i += blockDim.x) {
         const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
         if (row_pos[r] == -2) continue;
@@ -213,7 +248,10 @@ __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const 
             o.w = fmaf(x.w, f, o.w);
         }
         const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
-        if (a.direct) {
+        if (a.cluster) {
+            *reinterpret_cast<float4*>(mine + r * hd + d) = o;
+            if (d == 0u) chunk_ml[r] = make_float2(top, sum);
+        } else if (a.direct) {
             const bool none = sum == 0.f;
             *reinterpret_cast<float4*>(a.out + row * hd + d) =
                 none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
@@ -222,6 +260,79 @@ __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const 
             if (d == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(top, sum);
         }
     }
+    if (!a.cluster) return;
+    cluster_sync();
+    const uint32_t n = a.chunks, ml_addr = smem_addr(chunk_ml), o_addr = smem_addr(mine);
+    for (uint32_t i = cluster_rank() * blockDim.x + tid; i < kFewRows * hd4; i += n * blockDim.x) {
+        const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
+        if (row_pos[r] == -2) continue;
+        float2 ml[kMaxCluster];
+        float4 x[kMaxCluster];
+        float top = -INFINITY;
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxCluster; ++k) {
+            ml[k] = make_float2(0.f, 0.f);
+            x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n) {
+                ml[k] = load2_cluster(map_rank(ml_addr + r * 8u, k));
+                x[k] = load4_cluster(map_rank(o_addr + (r * hd + d) * 4u, k));
+            }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxCluster; ++k)
+            if (ml[k].y != 0.f) top = fmaxf(top, ml[k].x);
+        float sum = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxCluster; ++k) {
+            if (ml[k].y == 0.f) continue;
+            const float f = exp2f(ml[k].x - top);
+            sum = fmaf(ml[k].y, f, sum);
+            o.x = fmaf(x[k].x, f, o.x);
+            o.y = fmaf(x[k].y, f, o.y);
+            o.z = fmaf(x[k].z, f, o.z);
+            o.w = fmaf(x[k].w, f, o.w);
+        }
+        const bool none = sum == 0.f;
+        *reinterpret_cast<float4*>(a.out + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd + d) =
+            none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
+    }
+    cluster_sync();  // no CTA leaves while another still reads its sums
+}
+
+// The last step of every CTA: a launch that may overlap the part before it (a.late) ends
+// after that part, whatever its CTAs found to do, because what runs next reads both.
+__device__ __forceinline__ void end_after_previous(const AttnArgs& a) {
+    if (a.late) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// A launch with a cluster of a.chunks CTAs where a.cluster says so, and, where a.late, while
+// the kernel before it may still be running (which then ends before this one does).
+template <typename... Args>
+cudaError_t launch_items(const AttnArgs& a, void (*kernel)(Args...), uint64_t items, uint32_t threads, size_t smem,
+                         cudaStream_t stream, Args... args) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<uint32_t>(items));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    uint32_t n = 0;
+    if (a.cluster) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = a.chunks;
+        attr[n].val.clusterDim.y = 1;
+        attr[n++].val.clusterDim.z = 1;
+    }
+    if (a.late) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // The few-rows kernels, up to kFewRows query rows per tile: F16 caches on the tensor cores

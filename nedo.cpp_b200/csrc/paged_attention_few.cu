@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
 }
 
 template <uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(AttnArgs a) {
+__device__ __forceinline__ void attention_few(const AttnArgs& a) {
     using F = Few<HD>;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ uint32_t row_tok[kFewRows], row_head[kFewRows];
@@ -248,12 +248,14 @@ __global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(AttnArgs a) 
 }
 
 template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(const __grid_constant__ AttnArgs a) {
+    attention_few<HD>(a);
+    end_after_previous(a);
+}
+
+template <uint32_t HD>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(attention_few_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(Few<HD>::kSmem));
-    if (e != cudaSuccess) return e;
-    attention_few_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Few<HD>::kSmem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_items(a, attention_few_kernel<HD>, items, kThreads, Few<HD>::kSmem, stream, a);
 }
 
 }  // namespace

@@ -61,7 +61,7 @@ __device__ __forceinline__ float exchange(float a, float b, bool up, uint32_t ma
 }
 
 template <uint32_t HD, uint32_t R>
-__global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) attention_few32_kernel(AttnArgs a) {
+__device__ __forceinline__ void attention_few32(const AttnArgs& a) {
     using F = Few32<HD>;
     constexpr uint32_t kD = F::kDims;
     constexpr uint32_t kGroup = R < 4u ? R : 4u;   // rows whose sums are exchanged together
@@ -265,12 +265,14 @@ __global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) attention_few32_k
 }
 
 template <uint32_t HD, uint32_t R>
+__global__ void __launch_bounds__(kThreads, HD == 256 ? 1 : 2) attention_few32_kernel(const __grid_constant__ AttnArgs a) {
+    attention_few32<HD, R>(a);
+    end_after_previous(a);
+}
+
+template <uint32_t HD, uint32_t R>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(attention_few32_kernel<HD, R>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(Few32<HD>::kSmem));
-    if (e != cudaSuccess) return e;
-    attention_few32_kernel<HD, R><<<static_cast<uint32_t>(items), kThreads, Few32<HD>::kSmem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_items(a, attention_few32_kernel<HD, R>, items, kThreads, Few32<HD>::kSmem, stream, a);
 }
 
 template <uint32_t HD>

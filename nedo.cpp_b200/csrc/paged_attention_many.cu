@@ -38,7 +38,7 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
 }
 
 template <uint32_t HD>
-__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many_kernel(AttnArgs a) {
+__device__ __forceinline__ void attention_many(const AttnArgs& a) {
     using M = Many<HD>;
     constexpr uint32_t kKeys = M::kKeys, kGroups = kKeys / 16u, kCols = kKeys / 8u;
     extern __shared__ __align__(128) uint8_t sm[];
@@ -395,12 +395,14 @@ __global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many_ke
 }
 
 template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, HD <= 128 ? 2 : 1) attention_many_kernel(const __grid_constant__ AttnArgs a) {
+    attention_many<HD>(a);
+    end_after_previous(a);
+}
+
+template <uint32_t HD>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(attention_many_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(Many<HD>::kSmem));
-    if (e != cudaSuccess) return e;
-    attention_many_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Many<HD>::kSmem, stream>>>(a);
-    return cudaGetLastError();
+    return launch_items(a, attention_many_kernel<HD>, items, kThreads, Many<HD>::kSmem, stream, a);
 }
 
 }  // namespace

@@ -124,8 +124,7 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
 }
 
 template <uint32_t HD>
-__global__ void __launch_bounds__(kThreads, 1)
-    attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_shift) {
+__device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs& a, uint32_t box_shift) {
     using T = Tc<HD>;
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
@@ -142,6 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t c = rest % a.chunks;
     rest /= a.chunks;
 
+    // what follows on the stream may come up where there is room (it waits for this kernel)
+    if (tid == 0u) asm volatile("griddepcontrol.launch_dependents;");
     // ---- the item: rows and keys
     uint32_t s = 0, r0 = 0, nrows, t0 = 0;
     PagedSeq sq{0u, 0u, 0u};
@@ -529,7 +530,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         // the halves meet: the odd tiles' sums through shared memory (the ring is done with)
-        asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
         constexpr uint32_t kPitch = HD + 4u;
         float* sums = reinterpret_cast<float*>(sm + (ring - s0)) + r * kPitch + side * kD;
         sum_l[half * 2u + side][r] = p >= 0 ? l : 0.f;  // padding sees nothing
@@ -584,6 +584,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
+template <uint32_t HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_shift) {
+    attention_tc<HD>(maps, a, box_shift);
+    end_after_previous(a);
+}
+
 bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows) {
     EncodeTiled encode = encode_tiled_fn();
     if (!encode) return false;
@@ -601,11 +608,8 @@ cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
     const uint32_t box_rows = std::min(a.kv.page_size, kKeys);
     if (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows))
         return cudaErrorInvalidValue;
-    cudaError_t e = cudaFuncSetAttribute(attention_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(Tc<HD>::kSmem));
-    if (e != cudaSuccess) return e;
-    attention_tc_kernel<HD><<<static_cast<uint32_t>(items), kThreads, Tc<HD>::kSmem, stream>>>(maps, a, std::min(a.kv.page_shift, 7u));
-    return cudaGetLastError();
+    return launch_items(a, attention_tc_kernel<HD>, items, kThreads, Tc<HD>::kSmem, stream, maps, a,
+                        std::min(a.kv.page_shift, 7u));
 }
 
 }  // namespace
