@@ -107,14 +107,10 @@ __device__ __forceinline__ void attention_simt(const AttnArgs& a) {
             kb = min(kb, first_key(row_pos[r], a.window));
             ke = max(ke, static_cast<uint32_t>(row_pos[r]) + 1u);
         }
-        uint32_t base = 0, first = 0;
-        if (a.part == kPartOwn) {
-            base = a.shared_len;
-            first = own_first_chunk(sq, a.window, base, a.chunk);
-        } else {
-            ke = min(ke, a.shared_len);
-        }
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        uint32_t base = 0;
+        if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
+        else ke = min(ke, a.shared_len);
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
         kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
         if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
         if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
@@ -283,9 +279,9 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
             e0 = (min(hi, a.shared_len) + a.prefix_chunk - 1u) / a.prefix_chunk;
         }
         if (hi > a.shared_len) {
-            const uint32_t first = own_first_chunk(sq, a.window, a.shared_len, chunk);
-            b1 = a.prefix_chunks + (max(lo, a.shared_len) - a.shared_len) / chunk - first;
-            e1 = a.prefix_chunks + (hi - 1u - a.shared_len) / chunk + 1u - first;
+            const uint32_t begin = own_begin(sq, a.window, a.shared_len);
+            b1 = a.prefix_chunks + (max(lo, begin) - begin) / chunk;
+            e1 = a.prefix_chunks + (hi - 1u - begin) / chunk + 1u;
         }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -381,7 +377,7 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 5000.0, 1.0};
         case Kernel::kFew32: {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
-            return {kFewRows, slots, 1024u, 8.0 * hd * slots / 6500.0, 4000.0, 0.45};
+            return {kFewRows, slots, 2048u, 8.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
         default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0, 1.0};
     }
@@ -475,13 +471,10 @@ bool plan_paged_attention(PagedAttention* a) {
     const uint64_t most = a->picks ? static_cast<uint64_t>(a->picks) << a->kv.page_shift
                                    : (a->b.max_kv_len > shared ? a->b.max_kv_len - shared : 0u);
     uint64_t keys = most;
-    if (!a->picks && a->window != 0u) keys = std::min<uint64_t>(keys, static_cast<uint64_t>(a->window) + a->b.max_q_len - 1u);
-    // chunks of at most `chunk` keys that a row tile's keys touch: a window that starts
-    // inside a chunk reaches one chunk further
-    auto chunks = [&](uint64_t chunk) {
-        const uint64_t n = ceil_div(keys, chunk);
-        return static_cast<uint32_t>(std::max<uint64_t>(n * chunk < most ? n + 1u : n, 1u));
-    };
+    // with a window the chunks begin up to 63 keys in front of it
+    if (!a->picks && a->window != 0u)
+        keys = std::min<uint64_t>(keys, static_cast<uint64_t>(a->window) + a->b.max_q_len - 1u + 63u);
+    auto chunks = [&](uint64_t chunk) { return static_cast<uint32_t>(std::max<uint64_t>(ceil_div(keys, chunk), 1u)); };
     const Kernel own = own_kernel(*a);
     const Cost c = cost_of(own, a->kv);
     units = (a->picks ? a->b.tokens * ceil_div(group, c.rows) : own_tiles(*a, c.rows)) * a->kv.kv_heads;

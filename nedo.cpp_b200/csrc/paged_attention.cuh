@@ -32,11 +32,12 @@ struct AttnArgs {
     DeviceStatus* st;
 };
 
-// First chunk of sequence `sq` that any of its rows sees (own part).
-__device__ __forceinline__ uint32_t own_first_chunk(const PagedSeq& sq, uint32_t window, uint32_t base, uint32_t chunk) {
+// Where the chunks of sequence `sq`'s own part begin: at the first key that any of its rows
+// sees, rounded down to 64 keys from `base`.
+__device__ __forceinline__ uint32_t own_begin(const PagedSeq& sq, uint32_t window, uint32_t base) {
     const int p0 = sq.pos(0) > 0 ? sq.pos(0) : 0;
     const uint32_t lo = first_key(p0, window);
-    return lo > base ? (lo - base) / chunk : 0u;
+    return lo > base ? base + ((lo - base) & ~63u) : base;
 }
 
 // One warp: the sequence and the tile within it that tile number `want` is, when every
@@ -170,14 +171,10 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
         kb = e0 << a.kv.page_shift;
         ke = e1 << a.kv.page_shift;
     } else {
-        uint32_t base = 0, first = 0;
-        if (a.part == kPartOwn) {
-            base = a.shared_len;
-            first = own_first_chunk(sq, a.window, base, a.chunk);
-        } else {
-            ke = min(ke, a.shared_len);
-        }
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        uint32_t base = 0;
+        if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
+        else ke = min(ke, a.shared_len);
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
         kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
         if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
         if (kb >= ke && !a.direct) return false;  // no row of the tile sees a key of this chunk

@@ -75,22 +75,26 @@ __device__ __forceinline__ void attention_few32(const AttnArgs& a) {
     FewItem it;
     if (!few_setup(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t kb = it.kb, ke = it.ke, kh = it.kh;
-    // this warp's tiles: tile i starts at key j0 + 8 (4 i + warp); lane i holds its page and
-    // the position of its first key
+    // this warp's tiles: tile i starts at key j0 + 8 (4 i + warp); lane i holds the pages of
+    // tiles i and i + 32 and the positions of their first keys
     const uint32_t j0 = kb & ~(kKeys - 1u);
     const uint32_t ntiles_all = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
     const uint32_t ntiles = ntiles_all > warp ? (ntiles_all - warp + kWarps - 1u) / kWarps : 0u;
-    uint32_t my_page = kNone, my_pos = 0;
-    if (lane < ntiles) {
-        const uint32_t j = j0 + kKeys * (kWarps * lane + warp);
+    uint32_t my_page[2] = {kNone, kNone}, my_pos[2] = {0u, 0u};
+#pragma unroll
+    for (uint32_t u = 0; u < 2u; ++u) {
+        if (lane + 32u * u >= ntiles) continue;
+        const uint32_t j = j0 + kKeys * (kWarps * (lane + 32u * u) + warp);
         const uint32_t lp = a.part == kPartBlocks ? list[j >> a.kv.page_shift] : j >> a.kv.page_shift;
         if (lp != kNone) {
-            my_pos = (lp << a.kv.page_shift) + (j & (a.kv.page_size - 1u));
+            my_pos[u] = (lp << a.kv.page_shift) + (j & (a.kv.page_size - 1u));
             // a list's last page may reach beyond the sequence
-            if (a.part != kPartBlocks || my_pos <= static_cast<uint32_t>(row_pos[0]))
-                my_page = load_page(a.b, a.kv, it.s, lp, a.st);
+            if (a.part != kPartBlocks || my_pos[u] <= static_cast<uint32_t>(row_pos[0]))
+                my_page[u] = load_page(a.b, a.kv, it.s, lp, a.st);
         }
     }
+    auto page_of = [&](uint32_t i) { return __shfl_sync(0xFFFFFFFFu, i < 32u ? my_page[0] : my_page[1], i & 31u); };
+    auto pos_of = [&](uint32_t i) { return __shfl_sync(0xFFFFFFFFu, i < 32u ? my_pos[0] : my_pos[1], i & 31u); };
     uint8_t* my_ring = ring + warp * kStages * F::kStageBytes;
     const uint32_t ring_addr = smem_addr(my_ring);
     if (hd < HD) {  // channels beyond the head stay zero
@@ -103,7 +107,7 @@ __device__ __forceinline__ void attention_few32(const AttnArgs& a) {
     const float* vbase = static_cast<const float*>(a.kv.v);
     auto fetch = [&](uint32_t i) {
         if (i < ntiles) {
-            const uint32_t page = __shfl_sync(0xFFFFFFFFu, my_page, i), pos = __shfl_sync(0xFFFFFFFFu, my_pos, i);
+            const uint32_t page = page_of(i), pos = pos_of(i);
             const uint32_t dst = ring_addr + (i % kStages) * F::kStageBytes;
             const size_t off = ((static_cast<size_t>(page == kNone ? 0u : page) * a.kv.kv_heads + kh) * a.kv.page_size +
                                 (pos & (a.kv.page_size - 1u))) * hd;
@@ -156,7 +160,7 @@ __device__ __forceinline__ void attention_few32(const AttnArgs& a) {
         __syncwarp();
         const uint8_t* ks = my_ring + (t % kStages) * F::kStageBytes;
         const uint8_t* vs = ks + F::kTileBytes;
-        const uint32_t page = __shfl_sync(0xFFFFFFFFu, my_page, t), pos = __shfl_sync(0xFFFFFFFFu, my_pos, t);
+        const uint32_t page = page_of(t), pos = pos_of(t);
         const bool whole = page != kNone && pos >= it.all_b && pos + kKeys <= it.all_e;
         float sc[kVals];
 #pragma unroll

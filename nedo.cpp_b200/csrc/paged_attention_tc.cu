@@ -193,14 +193,10 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         }
         kb = __reduce_min_sync(0xFFFFFFFFu, lo);
         ke = __reduce_max_sync(0xFFFFFFFFu, hi);
-        uint32_t base = 0, first = 0;
-        if (a.part == kPartOwn) {
-            base = a.shared_len;
-            first = own_first_chunk(sq, a.window, base, a.chunk);
-        } else {
-            ke = min(ke, a.shared_len);
-        }
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(first + c) * a.chunk;
+        uint32_t base = 0;
+        if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
+        else ke = min(ke, a.shared_len);
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
         kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
         if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
         if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
