@@ -10,9 +10,9 @@
 // every number.
 //
 // Bound by reading the pages' bounds (4 hd bytes of an F16 cache per page and KV head).  A
-// cluster of CTAs takes one token and KV head, its warps eight pages at a time with the next
-// eight pages' loads in flight; the halves of a page's bounds lie next to each other, so a
-// lane takes 16 bytes of them with its own factors in registers.
+// cluster of CTAs takes one token and KV head, its warps eight pages at a time through a ring of
+// their own (cp.async, two stages); the halves of a page's bounds lie next to each
+// other, so a lane takes 16 bytes of them, its own copy, with its own factors in registers.
 //
 // The scores are first formed in 32 bits, with a bound on what that can be off: every sum of
 // n terms is n + 13 roundings (in the factors, the products, the sums along a lane and across
@@ -25,13 +25,15 @@
 #include <algorithm>
 
 #include "paged.cuh"
+#include "paged_mma.cuh"
 
 namespace nedo_gpu {
 namespace {
 
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kThreads = 128;
 constexpr uint32_t kWarps = kThreads / 32u;
 constexpr uint32_t kGroup = 8;  // pages a warp scores at once
+constexpr uint32_t kOpen = 64;  // pages that are scored again in 64 bits at most
 
 // Order-preserving 64-bit key of a score: 0 is kept for "no page", NaN is 1.
 __device__ __forceinline__ uint64_t score_key(double v) {
@@ -48,16 +50,24 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// A store, and a maximum, at `addr` of the first CTA's shared memory.
-__device__ __forceinline__ void store_first(uint32_t addr, uint32_t v) {
+// A store, and a maximum, union and intersection of bits, at `addr` of the first CTA's shared
+// memory.
+__device__ __forceinline__ uint32_t first_cta(uint32_t addr) {
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(addr));
+    return remote;
+}
+__device__ __forceinline__ void store_first(uint32_t remote, uint32_t v) {
     asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
 }
-__device__ __forceinline__ void max_first(uint32_t addr, uint32_t v) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(addr));
+__device__ __forceinline__ void max_first(uint32_t remote, uint32_t v) {
     asm volatile("red.shared::cluster.max.u32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+__device__ __forceinline__ void or_first(uint32_t remote, uint32_t v) {
+    asm volatile("red.shared::cluster.or.b32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
+}
+__device__ __forceinline__ void and_first(uint32_t remote, uint32_t v) {
+    asm volatile("red.shared::cluster.and.b32 [%0], %1;" ::"r"(remote), "r"(v) : "memory");
 }
 
 // A 16-byte piece of the bounds: its values, and the largest magnitude among them and `top`
@@ -125,79 +135,64 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
     return v + before;
 }
 
-// The `left`-th largest of key[0..n) (one CTA), to `shift` bits: *prefix holds its bits from
-// `shift` up, and the first return value how many of the keys that share them are to be taken.
-// Stops early where the keys that share them are all taken, unless the key is wanted whole.
+// The `left`-th largest of key[0..n) (one CTA): its bits from *shift up, in *prefix, and how
+// many of the keys that share them are still to be taken (returned).  All keys share the bits
+// outside `differ`; *prefix comes with those.  Stops where at most `few` keys share the bits.
 template <typename K>
-__device__ uint32_t find_largest(const K* key, uint32_t n, uint32_t left, bool whole, K* prefix_out, int* shift_out,
-                                 uint32_t* hist, uint32_t* warp_sums, uint32_t* found, K (*masks)[kWarps]) {
+__device__ uint32_t find_largest(const K* key, uint32_t n, uint32_t left, uint32_t few, uint64_t differ, K* prefix, int* shift,
+                                 uint32_t* hist, uint32_t* warp_sums, uint32_t* found) {
     constexpr int kBits = 8 * sizeof(K);
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    K any = 0, every = ~static_cast<K>(0);
-    for (uint32_t i = tid; i < n; i += kThreads) {
-        any |= key[i];
-        every &= key[i];
-    }
-    for (int o = 16; o > 0; o >>= 1) {
-        any |= __shfl_xor_sync(0xFFFFFFFFu, any, o);
-        every &= __shfl_xor_sync(0xFFFFFFFFu, every, o);
-    }
-    __syncthreads();
-    if (lane == 0u) {
-        masks[0][warp] = any;
-        masks[1][warp] = every;
-    }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t w = 0; w < kWarps; ++w) {
-        any |= masks[0][w];
-        every &= masks[1][w];
-    }
-    const uint64_t differ = any ^ every;
-    int shift = differ ? 64 - __clzll(static_cast<long long>(differ)) : 0;  // all keys share the bits from here up
-    K prefix = shift < kBits ? any >> shift << shift : 0;
-    bool done = shift == 0;  // all keys are the same
+    const uint32_t tid = threadIdx.x;
+    int at = differ ? 64 - __clzll(static_cast<long long>(differ)) : 0;
+    K bits = at < kBits ? *prefix >> at << at : 0;
+    bool done = at == 0 || n <= few;
     while (!done) {
-        const int next = max(0, shift - 8);
-        const uint32_t mask = (1u << (shift - next)) - 1u;
+        const int next = max(0, at - 8);
+        const uint32_t mask = (1u << (at - next)) - 1u;
         uint32_t total;
-        hist[tid] = 0u;
+        hist[2u * tid] = hist[2u * tid + 1u] = 0u;
         __syncthreads();
         for (uint32_t i = tid; i < n; i += kThreads) {
             const K k = key[i];
-            if (shift == kBits || (k >> shift) == (prefix >> shift))
-                atomicAdd(&hist[static_cast<uint32_t>(k >> next) & mask], 1u);
+            if (at == kBits || (k >> at) == (bits >> at)) atomicAdd(&hist[static_cast<uint32_t>(k >> next) & mask], 1u);
         }
         __syncthreads();
-        const uint32_t mine = hist[255u - tid];  // bins from the top
-        const uint32_t upto = block_scan(mine, warp_sums, &total);
-        if (upto >= left && upto - mine < left) {
-            found[0] = 255u - tid;
-            found[1] = left - (upto - mine);
+        const uint32_t high = hist[255u - 2u * tid], low = hist[254u - 2u * tid];  // two bins, from the top
+        const uint32_t upto = block_scan(high + low, warp_sums, &total), before = upto - high - low;
+        if (upto >= left && before < left) {
+            const bool first = before + high >= left;
+            found[0] = 255u - 2u * tid - (first ? 0u : 1u);
+            found[1] = left - before - (first ? 0u : high);
+            found[2] = first ? high : low;
         }
         __syncthreads();
-        prefix |= static_cast<K>(found[0]) << next;
+        bits |= static_cast<K>(found[0]) << next;
         left = found[1];
-        shift = next;
-        done = shift == 0 || (!whole && hist[found[0]] == left);
+        at = next;
+        done = at == 0 || found[2] <= few;
         __syncthreads();
     }
-    *prefix_out = prefix;
-    *shift_out = shift;
+    *prefix = bits;
+    *shift = at;
     return left;
 }
 
-// PIECES: 16-byte pieces of a page's bounds per lane.
+constexpr uint32_t kStages = 2;  // three run no faster: fewer CTAs fit (48 tokens x 4 heads: 26.2 us with two, 27.2 with three)
+
+// PIECES: 16-byte pieces of a page's bounds per lane.  Dynamic shared memory: key_words words of
+// 64 bits for the keys, then the warps' rings.
 template <typename T, uint32_t PIECES>
 __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, PagedBatch b, uint32_t heads,
                                                                 const float* __restrict__ q, uint32_t picks,
                                                                 uint32_t* __restrict__ blocks, uint32_t cluster,
-                                                                DeviceStatus* st) {
+                                                                uint32_t key_words, DeviceStatus* st) {
     using P = Piece<T>;
+
     extern __shared__ __align__(16) uint64_t key64[];
     uint32_t* const key = reinterpret_cast<uint32_t*>(key64);
-    __shared__ uint32_t hist[256], warp_sums[kWarps], found[2], top_bits, cand[256], cands;
-    __shared__ uint64_t masks[2][kWarps], cand_key[256];
+    __shared__ uint32_t hist[256], warp_sums[kWarps], found[3], top_bits, any_bits, all_bits, cand[kOpen], cands;
+    __shared__ uint64_t cand_key[kOpen], masks[2][kWarps];
+    __shared__ double factor[2][256];
     const uint32_t unit = blockIdx.x / cluster, rank = cluster_rank();
     const uint32_t t = unit / kv.kv_heads, kh = unit % kv.kv_heads, tid = threadIdx.x;
     const uint32_t warp = tid >> 5, lane = tid & 31u, hd = kv.head_dim, group = heads / kv.kv_heads;
@@ -214,12 +209,44 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
         return;
     }
     if (tid == 0u) {
-        top_bits = 0u;
-        cands = 0u;
+        top_bits = any_bits = cands = 0u;
+        all_bits = 0xFFFFFFFFu;
     }
     cluster_arrive();  // the first CTA runs, and has set these, before anything is stored into its memory
-    // this lane's factors: of its pieces of the bounds (lowest values first, then highest)
+    // the n - 1 pages in front of the token's own one, whose page is always taken
+    const uint32_t others = n - 1u, stride = cluster * kWarps * kGroup;
     const uint32_t half_pieces = hd / P::kCount;
+    const uint4* bounds = static_cast<const uint4*>(kv.bounds);
+    // group k of this warp: pages i0 + k * stride .. + 7.  Lane 8 g + j holds the id of page j of
+    // group 4 m + g (now) and of group 4 m + 4 + g (then).
+    const uint32_t i0 = (rank * kWarps + warp) * kGroup, ng = i0 < others ? (others - i0 + stride - 1u) / stride : 0u;
+    auto look_up = [&](uint32_t m) {
+        const uint32_t k = 4u * m + (lane >> 3), i = i0 + k * stride + (lane & 7u);
+        return k < ng && i < others ? load_page(b, kv, s, i, st) : kNone;
+    };
+    uint4* const ring = reinterpret_cast<uint4*>(key64 + key_words) + warp * kStages * kGroup * PIECES * 32u;
+    uint32_t now = look_up(0), then = look_up(1), top = 0u;
+    auto fetch = [&](uint32_t k, uint32_t m) {
+        if (k < ng) {
+            const uint32_t ids = k >> 2 == m ? now : then;
+#pragma unroll
+            for (uint32_t j = 0; j < kGroup; ++j) {
+                const uint32_t page = __shfl_sync(0xFFFFFFFFu, ids, (k & 3u) * 8u + j);
+#pragma unroll
+                for (uint32_t i = 0; i < PIECES; ++i) {
+                    const bool there = page != kNone && lane + 32u * i < 2u * half_pieces;
+                    const size_t at = (static_cast<size_t>(there ? page : 0u) * kv.kv_heads + kh) * 2u * half_pieces +
+                                      (there ? lane + 32u * i : 0u);
+                    cp_async16(smem_addr(ring + (((k % kStages) * kGroup + j) * PIECES + i) * 32u + lane), bounds + at,
+                               there ? 16u : 0u);
+                }
+            }
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (uint32_t k = 0; k + 1u < kStages; ++k) fetch(k, 0u);
+    // this lane's factors: of its pieces of the bounds (lowest values first, then highest)
     const float* qh = q + (static_cast<size_t>(t) * heads + kh * group) * hd;
     float f[PIECES][P::kCount], size = 0.f;
 #pragma unroll
@@ -230,6 +257,7 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
         if (piece < 2u * half_pieces) {
             const bool high = piece >= half_pieces;
             const float* src = qh + (high ? piece - half_pieces : piece) * P::kCount;
+#pragma unroll 4
             for (uint32_t g = 0; g < group; ++g)
 #pragma unroll
                 for (uint32_t e = 0; e < P::kCount; e += 4u) {
@@ -244,52 +272,28 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
         for (uint32_t e = 0; e < P::kCount; ++e) size += fabsf(f[i][e]);
     }
     size = warp_sum(size);
-    // the n - 1 pages in front of the token's own one, whose page is always taken
-    const uint32_t others = n - 1u, stride = cluster * kWarps * kGroup;
-    const uint4* bounds = static_cast<const uint4*>(kv.bounds);
-    auto look_up = [&](uint32_t i0) {
-        return lane < kGroup && i0 + lane < others ? load_page(b, kv, s, i0 + lane, st) : kNone;
-    };
-    // with one piece per lane there are registers for the next group's loads to be in flight
-    // while this one is added up
-    constexpr bool kAhead = PIECES == 1u;
-    uint4 x[kGroup][PIECES], ahead[kGroup][PIECES];
-    auto fetch = [&](uint32_t of) {  // of: the group's page ids, one per lane
-#pragma unroll
-        for (uint32_t j = 0; j < kGroup; ++j) {
-            const uint32_t page = __shfl_sync(0xFFFFFFFFu, of, j);
-#pragma unroll
-            for (uint32_t i = 0; i < PIECES; ++i) {
-                ahead[j][i] = make_uint4(0u, 0u, 0u, 0u);
-                if (page != kNone && lane + 32u * i < 2u * half_pieces)
-                    ahead[j][i] = __ldg(bounds + (static_cast<size_t>(page) * kv.kv_heads + kh) * 2u * half_pieces + lane + 32u * i);
-            }
-        }
-    };
-    uint32_t i0 = (rank * kWarps + warp) * kGroup;
-    uint32_t next = look_up(i0), pages = kNone, after = look_up(i0 + stride), top = 0u;
-    if (kAhead) fetch(next);
+    const uint32_t key_addr = first_cta(smem_addr(key));
+    uint32_t any = 0u, every = 0xFFFFFFFFu;
     bool waited = false;
-    for (; i0 < others; i0 += stride) {
-        if (!kAhead) fetch(next);
-#pragma unroll
-        for (uint32_t j = 0; j < kGroup; ++j)
-#pragma unroll
-            for (uint32_t i = 0; i < PIECES; ++i) x[j][i] = ahead[j][i];
-        pages = next;
-        next = after;
-        if (kAhead && i0 + stride < others) fetch(next);
-        after = look_up(i0 + 2u * stride);
+    for (uint32_t k = 0; k < ng; ++k) {
+        const uint32_t first = i0 + k * stride, pages = __shfl_sync(0xFFFFFFFFu, now, (k & 3u) * 8u + (lane >> 2));
+        fetch(k + kStages - 1u, k >> 2);
+        if ((k & 3u) == 3u) {
+            now = then;
+            then = look_up((k >> 2) + 2u);
+        }
+        cp_wait<kStages - 1>();
         float v[kGroup];
 #pragma unroll
         for (uint32_t j = 0; j < kGroup; ++j) {
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (uint32_t i = 0; i < PIECES; ++i) {
-                P::magnitude(x[j][i], &top);
+                const uint4 x = ring[(((k % kStages) * kGroup + j) * PIECES + i) * 32u + lane];  // this lane's own copy
+                P::magnitude(x, &top);
 #pragma unroll
                 for (uint32_t e = 0; e < P::kCount / 2u; ++e)
-                    sum = ffma2(P::pair(x[j][i], e), make_float2(f[i][2u * e], f[i][2u * e + 1u]), sum);
+                    sum = ffma2(P::pair(x, e), make_float2(f[i][2u * e], f[i][2u * e + 1u]), sum);
             }
             v[j] = sum.x + sum.y;
         }
@@ -301,39 +305,55 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
         float z = exchange(y[0], y[1], lane & 4u, 4u);  // page lane / 4
         z += __shfl_xor_sync(0xFFFFFFFFu, z, 2);
         z += __shfl_xor_sync(0xFFFFFFFFu, z, 1);
-        const uint32_t mine = __shfl_sync(0xFFFFFFFFu, pages, lane >> 2);
         if (!waited) {
             cluster_wait();
             waited = true;
         }
-        // a page that is none: below all others
-        if ((lane & 3u) == 0u && i0 + (lane >> 2) < others)
-            store_first(smem_addr(key + i0 + (lane >> 2)), mine != kNone ? key_of(z == 0.f ? 0.f : z) : 0u);
+        if ((lane & 3u) == 0u && first + (lane >> 2) < others) {
+            const uint32_t x = pages != kNone ? key_of(z == 0.f ? 0.f : z) : 0u;  // a page that is none: below all others
+            store_first(key_addr + 4u * (first + (lane >> 2)), x);
+            any |= x;
+            every &= x;
+        }
         __syncwarp();
     }
     if (!waited) cluster_wait();
-    // the largest magnitude of all bounds, as a number's bits
+    // the largest magnitude of all bounds, as a number's bits, and the bits of the keys
     const uint32_t largest = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(P::largest(top)));
-    if (lane == 0u) max_first(smem_addr(&top_bits), largest);
+    any = __reduce_or_sync(0xFFFFFFFFu, any);
+    every = __reduce_and_sync(0xFFFFFFFFu, every);
+    if (lane == 0u) {
+        max_first(first_cta(smem_addr(&top_bits)), largest);
+        or_first(first_cta(smem_addr(&any_bits)), any);
+        and_first(first_cta(smem_addr(&all_bits)), every);
+    }
     cluster_arrive();
     if (rank != 0u) return;
     cluster_wait();
 
-    // a page's score in 64 bits, by one warp
-    auto exact_key = [&](uint32_t i) -> uint64_t {
-        const uint32_t page = load_page(b, kv, s, i, st);
-        if (page == kNone) return 0ull;
-        const T* lo = static_cast<const T*>(kv.bounds) + (static_cast<size_t>(page) * kv.kv_heads + kh) * 2u * hd;
-        double z = 0.0;
-        for (uint32_t d = lane; d < hd; d += 32u) {
+    // a page's score in 64 bits, by one warp, from the factors in shared memory
+    auto factors = [&]() {
+        for (uint32_t d = tid; d < hd; d += kThreads) {
             double up = 0.0, down = 0.0;
+#pragma unroll 4
             for (uint32_t g = 0; g < group; ++g) {
                 const double y = qh[static_cast<size_t>(g) * hd + d];
                 if (y < 0.0) down += y;
                 else up += y;
             }
-            z += up * static_cast<double>(kv_float(lo[hd + d])) + down * static_cast<double>(kv_float(lo[d]));
+            factor[0][d] = down;
+            factor[1][d] = up;
         }
+        __syncthreads();
+    };
+    auto exact_key = [&](uint32_t i) -> uint64_t {
+        const uint32_t page = load_page(b, kv, s, i, st);
+        if (page == kNone) return 0ull;
+        const T* lo = static_cast<const T*>(kv.bounds) + (static_cast<size_t>(page) * kv.kv_heads + kh) * 2u * hd;
+        double z = 0.0;
+#pragma unroll 4
+        for (uint32_t d = lane; d < hd; d += 32u)
+            z += factor[1][d] * static_cast<double>(kv_float(lo[hd + d])) + factor[0][d] * static_cast<double>(kv_float(lo[d]));
         for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, o);
         return score_key(z);
     };
@@ -342,90 +362,120 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
     // what a score can be off, rounded up (nothing where all of them are zero)
     const float most = size * __uint_as_float(top_bits) * 1.01f;
     const float off = most == 0.f ? 0.f : (PIECES * P::kCount + group + 13u) * 6.0e-8f * most + 1e-37f;
-    uint32_t prefix = 0, total, sure = 0, left = 0;
-    int shift = 0;
-    bool all64 = !(most < INFINITY);
-    float above = 0.f, below = 0.f;
-    if (!all64) {
-        left = find_largest<uint32_t>(key, others, want, true, &prefix, &shift, hist, warp_sums, found,
-                                      reinterpret_cast<uint32_t(*)[kWarps]>(masks));
-        if (off > 0.f && prefix != 0u) {
-            // the pages that 32 bits leave open
-            above = number_of(prefix) + 2.f * off;
-            below = number_of(prefix) - 2.f * off;
+    // a thread's share of the pages, in order
+    const uint32_t run = (others + kThreads - 1u) / kThreads, a0 = min(others, tid * run), a1 = min(others, a0 + run);
+    uint32_t total;
+    if (most < INFINITY && off > 0.f) {
+        uint32_t prefix = any_bits;
+        int shift;
+        find_largest<uint32_t>(key, others, want, 1u, any_bits ^ all_bits, &prefix, &shift, hist,
+                                                     warp_sums, found);
+        // the threshold lies between these; pages above are taken, below not, the others are open
+        const uint32_t high = prefix | (shift < 32 ? (1u << shift) - 1u : 0xFFFFFFFFu);
+        if (prefix != 0u && high < 0xFF800000u) {
+            float above = number_of(high) + 2.f * off, below = number_of(prefix) - 2.f * off;
             above += fabsf(above) * 2.4e-7f;  // these sums round too
             below -= fabsf(below) * 2.4e-7f;
-            uint32_t taken = 0;
-            for (uint32_t i = tid; i < others; i += kThreads) {
-                const uint32_t k = key[i];
-                if (k == 0u) continue;
-                const float z = number_of(k);
+            uint32_t taken = 0, which = 0;  // which: of the thread's first 32 pages
+            for (uint32_t i = a0; i < a1; ++i) {
+                const float z = number_of(key[i]);
                 if (z > above) {
                     ++taken;
+                    if (i - a0 < 32u) which |= 1u << (i - a0);
                 } else if (z >= below) {
                     const uint32_t c = atomicAdd(&cands, 1u);
-                    if (c < 256u) cand[c] = i;
+                    if (c < kOpen) cand[c] = i;
                 }
             }
-            block_scan(taken, warp_sums, &sure);
+            const uint32_t before = block_scan(taken, warp_sums, &total) - taken;
             __syncthreads();
-            left = want - sure;
-            all64 = cands > 256u;
-            if (!all64 && cands > left) {
-                const uint32_t count = cands;
-                for (uint32_t c = warp; c < count; c += kWarps) {
-                    const uint64_t k = exact_key(cand[c]);
-                    if (lane == 0u) cand_key[c] = k;
-                }
-                __syncthreads();
-                // those that `left` others beat are not taken
-                if (tid < count) {
-                    const uint64_t mine = cand_key[tid];
-                    const uint32_t at = cand[tid];
+            const uint32_t left = want - total, count = cands;
+            if (count <= kOpen) {
+                if (count > left) {
+                    factors();
+                    for (uint32_t c = warp; c < count; c += kWarps) {
+                        const uint64_t k = exact_key(cand[c]);
+                        if (lane == 0u) cand_key[c] = k;
+                    }
+                    __syncthreads();
+                    // those that `left` others beat are not taken
                     uint32_t better = 0;
-                    for (uint32_t c = 0; c < count; ++c)
-                        better += cand_key[c] > mine || (cand_key[c] == mine && cand[c] < at);
-                    if (better >= left) key[at] = 0u;
+                    if (tid < count)
+                        for (uint32_t c = 0; c < count; ++c)
+                            better += cand_key[c] > cand_key[tid] || (cand_key[c] == cand_key[tid] && cand[c] < cand[tid]);
+                    __syncthreads();
+                    if (tid < count && better >= left) cand[tid] = kNone;
+                    __syncthreads();
                 }
-                __syncthreads();
+                // in page order: a page comes behind the taken ones in front of it
+                uint32_t in = before;
+                auto put = [&](uint32_t i) {
+                    uint32_t open = 0;
+                    for (uint32_t c = 0; c < count; ++c) open += cand[c] < i;
+                    out[in + open] = i;
+                    ++in;
+                };
+                for (uint32_t m = which; m != 0u; m &= m - 1u) put(a0 + __ffs(m) - 1u);
+                for (uint32_t i = a0 + 32u; i < a1; ++i)
+                    if (number_of(key[i]) > above) put(i);
+                // an open page that is taken: its thread counts the certain ones in front of it
+                for (uint32_t c = 0; c < count; ++c) {
+                    const uint32_t i = cand[c];
+                    if (i == kNone || i < a0 || i >= a1) continue;
+                    uint32_t at = before;
+                    for (uint32_t k = a0; k < i; ++k) at += number_of(key[k]) > above;
+                    for (uint32_t k = 0; k < count; ++k) at += cand[k] < i;
+                    out[at] = i;
+                }
+                if (tid == 0u) out[want] = n - 1u;  // the token's own page
+                return;
             }
         }
     }
-    uint64_t prefix64 = 0;
-    if (all64) {
-        for (uint32_t i = warp; i < others; i += kWarps) {
-            const uint64_t k = exact_key(i);
-            if (lane == 0u) key64[i] = k;
-        }
-        __syncthreads();
-        left = find_largest<uint64_t>(key64, others, want, false, &prefix64, &shift, hist, warp_sums, found, masks);
+    if (most == 0.f && all_bits == any_bits) {  // all scores are zero: the first pages
+        for (uint32_t i = tid; i < picks; i += kThreads) out[i] = i < want ? i : n - 1u;
+        return;
     }
-    // in page order: the pages that are taken for certain (2), and the first `left` of those that
-    // share the threshold (1)
-    const bool bounded = !all64 && off > 0.f && prefix != 0u;
-    auto rank_of = [&](uint32_t i) -> uint32_t {
-        if (all64) {
-            if (shift == 64) return 1u;
-            const uint64_t x = key64[i] >> shift, y = prefix64 >> shift;
-            return x > y ? 2u : x == y ? 1u : 0u;
-        }
-        const uint32_t k = key[i];
-        if (bounded) return k != 0u && number_of(k) >= below ? 2u : 0u;
-        return k > prefix ? 2u : k == prefix ? 1u : 0u;
-    };
-    const uint32_t run = (others + kThreads - 1u) / kThreads, a0 = min(others, tid * run), a1 = min(others, a0 + run);
-    uint32_t count = 0;  // taken in the low half, sharing in the high half (at most 16384 each)
-    for (uint32_t i = a0; i < a1; ++i) {
-        const uint32_t c = rank_of(i);
-        count += c == 2u ? 1u : c == 1u ? 0x10000u : 0u;
+    // all scores in 64 bits
+    factors();
+    for (uint32_t i = warp; i < others; i += kWarps) {
+        const uint64_t k = exact_key(i);
+        __syncwarp();
+        if (lane == 0u) key64[i] = k;
     }
+    __syncthreads();
+    uint64_t any64 = 0, every64 = ~0ull;
+    for (uint32_t i = tid; i < others; i += kThreads) {
+        any64 |= key64[i];
+        every64 &= key64[i];
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+        any64 |= __shfl_xor_sync(0xFFFFFFFFu, any64, o);
+        every64 &= __shfl_xor_sync(0xFFFFFFFFu, every64, o);
+    }
+    if (lane == 0u) {
+        masks[0][warp] = any64;
+        masks[1][warp] = every64;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w) {
+        any64 |= masks[0][w];
+        every64 &= masks[1][w];
+    }
+    uint64_t prefix = any64;
+    int shift;
+    const uint32_t left = find_largest<uint64_t>(key64, others, want, 0u, any64 ^ every64, &prefix, &shift, hist, warp_sums, found);
+    // in page order: the keys above it, and the first `left` of those that equal it
+    uint32_t count = 0;  // above in the low half, equal in the high half (at most 16384 each)
+    for (uint32_t i = a0; i < a1; ++i) count += key64[i] > prefix ? 1u : key64[i] == prefix ? 0x10000u : 0u;
     const uint32_t before = block_scan(count, warp_sums, &total) - count;
     uint32_t in = before & 0xFFFFu, same = before >> 16;
     for (uint32_t i = a0; i < a1; ++i) {
-        const uint32_t c = rank_of(i);
-        if (c == 2u || (c == 1u && same < left)) out[in + min(same, left)] = i;
-        in += c == 2u;
-        same += c == 1u;
+        const bool above = key64[i] > prefix, equal = key64[i] == prefix;
+        if (above || (equal && same < left)) out[in + min(same, left)] = i;
+        in += above;
+        same += equal;
     }
     if (tid == 0u) out[want] = n - 1u;  // the token's own page
 }
@@ -434,15 +484,16 @@ template <typename T, uint32_t PIECES>
 cudaError_t launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* q, uint32_t picks,
                    uint32_t* blocks, DeviceStatus* st, cudaStream_t stream) {
     const uint32_t pages = (b.max_kv_len + kv.page_size - 1u) >> kv.page_shift;
-    const size_t smem = static_cast<size_t>(pages) * sizeof(uint64_t) + 16u;
+    const uint32_t key_words = (pages + 1u) & ~1u;
+    const size_t smem = key_words * sizeof(uint64_t) + kWarps * kStages * kGroup * PIECES * 512u;
     cudaError_t e = cudaFuncSetAttribute(block_select_kernel<T, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;
-    // CTAs per token and KV head: enough for two to an SM, each with pages for its warps (48
-    // tokens x 4 heads x up to 1024 pages: 51 us with one, 47 with two, 50 with four, 67 with eight)
+    // CTAs per token and KV head: as many as run at once on 148 SMs, with pages for every warp
     const uint64_t units = static_cast<uint64_t>(b.tokens) * kv.kv_heads;
+    const uint64_t at_once = 148u * (224u * 1024u / (smem + 8192u));
     uint32_t cluster = 1;
-    while (cluster < 8u && units * cluster < 2u * 148u && pages > cluster * kWarps * kGroup) cluster *= 2u;
+    while (cluster < 8u && units * (cluster + 1u) <= at_once && pages > cluster * kWarps * kGroup) ++cluster;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<uint32_t>(units * cluster));
     cfg.blockDim = dim3(kThreads);
@@ -455,7 +506,8 @@ cudaError_t launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, block_select_kernel<T, PIECES>, kv, b, heads, q, picks, blocks, cluster, st);
+    return cudaLaunchKernelEx(&cfg, block_select_kernel<T, PIECES>, kv, b, heads, q, picks, blocks, cluster,
+                              key_words, st);
 }
 
 }  // namespace
