@@ -9,13 +9,16 @@
 // nothing that matters at any position (32 bits are 1e-3 of a turn off at position
 // 10^5), and the sine and cosine of the remaining fraction are taken in 32 bits.
 //
-// One launch with two kinds of CTAs.  The first take one page that the call writes and
-// one KV head: keys, and the page's channel bounds, whose minimum and maximum over the new
-// tokens need them in one place (16 bytes of a token per thread, the tokens of the page
-// spread over the thread groups, one round of loads for a page of 64).  The others take
-// one or four token rows: all query heads and the values, with the rows' sines and
-// cosines computed once for all heads.  Bound by the copies, and for single tokens by the
-// launch and three dependent loads.
+// One launch with two kinds of CTAs, bound by the copies, and for single tokens by the launch
+// and three dependent loads.
+//   * Rows: a CTA takes one or four token rows and up to 256 pieces of 16 bytes of each (a
+//     piece pair of a query head, a piece of a value), one per thread, so that a thread's loads
+//     are all on their way before the first is used, and before the rows' sequences and pages
+//     are known; their sines and cosines are computed once for the CTA.
+//   * Keys, where a sequence can have several new tokens: a CTA takes one page that the call
+//     writes and one KV head, because the minimum and maximum of the page's channels over the
+//     new tokens need them in one place (the tokens spread over the thread groups, one round of
+//     loads for a page of 64).  With one token per sequence they are pieces of its row.
 #include "paged.cuh"
 
 namespace nedo_gpu {
@@ -32,7 +35,9 @@ struct AppendArgs {
     uint32_t heads, rotate;
     uint32_t segs;      // pages that a sequence's new tokens can touch
     uint32_t key_ctas;  // CTAs of the first kind
-    uint32_t rows;      // token rows of a CTA of the second kind
+    uint32_t rows;      // token rows of a CTA of the other kind
+    uint32_t pieces, blocks;  // 16-byte pieces (pairs) of a row, and CTAs that share them
+    uint32_t row_keys;  // the keys are pieces of their rows
     DeviceStatus* st;
 };
 
@@ -149,14 +154,30 @@ __device__ void append_keys(const AppendArgs& a, float4* sums) {
     }
 }
 
-// The query heads and the values of a.rows token rows.
-template <typename T>
+// One piece of ROWS token rows per thread: of the query heads, of the keys (a.row_keys), of the
+// values.
+template <typename T, uint32_t ROWS>
 __device__ void append_rows(const AppendArgs& a, float2 (*cs)[128]) {
     __shared__ int row_pos[kMaxRows];
     __shared__ uint32_t row_page[kMaxRows];
-    const uint32_t t0 = (blockIdx.x - a.key_ctas) * a.rows, tid = threadIdx.x, nt = blockDim.x;
-    const uint32_t hd = a.kv.head_dim, half = hd / 2u, kvh = a.kv.kv_heads;
-    if (tid < a.rows) {
+    const uint32_t item = blockIdx.x - a.key_ctas, t0 = item / a.blocks * ROWS, tid = threadIdx.x, nt = blockDim.x;
+    const uint32_t hd = a.kv.head_dim, half = hd / 2u, kvh = a.kv.kv_heads, quads = half / 4u;
+    const uint32_t piece = item % a.blocks * nt + tid, turned = (a.heads + (a.row_keys ? kvh : 0u)) * quads;
+    const bool turns = piece < turned, there = piece < a.pieces;
+    // where the piece is in its row: a pair of pieces half a head apart, or one of the values
+    const uint32_t h = piece / quads, d = (piece - h * quads) * 4u;
+    const uint32_t off = turns ? h * hd + d : (a.heads + kvh) * hd + (piece - turned) * 4u;
+    const size_t width = static_cast<size_t>(a.heads + 2u * kvh) * hd;
+    float4 x[ROWS], y[ROWS];
+#pragma unroll
+    for (uint32_t r = 0; r < ROWS; ++r) {
+        x[r] = y[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!there || t0 + r >= a.b.tokens) continue;
+        const float* src = a.qkv + (t0 + r) * width + off;
+        x[r] = __ldg(reinterpret_cast<const float4*>(src));
+        if (turns) y[r] = __ldg(reinterpret_cast<const float4*>(src + half));
+    }
+    if (tid < ROWS) {
         int p = -1;
         uint32_t page = kNone;
         if (t0 + tid < a.b.tokens) {
@@ -172,36 +193,48 @@ __device__ void append_rows(const AppendArgs& a, float2 (*cs)[128]) {
     }
     __syncthreads();
     if (a.rotate) {
-        // rows innermost: a thread's pairs, and with them the frequencies, stay the same
-        for (uint32_t i = tid; i < half; i += nt) {
-            const double turns = turns_of(a, i);
-            for (uint32_t r = 0; r < a.rows; ++r)
-                if (row_pos[r] >= 0) cs[r][i] = rotation(row_pos[r], turns);
+        for (uint32_t i = tid; i < half * ROWS; i += nt) {
+            const uint32_t r = i / half, k = i - r * half;
+            if (row_pos[r] >= 0) cs[r][k] = rotation(row_pos[r], turns_of(a, k));
         }
         __syncthreads();
     }
-    const uint32_t quads = half / 4u, qn = a.heads * quads, vn = kvh * hd / 4u;
-    const size_t width = static_cast<size_t>(a.heads + 2u * kvh) * hd;
-    for (uint32_t i = tid; i < a.rows * (qn + vn); i += nt) {
-        const uint32_t r = i / (qn + vn), k = i - r * (qn + vn);
+    if (!there) return;
+#pragma unroll
+    for (uint32_t r = 0; r < ROWS; ++r) {
         const int p = row_pos[r];
         if (p < 0) continue;
-        const float* row = a.qkv + (t0 + r) * width;
-        if (k < qn) {
-            const uint32_t h = k / quads, d = (k - h * quads) * 4u;
-            float4 x = *reinterpret_cast<const float4*>(row + h * hd + d);
-            float4 y = *reinterpret_cast<const float4*>(row + h * hd + d + half);
-            if (a.rotate) rotate4(x, y, &cs[r][d]);
+        if (turns && a.rotate) rotate4(x[r], y[r], &cs[r][d]);
+        if (piece < a.heads * quads) {
             float* o = a.q_out + (static_cast<size_t>(t0 + r) * a.heads + h) * hd + d;
-            *reinterpret_cast<float4*>(o) = x;
-            *reinterpret_cast<float4*>(o + half) = y;
+            *reinterpret_cast<float4*>(o) = x[r];
+            *reinterpret_cast<float4*>(o + half) = y[r];
         } else if (row_page[r] != kNone) {
-            const uint32_t e = (k - qn) * 4u, h = e / hd, d = e - h * hd;
-            float4 x = *reinterpret_cast<const float4*>(row + (a.heads + kvh) * hd + e);
-            store4(static_cast<T*>(a.kv.v) +
-                       ((static_cast<size_t>(row_page[r]) * kvh + h) * a.kv.page_size +
-                        (static_cast<uint32_t>(p) & (a.kv.page_size - 1u))) * hd + d,
-                   x);
+            const uint32_t e = (piece - turned) * 4u, kh = turns ? h - a.heads : e / hd;
+            const size_t head = static_cast<size_t>(row_page[r]) * kvh + kh;
+            const uint32_t slot = static_cast<uint32_t>(p) & (a.kv.page_size - 1u);
+            if (!turns) {
+                store4(static_cast<T*>(a.kv.v) + (head * a.kv.page_size + slot) * hd + (e - kh * hd), x[r]);
+                continue;
+            }
+            T* dst = static_cast<T*>(a.kv.k) + (head * a.kv.page_size + slot) * hd + d;
+            store4(dst, x[r]);
+            store4(dst + half, y[r]);
+            if (a.kv.bounds == nullptr) continue;
+            T* bo = static_cast<T*>(a.kv.bounds) + head * 2u * hd + d;
+#pragma unroll
+            for (uint32_t k = 0; k < 2u; ++k) {
+                const float4 v = k ? y[r] : x[r], none = make_float4(INFINITY, INFINITY, INFINITY, INFINITY);
+                const float4 least = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                T* o = bo + k * half;
+                float4 lo = min4(none, v), hi = max4(least, v);
+                if (slot != 0u) {  // a page whose first slot is written begins anew
+                    lo = min4(lo, make_float4(kv_float(o[0]), kv_float(o[1]), kv_float(o[2]), kv_float(o[3])));
+                    hi = max4(hi, make_float4(kv_float(o[hd]), kv_float(o[hd + 1]), kv_float(o[hd + 2]), kv_float(o[hd + 3])));
+                }
+                store4(o, lo);
+                store4(o + hd, hi);
+            }
         }
     }
 }
@@ -210,7 +243,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
     __shared__ __align__(16) uint8_t sm[256 * 4 * sizeof(float4)];
     if (blockIdx.x < a.key_ctas) append_keys<T>(a, reinterpret_cast<float4*>(sm));
-    else append_rows<T>(a, reinterpret_cast<float2(*)[128]>(sm));
+    else if (a.rows == 1u) append_rows<T, 1>(a, reinterpret_cast<float2(*)[128]>(sm));
+    else append_rows<T, kMaxRows>(a, reinterpret_cast<float2(*)[128]>(sm));
 }
 
 }  // namespace
@@ -226,14 +260,17 @@ cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t he
     a.log2_theta = a.rotate ? log2(theta) : 0.0;
     a.heads = heads;
     a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
-    a.rows = b.tokens >= 8u * 148u ? kMaxRows : 1u;
+    a.rows = b.tokens >= 4u * 148u ? kMaxRows : 1u;  // four rows share their sines where there are CTAs enough
+    a.row_keys = b.max_q_len <= 1u;
+    const uint32_t quads = kv.head_dim / 8u;
+    a.pieces = (heads + (a.row_keys ? kv.kv_heads : 0u)) * quads + kv.kv_heads * kv.head_dim / 4u;
+    a.blocks = (a.pieces + 255u) / 256u;
+    const uint32_t threads = ((a.pieces + a.blocks - 1u) / a.blocks + 31u) / 32u * 32u;
     a.st = st;
-    const uint64_t keys = static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
-    const uint64_t grid = keys + (b.tokens + a.rows - 1u) / a.rows;
+    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
+    const uint64_t grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
     if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     a.key_ctas = static_cast<uint32_t>(keys);
-    // a page's tokens want more thread groups than one token per sequence does
-    const uint32_t threads = b.max_q_len > 4u ? 256u : 128u;
     if (kv.type == kF16) kv_append_kernel<__half><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
     else kv_append_kernel<float><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
     return cudaGetLastError();
