@@ -8,18 +8,21 @@
 // them, so a tile's O starts from zero in TMEM and is added to the running sums in fp32
 // registers, together with the rescaling by 2^(m_old - m_new).
 //
-// Work.  A CTA (one per SM, 640 threads) takes 128 rows through their keys in tiles of 128:
-//   * warp 16 brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
+// Work.  A CTA (one per SM, 896 threads) takes 128 rows through their keys in tiles of 128:
+//   * one warp brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
 //     swizzle), in the order of their use, four half-tile slots deep.  Of a tile that the
 //     item's key range cuts it zeroes the values outside, whatever the pages hold there;
-//   * one thread of warp 17 issues the MMAs: Q K^T of tile i + 1 before P V of tile i, so the
-//     tensor core works while a softmax runs;
-//   * warps 0-7 take the even and warps 8-15 the odd tiles, two threads to a row, each with
-//     half of the tile's keys and half of the channels: they read S from TMEM, agree on the
-//     row's maximum, write the split weights over S (the A operand of P V), and add O to their
-//     running sums.  The even and the odd sums meet at the end in shared memory.
-// TMEM: two S/P and two O tiles of 128 columns each.  Registers: the softmax threads hold 64
-// sums each, so they take 104 registers and the other warps give theirs up.
+//   * one thread issues the MMAs: Q K^T three tiles ahead of P V;
+//   * warps 0-7 take the even and warps 8-15 the odd tiles, two threads to a row, each with half
+//     of the tile's keys: they read S from TMEM, agree on the row's maximum, and write the split
+//     weights over S (the A operand of P V);
+//   * warps 16-23 add every tile's O to the running sums, two threads to a row, each with half
+//     of the channels, rescaling both to the larger of the maxima they go by (the even and the
+//     odd tiles keep maxima of their own, so neither half waits for the other).
+// TMEM: three S/P tiles and one O tile of 128 columns each.  A softmax thread never waits for
+// its own P V, so the tensor core has work while weights are formed (with S/P and O twice each
+// and the sums kept by the softmax threads, a tile took 3900 cycles of which the MMAs are 2100).
+// Registers: 64 for the softmax, 96 for the sums, 56 for the others.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -31,10 +34,12 @@ namespace {
 constexpr uint32_t kRows = kTcRows;     // 128
 constexpr uint32_t kKeys = 128;         // keys per tile
 constexpr uint32_t kSlots = 4;          // ring slots: the keys or the values of one tile
-constexpr uint32_t kSoftmax = 512;      // softmax threads: four to a row
-constexpr uint32_t kThreads = kSoftmax + 128;
+constexpr uint32_t kSoftmax = 512;      // softmax threads: two to a row, for the even and the odd tiles
+constexpr uint32_t kSums = 256;         // threads of the running sums: two to a row
+constexpr uint32_t kThreads = kSoftmax + kSums + 128;
+constexpr uint32_t kBuffers = 3;        // S/P tiles
 constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
-constexpr uint32_t kLoadWarp = 16, kMmaWarp = 17;
+constexpr uint32_t kSumWarp = kSoftmax / 32u, kLoadWarp = kSumWarp + kSums / 32u, kMmaWarp = kLoadWarp + 1u;
 
 template <uint32_t HD>
 struct Tc {
@@ -129,9 +134,9 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float row_unscale[kRows], tile_max[4][kRows], sum_l[4][kRows], sum_m[2][kRows];
-    __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[2], p_full[2], o_full[2], done;
-    __shared__ uint32_t found[2], tmem_slot, gaps[4];
+    __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
+    __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
+    __shared__ uint32_t found[2], tmem_slot, gaps[8];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
     uint8_t* const sm = sm_raw + (s0 - smem_addr(sm_raw));
     const uint32_t q_addr = s0, ring = s0 + 2u * T::kTile;
@@ -210,11 +215,13 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             mbar_init(&empty[i], 1);
         }
         mbar_init(&cut, 1);
-        for (uint32_t i = 0; i < 2u; ++i) {
+        for (uint32_t i = 0; i < kBuffers; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 256);
-            mbar_init(&o_full[i], 1);
         }
+        mbar_init(&o_full, 1);
+        mbar_init(&o_empty, kSums);
+        mbar_init(&q_full, kSoftmax);
         mbar_init(&done, 1);
         fence_barrier_init();
     }
@@ -223,48 +230,18 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    if (tid < 256u) {  // a row per two threads: scaled, split, stored
-        const uint32_t r = tid >> 1;
-        const int p = row_pos[r];
-        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
-        float big = 0.f;
-        if (p >= 0)
-            for (uint32_t d = (tid & 1u) * 8u; d < hd; d += 16u)
-#pragma unroll
-                for (uint32_t e = 0; e < 8; e += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(q + d + e);
-                    big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
-                                           fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
-                }
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-        const int e2 = up_exponent(big);
-        const float up = power_of_two(e2);
-        if ((tid & 1u) == 0u) row_unscale[r] = power_of_two(-e2);
-        for (uint32_t d = (tid & 1u) * 8u; d < HD; d += 16u) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-                float2 x = make_float2(0.f, 0.f);
-                if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
-                split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
-            }
-            *reinterpret_cast<uint4*>(sm + at(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(sm + T::kTile + at(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
 
-    // Ring order: K0, K1, V0, K2, V1, ..., V(last): the order in which the MMAs use them.
-    auto k_at = [&](uint32_t i) { return i == 0u ? 0u : 2u * i - 1u; };
-    auto v_at = [&](uint32_t i) { return i + 1u < ntiles ? 2u * i + 2u : 2u * ntiles - 1u; };
+    // Ring order: K0, K1, K2, V0, K3, V1, ..., V(last): the order in which the MMAs use them.
+    auto k_at = [&](uint32_t i) { return i + (i > 2u ? i - 2u : 0u); };
+    auto v_at = [&](uint32_t i) { return i + min(ntiles, i + kBuffers); };
 
     if (warp >= kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kLoadWarp) {
             // ---- loads
             const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
@@ -289,7 +266,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 const bool patch = values && !whole;
                 uint64_t* bar = patch ? &cut : &full[slot];
                 if (lane == 0u) {
-                    if (!values) gaps[i & 3u] = want & ~there;
+                    if (!values) gaps[i & 7u] = want & ~there;
                     const uint32_t bytes = __popc(there) * T::kBlocks * box_bytes;
                     if (bytes != 0u) mbar_arrive_expect_tx(bar, bytes);
                     else mbar_arrive(bar);
@@ -319,16 +296,18 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 }
                 issued = n + 1u;
             };
-            uint32_t before = kNone, now = look_up(0), next = look_up(1);
-            for (uint32_t i = 0; i < ntiles && ok; ++i) {
+            // pages of the tiles whose keys come next and of those whose values do, three behind
+            uint32_t pages[4] = {look_up(0), kNone, kNone, kNone}, next = look_up(1);
+            for (uint32_t i = 0; i < ntiles + kBuffers && ok; ++i) {
                 const uint32_t after = look_up(i + 2u);
-                load(k_at(i), i, now, false);
-                if (i > 0u && ok) load(v_at(i - 1u), i - 1u, before, true);
-                before = now;
-                now = next;
+                if (i < ntiles) load(k_at(i), i, pages[0], false);
+                if (i >= 2u && i - 2u < ntiles && ok) load(v_at(i - 2u), i - 2u, pages[2], true);
+                pages[3] = pages[2];
+                pages[2] = pages[1];
+                pages[1] = pages[0];
+                pages[0] = next;
                 next = after;
             }
-            if (ntiles != 0u && ok) load(v_at(ntiles - 1u), ntiles - 1u, before, true);
             // the last copies into every slot have landed before the CTA ends
             for (uint32_t n = issued > kSlots ? issued - kSlots : 0u; n < issued; ++n)
                 mbar_wait_bounded(&full[n % kSlots], (n / kSlots) & 1u, a.st, 63u);
@@ -342,7 +321,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     ok = mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 64u);
                     if (!ok) return;
                     tc_fence_after();
-                    const uint32_t d = tmem + (i & 1u) * 128u;
+                    const uint32_t d = tmem + i % kBuffers * 128u;
 #pragma unroll
                     for (uint32_t half = 0; half < 2u; ++half)  // low halves first
 #pragma unroll
@@ -351,26 +330,28 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                             mma_ss(d, desc(q_addr + (half ? 0u : T::kTile) + off, 16u), desc(ring + slot * T::kTile + off, 16u),
                                    kS, half + k != 0u);
                         }
-                    tc_commit(&s_full[i & 1u]);
+                    tc_commit(&s_full[i % kBuffers]);
                     tc_commit(&empty[slot]);
                 };
-                if (ntiles != 0u) qk(0);
+                if (ntiles != 0u) ok = mbar_wait_bounded(&q_full, 0u, a.st, 71u);
+                for (uint32_t i = 0; i < kBuffers && i < ntiles && ok; ++i) qk(i);
                 for (uint32_t i = 0; i < ntiles && ok; ++i) {
-                    if (i + 1u < ntiles) qk(i + 1u);
                     const uint32_t n = v_at(i), slot = n % kSlots;
-                    ok = ok && mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 65u);
-                    ok = ok && mbar_wait_bounded(&p_full[i & 1u], (i >> 1) & 1u, a.st, 66u);
+                    ok = mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 65u) &&
+                         mbar_wait_bounded(&p_full[i % kBuffers], (i / kBuffers) & 1u, a.st, 66u) &&
+                         (i == 0u || mbar_wait_bounded(&o_empty, (i - 1u) & 1u, a.st, 72u));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t d = tmem + 256u + (i & 1u) * 128u, p = tmem + (i & 1u) * 128u;
+                    const uint32_t d = tmem + kBuffers * 128u, p = tmem + i % kBuffers * 128u;
 #pragma unroll
                     for (uint32_t half = 0; half < 2u; ++half)
 #pragma unroll
                         for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 + 8 columns of weights, 2048 bytes of values
                             mma_ts(d, p + k * 16u + (half ? 0u : 8u),
                                    desc(ring + slot * T::kTile + k * 2048u, kBlock), kO, half + k != 0u);
-                    tc_commit(&o_full[i & 1u]);
+                    tc_commit(&o_full);
                     tc_commit(&empty[slot]);
+                    if (i + kBuffers < ntiles) qk(i + kBuffers);
                 }
                 tc_commit(&done);  // every MMA issued above has completed when this arrives
                 mbar_wait_bounded(&done, 0u, a.st, 67u);
@@ -378,196 +359,232 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             __syncwarp();
         }
     } else {
-        // ---- softmax: tiles half, half + 2, ...; keys and channels of this side
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-        const uint32_t half = warp >> 3, side = (warp >> 2) & 1u, r = tid & 127u;
-        constexpr uint32_t kD = HD / 2u, kC = kKeys / 32u;  // channels and 16-key pieces of a side
+        const uint32_t r = tid & 127u, side = (warp >> 2) & 1u;
         const uint32_t lanes = tmem + ((warp & 3u) << 21);  // the warp's 32 TMEM lanes
-        const uint32_t st_addr = lanes + half * 128u + side * 64u, o_addr = lanes + 256u + half * 128u + side * kD;
         const int p = row_pos[r];
-        const float unscale = row_unscale[r];
         const uint32_t lo_key = p >= 0 ? first_key(p, a.window) : kNone, hi_key = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
         // keys that some / every row of the warp sees
         const uint32_t wb = __reduce_min_sync(0xFFFFFFFFu, lo_key), we = __reduce_max_sync(0xFFFFFFFFu, hi_key);
-        const uint32_t all_b = __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? lo_key : 0u);
-        const uint32_t all_e = __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? hi_key : kNone);
-        float acc[kD];
-#pragma unroll
-        for (uint32_t d = 0; d < kD; ++d) acc[d] = 0.f;
-        float m = -INFINITY, l = 0.f;
+        const uint32_t all_b = max(kb, __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? lo_key : 0u));
+        const uint32_t all_e = min(ke, __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? hi_key : kNone));
+        const uint32_t row_b = max(lo_key, kb), row_e = min(hi_key, ke);
+        // which of 16 keys from key 16 k of the tile at j on this row sees
+        auto seen = [&](uint32_t j, uint32_t gap, uint32_t k) -> uint32_t {
+            const uint32_t at = j + 16u * k, b = min(max(row_b, at) - at, 16u), e = min(max(row_e, at) - at, 16u);
+            return gap >> ((16u * k) >> box_shift) & 1u ? 0u : (0xFFFFu << b) & ((1u << e) - 1u);
+        };
         bool ok = true;
-        for (uint32_t i = half; i < ntiles && ok; i += 2u) {
-            const uint32_t ph = (i >> 1) & 1u, j = j0 + i * kKeys;
-            ok = mbar_wait_bounded(&s_full[half], ph, a.st, 68u);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            const bool mine = j < we && j + kKeys > wb;  // a tile that none of the warp's rows sees is passed over
-            float alpha = 1.f, ref = 0.f;
-            bool whole = true;
-            uint32_t gap = 0u;
-            // keys of the tile that this row sees: bits of 16 keys from key 16 k on
-            const uint32_t from = max(max(lo_key, kb), j) - j, to = min(min(hi_key, ke), j + kKeys) - min(j, min(hi_key, ke));
-            auto seen = [&](uint32_t k) -> uint32_t {
-                const uint32_t b = min(max(from, 16u * k) - 16u * k, 16u), e = min(max(to, 16u * k) - 16u * k, 16u);
-                return gap >> ((16u * k) >> box_shift) & 1u ? 0u : (0xFFFFu << b) & ((1u << e) - 1u);
-            };
-            auto mask = [&](uint32_t (&x)[16], uint32_t k) {
-                const uint32_t bits = seen(kC * side + k);
-#pragma unroll
-                for (uint32_t e = 0; e < 16u; ++e)
-                    if (!(bits >> e & 1u)) x[e] = 0xFF800000u;
-            };
-            if (mine) {
-                gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 3u]);
-                whole = gap == 0u && j >= max(all_b, kb) && j + kKeys <= min(all_e, ke);
-                float mt[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-                for (uint32_t k = 0; k < kC; k += 2u) {
-                    uint32_t x[2][16];
-                    tmem_load(st_addr + 16u * k, x[0]);
-                    tmem_load(st_addr + 16u * (k + 1u), x[1]);
-                    tmem_ready(x[0]);
-                    tmem_ready(x[1]);
-#pragma unroll
-                    for (uint32_t u = 0; u < 2u; ++u) {
-                        if (!whole) mask(x[u], k + u);
-#pragma unroll
-                        for (uint32_t e = 0; e < 16u; e += 2u)
-                            mt[(e >> 1) & 1u] =
-                                fmaxf(fmaxf(mt[(e >> 1) & 1u], __uint_as_float(x[u][e])), __uint_as_float(x[u][e + 1]));
+        if (warp < kSumWarp) {
+            // ---- softmax: tiles half, half + 2, ...; keys of this side
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+            const uint32_t half = warp >> 3;
+            constexpr uint32_t kC = kKeys / 32u;  // 16-key pieces of a side
+            {
+                // queries: a row per four threads, scaled, split, stored
+                const uint32_t rq = tid >> 2, part = tid & 3u;
+                const int pq = row_pos[rq];
+                const float* q = a.q + (static_cast<size_t>(row_tok[rq]) * a.heads + row_head[rq]) * hd;
+                float big = 0.f;
+                if (pq >= 0)
+                    for (uint32_t d = part * 4u; d < hd; d += 16u) {
+                        const float4 x = *reinterpret_cast<const float4*>(q + d);
+                        big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
+                                               fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
                     }
+                big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+                const int e2 = up_exponent(big);
+                const float up = power_of_two(e2);
+                if (part == 0u) row_unscale[rq] = power_of_two(-e2);
+                for (uint32_t d = part * 8u; d < HD; d += 32u) {
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e += 2) {
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (pq >= 0 && d < hd) x = *reinterpret_cast<const float4*>(q + d + 2u * e);
+                        split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
+                        split(x.z * a.scale_log2 * up, x.w * a.scale_log2 * up, &hi[e + 1u], &lo[e + 1u]);
+                    }
+                    *reinterpret_cast<uint4*>(sm + at(rq, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(sm + T::kTile + at(rq, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
-                tile_max[half * 2u + side][r] = fmaxf(mt[0], mt[1]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&q_full);
+                named_barrier_sync(3, kSoftmax);
             }
-            named_barrier_sync(1u + half, 256);
-            if (mine) {
-                const float mt = fmaxf(tile_max[half * 2u][r], tile_max[half * 2u + 1u][r]);
-                const float mn = fmaxf(m, mt * unscale);
-                alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
-                m = mn;
-                ref = (mn == -INFINITY ? 0.f : mn) - kUp;
-                float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                const float2 unscale2 = make_float2(unscale, unscale), ref2 = make_float2(-ref, -ref);
+            const float unscale = row_unscale[r];
+            float m = -INFINITY, l = 0.f;
+            for (uint32_t i = half; i < ntiles && ok; i += 2u) {
+                const uint32_t buf = i % kBuffers, j = j0 + i * kKeys, st_addr = lanes + buf * 128u + side * 64u;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[buf], (i / kBuffers) & 1u, a.st, 68u));
+                if (!ok) break;
+                tc_fence_after();
+                const bool mine = j < we && j + kKeys > wb;  // a tile that none of the warp's rows sees is passed over
+                const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 7u]);
+                const bool whole = gap == 0u && j >= all_b && j + kKeys <= all_e;
+                auto mask = [&](uint32_t (&x)[16], uint32_t k) {
+                    const uint32_t bits = seen(j, gap, kC * side + k);
+#pragma unroll
+                    for (uint32_t e = 0; e < 16u; ++e)
+                        if (!(bits >> e & 1u)) x[e] = 0xFF800000u;
+                };
+                if (mine) {
+                    float mt[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-                for (uint32_t k = 0; k < kC; ++k) {
-                    uint32_t x[16], w[16];  // w: 8 columns of high halves, 8 of low halves
-                    tmem_load(st_addr + 16u * k, x);
-                    tmem_ready(x);
-                    if (!whole) mask(x, k);
+                    for (uint32_t k = 0; k < kC; k += 2u) {
+                        uint32_t x[2][16];
+                        tmem_load(st_addr + 16u * k, x[0]);
+                        tmem_load(st_addr + 16u * (k + 1u), x[1]);
+                        tmem_ready(x[0]);
+                        tmem_ready(x[1]);
 #pragma unroll
-                    for (uint32_t e = 0; e < 8u; ++e) {
-                        float2 v = ffma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), unscale2, ref2);
-                        v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
-                        part[e & 1u] = fadd2(part[e & 1u], v);
-                        split(v, &w[e], &w[8 + e]);
-                    }
-                    tmem_store(st_addr + 16u * k, w);
-                }
-                l = fmaf(l, alpha, (part[0].x + part[1].x) + (part[0].y + part[1].y));
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            }
-            tc_fence_before();
-            mbar_arrive(&p_full[half]);
-            ok = mbar_wait_bounded(&o_full[half], ph, a.st, 70u);
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (mine) {
-                bool odd = false;
-                uint32_t x[2][16];
-                if (!whole) {
-                    // a value that is not finite must not reach the rows that do not see it, yet
-                    // 0 * inf is in their sums: then the tile is done key by key
-                    float t = 0.f;
-                    tmem_load(o_addr, x[0]);
+                        for (uint32_t u = 0; u < 2u; ++u) {
+                            if (!whole) mask(x[u], k + u);
 #pragma unroll
-                    for (uint32_t k = 0; k < kD / 16u; ++k) {
-                        tmem_ready(x[k & 1u]);
-                        if (k + 1u < kD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
-#pragma unroll
-                        for (uint32_t e = 0; e < 16u; ++e) t = fmaf(__uint_as_float(x[k & 1u][e]), 0.f, t);
-                    }
-                    odd = p >= 0 && t != 0.f;
-                }
-                if (!__any_sync(0xFFFFFFFFu, odd)) {
-                    tmem_load(o_addr, x[0]);
-#pragma unroll
-                    for (uint32_t k = 0; k < kD / 16u; ++k) {
-                        tmem_ready(x[k & 1u]);
-                        if (k + 1u < kD / 16u) tmem_load(o_addr + 16u * (k + 1u), x[(k + 1u) & 1u]);
-#pragma unroll
-                        for (uint32_t e = 0; e < 16u; e += 2u) {
-                            const float2 y = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), make_float2(alpha, alpha),
-                                                   make_float2(__uint_as_float(x[k & 1u][e]), __uint_as_float(x[k & 1u][e + 1u])));
-                            acc[16u * k + e] = y.x;
-                            acc[16u * k + e + 1u] = y.y;
+                            for (uint32_t e = 0; e < 16u; e += 2u)
+                                mt[(e >> 1) & 1u] =
+                                    fmaxf(fmaxf(mt[(e >> 1) & 1u], __uint_as_float(x[u][e])), __uint_as_float(x[u][e + 1]));
                         }
                     }
-                } else {
-#pragma unroll
-                    for (uint32_t d = 0; d < kD; ++d) acc[d] *= alpha;
-                    const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
-                    for (uint32_t k = from; k < to; ++k) {
-                        if (!(seen(k >> 4) >> (k & 15u) & 1u)) continue;
-                        const uint32_t page = a.b.table[static_cast<size_t>(s) * a.b.max_pages + ((j + k) >> a.kv.page_shift)];
-                        const size_t off = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size +
-                                            ((j + k) & (a.kv.page_size - 1u))) * hd;
-                        const __half *kr = static_cast<const __half*>(a.kv.k) + off, *vr = static_cast<const __half*>(a.kv.v) + off;
-                        float sum = 0.f;
-                        for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, __half2float(kr[d]), sum);
-                        const float w = exp2_fast(sum - ref);
-#pragma unroll
-                        for (uint32_t d = 0; d < kD; ++d)
-                            if (side * kD + d < hd) acc[d] = fmaf(w, __half2float(vr[side * kD + d]), acc[d]);
-                    }
-                    __syncwarp();
+                    side_max[(i >> 1) & 1u][half * 2u + side][r] = fmaxf(mt[0], mt[1]);
                 }
+                named_barrier_sync(1u + half, 256);
+                if (mine) {
+                    // (taken in turns: a quick thread may be a tile ahead of its pair)
+                    const float(*both)[kRows] = side_max[(i >> 1) & 1u] + half * 2u;
+                    const float mn = fmaxf(m, fmaxf(both[0][r], both[1][r]) * unscale);
+                    const float alpha = mn == -INFINITY ? 1.f : exp2_fast(m - mn);
+                    m = mn;
+                    const float ref = (mn == -INFINITY ? 0.f : mn) - kUp;
+                    float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    const float2 unscale2 = make_float2(unscale, unscale), ref2 = make_float2(-ref, -ref);
+#pragma unroll 1
+                    for (uint32_t k = 0; k < kC; ++k) {
+                        uint32_t x[16], w[16];  // w: 8 columns of high halves, 8 of low halves
+                        tmem_load(st_addr + 16u * k, x);
+                        tmem_ready(x);
+                        if (!whole) mask(x, k);
+#pragma unroll
+                        for (uint32_t e = 0; e < 8u; ++e) {
+                            float2 v = ffma2(make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), unscale2, ref2);
+                            v = make_float2(exp2_fast(v.x), exp2_fast(v.y));
+                            part[e & 1u] = fadd2(part[e & 1u], v);
+                            split(v, &w[e], &w[8 + e]);
+                        }
+                        tmem_store(st_addr + 16u * k, w);
+                    }
+                    l = fmaf(l, alpha, (part[0].x + part[1].x) + (part[0].y + part[1].y));
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                }
+                // read behind P V: its place is free again once the sums have come three tiles further
+                if (side == 0u) tile_ref[i % (2u * kBuffers)][r] = m;
+                tc_fence_before();
+                mbar_arrive(&p_full[buf]);
             }
-        }
-        // the halves meet: the odd tiles' sums through shared memory (the ring is done with)
-        constexpr uint32_t kPitch = HD + 4u;
-        float* sums = reinterpret_cast<float*>(sm + (ring - s0)) + r * kPitch + side * kD;
-        sum_l[half * 2u + side][r] = p >= 0 ? l : 0.f;  // padding sees nothing
-        if (side == 0u) sum_m[half][r] = m == -INFINITY ? 0.f : m;
-        named_barrier_sync(3, kSoftmax);
-        if (half == 1u) {
+            sum_l[half * 2u + side][r] = p >= 0 ? l : 0.f;  // padding sees nothing
+            if (side == 0u) sum_m[half][r] = m == -INFINITY ? 0.f : m;
+            asm volatile("bar.arrive 4, %0;" ::"n"(kSoftmax + kSums) : "memory");
+        } else {
+            // ---- running sums: channels of this side
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+            constexpr uint32_t kD = HD / 2u;
+            const uint32_t o_addr = lanes + kBuffers * 128u + side * kD;
+            float acc[kD], top = -INFINITY;
+#pragma unroll
+            for (uint32_t d = 0; d < kD; ++d) acc[d] = 0.f;
+            for (uint32_t i = 0; i < ntiles && ok; ++i) {
+                const uint32_t j = j0 + i * kKeys;
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&o_full, i & 1u, a.st, 70u));
+                if (!ok) break;
+                tc_fence_after();
+                if (j < we && j + kKeys > wb) {
+                    const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 7u]);
+                    const bool whole = gap == 0u && j >= all_b && j + kKeys <= all_e;
+                    // the tile's weights go by its half's maximum, the sums by the largest so far
+                    const float ref = tile_ref[i % (2u * kBuffers)][r], most = fmaxf(top, ref);
+                    const float alpha = most == -INFINITY ? 1.f : exp2_fast(top - most);
+                    const float beta = ref == -INFINITY ? 0.f : exp2_fast(ref - most);
+                    top = most;
+                    uint32_t x[16];
+                    bool odd = false;
+                    if (!whole) {
+                        // a value that is not finite must not reach the rows that do not see it, yet
+                        // 0 * inf is in their sums: then the tile is done key by key
+                        float t = 0.f;
+#pragma unroll 1
+                        for (uint32_t k = 0; k < kD / 16u; ++k) {
+                            tmem_load(o_addr + 16u * k, x);
+                            tmem_ready(x);
+#pragma unroll
+                            for (uint32_t e = 0; e < 16u; ++e) t = fmaf(__uint_as_float(x[e]), 0.f, t);
+                        }
+                        odd = p >= 0 && t != 0.f;
+                    }
+                    const float2 alpha2 = make_float2(alpha, alpha), beta2 = make_float2(beta, beta);
+                    if (!__any_sync(0xFFFFFFFFu, odd)) {
+#pragma unroll
+                        for (uint32_t k = 0; k < kD / 16u; ++k) {
+                            tmem_load(o_addr + 16u * k, x);
+                            tmem_ready(x);
+#pragma unroll
+                            for (uint32_t e = 0; e < 16u; e += 2u) {
+                                const float2 o = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1u]));
+                                const float2 y = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), alpha2, __fmul2_rn(o, beta2));
+                                acc[16u * k + e] = y.x;
+                                acc[16u * k + e + 1u] = y.y;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (uint32_t d = 0; d < kD; ++d) acc[d] *= alpha;
+                        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+                        for (uint32_t key = max(row_b, j); key < min(row_e, j + kKeys); ++key) {
+                            if (!(seen(j, gap, (key - j) >> 4) >> ((key - j) & 15u) & 1u)) continue;
+                            const uint32_t page = a.b.table[static_cast<size_t>(s) * a.b.max_pages + (key >> a.kv.page_shift)];
+                            const size_t off = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size +
+                                                (key & (a.kv.page_size - 1u))) * hd;
+                            const __half *kr = static_cast<const __half*>(a.kv.k) + off, *vr = static_cast<const __half*>(a.kv.v) + off;
+                            float sum = 0.f;
+                            for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, __half2float(kr[d]), sum);
+                            const float w = exp2_fast(sum - (most - kUp));
+#pragma unroll
+                            for (uint32_t d = 0; d < kD; ++d)
+                                if (side * kD + d < hd) acc[d] = fmaf(w, __half2float(vr[side * kD + d]), acc[d]);
+                        }
+                        __syncwarp();
+                    }
+                }
+                tc_fence_before();
+                mbar_arrive(&o_empty);
+            }
+            // the weight sums of both halves, then the rows' results through shared memory (the ring
+            // is done with)
+            asm volatile("bar.sync 4, %0;" ::"n"(kSoftmax + kSums) : "memory");
+            constexpr uint32_t kPitch = HD + 4u;
+            float* sums = reinterpret_cast<float*>(sm + (ring - s0));
+            const float l0 = sum_l[0][r] + sum_l[1][r], l1 = sum_l[2][r] + sum_l[3][r];
+            const float ref = top == -INFINITY ? 0.f : top;
+            const float sum = (l0 == 0.f ? 0.f : l0 * exp2_fast(sum_m[0][r] - ref)) + (l1 == 0.f ? 0.f : l1 * exp2_fast(sum_m[1][r] - ref));
+            const float scale = a.direct ? 1.f / sum : 1.f;
 #pragma unroll
             for (uint32_t d = 0; d < kD; d += 4u)
-                *reinterpret_cast<float4*>(sums + d) = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
-        }
-        named_barrier_sync(3, kSoftmax);
-        const float l0 = sum_l[0][r] + sum_l[1][r], l1 = sum_l[2][r] + sum_l[3][r];
-        const float top = l0 == 0.f ? sum_m[1][r] : l1 == 0.f ? sum_m[0][r] : fmaxf(sum_m[0][r], sum_m[1][r]);
-        const float f0 = l0 == 0.f ? 0.f : exp2_fast(sum_m[0][r] - top), f1 = l1 == 0.f ? 0.f : exp2_fast(sum_m[1][r] - top);
-        const float sum = l0 * f0 + l1 * f1;
-        if (half == 0u) {
-            const float scale = a.direct && sum != 0.f ? 1.f / sum : 1.f;
-#pragma unroll
-            for (uint32_t d = 0; d < kD; d += 4u) {
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (l1 != 0.f) x = *reinterpret_cast<const float4*>(sums + d);
-                if (l1 != 0.f) x = make_float4(x.x * f1, x.y * f1, x.z * f1, x.w * f1);
-                if (l0 != 0.f)
-                    x = make_float4(fmaf(acc[d], f0, x.x), fmaf(acc[d + 1], f0, x.y), fmaf(acc[d + 2], f0, x.z),
-                                    fmaf(acc[d + 3], f0, x.w));
-                *reinterpret_cast<float4*>(sums + d) = make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale);
-            }
-        }
-        const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-        if (ok && half == 0u && side == 0u && !a.direct && p != -2)
-            a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]] =
-                make_float2(top - kUp, sum);
-        named_barrier_sync(3, kSoftmax);
-        if (ok) {
-            const float* all = reinterpret_cast<const float*>(sm + (ring - s0));
-            const uint32_t hd4 = hd / 4u;
-            for (uint32_t x = tid; x < kRows * hd4; x += kSoftmax) {
-                const uint32_t rr = x / hd4, d = (x - rr * hd4) * 4u;
-                if (row_pos[rr] == -2) continue;
-                const size_t row = static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr];
-                float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
-                *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(all + rr * kPitch + d);
+                *reinterpret_cast<float4*>(sums + r * kPitch + side * kD + d) =
+                    sum == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                               : make_float4(acc[d] * scale, acc[d + 1] * scale, acc[d + 2] * scale, acc[d + 3] * scale);
+            const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+            if (ok && side == 0u && !a.direct && p != -2)
+                a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]] =
+                    make_float2(ref - kUp, sum);
+            named_barrier_sync(5, kSums);
+            if (ok) {
+                const uint32_t hd4 = hd / 4u;
+                for (uint32_t x = tid - kSoftmax; x < kRows * hd4; x += kSums) {
+                    const uint32_t rr = x / hd4, d = (x - rr * hd4) * 4u;
+                    if (row_pos[rr] == -2) continue;
+                    const size_t row = static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr];
+                    float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
+                    *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(sums + rr * kPitch + d);
+                }
             }
         }
     }
