@@ -20,219 +20,6 @@
 namespace nedo_gpu {
 namespace {
 
-// ---- the general kernel: any type, any head size, CUDA cores ----------------
-constexpr uint32_t kRows = 8;   // query rows per tile
-constexpr uint32_t kTile = 32;  // keys per step: one per lane
-constexpr uint32_t kThreads = 128;
-
-size_t simt_smem(uint32_t hd) { return (kRows + 2u * kTile) * static_cast<size_t>(hd + 4u) * sizeof(float); }
-
-template <typename T>
-__device__ __forceinline__ void attention_simt(const AttnArgs& a) {
-    extern __shared__ __align__(16) float sm[];
-    __shared__ uint32_t row_tok[kRows], row_head[kRows];
-    __shared__ int row_pos[kRows];
-    __shared__ float pw[kRows][kTile], alpha[kRows], lsum[kRows];
-    __shared__ float mrow[kRows];
-    __shared__ uint64_t koff[kTile];
-    __shared__ uint32_t kpos[kTile];
-    __shared__ uint32_t found[2];
-    __shared__ uint32_t list[kMaxPicks];
-    const uint32_t hd = a.kv.head_dim, pitch = hd + 4u, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-    float* qs = sm;
-    float* ks = qs + kRows * pitch;
-    float* vs = ks + kTile * pitch;
-    const uint32_t c = blockIdx.x % a.chunks;
-    uint32_t rest = blockIdx.x / a.chunks;
-    const uint32_t kh = rest % a.kv.kv_heads;
-    rest /= a.kv.kv_heads;
-
-    // the tile's rows
-    uint32_t s = kNone, r0 = 0, nrows = 0, t0 = 0;
-    PagedSeq sq{0u, 0u, 0u};
-    if (a.part == kPartOwn) {
-        if (warp == 0) {
-            uint32_t tile;
-            const uint32_t seq = find_tile(a, rest, kRows, &tile);
-            if (lane == 0) {
-                found[0] = seq;
-                found[1] = tile;
-            }
-        }
-        __syncthreads();
-        s = found[0];
-        if (s == kNone) return;
-        sq = load_seq(a.b, s, a.st);
-        t0 = sq.t0;
-        r0 = found[1] * kRows;
-        nrows = min(kRows, sq.n * a.group - r0);
-    } else if (a.part == kPartPrefix) {
-        r0 = rest * kRows;
-        nrows = min(kRows, a.b.tokens * a.group - r0);
-    } else {
-        t0 = rest / a.row_blocks;
-        r0 = (rest % a.row_blocks) * kRows;
-        nrows = min(kRows, a.group - r0);
-        s = seq_of_token(a.b, t0);
-        if (s == kNone) return;
-        sq = load_seq(a.b, s, a.st);
-        if (sq.n == 0u) return;
-    }
-    if (tid < kRows) {
-        int p = -2;  // no row here
-        uint32_t tok = 0, head = 0;
-        if (tid < nrows) {
-            tok = t0 + (r0 + tid) / a.group;
-            head = kh * a.group + (r0 + tid) % a.group;
-            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
-        }
-        row_tok[tid] = tok;
-        row_head[tid] = head;
-        row_pos[tid] = p;
-        mrow[tid] = -INFINITY;
-        lsum[tid] = 0.f;
-    }
-    __syncthreads();
-    // the tile's keys in this chunk: [kb, ke) positions, or list entries
-    uint32_t kb = kNone, ke = 0;
-    if (a.part == kPartBlocks) {
-        const uint32_t* l = a.blocks + (static_cast<size_t>(t0) * a.kv.kv_heads + kh) * a.picks;
-        if (warp == 0) checked_list(l, a.picks, row_pos[0], a.kv.page_shift, list);
-        __syncthreads();
-        kb = c * a.chunk;
-        ke = min(kb + a.chunk, a.picks << a.kv.page_shift);
-    } else {
-        for (uint32_t r = 0; r < kRows; ++r) {
-            if (row_pos[r] < 0) continue;
-            kb = min(kb, first_key(row_pos[r], a.window));
-            ke = max(ke, static_cast<uint32_t>(row_pos[r]) + 1u);
-        }
-        uint32_t base = 0;
-        if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
-        else ke = min(ke, a.shared_len);
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
-        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
-        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
-        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
-        if (a.part == kPartPrefix) s = 0;
-    }
-    for (uint32_t i = tid; i < kRows * hd; i += kThreads) {
-        const uint32_t r = i / hd, d = i - r * hd;
-        qs[r * pitch + d] =
-            row_pos[r] >= 0 ? a.q[(static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd + d] * a.scale_log2 : 0.f;
-    }
-    float acc[kRows][2];
-#pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r) acc[r][0] = acc[r][1] = 0.f;
-
-    for (uint32_t j0 = kb; j0 < ke; j0 += kTile) {
-        __syncthreads();
-        if (tid < kTile) {
-            const uint32_t j = j0 + tid;
-            uint32_t pos = kNone;
-            uint64_t off = ~0ull;
-            if (j < ke) {
-                const uint32_t lp = a.part == kPartBlocks ? list[j >> a.kv.page_shift] : j >> a.kv.page_shift;
-                const uint32_t slot = j & (a.kv.page_size - 1u);
-                if (lp != kNone) {
-                    const uint32_t at = (lp << a.kv.page_shift) + slot;
-                    const uint32_t page = at < sq.kv || a.part == kPartPrefix ? load_page(a.b, a.kv, s, lp, a.st) : kNone;
-                    if (page != kNone) {
-                        pos = at;
-                        off = ((static_cast<uint64_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size + slot) * hd;
-                    }
-                }
-            }
-            kpos[tid] = pos;
-            koff[tid] = off;
-        }
-        __syncthreads();
-        for (uint32_t i = tid; i < kTile * hd; i += kThreads) {
-            const uint32_t j = i / hd, d = i - j * hd;
-            const uint64_t off = koff[j];
-            // unseen keys count as zero, whatever their memory holds
-            ks[j * pitch + d] = off != ~0ull ? kv_float(static_cast<const T*>(a.kv.k)[off + d]) : 0.f;
-            vs[j * pitch + d] = off != ~0ull ? kv_float(static_cast<const T*>(a.kv.v)[off + d]) : 0.f;
-        }
-        __syncthreads();
-        for (uint32_t r = warp; r < kRows; r += kThreads / 32u) {
-            float sc = 0.f;
-            for (uint32_t d = 0; d < hd; d += 4u) {
-                const float4 kk = *reinterpret_cast<const float4*>(ks + lane * pitch + d);
-                const float4 qq = *reinterpret_cast<const float4*>(qs + r * pitch + d);
-                sc = fmaf(kk.x, qq.x, sc);
-                sc = fmaf(kk.y, qq.y, sc);
-                sc = fmaf(kk.z, qq.z, sc);
-                sc = fmaf(kk.w, qq.w, sc);
-            }
-            const uint32_t at = kpos[lane];
-            const int p = row_pos[r];
-            const bool see = p >= 0 && at <= static_cast<uint32_t>(p) && at >= first_key(p, a.window);
-            if (!see) sc = -INFINITY;
-            float m = sc;
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-            const float m0 = mrow[r];
-            m = fmaxf(m, m0);
-            // rows that have seen nothing yet keep m = -inf, factor 1 and weights 0
-            const float al = m == -INFINITY ? 1.f : exp2f(m0 - m);
-            const float e = see ? exp2f(sc - m) : 0.f;
-            const float l = warp_sum(e);
-            pw[r][lane] = e;
-            __syncwarp();
-            if (lane == 0) {
-                alpha[r] = al;
-                mrow[r] = m;
-                lsum[r] = lsum[r] * al + l;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t u = 0; u < 2u; ++u) {
-            const uint32_t d = tid + u * kThreads;
-            if (d >= hd) continue;
-#pragma unroll
-            for (uint32_t r = 0; r < kRows; ++r) {
-                float o = acc[r][u] * alpha[r];
-                for (uint32_t j = 0; j < kTile; ++j) {
-                    const float w = pw[r][j];
-                    if (w != 0.f) o = fmaf(w, vs[j * pitch + d], o);  // an unseen value never enters
-                }
-                acc[r][u] = o;
-            }
-        }
-    }
-    __syncthreads();
-    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-#pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r) {
-        if (row_pos[r] == -2) continue;
-        const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
-        const float l = lsum[r];
-#pragma unroll
-        for (uint32_t u = 0; u < 2u; ++u) {
-            const uint32_t d = tid + u * kThreads;
-            if (d >= hd) continue;
-            if (a.direct) {
-                a.out[row * hd + d] = l == 0.f ? 0.f : acc[r][u] / l;  // l = 0: no key seen
-            } else {
-                a.part_o[((a.slot0 + c) * rows_all + row) * hd + d] = acc[r][u];
-            }
-        }
-        if (!a.direct && tid == 0) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(mrow[r], l);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) attention_simt_kernel(const __grid_constant__ AttnArgs a) {
-    attention_simt<T>(a);
-    end_after_previous(a);
-}
-
-cudaError_t launch_simt(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    return launch_items(a, a.kv.type == kF16 ? attention_simt_kernel<__half> : attention_simt_kernel<float>, items, kThreads,
-                        simt_smem(a.kv.head_dim), stream, a);
-}
-
 // ---- adding a row's chunks ---------------------------------------------------
 struct CombineArgs {
     PagedKv kv;
@@ -354,7 +141,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kFew32, kMany, kTc, kSimt };
+enum class Kernel { kFew, kFew32, kMany, kMany32, kTc };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -379,7 +166,8 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {kFewRows, slots, 2048u, 8.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
-        default: return {kRows, 148u * 3u, 0u, 40.0, 5000.0, 1.0};
+        default:  // kMany32: three products each way
+            return {many32_rows(hd), 148u, 0u, hd <= 64u ? 24.0 : 48.0, 5000.0, 1.0};
     }
 }
 
@@ -429,7 +217,7 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 
 // The kernel of a part whose row tiles have up to `rows` rows.
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
-    if (kv.type != kF16) return rows <= kFewRows ? Kernel::kFew32 : Kernel::kSimt;
+    if (kv.type != kF16) return rows <= kFewRows ? Kernel::kFew32 : Kernel::kMany32;
     if (rows <= kFewRows) return Kernel::kFew;
     const bool tc = kv.head_dim <= 128u && static_cast<uint64_t>(kv.num_pages) * kv.kv_heads < (1ull << 31);
     return tc ? Kernel::kTc : Kernel::kMany;
@@ -450,7 +238,7 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
         case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
         case Kernel::kMany: return launch_attention_many(a, tiles, stream);
         case Kernel::kTc: return launch_attention_tc(a, tiles, stream);
-        default: return launch_simt(a, items, stream);
+        default: return launch_attention_many32(a, tiles, stream);
     }
 }
 

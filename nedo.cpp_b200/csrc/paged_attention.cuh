@@ -340,6 +340,10 @@ cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_
 // tiles of kManyRows.
 constexpr uint32_t kManyRows = 64;
 cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
+// Tiles of many32_rows(head_dim) rows of F32 caches on the tensor cores
+// (paged_attention_many32.cu).
+uint32_t many32_rows(uint32_t head_dim);
+cudaError_t launch_attention_many32(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
 // Tiles of kTcRows rows on the 5th-generation tensor cores (paged_attention_tc.cu): F16
 // caches, heads of up to 128 channels, num_pages * kv_heads below 2^31.
 constexpr uint32_t kTcRows = 128;

@@ -1,0 +1,469 @@
+// paged_attention_many32.cu -- attention over a paged F32 cache for tiles of many query rows
+// (prompts, and the tokens of a whole batch over their shared prefix): bound by the tensor
+// cores.
+//
+// Mathematics.  Both factors of each product are fp32 here, so both are split in two fp16
+// halves (22 bits) and three of the four products are formed, the small ones first:
+// lo hi + hi lo + hi hi; what is left out is 2^-22 of the product.  Queries are scaled by a
+// power of two per row, keys and values by one per tile, to where the low halves are normal
+// numbers; the weights as in the other kernels.  A tile's weighted values are summed from zero
+// and added to the running sums in fp32, which also takes the tile's scale back.
+//
+// Work.  A CTA of one warp for 16 rows (128 rows, 64 for heads above 128) takes its rows through
+// their keys in tiles of 64 (32).  The next tile's keys and values are on their way (cp.async)
+// while this one is multiplied; a tile that has landed is read once by all threads, its largest
+// magnitudes found, and its halves written next to it for ldmatrix, once for all warps.
+#include "paged_attention.cuh"
+#include "paged_mma.cuh"
+
+namespace nedo_gpu {
+namespace {
+
+template <uint32_t HD>
+struct Many32 {
+    static constexpr uint32_t kRows = HD <= 128u ? 128u : 64u;
+    static constexpr uint32_t kWarps = kRows / 16u;
+    static constexpr uint32_t kThreads = 32u * kWarps;
+    static constexpr uint32_t kKeys = HD <= 128u ? 64u : 32u;
+    static constexpr uint32_t kRowBytes = HD * 2u;                     // a row of halves
+    static constexpr uint32_t kQBytes = kRows * kRowBytes;             // one half of the queries
+    static constexpr uint32_t kHalfBytes = kKeys * kRowBytes;          // one half of a tile's keys or values
+    static constexpr uint32_t kRawBytes = kKeys * HD * 4u;             // a tile's keys or values as they come
+    static constexpr uint32_t kSmem = 2u * kQBytes + 4u * kHalfBytes + 2u * kRawBytes;
+};
+
+template <uint32_t HD>
+__device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
+    return r * Many32<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
+}
+
+__device__ __forceinline__ float finite_size(float x) {
+    const float s = fabsf(x);
+    return s < INFINITY ? s : 0.f;
+}
+// Two values as halves {hi, lo}; an infinity or NaN is all in the high half.
+__device__ __forceinline__ void split_any(float x, float y, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    *hi = pack(h);
+    *lo = pack(__floats2half2_rn(fabsf(f.x) < INFINITY ? x - f.x : 0.f, fabsf(f.y) < INFINITY ? y - f.y : 0.f));
+}
+
+template <uint32_t HD>
+__device__ __forceinline__ void attention_many32(const AttnArgs& a) {
+    using M = Many32<HD>;
+    constexpr uint32_t kRows = M::kRows, kKeys = M::kKeys, kGroups = kKeys / 16u, kCols = kKeys / 8u, kThreads = M::kThreads;
+    extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint32_t row_tok[kRows], row_head[kRows];
+    __shared__ int row_pos[kRows];
+    __shared__ float row_unscale[kRows], size[2][M::kWarps];
+    __shared__ uint32_t found[2], odd_warp[M::kWarps];
+    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t kh = blockIdx.x % a.kv.kv_heads;
+    uint32_t rest = blockIdx.x / a.kv.kv_heads;
+    const uint32_t c = rest % a.chunks;
+    rest /= a.chunks;
+
+    // rows
+    uint32_t s = 0, r0 = 0, nrows, t0 = 0;
+    PagedSeq sq{0u, 0u, 0u};
+    if (a.part == kPartPrefix) {
+        r0 = rest * kRows;
+        nrows = min(kRows, a.b.tokens * a.group - r0);
+    } else {
+        // the last tiles first: with causal rows they have the most keys
+        if (warp == 0) {
+            uint32_t tile;
+            const uint32_t seq = find_tile(a, a.tiles - 1u - rest, kRows, &tile);
+            if (lane == 0u) {
+                found[0] = seq;
+                found[1] = tile;
+            }
+        }
+        __syncthreads();
+        s = found[0];
+        if (s == kNone) return;
+        sq = load_seq(a.b, s, a.st);
+        t0 = sq.t0;
+        r0 = found[1] * kRows;
+        nrows = min(kRows, sq.n * a.group - r0);
+    }
+    if (tid < kRows) {
+        int p = -2;
+        uint32_t tok = 0, head = 0;
+        if (tid < nrows) {
+            tok = t0 + (r0 + tid) / a.group;
+            head = kh * a.group + (r0 + tid) % a.group;
+            p = a.part == kPartPrefix ? row_position(a, tok) : max(-1, sq.pos(tok - sq.t0));
+        }
+        row_tok[tid] = tok;
+        row_head[tid] = head;
+        row_pos[tid] = p;
+    }
+    __syncthreads();
+    // keys [kb, ke) of the tile and [wb, we) of this warp; [all_b, all_e): seen by all its rows
+    uint32_t kb = kNone, ke = 0, wb = kNone, we = 0, all_b = 0, all_e = kNone;
+    {
+        uint32_t lo = kNone, hi = 0;
+#pragma unroll
+        for (uint32_t u = 0; u < kRows / 32u; ++u) {
+            const int p = row_pos[lane + 32u * u];
+            if (p >= 0) {
+                lo = min(lo, first_key(p, a.window));
+                hi = max(hi, static_cast<uint32_t>(p) + 1u);
+            }
+        }
+        kb = __reduce_min_sync(0xFFFFFFFFu, lo);
+        ke = __reduce_max_sync(0xFFFFFFFFu, hi);
+        const int p = row_pos[warp * 16u + (lane & 15u)];
+        const uint32_t l1 = p >= 0 ? first_key(p, a.window) : kNone, h1 = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        wb = __reduce_min_sync(0xFFFFFFFFu, l1);
+        we = __reduce_max_sync(0xFFFFFFFFu, h1);
+        all_b = __reduce_max_sync(0xFFFFFFFFu, p >= 0 ? l1 : 0u);
+        all_e = __reduce_min_sync(0xFFFFFFFFu, p >= 0 ? h1 : kNone);
+    }
+    {
+        uint32_t base = 0;
+        if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
+        else ke = min(ke, a.shared_len);
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
+        kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
+        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
+        if (kb >= ke && !a.direct) return;  // no row of the tile sees a key of this chunk
+    }
+    const uint32_t j0 = kb & ~(kKeys - 1u), ntiles = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
+
+    uint8_t* const halves = sm + 2u * M::kQBytes;                 // keys hi, lo, values hi, lo
+    uint8_t* const raw = halves + 4u * M::kHalfBytes;             // keys, values
+    const uint32_t q_addr = smem_addr(sm), k_addr = smem_addr(halves), v_addr = k_addr + 2u * M::kHalfBytes;
+    if (hd < HD) {  // channels beyond the head stay zero
+        for (uint32_t i = tid; i < M::kSmem / 16u; i += kThreads) reinterpret_cast<uint4*>(sm)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+    }
+    const uint32_t chunks16 = hd >> 2;
+    const float* kbase = static_cast<const float*>(a.kv.k);
+    const float* vbase = static_cast<const float*>(a.kv.v);
+    // pages of the next tile's groups of 16 keys (a group lies within one page)
+    uint32_t pages[kGroups];
+    auto look_up = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t u = 0; u < kGroups; ++u) {
+            const uint32_t j = j0 + i * kKeys + u * 16u;
+            pages[u] = i < ntiles && j < ke && j + 16u > kb ? load_page(a.b, a.kv, s, j >> a.kv.page_shift, a.st) : kNone;
+        }
+    };
+    uint32_t there = 0;  // groups of the tile on its way whose page is a page, or that no row sees
+    // 16-byte pieces x of a tile: the same ones are copied and read back by the same thread
+    constexpr uint32_t kPieces = kKeys * (HD / 4u) / kThreads, kAtOnce = kThreads / (HD / 4u);
+    const uint32_t piece_ch = tid % (HD / 4u), piece_row = tid / (HD / 4u);
+    auto fetch = [&](uint32_t i) {
+        if (i < ntiles) {
+            there = 0u;
+#pragma unroll
+            for (uint32_t u = 0; u < kGroups; ++u) {
+                const uint32_t j = j0 + i * kKeys + u * 16u;
+                if (pages[u] != kNone || j >= ke || j + 16u <= kb) there |= 1u << u;
+            }
+            if (piece_ch < chunks16) {
+#pragma unroll
+                for (uint32_t x = 0; x < kPieces; ++x) {
+                    const uint32_t r = piece_row + x * kAtOnce, j = j0 + i * kKeys + r;
+                    uint32_t page = pages[0];
+#pragma unroll
+                    for (uint32_t u = 1; u < kGroups; ++u) page = r >= 16u * u ? pages[u] : page;
+                    const bool in = page != kNone && j >= kb && j < ke;
+                    const size_t o = (((in ? static_cast<size_t>(page) : 0u) * a.kv.kv_heads + kh) * a.kv.page_size +
+                                      (in ? j & (a.kv.page_size - 1u) : 0u)) * hd + piece_ch * 4u;
+                    const uint32_t dst = smem_addr(raw) + (r * (HD / 4u) + piece_ch) * 16u;
+                    cp_async16(dst, kbase + o, in ? 16u : 0u);
+                    cp_async16(dst + M::kRawBytes, vbase + o, in ? 16u : 0u);
+                }
+            }
+        }
+        cp_commit();
+    };
+    look_up(0);
+    fetch(0);
+    look_up(1);
+
+    // queries: scaled, split and stored; a row per two threads
+    {
+        const uint32_t r = tid >> 1;
+        const int p = row_pos[r];
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+        float big = 0.f;
+        if (p >= 0)
+            for (uint32_t d = (tid & 1u) * 4u; d < hd; d += 8u) {
+                const float4 x = *reinterpret_cast<const float4*>(q + d);
+                big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
+                                       fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
+            }
+        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+        const int e2 = up_exponent(big);
+        const float up = power_of_two(e2);
+        if ((tid & 1u) == 0u) row_unscale[r] = power_of_two(-e2);
+        for (uint32_t d = (tid & 1u) * 8u; d < HD; d += 16u) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                float2 x = make_float2(0.f, 0.f);
+                if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
+                split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
+            }
+            *reinterpret_cast<uint4*>(sm + at<HD>(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(sm + M::kQBytes + at<HD>(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+    __syncthreads();
+
+    // this thread's rows g and g + 8 of the warp's 16
+    const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u, mi = lane >> 3, mr = lane & 7u;
+    float unscale[2], m[2], l[2];
+    uint32_t lo_key[2], hi_key[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        const uint32_t r = warp * 16u + g + 8u * h;
+        const int p = row_pos[r];
+        unscale[h] = row_unscale[r];
+        lo_key[h] = p >= 0 ? first_key(p, a.window) : kNone;
+        hi_key[h] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+    }
+    float acc[HD / 8][4];
+#pragma unroll
+    for (uint32_t n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+
+    for (uint32_t i = 0; i < ntiles; ++i) {
+        const uint32_t have = there, j = j0 + i * kKeys;
+        cp_wait<0>();
+        // the tile as halves: every thread its own pieces (the ones it copied), first their sizes
+        float big[2] = {0.f, 0.f};
+        bool odd = false;
+#pragma unroll 4
+        for (uint32_t x = 0; x < kPieces; ++x) {
+            const uint32_t piece = (piece_row + x * kAtOnce) * (HD / 4u) + piece_ch;
+#pragma unroll
+            for (uint32_t kv = 0; kv < 2u; ++kv) {
+                const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
+                big[kv] = fmaxf(big[kv], fmaxf(fmaxf(finite_size(v.x), finite_size(v.y)), fmaxf(finite_size(v.z), finite_size(v.w))));
+                if (kv == 1u) odd |= !(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) < INFINITY) ||
+                                     v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+            }
+        }
+#pragma unroll
+        for (uint32_t kv = 0; kv < 2u; ++kv) {
+            for (int o = 16; o > 0; o >>= 1) big[kv] = fmaxf(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], o));
+            if (lane == 0u) size[kv][warp] = big[kv];
+        }
+        odd = __any_sync(0xFFFFFFFFu, odd);
+        if (lane == 0u) odd_warp[warp] = odd;
+        __syncthreads();  // also: all warps are done with the halves of the tile before
+        odd = false;
+#pragma unroll
+        for (uint32_t w = 0; w < M::kWarps; ++w) {
+            big[0] = fmaxf(big[0], size[0][w]);
+            big[1] = fmaxf(big[1], size[1][w]);
+            odd |= odd_warp[w] != 0u;
+        }
+        const int ek = up_exponent(big[0]), ev = up_exponent(big[1]);
+        const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek), v_down = power_of_two(-ev);
+#pragma unroll 4
+        for (uint32_t x = 0; x < kPieces; ++x) {
+            const uint32_t r = piece_row + x * kAtOnce, piece = r * (HD / 4u) + piece_ch;
+#pragma unroll
+            for (uint32_t kv = 0; kv < 2u; ++kv) {
+                const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
+                const float up = kv ? v_up : k_up;
+                uint32_t hi[2], lo[2];
+                split_any(v.x * up, v.y * up, &hi[0], &lo[0]);
+                split_any(v.z * up, v.w * up, &hi[1], &lo[1]);
+                uint8_t* dst = halves + kv * 2u * M::kHalfBytes + at<HD>(r, piece_ch >> 1) + (piece_ch & 1u) * 8u;
+                *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(dst + M::kHalfBytes) = make_uint2(lo[0], lo[1]);
+            }
+        }
+        fetch(i + 1u);  // into the thread's own pieces, which it has read
+        look_up(i + 2u);
+        __syncthreads();
+        if (j < we && j + kKeys > wb) {
+            float sc[kCols][4];
+#pragma unroll
+            for (uint32_t n = 0; n < kCols; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+            for (uint32_t turn = 0; turn < 3u; ++turn) {  // lo hi, hi lo, hi hi
+#pragma unroll
+                for (uint32_t k = 0; k < HD / 16; ++k) {
+                    uint32_t qf[4];
+                    ldsm4(qf, q_addr + (turn == 0u ? M::kQBytes : 0u) + at<HD>(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1)));
+#pragma unroll
+                    for (uint32_t n = 0; n < kGroups; ++n) {
+                        uint32_t b[4];
+                        ldsm4(b, k_addr + (turn == 1u ? M::kHalfBytes : 0u) + at<HD>(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
+                        mma(sc[2 * n], qf, b[0], b[1]);
+                        mma(sc[2 * n + 1], qf, b[2], b[3]);
+                    }
+                }
+            }
+            const bool whole = have == (1u << kGroups) - 1u && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
+            if (!whole) {
+#pragma unroll
+                for (uint32_t n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        const uint32_t key = j + n * 8u + t2 + (e & 1u), h = e >> 1;
+                        if (key < lo_key[h] || key >= hi_key[h] || key < kb || key >= ke || !(have >> (n >> 1) & 1u))
+                            sc[n][e] = -INFINITY;
+                    }
+            }
+            float alpha[2], ref[2], down[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                float mt = sc[0][2 * h];
+#pragma unroll
+                for (uint32_t n = 0; n < kCols; ++n) mt = fmaxf(mt, fmaxf(sc[n][2 * h], sc[n][2 * h + 1]));
+                mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
+                mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
+                // the two powers one after the other: together they may leave fp32's range
+                down[h] = unscale[h];
+                const float mn = fmaxf(m[h], mt * down[h] * k_down);
+                alpha[h] = mn == -INFINITY ? 1.f : exp2_fast(m[h] - mn);
+                m[h] = mn;
+                ref[h] = (mn == -INFINITY ? 0.f : mn) - kUp;
+                l[h] *= alpha[h];
+            }
+            uint32_t phi[kGroups][4], plo[kGroups][4];
+#pragma unroll
+            for (uint32_t n = 0; n < kCols; ++n) {
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) {
+                    sc[n][e] = exp2_fast(fmaf(sc[n][e] * down[e >> 1], k_down, -ref[e >> 1]));
+                    l[e >> 1] += sc[n][e];
+                }
+                split(sc[n][0], sc[n][1], &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
+                split(sc[n][2], sc[n][3], &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
+            }
+            if (whole || !odd) {
+#pragma unroll
+                for (uint32_t n = 0; n < HD / 16; ++n) {
+                    float o[2][4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+                    uint32_t b[kGroups][4];
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k)
+                        ldsm4t(b[k], v_addr + M::kHalfBytes + at<HD>(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k) {
+                        mma(o[0], phi[k], b[k][0], b[k][1]);
+                        mma(o[1], phi[k], b[k][2], b[k][3]);
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k)
+                        ldsm4t(b[k], v_addr + at<HD>(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k) {
+                        mma(o[0], plo[k], b[k][0], b[k][1]);
+                        mma(o[1], plo[k], b[k][2], b[k][3]);
+                    }
+#pragma unroll
+                    for (uint32_t k = 0; k < kGroups; ++k) {
+                        mma(o[0], phi[k], b[k][0], b[k][1]);
+                        mma(o[1], phi[k], b[k][2], b[k][3]);
+                    }
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        acc[2 * n][e] = fmaf(acc[2 * n][e], alpha[e >> 1], o[0][e] * v_down);
+                        acc[2 * n + 1][e] = fmaf(acc[2 * n + 1][e], alpha[e >> 1], o[1][e] * v_down);
+                    }
+                }
+            } else {
+                // a value that is not finite must not reach the rows that do not see it (0 * inf)
+#pragma unroll
+                for (uint32_t n = 0; n < HD / 8; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) acc[n][e] *= alpha[e >> 1];
+#pragma unroll
+                for (uint32_t n8 = 0; n8 < kCols; ++n8) {
+                    for (uint32_t jj = 0; jj < 8; ++jj) {
+                        const uint32_t from = (lane & ~3u) | (jj >> 1), key = j + n8 * 8u + jj;
+                        float w[2];
+#pragma unroll
+                        for (uint32_t h = 0; h < 2; ++h) {
+                            const float w0 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h], from);
+                            const float w1 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h + 1], from);
+                            w[h] = jj & 1u ? w1 : w0;
+                        }
+                        const bool in = key >= kb && key < ke && (have >> (n8 >> 1) & 1u);
+                        const bool see0 = in && key >= lo_key[0] && key < hi_key[0], see1 = in && key >= lo_key[1] && key < hi_key[1];
+#pragma unroll
+                        for (uint32_t n = 0; n < HD / 8; ++n) {
+                            const uint8_t* at_v = halves + 2u * M::kHalfBytes + at<HD>(n8 * 8u + jj, n) + t2 * 2u;
+                            const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(at_v));
+                            const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(at_v + M::kHalfBytes));
+                            const float f0 = (fh.x + fl.x) * v_down, f1 = (fh.y + fl.y) * v_down;
+                            if (see0) {
+                                acc[n][0] = fmaf(w[0], f0, acc[n][0]);
+                                acc[n][1] = fmaf(w[0], f1, acc[n][1]);
+                            }
+                            if (see1) {
+                                acc[n][2] = fmaf(w[1], f0, acc[n][2]);
+                                acc[n][3] = fmaf(w[1], f1, acc[n][3]);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    cp_wait<0>();
+    asm volatile("griddepcontrol.launch_dependents;");
+    const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+        const uint32_t r = warp * 16u + g + 8u * h;
+        const int p = row_pos[r];
+        if (p == -2) continue;
+        if (p < 0) l[h] = 0.f;  // padding sees nothing
+        const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
+        float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
+        const bool none = l[h] == 0.f;
+#pragma unroll
+        for (uint32_t n = 0; n < HD / 8; ++n) {
+            if (n * 8u >= hd) continue;
+            const float f = a.direct ? l[h] : 1.f;
+            *reinterpret_cast<float2*>(o + n * 8u + t2) =
+                none ? make_float2(0.f, 0.f) : make_float2(acc[n][2 * h] / f, acc[n][2 * h + 1] / f);
+        }
+        if (!a.direct && (lane & 3u) == 0u)
+            a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2((m[h] == -INFINITY ? 0.f : m[h]) - kUp, l[h]);
+    }
+}
+
+template <uint32_t HD>
+__global__ void __launch_bounds__(Many32<HD>::kThreads, 1) attention_many32_kernel(const __grid_constant__ AttnArgs a) {
+    attention_many32<HD>(a);
+    end_after_previous(a);
+}
+
+template <uint32_t HD>
+cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    return launch_items(a, attention_many32_kernel<HD>, items, Many32<HD>::kThreads, Many32<HD>::kSmem, stream, a);
+}
+
+}  // namespace
+
+uint32_t many32_rows(uint32_t head_dim) { return head_dim <= 128u ? 128u : 64u; }
+
+cudaError_t launch_attention_many32(const AttnArgs& args, uint64_t tiles, cudaStream_t stream) {
+    AttnArgs a = args;
+    a.tiles = static_cast<uint32_t>(tiles);
+    const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
+    if (a.kv.head_dim <= 64u) return launch<64>(a, items, stream);
+    if (a.kv.head_dim <= 128u) return launch<128>(a, items, stream);
+    return launch<256>(a, items, stream);
+}
+
+}  // namespace nedo_gpu
