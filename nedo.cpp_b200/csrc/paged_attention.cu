@@ -217,8 +217,8 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 
 // The kernel of a part whose row tiles have up to `rows` rows.
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
-    if (kv.type != kF16) return rows <= kFewRows ? Kernel::kFew32 : Kernel::kMany32;
-    if (rows <= kFewRows) return Kernel::kFew;
+    if (kv.type != kF16) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
+    if (rows <= kFewMax) return Kernel::kFew;
     const bool tc = kv.head_dim <= 128u && static_cast<uint64_t>(kv.num_pages) * kv.kv_heads < (1ull << 31);
     return tc ? Kernel::kTc : Kernel::kMany;
 }
@@ -265,14 +265,17 @@ bool plan_paged_attention(PagedAttention* a) {
     auto chunks = [&](uint64_t chunk) { return static_cast<uint32_t>(std::max<uint64_t>(ceil_div(keys, chunk), 1u)); };
     const Kernel own = own_kernel(*a);
     const Cost c = cost_of(own, a->kv);
-    units = (a->picks ? a->b.tokens * ceil_div(group, c.rows) : own_tiles(*a, c.rows)) * a->kv.kv_heads;
+    units = (a->picks          ? a->b.tokens * ceil_div(group, c.rows)
+             : takes_few(own) ? a->b.seqs * ceil_div(a->b.max_q_len * group, c.rows)
+                              : own_tiles(*a, c.rows)) *
+            a->kv.kv_heads;
     const bool alone = shared == 0u;
     a->own_chunk = chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(own));
     a->own_chunks = chunks(a->own_chunk);
     a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
     if (!takes_few(own) && a->b.seqs > 1u) {
-        const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads;
+        const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / kFewRows);
         a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv), alone);
         a->few_chunks = chunks(a->few_chunk);
         a->few_cluster = alone && a->few_chunks > 1u && a->few_chunks <= kMaxCluster;
@@ -316,6 +319,7 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         a.slot0 = 0;
         const Kernel k = prefix_kernel(p);
         const uint64_t all = static_cast<uint64_t>(p.b.tokens) * a.group;
+        a.row_blocks = static_cast<uint32_t>(ceil_div(all, kFewRows));
         e = launch_part(k, a, ceil_div(all, cost_of(k, p.kv).rows), all, stream);
         if (e != cudaSuccess) return e;
         a.late = 1u;
@@ -337,17 +341,20 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         const bool mixed = p.few_chunks != 0u;
         const uint64_t max_rows = static_cast<uint64_t>(p.b.max_q_len) * a.group;
         a.part = kPartOwn;
-        a.rows_from = mixed ? kFewRows + 1u : 0u;
-        e = launch_part(k, a, takes_few(k) ? p.b.seqs : own_tiles(p, tile), max_rows, stream);
+        a.rows_from = mixed ? kFewMax + 1u : 0u;
+        a.row_blocks = takes_few(k) ? static_cast<uint32_t>(ceil_div(max_rows, tile)) : 1u;
+        e = launch_part(k, a, takes_few(k) ? static_cast<uint64_t>(p.b.seqs) * a.row_blocks : own_tiles(p, tile), max_rows, stream);
         if (e == cudaSuccess && mixed) {
             a.rows_from = 0u;
-            a.rows_to = kFewRows;
+            a.rows_to = kFewMax;
+            a.row_blocks = kFewMax / kFewRows;
             a.chunk = p.few_chunk;
             a.chunks = p.few_chunks;
             a.direct = few_direct;
             a.cluster = p.few_cluster;
             a.late = 1u;
-            e = launch_part(p.kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a, p.b.seqs, kFewRows, stream);
+            e = launch_part(p.kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a,
+                            static_cast<uint64_t>(p.b.seqs) * a.row_blocks, kFewRows, stream);
         }
     }
     if (e != cudaSuccess || (own_direct && few_direct)) return e;
@@ -364,7 +371,7 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     c.own_chunks = p.own_chunks;
     c.prefix_chunk = p.prefix_chunk;
     c.prefix_chunks = p.prefix_chunks;
-    c.few_rows = p.few_chunks != 0u ? kFewRows : 0u;
+    c.few_rows = p.few_chunks != 0u ? kFewMax : 0u;
     c.few_chunk = p.few_chunk;
     c.own_direct = own_direct;
     c.few_direct = few_direct;

@@ -101,6 +101,7 @@ __device__ __forceinline__ void checked_list(const uint32_t* __restrict__ l, uin
 }
 
 constexpr uint32_t kFewRows = 8;
+constexpr uint32_t kFewMax = 16;     // rows of a sequence that still go to the few-rows kernels, in tiles of kFewRows
 constexpr uint32_t kMaxCluster = 8;  // chunks that a cluster can hold
 // The work item of a few-rows CTA: its row tile (into shared memory: token, head and
 // position of each row, position -2 where there is none) and its keys.
@@ -121,22 +122,25 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     // rows
     uint32_t s = 0, r0 = 0, nrows, t0 = 0;
     PagedSeq sq{0u, 0u, 0u};
+    r0 = rest % a.row_blocks * kFewRows;
+    rest /= a.row_blocks;
     if (a.part == kPartPrefix) {
-        nrows = a.b.tokens * a.group;
+        nrows = min(kFewRows, a.b.tokens * a.group - r0);
     } else {
         if (a.part == kPartOwn) {
             s = rest;
         } else {
-            t0 = rest / a.row_blocks;
-            r0 = (rest % a.row_blocks) * kFewRows;
+            t0 = rest;
             s = seq_of_token(a.b, t0);
             if (s == kNone) return false;
         }
         sq = load_seq(a.b, s, a.st);
         if (sq.n == 0u) return false;
+        const uint32_t rows = a.part == kPartOwn ? sq.n * a.group : a.group;
         if (a.part == kPartOwn) t0 = sq.t0;
-        if (a.part == kPartOwn && sq.n * a.group > a.rows_to) return false;  // the many-rows kernel's
-        nrows = a.part == kPartOwn ? sq.n * a.group : min(kFewRows, a.group - r0);
+        if (a.part == kPartOwn && rows > a.rows_to) return false;  // the many-rows kernel's
+        if (r0 >= rows) return false;
+        nrows = min(kFewRows, rows - r0);
     }
     if (tid < kFewRows) {
         int p = -2;
