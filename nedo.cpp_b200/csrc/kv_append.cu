@@ -49,9 +49,11 @@ __device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
 __device__ __forceinline__ float2 rotation(int p, double turns) {
     double turn = static_cast<double>(p) * turns;
     turn -= rint(turn);
-    float2 c;
-    sincospif(2.f * static_cast<float>(turn), &c.y, &c.x);
-    return c;
+    // what the fraction loses in 32 bits turns the result by the rest of the angle
+    const float f = static_cast<float>(turn), rest = static_cast<float>((turn - f) * 6.283185307179586);
+    float c, s;
+    sincospif(2.f * f, &s, &c);
+    return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
 }
 __device__ __forceinline__ void rotate4(float4& x, float4& y, const float2* c) {
     const float4 u = x, w = y;

@@ -22,7 +22,7 @@
 // TMEM: three S/P tiles and one O tile of 128 columns each.  A softmax thread never waits for
 // its own P V, so the tensor core has work while weights are formed (with S/P and O twice each
 // and the sums kept by the softmax threads, a tile took 3900 cycles of which the MMAs are 2100).
-// Registers: 64 for the softmax, 96 for the sums, 56 for the others.
+// Registers: 56 for the softmax, 112 for the sums, 56 for the others.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -376,7 +376,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         bool ok = true;
         if (warp < kSumWarp) {
             // ---- softmax: tiles half, half + 2, ...; keys of this side
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
             const uint32_t half = warp >> 3;
             constexpr uint32_t kC = kKeys / 32u;  // 16-key pieces of a side
             {
@@ -486,7 +486,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             asm volatile("bar.arrive 4, %0;" ::"n"(kSoftmax + kSums) : "memory");
         } else {
             // ---- running sums: channels of this side
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
             constexpr uint32_t kD = HD / 2u;
             const uint32_t o_addr = lanes + kBuffers * 128u + side * kD;
             float acc[kD], top = -INFINITY;
@@ -523,15 +523,18 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     const float2 alpha2 = make_float2(alpha, alpha), beta2 = make_float2(beta, beta);
                     if (!__any_sync(0xFFFFFFFFu, odd)) {
 #pragma unroll
-                        for (uint32_t k = 0; k < kD / 16u; ++k) {
-                            tmem_load(o_addr + 16u * k, x);
-                            tmem_ready(x);
+                        for (uint32_t k = 0; k < kD / 16u; k += 2u) {
+                            uint32_t y[2][16];
+                            tmem_load(o_addr + 16u * k, y[0]);
+                            tmem_load(o_addr + 16u * (k + 1u), y[1]);
+                            tmem_ready(y[0]);
+                            tmem_ready(y[1]);
 #pragma unroll
-                            for (uint32_t e = 0; e < 16u; e += 2u) {
-                                const float2 o = make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1u]));
-                                const float2 y = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), alpha2, __fmul2_rn(o, beta2));
-                                acc[16u * k + e] = y.x;
-                                acc[16u * k + e + 1u] = y.y;
+                            for (uint32_t e = 0; e < 32u; e += 2u) {
+                                const float2 o = make_float2(__uint_as_float(y[e >> 4][e & 15u]), __uint_as_float(y[e >> 4][(e & 15u) + 1u]));
+                                const float2 z = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), alpha2, __fmul2_rn(o, beta2));
+                                acc[16u * k + e] = z.x;
+                                acc[16u * k + e + 1u] = z.y;
                             }
                         }
                     } else {
