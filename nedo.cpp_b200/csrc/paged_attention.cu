@@ -341,6 +341,9 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         const bool mixed = p.few_chunks != 0u;
         const uint64_t max_rows = static_cast<uint64_t>(p.b.max_q_len) * a.group;
         a.part = kPartOwn;
+        // (one sequence is in order, many end with small tiles anyway and take longer to look through)
+        const uint64_t most = p.window ? std::min<uint64_t>(p.window, p.b.max_kv_len) : p.b.max_kv_len;
+        a.depth = p.b.seqs > 1u && p.b.seqs <= 64u ? static_cast<uint32_t>(ceil_div(most, 8u)) : 0u;
         a.rows_from = mixed ? kFewMax + 1u : 0u;
         a.row_blocks = takes_few(k) ? static_cast<uint32_t>(ceil_div(max_rows, tile)) : 1u;
         e = launch_part(k, a, takes_few(k) ? static_cast<uint64_t>(p.b.seqs) * a.row_blocks : own_tiles(p, tile), max_rows, stream);

@@ -24,7 +24,7 @@ struct AttnArgs {
     uint32_t late;           // launched while another part's kernel may still run
     float* part_o;           // [slots][tokens * heads][head_dim]
     float2* part_ml;         // [slots][tokens * heads]
-    uint32_t tiles;          // many-rows kernel: row tiles of the launch
+    uint32_t depth;          // many-rows kernels: keys by which a launch's tiles are put in order
     // own part: rows per sequence that this launch takes, from .. to (the others are another's)
     uint32_t rows_from, rows_to;
     const uint32_t* blocks;
@@ -40,30 +40,57 @@ __device__ __forceinline__ uint32_t own_begin(const PagedSeq& sq, uint32_t windo
     return lo > base ? base + ((lo - base) & ~63u) : base;
 }
 
-// One warp: the sequence and the tile within it that tile number `want` is, when every
-// sequence that this launch takes has ceil(rows / tile_rows) tiles, in order (kNone: there
-// is no such tile).
+// First of a sequence's row tiles with rows that see more than `keys` keys (or as many tiles
+// as it has): with causal rows the later tiles have the most keys, up to the window.
+__device__ __forceinline__ uint32_t first_tile_above(const AttnArgs& a, const PagedSeq& sq, uint32_t tiles, uint32_t tile_rows,
+                                                     uint32_t keys) {
+    if (a.window != 0u && keys >= a.window) return tiles;
+    const int token = static_cast<int>(keys) - static_cast<int>(sq.kv - min(sq.kv, sq.n));  // the first token that does
+    if (token <= 0) return 0u;
+    if (token >= static_cast<int>(sq.n)) return tiles;
+    const uint32_t t = (static_cast<uint32_t>(token) * a.group + tile_rows) / tile_rows;  // tiles up to the one with its first row
+    return min(tiles, t - 1u);
+}
+
+// One warp: the sequence, and the tile within it, that work item `want` is (kNone: there is no
+// such item).  Every sequence that this launch takes has ceil(rows / tile_rows) tiles.  Those with
+// many keys come first, in steps of an eighth of the most keys that a row can see (a.depth; 0:
+// not in steps), so that the launch does not end with one of them.
 __device__ __forceinline__ uint32_t find_tile(const AttnArgs& a, uint32_t want, uint32_t tile_rows, uint32_t* tile) {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-        uint32_t cnt = 0;
-        if (s0 + lane < a.b.seqs) {
-            const uint32_t rows = load_seq(a.b, s0 + lane, a.st).n * a.group;
-            if (rows >= a.rows_from && rows <= a.rows_to) cnt = (rows + tile_rows - 1u) / tile_rows;
+    uint32_t before = 0, loaded = kNone;
+    PagedSeq sq{0u, 0u, 0u};
+    for (uint32_t step = a.depth != 0u ? 8u : 1u; step-- > 0u;) {
+        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
+            uint32_t cnt = 0, first = 0;
+            if (s0 + lane < a.b.seqs) {
+                if (loaded != s0) sq = load_seq(a.b, s0 + lane, a.st);
+                loaded = s0;
+                const uint32_t rows = sq.n * a.group;
+                if (rows >= a.rows_from && rows <= a.rows_to) {
+                    cnt = (rows + tile_rows - 1u) / tile_rows;
+                    if (a.depth != 0u) {
+                        if (step != 0u) first = first_tile_above(a, sq, cnt, tile_rows, step * a.depth);
+                        const uint32_t end = step != 7u ? first_tile_above(a, sq, cnt, tile_rows, (step + 1u) * a.depth) : cnt;
+                        cnt = end - first;
+                    }
+                }
+            }
+            uint32_t inc = cnt;
+            for (uint32_t o = 1; o < 32u; o <<= 1) {
+                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > want);
+            if (hit != 0u) {
+                const uint32_t w = __ffs(hit) - 1u;
+                // within a sequence the last tile first
+                const uint32_t at = want - before - __shfl_sync(0xFFFFFFFFu, inc - cnt, w);
+                *tile = __shfl_sync(0xFFFFFFFFu, first + cnt, w) - 1u - at;
+                return s0 + w;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, inc, 31);
         }
-        uint32_t inc = cnt;
-        for (uint32_t o = 1; o < 32u; o <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > want);
-        if (hit != 0u) {
-            const uint32_t w = __ffs(hit) - 1u;
-            *tile = want - before - __shfl_sync(0xFFFFFFFFu, inc - cnt, w);
-            return s0 + w;
-        }
-        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
     *tile = 0;
     return kNone;

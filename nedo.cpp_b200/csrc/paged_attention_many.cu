@@ -59,10 +59,9 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         r0 = rest * kManyRows;
         nrows = min(kManyRows, a.b.tokens * a.group - r0);
     } else {
-        // the last tiles first: with causal rows they have the most keys
         if (warp == 0) {
             uint32_t tile;
-            const uint32_t seq = find_tile(a, a.tiles - 1u - rest, kManyRows, &tile);
+            const uint32_t seq = find_tile(a, rest, kManyRows, &tile);
             if (lane == 0u) {
                 found[0] = seq;
                 found[1] = tile;
@@ -403,9 +402,7 @@ cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_attention_many(const AttnArgs& args, uint64_t tiles, cudaStream_t stream) {
-    AttnArgs a = args;
-    a.tiles = static_cast<uint32_t>(tiles);
+cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream) {
     const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
     if (a.kv.head_dim <= 64u) return launch<64>(a, items, stream);
     if (a.kv.head_dim <= 128u) return launch<128>(a, items, stream);

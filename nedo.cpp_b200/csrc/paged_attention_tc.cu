@@ -12,17 +12,22 @@
 //   * one warp brings keys and values in by TMA (one 64-channel box per page piece, 128-byte
 //     swizzle), in the order of their use, four half-tile slots deep.  Of a tile that the
 //     item's key range cuts it zeroes the values outside, whatever the pages hold there;
-//   * one thread issues the MMAs: Q K^T three tiles ahead of P V;
+//   * one warp issues the MMAs: Q K^T three tiles ahead of P V;
 //   * warps 0-7 take the even and warps 8-15 the odd tiles, two threads to a row, each with half
 //     of the tile's keys: they read S from TMEM, agree on the row's maximum, and write the split
 //     weights over S (the A operand of P V);
 //   * warps 16-23 add every tile's O to the running sums, two threads to a row, each with half
 //     of the channels, rescaling both to the larger of the maxima they go by (the even and the
 //     odd tiles keep maxima of their own, so neither half waits for the other).
-// TMEM: three S/P tiles and one O tile of 128 columns each.  A softmax thread never waits for
-// its own P V, so the tensor core has work while weights are formed (with S/P and O twice each
-// and the sums kept by the softmax threads, a tile took 3900 cycles of which the MMAs are 2100).
+// TMEM, 512 columns: three S/P tiles and one O tile.  Two of them with the queries' halves in TMEM
+// as well (and six ring slots) took 130 us where this takes 126.
 // Registers: 56 for the softmax, 112 for the sums, 56 for the others.
+//
+// What bounds it: 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two
+// sequences over 4096 and 2550 keys, window 2048: 126 us, 688 TFLOP/s of fp16 MMAs (two for each
+// product of the formula), a tile about 3100 cycles of which the MMAs run 2050.  The rest is the round trip of
+// a tile: the softmax of its half, some 3300 cycles of exponentials, splits and TMEM traffic in
+// each of the two halves, and the waits on barriers between the roles.
 #include <algorithm>
 
 #include "paged_attention.cuh"
@@ -38,14 +43,16 @@ constexpr uint32_t kSoftmax = 512;      // softmax threads: two to a row, for th
 constexpr uint32_t kSums = 256;         // threads of the running sums: two to a row
 constexpr uint32_t kThreads = kSoftmax + kSums + 128;
 constexpr uint32_t kBuffers = 3;        // S/P tiles
+constexpr uint32_t kOColumn = kBuffers * 128u;  // TMEM columns of O
+constexpr uint32_t kTmem = 0u;          // where an allocation of the whole TMEM lies
 constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
 constexpr uint32_t kSumWarp = kSoftmax / 32u, kLoadWarp = kSumWarp + kSums / 32u, kMmaWarp = kLoadWarp + 1u;
 
 template <uint32_t HD>
 struct Tc {
     static constexpr uint32_t kBlocks = HD / 64u;
-    static constexpr uint32_t kTile = kBlocks * kBlock;   // one half of the queries, or a ring slot
-    static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u;
+    static constexpr uint32_t kTile = kBlocks * kBlock;   // a ring slot
+    static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u;  // the queries' high and low halves, the ring
 };
 
 struct TcMaps {
@@ -66,20 +73,23 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                  : "memory");
 }
-// D (TMEM) = A (shared memory) * B (shared memory) [+ D]
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// D (TMEM) = A (TMEM) * B (shared memory, the low word of its descriptor and the high one) [+ D].
+// All operands are the same in the whole warp, so that they live in uniform registers: built
+// per lane, each MMA took some 110 cycles to issue, of which it runs 64.
+template <uint32_t HIGH, uint32_t IDESC>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
-// D (TMEM) = A (TMEM) * B (shared memory) [+ D]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+template <uint32_t HIGH, uint32_t IDESC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(a_low), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
 // 16 columns of this warp's 32 lanes, a row per thread: the load is under way until
@@ -108,21 +118,43 @@ __device__ __forceinline__ void tmem_store(uint32_t addr, const uint32_t (&v)[16
 }
 
 // Shared-memory matrix descriptors, 128-byte swizzle, 8-row atoms of 1024 bytes.
-// K-major (queries, keys: rows of 64 channels): the next 8 rows 1024 bytes on.
+// K-major (keys: rows of 64 channels): the next 8 rows 1024 bytes on.
 // MN-major (values: N = channels contiguous, K = keys): 8 keys 1024 bytes on, the next 64
 // channels one block on.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
-    uint64_t d = static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(lbo >> 4) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;  // descriptor version of sm_100
-    d |= static_cast<uint64_t>(2u) << 61;  // SWIZZLE_128B
-    return d;
-}
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t lbo) { return ((addr >> 4) & 0x3FFFu) | (lbo >> 4) << 16; }
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;  // stride, sm_100's version, SWIZZLE_128B
 // kind::f16: fp16 operands, fp32 sums, M = 128, N = n; B K-major or MN-major.
 __host__ __device__ constexpr uint32_t idesc(uint32_t n, bool b_mn) {
     return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
+// Whether a phase is complete, without waiting.  A look at a barrier takes some 330 cycles here
+// (it queues behind the softmax warps' exponentials), so the warp that issues the MMAs looks at
+// all that it needs at once and waits only for what is not there.
+__device__ __forceinline__ uint32_t is_complete(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok;
+}
+// True in one lane of the (whole) warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0u;
+}
+// One arrival, and one waiting thread, for a whole warp: 32 of them on one barrier are taken one
+// after the other (256 arrivals came to some 700 cycles of every tile).
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31u) == 0u) mbar_arrive(bar);
+}
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, DeviceStatus* st, uint32_t site) {
+    return __all_sync(0xFFFFFFFFu, mbar_wait_bounded(bar, parity, st, site));
+}
+
 // Byte offset of 16-byte chunk c (of all the row's channels) of row r.
 __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return (c >> 3) * kBlock + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
@@ -134,12 +166,12 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
+    __shared__ float side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
     __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
     __shared__ uint32_t found[2], tmem_slot, gaps[8];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
     uint8_t* const sm = sm_raw + (s0 - smem_addr(sm_raw));
-    const uint32_t q_addr = s0, ring = s0 + 2u * T::kTile;
+    const uint32_t ring = s0 + 2u * T::kTile;
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t kh = blockIdx.x % a.kv.kv_heads;
     uint32_t rest = blockIdx.x / a.kv.kv_heads;
@@ -155,10 +187,9 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         r0 = rest * kRows;
         nrows = min(kRows, a.b.tokens * a.group - r0);
     } else {
-        // the last tiles first: with causal rows they have the most keys
         if (warp == 0) {
             uint32_t tile;
-            const uint32_t seq = find_tile(a, a.tiles - 1u - rest, kRows, &tile);
+            const uint32_t seq = find_tile(a, rest, kRows, &tile);
             if (lane == 0u) {
                 found[0] = seq;
                 found[1] = tile;
@@ -217,11 +248,11 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         mbar_init(&cut, 1);
         for (uint32_t i = 0; i < kBuffers; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 256);
+            mbar_init(&p_full[i], 8);
         }
         mbar_init(&o_full, 1);
-        mbar_init(&o_empty, kSums);
-        mbar_init(&q_full, kSoftmax);
+        mbar_init(&o_empty, kSums / 32u);
+        mbar_init(&q_full, kSoftmax / 32u);
         mbar_init(&done, 1);
         fence_barrier_init();
     }
@@ -234,10 +265,11 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_slot;
+    // all 512 columns: they begin at 0
+    constexpr uint32_t tmem = kTmem;
 
-    // Ring order: K0, K1, K2, V0, K3, V1, ..., V(last): the order in which the MMAs use them.
-    auto k_at = [&](uint32_t i) { return i + (i > 2u ? i - 2u : 0u); };
+    // Ring order: K0, K1, V0, K2, V1, ..., V(last): the order in which the MMAs use them.
+    auto k_at = [&](uint32_t i) { return i + (i >= kBuffers ? i - kBuffers + 1u : 0u); };
     auto v_at = [&](uint32_t i) { return i + min(ntiles, i + kBuffers); };
 
     if (warp >= kLoadWarp) {
@@ -256,8 +288,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             uint32_t issued = 0, cuts = 0;
             auto load = [&](uint32_t n, uint32_t i, uint32_t pages, bool values) {
                 const uint32_t slot = n % kSlots, dst = ring + slot * T::kTile;
-                if (ok && n >= kSlots) ok = mbar_wait_bounded(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u);
-                ok = __all_sync(0xFFFFFFFFu, ok);
+                if (ok && n >= kSlots) ok = warp_wait(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u);
                 if (!ok) return;
                 const uint32_t j = j0 + i * kKeys, there = __ballot_sync(0xFFFFFFFFu, pages != kNone);
                 const uint32_t want = __ballot_sync(
@@ -282,7 +313,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 }
                 if (patch) {
                     // values outside the item's keys count as zero
-                    ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&cut, cuts & 1u, a.st, 62u));
+                    ok = warp_wait(&cut, cuts & 1u, a.st, 62u);
                     ++cuts;
                     if (!ok) return;
                     for (uint32_t x = lane; x < kKeys * 8u * T::kBlocks; x += 32u) {
@@ -296,15 +327,14 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 }
                 issued = n + 1u;
             };
-            // pages of the tiles whose keys come next and of those whose values do, three behind
+            // pages of the tiles whose keys are in and whose values are not yet
             uint32_t pages[4] = {look_up(0), kNone, kNone, kNone}, next = look_up(1);
-            for (uint32_t i = 0; i < ntiles + kBuffers && ok; ++i) {
+            for (uint32_t i = 0; i < ntiles + kBuffers - 1u && ok; ++i) {
                 const uint32_t after = look_up(i + 2u);
                 if (i < ntiles) load(k_at(i), i, pages[0], false);
-                if (i >= 2u && i - 2u < ntiles && ok) load(v_at(i - 2u), i - 2u, pages[2], true);
-                pages[3] = pages[2];
-                pages[2] = pages[1];
-                pages[1] = pages[0];
+                if (i >= kBuffers - 1u && ok) load(v_at(i - (kBuffers - 1u)), i - (kBuffers - 1u), pages[kBuffers - 1u], true);
+#pragma unroll
+                for (uint32_t u = 3; u > 0u; --u) pages[u] = pages[u - 1u];
                 pages[0] = next;
                 next = after;
             }
@@ -312,51 +342,65 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             for (uint32_t n = issued > kSlots ? issued - kSlots : 0u; n < issued; ++n)
                 mbar_wait_bounded(&full[n % kSlots], (n / kSlots) & 1u, a.st, 63u);
         } else if (warp == kMmaWarp) {
-            if (lane == 0u) {
-                // ---- MMAs
-                bool ok = true;
-                constexpr uint32_t kS = idesc(kKeys, false), kO = idesc(HD, true);
-                auto qk = [&](uint32_t i) {
-                    const uint32_t n = k_at(i), slot = n % kSlots;
-                    ok = mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 64u);
-                    if (!ok) return;
-                    tc_fence_after();
-                    const uint32_t d = tmem + i % kBuffers * 128u;
+            // ---- MMAs: the whole warp waits, one lane issues
+            bool ok = true;
+            constexpr uint32_t kS = idesc(kKeys, false), kO = idesc(HD, true);
+            uint32_t slot = 0, turn = 0;  // ring slot of the next keys or values, and its phase
+            auto advance = [&]() {
+                slot = slot + 1u == kSlots ? 0u : slot + 1u;
+                turn ^= slot == 0u;
+            };
+            auto qk = [&](uint32_t buf, bool there) {
+                if (!there) ok = warp_wait(&full[slot], turn, a.st, 64u);
+                if (!ok) return;
+                tc_fence_after();
+                const uint32_t d = kTmem + buf * 128u, k0 = desc_low(ring + slot * T::kTile, 16u), q0 = desc_low(s0, 16u);
+                if (elect_one()) {
 #pragma unroll
                     for (uint32_t half = 0; half < 2u; ++half)  // low halves first
 #pragma unroll
-                        for (uint32_t k = 0; k < HD / 16u; ++k) {
-                            const uint32_t off = (k >> 2) * kBlock + (k & 3u) * 32u;
-                            mma_ss(d, desc(q_addr + (half ? 0u : T::kTile) + off, 16u), desc(ring + slot * T::kTile + off, 16u),
-                                   kS, half + k != 0u);
-                        }
-                    tc_commit(&s_full[i % kBuffers]);
+                        for (uint32_t k = 0; k < HD / 16u; ++k)
+                            mma_ss<kDescHigh, kS>(d, q0 + (((half ? 0u : T::kTile) + (k >> 2) * kBlock + (k & 3u) * 32u) >> 4),
+                                                  k0 + (((k >> 2) * kBlock + (k & 3u) * 32u) >> 4), half + k != 0u);
+                    tc_commit(&s_full[buf]);
                     tc_commit(&empty[slot]);
-                };
-                if (ntiles != 0u) ok = mbar_wait_bounded(&q_full, 0u, a.st, 71u);
-                for (uint32_t i = 0; i < kBuffers && i < ntiles && ok; ++i) qk(i);
-                for (uint32_t i = 0; i < ntiles && ok; ++i) {
-                    const uint32_t n = v_at(i), slot = n % kSlots;
-                    ok = mbar_wait_bounded(&full[slot], (n / kSlots) & 1u, a.st, 65u) &&
-                         mbar_wait_bounded(&p_full[i % kBuffers], (i / kBuffers) & 1u, a.st, 66u) &&
-                         (i == 0u || mbar_wait_bounded(&o_empty, (i - 1u) & 1u, a.st, 72u));
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t d = tmem + kBuffers * 128u, p = tmem + i % kBuffers * 128u;
+                }
+                __syncwarp();
+                advance();
+            };
+            if (ntiles != 0u) ok = warp_wait(&q_full, 0u, a.st, 71u);
+            for (uint32_t i = 0; i < kBuffers && i < ntiles && ok; ++i) qk(i, false);
+            for (uint32_t i = 0; i < ntiles && ok; ++i) {
+                const uint32_t buf = i % kBuffers, p_turn = (i / kBuffers) & 1u;
+                // the values, the weights, the sums' leave to write O, and the next keys
+                const uint32_t slot1 = slot + 1u == kSlots ? 0u : slot + 1u;
+                const uint32_t v_there = is_complete(&full[slot], turn), p_there = is_complete(&p_full[buf], p_turn);
+                const uint32_t o_there = i == 0u ? 1u : is_complete(&o_empty, (i - 1u) & 1u);
+                const uint32_t k_there = is_complete(&full[slot1], turn ^ (slot1 == 0u));
+                const bool k_now = __all_sync(0xFFFFFFFFu, k_there);
+                ok = (__all_sync(0xFFFFFFFFu, v_there) || warp_wait(&full[slot], turn, a.st, 65u)) &&
+                     (__all_sync(0xFFFFFFFFu, p_there) || warp_wait(&p_full[buf], p_turn, a.st, 66u)) &&
+                     (__all_sync(0xFFFFFFFFu, o_there) || warp_wait(&o_empty, (i - 1u) & 1u, a.st, 72u));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t p = kTmem + buf * 128u, v0 = desc_low(ring + slot * T::kTile, kBlock);
+                if (elect_one()) {
 #pragma unroll
                     for (uint32_t half = 0; half < 2u; ++half)
 #pragma unroll
                         for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 + 8 columns of weights, 2048 bytes of values
-                            mma_ts(d, p + k * 16u + (half ? 0u : 8u),
-                                   desc(ring + slot * T::kTile + k * 2048u, kBlock), kO, half + k != 0u);
+                            mma_ts<kDescHigh, kO>(kTmem + kOColumn, p + k * 16u + (half ? 0u : 8u), v0 + k * (2048u >> 4),
+                                                  half + k != 0u);
                     tc_commit(&o_full);
                     tc_commit(&empty[slot]);
-                    if (i + kBuffers < ntiles) qk(i + kBuffers);
                 }
-                tc_commit(&done);  // every MMA issued above has completed when this arrives
-                mbar_wait_bounded(&done, 0u, a.st, 67u);
+                __syncwarp();
+                advance();
+                if (i + kBuffers < ntiles) qk(buf, k_now);
             }
+            if (elect_one()) tc_commit(&done);  // every MMA issued above has completed when this arrives
             __syncwarp();
+            warp_wait(&done, 0u, a.st, 67u);
         }
     } else {
         const uint32_t r = tid & 127u, side = (warp >> 2) & 1u;
@@ -379,45 +423,49 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
             const uint32_t half = warp >> 3;
             constexpr uint32_t kC = kKeys / 32u;  // 16-key pieces of a side
+            float unscale;
             {
                 // queries: a row per four threads, scaled, split, stored
-                const uint32_t rq = tid >> 2, part = tid & 3u;
-                const int pq = row_pos[rq];
-                const float* q = a.q + (static_cast<size_t>(row_tok[rq]) * a.heads + row_head[rq]) * hd;
+                constexpr uint32_t kPart = HD / 4u;  // channels of a thread
+                const uint32_t part = warp >> 2;
+                const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd + part * kPart;
+                float4 x[kPart / 4u];
                 float big = 0.f;
-                if (pq >= 0)
-                    for (uint32_t d = part * 4u; d < hd; d += 16u) {
-                        const float4 x = *reinterpret_cast<const float4*>(q + d);
-                        big = fmaxf(big, fmaxf(fmaxf(fabsf(x.x * a.scale_log2), fabsf(x.y * a.scale_log2)),
-                                               fmaxf(fabsf(x.z * a.scale_log2), fabsf(x.w * a.scale_log2))));
-                    }
-                big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-                big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+#pragma unroll
+                for (uint32_t e = 0; e < kPart / 4u; ++e) {
+                    x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (p >= 0 && part * kPart + 4u * e < hd) x[e] = *reinterpret_cast<const float4*>(q + 4u * e);
+                    x[e] = make_float4(x[e].x * a.scale_log2, x[e].y * a.scale_log2, x[e].z * a.scale_log2, x[e].w * a.scale_log2);
+                    big = fmaxf(big, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
+                }
+                side_max[0][part][r] = big;
+                named_barrier_sync(3, kSoftmax);
+                big = fmaxf(fmaxf(side_max[0][0][r], side_max[0][1][r]), fmaxf(side_max[0][2][r], side_max[0][3][r]));
                 const int e2 = up_exponent(big);
                 const float up = power_of_two(e2);
-                if (part == 0u) row_unscale[rq] = power_of_two(-e2);
-                for (uint32_t d = part * 8u; d < HD; d += 32u) {
-                    uint32_t hi[4], lo[4];
+                unscale = power_of_two(-e2);
+                uint32_t hi[kPart / 2u], lo[kPart / 2u];
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; e += 2) {
-                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (pq >= 0 && d < hd) x = *reinterpret_cast<const float4*>(q + d + 2u * e);
-                        split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
-                        split(x.z * a.scale_log2 * up, x.w * a.scale_log2 * up, &hi[e + 1u], &lo[e + 1u]);
-                    }
-                    *reinterpret_cast<uint4*>(sm + at(rq, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(sm + T::kTile + at(rq, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                for (uint32_t e = 0; e < kPart / 4u; ++e) {
+                    split(x[e].x * up, x[e].y * up, &hi[2u * e], &lo[2u * e]);
+                    split(x[e].z * up, x[e].w * up, &hi[2u * e + 1u], &lo[2u * e + 1u]);
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < kPart / 8u; ++e) {
+                    const uint32_t ch = part * (kPart / 8u) + e;
+                    *reinterpret_cast<uint4*>(sm + at(r, ch)) = make_uint4(hi[4u * e], hi[4u * e + 1u], hi[4u * e + 2u], hi[4u * e + 3u]);
+                    *reinterpret_cast<uint4*>(sm + T::kTile + at(r, ch)) =
+                        make_uint4(lo[4u * e], lo[4u * e + 1u], lo[4u * e + 2u], lo[4u * e + 3u]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&q_full);
-                named_barrier_sync(3, kSoftmax);
+                warp_arrive(&q_full);
+                named_barrier_sync(3, kSoftmax);  // the maxima have been read: their place serves the tiles
             }
-            const float unscale = row_unscale[r];
             float m = -INFINITY, l = 0.f;
-            for (uint32_t i = half; i < ntiles && ok; i += 2u) {
+            for (uint32_t i = half; i < ntiles; i += 2u) {
                 const uint32_t buf = i % kBuffers, j = j0 + i * kKeys, st_addr = lanes + buf * 128u + side * 64u;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&s_full[buf], (i / kBuffers) & 1u, a.st, 68u));
-                if (!ok) break;
+                // (a warp whose wait ran out goes on through the barriers that it shares with others)
+                if (ok) ok = warp_wait(&s_full[buf], (i / kBuffers) & 1u, a.st, 68u);
                 tc_fence_after();
                 const bool mine = j < we && j + kKeys > wb;  // a tile that none of the warp's rows sees is passed over
                 const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 7u]);
@@ -479,7 +527,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 // read behind P V: its place is free again once the sums have come three tiles further
                 if (side == 0u) tile_ref[i % (2u * kBuffers)][r] = m;
                 tc_fence_before();
-                mbar_arrive(&p_full[buf]);
+                warp_arrive(&p_full[buf]);
             }
             sum_l[half * 2u + side][r] = p >= 0 ? l : 0.f;  // padding sees nothing
             if (side == 0u) sum_m[half][r] = m == -INFINITY ? 0.f : m;
@@ -488,13 +536,13 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             // ---- running sums: channels of this side
             asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
             constexpr uint32_t kD = HD / 2u;
-            const uint32_t o_addr = lanes + kBuffers * 128u + side * kD;
+            const uint32_t o_addr = lanes + kOColumn + side * kD;
             float acc[kD], top = -INFINITY;
 #pragma unroll
             for (uint32_t d = 0; d < kD; ++d) acc[d] = 0.f;
             for (uint32_t i = 0; i < ntiles && ok; ++i) {
                 const uint32_t j = j0 + i * kKeys;
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&o_full, i & 1u, a.st, 70u));
+                ok = warp_wait(&o_full, i & 1u, a.st, 70u);
                 if (!ok) break;
                 tc_fence_after();
                 if (j < we && j + kKeys > wb) {
@@ -558,7 +606,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(&o_empty);
+                warp_arrive(&o_empty);
             }
             // the weight sums of both halves, then the rows' results through shared memory (the ring
             // is done with)
@@ -596,7 +644,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     __syncthreads();
     if (warp == kMmaWarp) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_slot), "r"(512u));
     }
 }
 
@@ -630,9 +678,7 @@ cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_attention_tc(const AttnArgs& args, uint64_t tiles, cudaStream_t stream) {
-    AttnArgs a = args;
-    a.tiles = static_cast<uint32_t>(tiles);
+cudaError_t launch_attention_tc(const AttnArgs& a, uint64_t tiles, cudaStream_t stream) {
     const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
     return a.kv.head_dim <= 64u ? launch<64>(a, items, stream) : launch<128>(a, items, stream);
 }
