@@ -180,7 +180,8 @@ __device__ uint32_t find_largest(const K* key, uint32_t n, uint32_t left, uint32
 constexpr uint32_t kStages = 2;  // three run no faster: fewer CTAs fit (48 tokens x 4 heads: 26.2 us with two, 27.2 with three)
 
 // PIECES: 16-byte pieces of a page's bounds per lane.  Dynamic shared memory: key_words words of
-// 64 bits for the keys, then the warps' rings.
+// 32 bits for the keys, then the warps' rings.  Keys of 64 bits lie over both: they are formed
+// when the rings are done with.
 template <typename T, uint32_t PIECES>
 __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, PagedBatch b, uint32_t heads,
                                                                 const float* __restrict__ q, uint32_t picks,
@@ -224,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
         const uint32_t k = 4u * m + (lane >> 3), i = i0 + k * stride + (lane & 7u);
         return k < ng && i < others ? load_page(b, kv, s, i, st) : kNone;
     };
-    uint4* const ring = reinterpret_cast<uint4*>(key64 + key_words) + warp * kStages * kGroup * PIECES * 32u;
+    uint4* const ring = reinterpret_cast<uint4*>(key + key_words) + warp * kStages * kGroup * PIECES * 32u;
     uint32_t now = look_up(0), then = look_up(1), top = 0u;
     auto fetch = [&](uint32_t k, uint32_t m) {
         if (k < ng) {
@@ -484,8 +485,8 @@ template <typename T, uint32_t PIECES>
 cudaError_t launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* q, uint32_t picks,
                    uint32_t* blocks, DeviceStatus* st, cudaStream_t stream) {
     const uint32_t pages = (b.max_kv_len + kv.page_size - 1u) >> kv.page_shift;
-    const uint32_t key_words = (pages + 1u) & ~1u;
-    const size_t smem = key_words * sizeof(uint64_t) + kWarps * kStages * kGroup * PIECES * 512u;
+    const uint32_t key_words = (pages + 3u) & ~3u;
+    const size_t smem = std::max(key_words * sizeof(uint64_t), key_words * sizeof(uint32_t) + kWarps * kStages * kGroup * PIECES * 512u);
     cudaError_t e = cudaFuncSetAttribute(block_select_kernel<T, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(smem));
     if (e != cudaSuccess) return e;

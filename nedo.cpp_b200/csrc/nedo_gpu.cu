@@ -1663,8 +1663,9 @@ int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_
         return fail(NEDO_GPU_ERR_ARG, w + "head_dim must be a multiple of 8 in 8..256");
     if (c->page_size < 16u || c->page_size > 256u || (c->page_size & (c->page_size - 1u)))
         return fail(NEDO_GPU_ERR_ARG, w + "page_size must be 16, 32, 64, 128 or 256");
-    if (c->num_pages == 0 || c->num_pages >= 0xFFFFFFFFull)
-        return fail(NEDO_GPU_ERR_ARG, w + "num_pages must be in 1..2^32-2");
+    // (512 GiB of keys at least; below it, a page and head is a signed TMA coordinate)
+    if (c->num_pages == 0 || c->num_pages >= 0x80000000ull || c->num_pages * c->kv_heads >= 0x80000000ull)
+        return fail(NEDO_GPU_ERR_ARG, w + "num_pages * kv_heads must be in 1..2^31-1");
     if (!c->k || !c->v) return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
     if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->bounds))
         return fail(NEDO_GPU_ERR_ARG, w + "cache buffers must be 16-byte aligned");
@@ -1676,6 +1677,7 @@ int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_
         return fail(NEDO_GPU_ERR_ARG, w + "shared_pages exceeds max_pages");
     if (b->seqs && b->tokens && (!b->q_start || !b->kv_len || (b->max_pages && !b->page_table)))
         return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    if (b->seqs && b->tokens && !b->max_q_len) return fail(NEDO_GPU_ERR_ARG, w + "max_q_len must be positive");
     uint32_t shift = 0;
     while ((1u << shift) < c->page_size) ++shift;
     kv->type = c->type;
@@ -1714,7 +1716,7 @@ int plan_attention(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_
                    uint32_t window, const uint32_t* blocks, uint32_t picks, PagedAttention* a) {
     if (int rc = check_paged(what, c, b, heads, &a->kv, &a->b)) return rc;
     a->heads = heads;
-    a->window = window;
+    a->window = window > b->max_kv_len ? 0u : window;  // wider than any sequence: no limit
     a->shared_pages = picks ? 0u : b->shared_pages;
     a->blocks = blocks;
     a->picks = picks;

@@ -156,10 +156,8 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
-        case Kernel::kMany: {  // 64 rows through the tensor cores, two items to an SM
-            const uint32_t slots = 148u * (hd <= 128u ? 2u : 1u);
-            return {kManyRows, slots, 0u, hd <= 64u ? 17.0 : 34.0, 5000.0, 1.0};
-        }
+        case Kernel::kMany:  // 64 rows of a head above 128 through the tensor cores, an item to an SM
+            return {kManyRows, 148u, 0u, 34.0, 5000.0, 1.0};
         case Kernel::kTc:  // 128 rows through 32 MMAs per 128 keys, an item to an SM
             return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 5000.0, 1.0};
         case Kernel::kFew32: {
@@ -219,8 +217,7 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
     if (kv.type != kF16) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
     if (rows <= kFewMax) return Kernel::kFew;
-    const bool tc = kv.head_dim <= 128u && static_cast<uint64_t>(kv.num_pages) * kv.kv_heads < (1ull << 31);
-    return tc ? Kernel::kTc : Kernel::kMany;
+    return kv.head_dim <= 128u ? Kernel::kTc : Kernel::kMany;
 }
 Kernel prefix_kernel(const PagedAttention& a) {
     return kernel_for(a.kv, static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads));

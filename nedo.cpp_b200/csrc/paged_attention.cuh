@@ -367,8 +367,8 @@ cudaError_t launch_items(const AttnArgs& a, void (*kernel)(Args...), uint64_t it
 // (paged_attention_few.cu), F32 caches on the CUDA cores (paged_attention_few32.cu).
 cudaError_t launch_attention_few(const AttnArgs& a, uint64_t items, cudaStream_t stream);
 cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_t items, cudaStream_t stream);
-// The many-rows kernel on the tensor cores (paged_attention_many.cu): F16 caches, row
-// tiles of kManyRows.
+// Tiles of kManyRows rows on the tensor cores (paged_attention_many.cu): F16 caches, heads
+// above 128.
 constexpr uint32_t kManyRows = 64;
 cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
 // Tiles of many32_rows(head_dim) rows of F32 caches on the tensor cores
@@ -376,7 +376,7 @@ cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_
 uint32_t many32_rows(uint32_t head_dim);
 cudaError_t launch_attention_many32(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
 // Tiles of kTcRows rows on the 5th-generation tensor cores (paged_attention_tc.cu): F16
-// caches, heads of up to 128 channels, num_pages * kv_heads below 2^31.
+// caches, heads of up to 128 channels.
 constexpr uint32_t kTcRows = 128;
 cudaError_t launch_attention_tc(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
 

@@ -7,7 +7,11 @@
 // lo hi + hi lo + hi hi; what is left out is 2^-22 of the product.  Queries are scaled by a
 // power of two per row, keys and values by one per tile, to where the low halves are normal
 // numbers; the weights as in the other kernels.  A tile's weighted values are summed from zero
-// and added to the running sums in fp32, which also takes the tile's scale back.
+// and added to the running sums in fp32, which also takes the tile's scale back.  Under the
+// tile's scale a number keeps 2^-38 of the tile's largest: less than its own 22 bits where it is
+// below 2^-16 of that.  A tile in which some key or value is that much smaller than another as
+// a whole (a row must not lose its digits to one that it may not even see) is done in fp32, key
+// by key; so is one with values that are not finite and rows that do not see all of it.
 //
 // Work.  A CTA of one warp for 16 rows (128 rows, 64 for heads above 128) takes its rows through
 // their keys in tiles of 64 (32).  The next tile's keys and values are on their way (cp.async)
@@ -56,7 +60,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float row_unscale[kRows], size[2][M::kWarps];
+    __shared__ float row_unscale[kRows], size[2][M::kWarps], least[2][M::kWarps];
     __shared__ uint32_t found[2], odd_warp[M::kWarps];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t kh = blockIdx.x % a.kv.kv_heads;
@@ -237,23 +241,35 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         const uint32_t have = there, j = j0 + i * kKeys;
         cp_wait<0>();
         // the tile as halves: every thread its own pieces (the ones it copied), first their sizes
-        float big[2] = {0.f, 0.f};
+        float big[2] = {0.f, 0.f}, small[2] = {INFINITY, INFINITY};
         bool odd = false;
+        constexpr uint32_t kLanes = HD / 4u < 32u ? HD / 4u : 32u;  // lanes that hold a key's (or half a key's) channels
+        const uint32_t lanes = kLanes == 32u ? 0xFFFFFFFFu : ((1u << kLanes) - 1u) << (lane & ~(kLanes - 1u));
 #pragma unroll 4
         for (uint32_t x = 0; x < kPieces; ++x) {
             const uint32_t piece = (piece_row + x * kAtOnce) * (HD / 4u) + piece_ch;
 #pragma unroll
             for (uint32_t kv = 0; kv < 2u; ++kv) {
                 const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
-                big[kv] = fmaxf(big[kv], fmaxf(fmaxf(finite_size(v.x), finite_size(v.y)), fmaxf(finite_size(v.z), finite_size(v.w))));
+                const float most = fmaxf(fmaxf(finite_size(v.x), finite_size(v.y)), fmaxf(finite_size(v.z), finite_size(v.w)));
+                // (magnitudes order like their bits)
+                const float row = __uint_as_float(__reduce_max_sync(lanes, __float_as_uint(most)));
+                big[kv] = fmaxf(big[kv], row);
+                if (row != 0.f) small[kv] = fminf(small[kv], row);
                 if (kv == 1u) odd |= !(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) < INFINITY) ||
                                      v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
             }
         }
 #pragma unroll
         for (uint32_t kv = 0; kv < 2u; ++kv) {
-            for (int o = 16; o > 0; o >>= 1) big[kv] = fmaxf(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], o));
-            if (lane == 0u) size[kv][warp] = big[kv];
+            if constexpr (kLanes < 32u) {
+                big[kv] = fmaxf(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], 16));
+                small[kv] = fminf(small[kv], __shfl_xor_sync(0xFFFFFFFFu, small[kv], 16));
+            }
+            if (lane == 0u) {
+                size[kv][warp] = big[kv];
+                least[kv][warp] = small[kv];
+            }
         }
         odd = __any_sync(0xFFFFFFFFu, odd);
         if (lane == 0u) odd_warp[warp] = odd;
@@ -261,10 +277,14 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         odd = false;
 #pragma unroll
         for (uint32_t w = 0; w < M::kWarps; ++w) {
-            big[0] = fmaxf(big[0], size[0][w]);
-            big[1] = fmaxf(big[1], size[1][w]);
+#pragma unroll
+            for (uint32_t kv = 0; kv < 2u; ++kv) {
+                big[kv] = fmaxf(big[kv], size[kv][w]);
+                small[kv] = fminf(small[kv], least[kv][w]);
+            }
             odd |= odd_warp[w] != 0u;
         }
+        const bool wild = big[0] > small[0] * 65536.f || big[1] > small[1] * 65536.f;
         const int ek = up_exponent(big[0]), ev = up_exponent(big[1]);
         const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek), v_down = power_of_two(-ev);
 #pragma unroll 4
@@ -286,9 +306,35 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         look_up(i + 2u);
         __syncthreads();
         if (j < we && j + kKeys > wb) {
+            const bool whole = have == (1u << kGroups) - 1u && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
+            const bool slow = wild || (odd && !whole);
             float sc[kCols][4];
 #pragma unroll
             for (uint32_t n = 0; n < kCols; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            // where key `key` of the tile lies in the cache, if it is one of the item's
+            auto in_tile = [&](uint32_t key) { return key >= kb && key < ke && (have >> ((key - j) >> 4) & 1u); };
+            auto place = [&](uint32_t key) -> size_t {
+                const uint32_t page = a.b.table[static_cast<size_t>(s) * a.b.max_pages + (key >> a.kv.page_shift)];
+                return ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size + (key & (a.kv.page_size - 1u))) * hd;
+            };
+            if (slow) {
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const uint32_t r = warp * 16u + g + 8u * h;
+                    const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+#pragma unroll
+                    for (uint32_t n = 0; n < kCols; ++n)
+#pragma unroll
+                        for (uint32_t e = 0; e < 2; ++e) {
+                            const uint32_t key = j + n * 8u + t2 + e;
+                            if (!in_tile(key) || key < lo_key[h] || key >= hi_key[h]) continue;
+                            const float* kr = kbase + place(key);
+                            float sum = 0.f;
+                            for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, kr[d], sum);
+                            sc[n][2 * h + e] = sum;
+                        }
+                }
+            } else {
 #pragma unroll
             for (uint32_t turn = 0; turn < 3u; ++turn) {  // lo hi, hi lo, hi hi
 #pragma unroll
@@ -304,7 +350,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                     }
                 }
             }
-            const bool whole = have == (1u << kGroups) - 1u && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
+            }
+            const float k_one = slow ? 1.f : k_down;
             if (!whole) {
 #pragma unroll
                 for (uint32_t n = 0; n < kCols; ++n)
@@ -324,8 +371,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                 mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
                 mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
                 // the two powers one after the other: together they may leave fp32's range
-                down[h] = unscale[h];
-                const float mn = fmaxf(m[h], mt * down[h] * k_down);
+                down[h] = slow ? 1.f : unscale[h];
+                const float mn = fmaxf(m[h], mt * down[h] * k_one);
                 alpha[h] = mn == -INFINITY ? 1.f : exp2_fast(m[h] - mn);
                 m[h] = mn;
                 ref[h] = (mn == -INFINITY ? 0.f : mn) - kUp;
@@ -336,13 +383,13 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
             for (uint32_t n = 0; n < kCols; ++n) {
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) {
-                    sc[n][e] = exp2_fast(fmaf(sc[n][e] * down[e >> 1], k_down, -ref[e >> 1]));
+                    sc[n][e] = exp2_fast(fmaf(sc[n][e] * down[e >> 1], k_one, -ref[e >> 1]));
                     l[e >> 1] += sc[n][e];
                 }
                 split(sc[n][0], sc[n][1], &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
                 split(sc[n][2], sc[n][3], &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
             }
-            if (whole || !odd) {
+            if (!slow) {
 #pragma unroll
                 for (uint32_t n = 0; n < HD / 16; ++n) {
                     float o[2][4];
@@ -377,7 +424,6 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                     }
                 }
             } else {
-                // a value that is not finite must not reach the rows that do not see it (0 * inf)
 #pragma unroll
                 for (uint32_t n = 0; n < HD / 8; ++n)
 #pragma unroll
@@ -393,14 +439,13 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                             const float w1 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h + 1], from);
                             w[h] = jj & 1u ? w1 : w0;
                         }
-                        const bool in = key >= kb && key < ke && (have >> (n8 >> 1) & 1u);
-                        const bool see0 = in && key >= lo_key[0] && key < hi_key[0], see1 = in && key >= lo_key[1] && key < hi_key[1];
+                        if (!in_tile(key)) continue;
+                        const bool see0 = key >= lo_key[0] && key < hi_key[0], see1 = key >= lo_key[1] && key < hi_key[1];
+                        const float* vr = vbase + place(key);
 #pragma unroll
                         for (uint32_t n = 0; n < HD / 8; ++n) {
-                            const uint8_t* at_v = halves + 2u * M::kHalfBytes + at<HD>(n8 * 8u + jj, n) + t2 * 2u;
-                            const float2 fh = __half22float2(*reinterpret_cast<const __half2*>(at_v));
-                            const float2 fl = __half22float2(*reinterpret_cast<const __half2*>(at_v + M::kHalfBytes));
-                            const float f0 = (fh.x + fl.x) * v_down, f1 = (fh.y + fl.y) * v_down;
+                            if (n * 8u >= hd) continue;
+                            const float f0 = vr[n * 8u + t2], f1 = vr[n * 8u + t2 + 1u];
                             if (see0) {
                                 acc[n][0] = fmaf(w[0], f0, acc[n][0]);
                                 acc[n][1] = fmaf(w[0], f1, acc[n][1]);

@@ -47,6 +47,7 @@ def calls(lib, c, b, heads=12):
     (dict(page_size=512), 12, nedo_gpu.ERR_ARG, "page_size"),
     (dict(num_pages=0), 12, nedo_gpu.ERR_ARG, "num_pages"),
     (dict(num_pages=1 << 32), 12, nedo_gpu.ERR_ARG, "num_pages"),
+    (dict(num_pages=1 << 29), 12, nedo_gpu.ERR_ARG, "num_pages"),
     (dict(k=None), 12, nedo_gpu.ERR_ARG, "null pointer"),
     (dict(v=None), 12, nedo_gpu.ERR_ARG, "null pointer"),
     (dict(k=A + 8), 12, nedo_gpu.ERR_ARG, "16-byte aligned"),
@@ -69,6 +70,7 @@ def test_bad_cache_refused(lib, kw, heads, code, msg):
     (dict(q_start=None), "null pointer"),
     (dict(kv_len=None), "null pointer"),
     (dict(page_table=None), "null pointer"),
+    (dict(max_q_len=0), "max_q_len"),
 ])
 def test_bad_batch_refused(lib, kw, msg):
     for call in calls(lib, cache(), batch(**kw)):

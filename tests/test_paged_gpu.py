@@ -155,6 +155,39 @@ def test_value_sizes(lib, cuda, type_):
 
 
 @pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,hd,window", [(6, 64, 0), (6, 128, 0), (2, 256, 0), (6, 40, 30)])
+def test_keys_and_values_of_very_different_size(lib, cuda, type_, heads, hd, window):
+    """Rows that do not see a far larger key or value next to theirs keep all their digits."""
+    s = Setup(type_, heads, 2, hd, 16, q=[70, 1, 90], kv=[150, 90, 91], seed=30)
+    large, small = (3e3, 1e-4) if type_ == F16 else (1e25, 1e-25)
+    for seq, pos, f in ((0, 146, large), (0, 100, small), (1, 88, small), (2, 30, large), (2, 31, small), (2, 88, large)):
+        at = s.table[seq, pos // 16], slice(None), pos % 16
+        s.v[at] = (s.v[at].astype(np.float64) * f).astype(s.v.dtype)
+        s.k[at] = (s.k[at].astype(np.float64) * (f if f < 1 else 1e3)).astype(s.k.dtype)
+    d = Device(lib, cuda, s)
+    check_attention(s, d.attention(window), s.attention(window))
+    lib.status()
+
+
+@pytest.mark.parametrize("q", [1, 9, 40])
+@pytest.mark.parametrize("type_", [F16, F32])
+def test_windows_wider_than_any_sequence(lib, cuda, type_, q):
+    d = dev(lib, cuda, type_, 6, 2, 64, 16, q=[q, q], kv=[200, 90], seed=31)
+    whole = d.attention().clone()
+    for window in (200, 201, 2 ** 31 - 1, 2 ** 31, 2 ** 32 - 1):
+        assert cuda.equal(d.attention(window), whole), window
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("q", [1, 40])
+def test_nothing_cached_anywhere(lib, cuda, type_, q):
+    d = dev(lib, cuda, type_, 6, 2, 64, 16, q=[q, 0, 1], kv=[0, 0, 0], tail=1, seed=32)
+    d.batch.max_pages, d.batch.page_table = 0, None
+    check_attention(d.s, d.attention(), d.s.attention())
+    lib.status()
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_values_that_are_not_finite(lib, cuda, type_, bad):
     """A value that is not finite reaches the rows that see it, in its channel, and no other row."""
@@ -392,6 +425,17 @@ def test_select_many_pages(lib, cuda, pages, picks):
     s = Setup(F16, 3, 1, 64, 16, q=[1, 1], kv=[pages * 16, pages * 11 + 5], seed=23)
     d = Device(lib, cuda, s)
     assert np.array_equal(d.select(picks).cpu().numpy().view(np.uint32), s.select(picks))
+
+
+@pytest.mark.parametrize("type_,hd", [(F16, 256), (F32, 256), (F32, 128)])
+def test_select_most_pages_of_wide_heads(lib, cuda, type_, hd):
+    """The most pages that a selection takes, their numbers and the copies in flight in shared
+    memory together; equal scores everywhere take the path that scores all pages in 64 bits."""
+    s = Setup(type_, 2, 1, hd, 16, q=[1], kv=[90], seed=33)
+    s.kv, s.max_pages = [16384 * 16], 16384
+    s.table = s.table[:, np.arange(16384) % 6]  # six pages, over and over
+    d = Device(lib, cuda, s)
+    assert np.array_equal(d.select(40).cpu().numpy().view(np.uint32), s.select(40))
 
 
 # ------------------------------------------------------ attention over picked pages
