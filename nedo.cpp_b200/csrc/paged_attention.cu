@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kFew32, kMany, kMany32, kTc };
+enum class Kernel { kFew, kFew16, kFew32, kMany, kMany32, kTc };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -152,9 +152,10 @@ struct Cost {
 Cost cost_of(Kernel k, const PagedKv& kv) {
     const uint32_t hd = kv.head_dim;
     switch (k) {
-        case Kernel::kFew: {  // reads 4 hd bytes per key of the SMs' common 6.5 TB/s
+        case Kernel::kFew:
+        case Kernel::kFew16: {  // reads 4 hd bytes per key of the SMs' common 6.5 TB/s
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
-            return {kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
+            return {k == Kernel::kFew ? kFewRows : 2u * kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
         case Kernel::kMany:  // 64 rows of a head above 128 through the tensor cores, an item to an SM
             return {kManyRows, 148u, 0u, 34.0, 5000.0, 1.0};
@@ -216,22 +217,27 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 // The kernel of a part whose row tiles have up to `rows` rows.
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
     if (kv.type != kF16) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
-    if (rows <= kFewMax) return Kernel::kFew;
+    if (rows <= kFewRows || (rows <= kFewMax && kv.head_dim > 128u)) return Kernel::kFew;
+    if (rows <= kFewMax) return Kernel::kFew16;
     return kv.head_dim <= 128u ? Kernel::kTc : Kernel::kMany;
 }
 Kernel prefix_kernel(const PagedAttention& a) {
     return kernel_for(a.kv, static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads));
 }
 Kernel own_kernel(const PagedAttention& a) {
-    return kernel_for(a.kv, a.picks ? 1u : static_cast<uint64_t>(a.b.max_q_len) * (a.heads / a.kv.kv_heads));
+    const uint32_t group = a.heads / a.kv.kv_heads;
+    return kernel_for(a.kv, a.picks ? std::min(group, kFewMax) : static_cast<uint64_t>(a.b.max_q_len) * group);
 }
-bool takes_few(Kernel k) { return k == Kernel::kFew || k == Kernel::kFew32; }
+// The kernel of the sequences with few rows among others with many: mostly single tokens.
+Kernel few_kernel(const PagedAttention& a) { return kernel_for(a.kv, std::min(a.heads / a.kv.kv_heads, kFewMax)); }
+bool takes_few(Kernel k) { return k == Kernel::kFew || k == Kernel::kFew16 || k == Kernel::kFew32; }
 
 // A part on its kernel: `tiles` row tiles of up to max_rows rows, times KV heads and chunks.
 cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t max_rows, cudaStream_t stream) {
     const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
     switch (k) {
-        case Kernel::kFew: return launch_attention_few(a, items, stream);
+        case Kernel::kFew: return launch_attention_few(a, kFewRows, items, stream);
+        case Kernel::kFew16: return launch_attention_few(a, 2u * kFewRows, items, stream);
         case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
         case Kernel::kMany: return launch_attention_many(a, tiles, stream);
         case Kernel::kTc: return launch_attention_tc(a, tiles, stream);
@@ -272,8 +278,9 @@ bool plan_paged_attention(PagedAttention* a) {
     a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
     if (!takes_few(own) && a->b.seqs > 1u) {
-        const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / kFewRows);
-        a->few_chunk = chunk_keys(keys, u, sums, a->kv, cost_of(a->kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a->kv), alone);
+        const Cost few = cost_of(few_kernel(*a), a->kv);
+        const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / few.rows);
+        a->few_chunk = chunk_keys(keys, u, sums, a->kv, few, alone);
         a->few_chunks = chunks(a->few_chunk);
         a->few_cluster = alone && a->few_chunks > 1u && a->few_chunks <= kMaxCluster;
         grid = std::max(grid, u * a->few_chunks);
@@ -316,8 +323,8 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         a.slot0 = 0;
         const Kernel k = prefix_kernel(p);
         const uint64_t all = static_cast<uint64_t>(p.b.tokens) * a.group;
-        a.row_blocks = static_cast<uint32_t>(ceil_div(all, kFewRows));
-        e = launch_part(k, a, ceil_div(all, cost_of(k, p.kv).rows), all, stream);
+        a.row_blocks = static_cast<uint32_t>(ceil_div(all, cost_of(k, p.kv).rows));
+        e = launch_part(k, a, a.row_blocks, all, stream);
         if (e != cudaSuccess) return e;
         a.late = 1u;
     }
@@ -347,14 +354,14 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         if (e == cudaSuccess && mixed) {
             a.rows_from = 0u;
             a.rows_to = kFewMax;
-            a.row_blocks = kFewMax / kFewRows;
+            const Kernel few = few_kernel(p);
+            a.row_blocks = kFewMax / cost_of(few, p.kv).rows;
             a.chunk = p.few_chunk;
             a.chunks = p.few_chunks;
             a.direct = few_direct;
             a.cluster = p.few_cluster;
             a.late = 1u;
-            e = launch_part(p.kv.type == kF16 ? Kernel::kFew : Kernel::kFew32, a,
-                            static_cast<uint64_t>(p.b.seqs) * a.row_blocks, kFewRows, stream);
+            e = launch_part(few, a, static_cast<uint64_t>(p.b.seqs) * a.row_blocks, kFewRows, stream);
         }
     }
     if (e != cudaSuccess || (own_direct && few_direct)) return e;

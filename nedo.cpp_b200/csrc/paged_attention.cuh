@@ -128,7 +128,7 @@ __device__ __forceinline__ void checked_list(const uint32_t* __restrict__ l, uin
 }
 
 constexpr uint32_t kFewRows = 8;
-constexpr uint32_t kFewMax = 16;     // rows of a sequence that still go to the few-rows kernels, in tiles of kFewRows
+constexpr uint32_t kFewMax = 16;     // rows of a sequence that still go to the few-rows kernels, in tiles of 8 or 16
 constexpr uint32_t kMaxCluster = 8;  // chunks that a cluster can hold
 // The work item of a few-rows CTA: its row tile (into shared memory: token, head and
 // position of each row, position -2 where there is none) and its keys.
@@ -137,7 +137,8 @@ struct FewItem {
     uint32_t kb, ke;         // keys: positions, or places in the page list (`list`)
     uint32_t all_b, all_e;   // positions seen by every row
 };
-// False: nothing to do.  All threads of the CTA.
+// False: nothing to do.  All threads of the CTA.  ROWS: rows of a tile.
+template <uint32_t ROWS>
 __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, uint32_t* row_head, int* row_pos,
                                           uint32_t* list, FewItem* it) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5;
@@ -149,10 +150,10 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     // rows
     uint32_t s = 0, r0 = 0, nrows, t0 = 0;
     PagedSeq sq{0u, 0u, 0u};
-    r0 = rest % a.row_blocks * kFewRows;
+    r0 = rest % a.row_blocks * ROWS;
     rest /= a.row_blocks;
     if (a.part == kPartPrefix) {
-        nrows = min(kFewRows, a.b.tokens * a.group - r0);
+        nrows = min(ROWS, a.b.tokens * a.group - r0);
     } else {
         if (a.part == kPartOwn) {
             s = rest;
@@ -167,9 +168,9 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
         if (a.part == kPartOwn) t0 = sq.t0;
         if (a.part == kPartOwn && rows > a.rows_to) return false;  // the many-rows kernel's
         if (r0 >= rows) return false;
-        nrows = min(kFewRows, rows - r0);
+        nrows = min(ROWS, rows - r0);
     }
-    if (tid < kFewRows) {
+    if (tid < ROWS) {
         int p = -2;
         uint32_t tok = 0, head = 0;
         if (tid < nrows) {
@@ -184,7 +185,7 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     __syncthreads();
     // keys [kb, ke): positions, or places in the page list; [all_b, all_e): seen by every row
     uint32_t kb = kNone, ke = 0, all_b = 0, all_e = kNone;
-    for (uint32_t r = 0; r < kFewRows; ++r) {
+    for (uint32_t r = 0; r < ROWS; ++r) {
         if (row_pos[r] < 0) continue;
         const uint32_t lo = first_key(row_pos[r], a.window), hi = static_cast<uint32_t>(row_pos[r]) + 1u;
         kb = min(kb, lo);
@@ -247,15 +248,15 @@ __device__ __forceinline__ float4 load4_cluster(uint32_t addr) {
 // in shared memory) added in warp order and written out, or to the chunk's place, or, where
 // the row tile's chunks are a cluster, into shared memory behind `part`: there every CTA adds
 // a share of the rows' channels over the chunks, in chunk order, and writes it out.
-template <uint32_t WARPS>
+template <uint32_t WARPS, uint32_t ROWS>
 __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const uint32_t* row_tok, const uint32_t* row_head,
-                                           const int* row_pos, const float (*wm)[kFewRows], const float (*wl)[kFewRows],
+                                           const int* row_pos, const float (*wm)[ROWS], const float (*wl)[ROWS],
                                            float* part, uint32_t pitch) {
-    __shared__ float2 chunk_ml[kFewRows];
+    __shared__ float2 chunk_ml[ROWS];
     const uint32_t tid = threadIdx.x, hd = a.kv.head_dim, hd4 = hd / 4u;
     const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-    float* const mine = part + WARPS * kFewRows * pitch;  // cluster: [row][hd]
-    for (uint32_t i = tid; i < kFewRows * hd4; i += blockDim.x) {
+    float* const mine = part + WARPS * ROWS * pitch;  // cluster: [row][hd]
+    for (uint32_t i = tid; i < ROWS * hd4; i += blockDim.x) {
         const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
         if (row_pos[r] == -2) continue;
         float top = -INFINITY;
@@ -268,7 +269,7 @@ __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const 
         for (uint32_t w = 0; w < WARPS; ++w) {
             if (wl[w][r] == 0.f) continue;  // nothing seen there
             const float f = exp2f(wm[w][r] - top);
-            const float4 x = *reinterpret_cast<const float4*>(part + (w * kFewRows + r) * pitch + d);
+            const float4 x = *reinterpret_cast<const float4*>(part + (w * ROWS + r) * pitch + d);
             sum = fmaf(wl[w][r], f, sum);
             o.x = fmaf(x.x, f, o.x);
             o.y = fmaf(x.y, f, o.y);
@@ -291,7 +292,7 @@ __device__ __forceinline__ void few_finish(const AttnArgs& a, uint32_t c, const 
     if (!a.cluster) return;
     cluster_sync();
     const uint32_t n = a.chunks, ml_addr = smem_addr(chunk_ml), o_addr = smem_addr(mine);
-    for (uint32_t i = cluster_rank() * blockDim.x + tid; i < kFewRows * hd4; i += n * blockDim.x) {
+    for (uint32_t i = cluster_rank() * blockDim.x + tid; i < ROWS * hd4; i += n * blockDim.x) {
         const uint32_t r = i / hd4, d = (i - r * hd4) * 4u;
         if (row_pos[r] == -2) continue;
         float2 ml[kMaxCluster];
@@ -363,9 +364,10 @@ cudaError_t launch_items(const AttnArgs& a, void (*kernel)(Args...), uint64_t it
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// The few-rows kernels, up to kFewRows query rows per tile: F16 caches on the tensor cores
-// (paged_attention_few.cu), F32 caches on the CUDA cores (paged_attention_few32.cu).
-cudaError_t launch_attention_few(const AttnArgs& a, uint64_t items, cudaStream_t stream);
+// The few-rows kernels: F16 caches on the tensor cores, tiles of `rows` 8 or (heads of up to
+// 128 channels) 16 query rows (paged_attention_few.cu), F32 caches on the CUDA cores, tiles of
+// 8 (paged_attention_few32.cu).
+cudaError_t launch_attention_few(const AttnArgs& a, uint32_t rows, uint64_t items, cudaStream_t stream);
 cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_t items, cudaStream_t stream);
 // Tiles of kManyRows rows on the tensor cores (paged_attention_many.cu): F16 caches, heads
 // above 128.

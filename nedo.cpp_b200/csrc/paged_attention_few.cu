@@ -1,5 +1,5 @@
-// paged_attention_few.cu -- attention over a paged F16 cache for tiles of at most
-// eight query rows (single tokens with their group of heads, a few tokens of small
+// paged_attention_few.cu -- attention over a paged F16 cache for tiles of up to eight or
+// sixteen query rows (single tokens with their group of heads, a few tokens of small
 // groups, the rows of a page list): the shape of decoding, bound by reading the cache.
 //
 // Mathematics.  Queries and weights are fp32 and the cache is fp16, so every product
@@ -9,12 +9,19 @@
 // weights p = 2^(s - m + 14) are taken up by the same factor in numerator and sum.  The
 // two halves ride in one m16n8k16 operand, rows 0-7 the high and rows 8-15 the low half
 // of the same eight query rows, so the split costs no extra instruction: both parts of a
-// row's sum land in the same thread, which adds them.
+// row's sum land in the same thread, which adds them.  With more than eight rows the halves
+// are operands of their own, and every tile's weighted values are summed from zero and added
+// in fp32.
 //
 // Work.  A CTA of four warps takes one row tile and one chunk of keys; each warp streams
 // every fourth 16-key tile through a ring of its own (cp.async, three stages), with its
 // own running maximum and sums, so the warps meet only at the end.  A 16-key tile lies
 // within one page.  Two CTAs share an SM.
+//
+// 32 single tokens of 12 query and 4 KV heads of 128 channels over 8191 to 32768 keys: 214 us,
+// 6.6 TB/s.  32 query heads over 2 KV heads, 5000 to 20000 keys: 86 us in tiles of 16 rows, 5.0
+// TB/s (118 us in two tiles of 8, which both read the cache).  Heads above 128 keep to 8: the
+// queries and sums of 16 rows would not stay in registers.
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
@@ -41,17 +48,18 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return r * Few<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
 }
 
-template <uint32_t HD>
+template <uint32_t HD, uint32_t ROWS>
 __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     using F = Few<HD>;
+    constexpr uint32_t kMine = ROWS / 8u;  // rows of a thread: g, and g + 8 of 16
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ uint32_t row_tok[kFewRows], row_head[kFewRows];
-    __shared__ int row_pos[kFewRows];
-    __shared__ float wm[kWarps][kFewRows], wl[kWarps][kFewRows];
+    __shared__ uint32_t row_tok[ROWS], row_head[ROWS];
+    __shared__ int row_pos[ROWS];
+    __shared__ float wm[kWarps][ROWS], wl[kWarps][ROWS];
     __shared__ uint32_t list[kMaxPicks];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     FewItem it;
-    if (!few_setup(a, row_tok, row_head, row_pos, list, &it)) return;
+    if (!few_setup<ROWS>(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t c = it.c, kh = it.kh, s = it.s, kb = it.kb, ke = it.ke, all_b = it.all_b, all_e = it.all_e;
     // this warp's tiles: tile i starts at key j0 + 16 (4 i + warp); lane i holds its page and
     // the position of its first key
@@ -103,13 +111,16 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
 #pragma unroll
     for (uint32_t i = 0; i + 1u < F::kStages; ++i) fetch(i);
 
-    // this thread's query row: g, channels 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
+    // this thread's query rows: g (and g + 8), channels 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
     const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u;
-    const int p = row_pos[g];
-    uint32_t qf[HD / 16][4];
-    float unscale;
-    {
-        const float* q = a.q + (static_cast<size_t>(row_tok[g]) * a.heads + row_head[g]) * hd;
+    uint32_t qf[kMine][HD / 16][4];  // 8 rows: both halves in one operand; 16: the high and the low halves
+    float unscale[kMine], m[kMine], l[kMine];
+    uint32_t p_lo[kMine], p_hi[kMine];
+#pragma unroll
+    for (uint32_t h = 0; h < kMine; ++h) {
+        const uint32_t r = g + 8u * h;
+        const int p = row_pos[r];
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
         float2 x[HD / 8];
         float big = 0.f;
 #pragma unroll
@@ -124,15 +135,20 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
         const int e = up_exponent(big);
         const float up = power_of_two(e);
-        unscale = power_of_two(-e);
+        unscale[h] = power_of_two(-e);
 #pragma unroll
-        for (uint32_t i = 0; i < HD / 16; ++i) {
-            split(x[2 * i].x * up, x[2 * i].y * up, &qf[i][0], &qf[i][1]);
-            split(x[2 * i + 1].x * up, x[2 * i + 1].y * up, &qf[i][2], &qf[i][3]);
-        }
+        for (uint32_t i = 0; i < HD / 16; ++i)
+#pragma unroll
+            for (uint32_t k = 0; k < 2u; ++k) {
+                uint32_t* const high = &qf[0][i][2u * k + h];
+                uint32_t* const low = kMine == 1u ? &qf[0][i][2u * k + 1u] : &qf[kMine - 1u][i][2u * k + h];
+                split(x[2 * i + k].x * up, x[2 * i + k].y * up, high, low);
+            }
+        p_lo[h] = p >= 0 ? first_key(p, a.window) : kNone;
+        p_hi[h] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+        m[h] = -INFINITY;
+        l[h] = 0.f;
     }
-    const uint32_t p_lo = p >= 0 ? first_key(p, a.window) : kNone, p_hi = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
-    float m = -INFINITY, l = 0.f;
     float acc[HD / 8][4];
 #pragma unroll
     for (uint32_t n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -143,52 +159,67 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
         cp_wait<F::kStages - 1>();
         __syncwarp();
         const uint32_t ks = ring_addr + (i % F::kStages) * F::kStageBytes, vs = ks + F::kTileBytes;
-        float sc[2][4];
+        float sc[kMine][2][4];  // 16 rows: from the high and from the low halves
 #pragma unroll
-        for (uint32_t n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+        for (uint32_t h = 0; h < kMine; ++h)
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) sc[h][n][0] = sc[h][n][1] = sc[h][n][2] = sc[h][n][3] = 0.f;
 #pragma unroll
         for (uint32_t k = 0; k < HD / 16; ++k) {
             uint32_t b[4];
             ldsm4(b, ks + at<HD>((mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
-            mma(sc[0], qf[k], b[0], b[1]);
-            mma(sc[1], qf[k], b[2], b[3]);
+#pragma unroll
+            for (uint32_t h = 0; h < kMine; ++h) {
+                mma(sc[h][0], qf[h][k], b[0], b[1]);
+                mma(sc[h][1], qf[h][k], b[2], b[3]);
+            }
         }
         const uint32_t page = __shfl_sync(0xFFFFFFFFu, my_page, i), pos = __shfl_sync(0xFFFFFFFFu, my_pos, i);
-        float v[4];  // keys pos + 2t, 2t + 1, 2t + 8, 2t + 9
-        v[0] = (sc[0][0] + sc[0][2]) * unscale;
-        v[1] = (sc[0][1] + sc[0][3]) * unscale;
-        v[2] = (sc[1][0] + sc[1][2]) * unscale;
-        v[3] = (sc[1][1] + sc[1][3]) * unscale;
         const bool whole = page != kNone && pos >= all_b && pos + kKeys <= all_e;
-        if (!whole) {
+        float v[kMine][4], mn[kMine];  // keys pos + 2t, 2t + 1, 2t + 8, 2t + 9
+        bool more = false;
+#pragma unroll
+        for (uint32_t h = 0; h < kMine; ++h) {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t at_key = pos + t2 + (j & 1u) + (j >> 1) * 8u;
-                if (page == kNone || at_key < p_lo || at_key >= p_hi) v[j] = -INFINITY;
+                const float high = sc[0][j >> 1][(j & 1u) + 2u * h];
+                const float low = kMine == 1u ? sc[0][j >> 1][(j & 1u) + 2u] : sc[kMine - 1u][j >> 1][(j & 1u) + 2u * h];
+                v[h][j] = (high + low) * unscale[h];
+                if (!whole) {
+                    const uint32_t at_key = pos + t2 + (j & 1u) + (j >> 1) * 8u;
+                    if (page == kNone || at_key < p_lo[h] || at_key >= p_hi[h]) v[h][j] = -INFINITY;
+                }
             }
+            float mt = fmaxf(fmaxf(v[h][0], v[h][1]), fmaxf(v[h][2], v[h][3]));
+            mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
+            mn[h] = fmaxf(m[h], mt);
+            more |= mt > m[h];
         }
-        float mt = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
-        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 1));
-        mt = fmaxf(mt, __shfl_xor_sync(0xFFFFFFFFu, mt, 2));
-        if (__any_sync(0xFFFFFFFFu, mt > m)) {
-            const float mn = fmaxf(m, mt), al = mn == -INFINITY ? 1.f : exp2f(m - mn);
-            m = mn;
-            l *= al;
+        if (__any_sync(0xFFFFFFFFu, more)) {
+            float al[kMine];
 #pragma unroll
-            for (uint32_t n = 0; n < HD / 8; ++n) {
-                acc[n][0] *= al;
-                acc[n][1] *= al;
-                acc[n][2] *= al;
-                acc[n][3] *= al;
+            for (uint32_t h = 0; h < kMine; ++h) {
+                al[h] = mn[h] == -INFINITY ? 1.f : exp2f(m[h] - mn[h]);
+                m[h] = mn[h];
+                l[h] *= al[h];
             }
-        }
-        const float ref = (m == -INFINITY ? 0.f : m) - kUp;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) v[j] = exp2_fast(v[j] - ref);
-        l += (v[0] + v[1]) + (v[2] + v[3]);
-        uint32_t pf[4];
-        split(v[0], v[1], &pf[0], &pf[1]);
-        split(v[2], v[3], &pf[2], &pf[3]);
+            for (uint32_t n = 0; n < HD / 8; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) acc[n][e] *= al[kMine == 1u ? 0u : e >> 1];
+        }
+        uint32_t pf[kMine][4];
+#pragma unroll
+        for (uint32_t h = 0; h < kMine; ++h) {
+            const float ref = (m[h] == -INFINITY ? 0.f : m[h]) - kUp;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) v[h][j] = exp2_fast(v[h][j] - ref);
+            l[h] += (v[h][0] + v[h][1]) + (v[h][2] + v[h][3]);
+#pragma unroll
+            for (uint32_t k = 0; k < 2u; ++k)
+                split(v[h][2u * k], v[h][2u * k + 1u], &pf[0][2u * k + h], kMine == 1u ? &pf[0][2u * k + 1u] : &pf[kMine - 1u][2u * k + h]);
+        }
         // a value that is not finite must not reach the rows that do not see it (0 * inf):
         // only tiles that some row sees in part can hold one, and those are few
         bool odd = false;
@@ -206,22 +237,41 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             for (uint32_t n = 0; n < HD / 16; ++n) {
                 uint32_t b[4];
                 ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
-                mma(acc[2 * n], pf, b[0], b[1]);
-                mma(acc[2 * n + 1], pf, b[2], b[3]);
+                if constexpr (kMine == 1u) {
+                    mma(acc[2 * n], pf[0], b[0], b[1]);
+                    mma(acc[2 * n + 1], pf[0], b[2], b[3]);
+                } else {
+                    // from zero, and added in fp32: the tensor core would cut the running sums twice a tile
+                    float o[2][4];
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+                    mma(o[0], pf[kMine - 1u], b[0], b[1]);
+                    mma(o[1], pf[kMine - 1u], b[2], b[3]);
+                    mma(o[0], pf[0], b[0], b[1]);
+                    mma(o[1], pf[0], b[2], b[3]);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        acc[2 * n][e] += o[0][e];
+                        acc[2 * n + 1][e] += o[1][e];
+                    }
+                }
             }
         } else {
             for (uint32_t j = 0; j < kKeys; ++j) {
                 const uint32_t from = (lane & ~3u) | ((j & 7u) >> 1);
-                const float w0 = __shfl_sync(0xFFFFFFFFu, v[0], from), w1 = __shfl_sync(0xFFFFFFFFu, v[1], from);
-                const float w2 = __shfl_sync(0xFFFFFFFFu, v[2], from), w3 = __shfl_sync(0xFFFFFFFFu, v[3], from);
-                const float w = j < 8u ? (j & 1u ? w1 : w0) : (j & 1u ? w3 : w2);
-                if (pos + j < p_lo || pos + j >= p_hi || page == kNone) continue;
 #pragma unroll
-                for (uint32_t n = 0; n < HD / 8; ++n) {
-                    const uint8_t* row = my_ring + (vs - ring_addr) + at<HD>(j, n) + t2 * 2u;
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(row));
-                    acc[n][0] = fmaf(w, f.x, acc[n][0]);
-                    acc[n][1] = fmaf(w, f.y, acc[n][1]);
+                for (uint32_t h = 0; h < kMine; ++h) {
+                    const float w0 = __shfl_sync(0xFFFFFFFFu, v[h][0], from), w1 = __shfl_sync(0xFFFFFFFFu, v[h][1], from);
+                    const float w2 = __shfl_sync(0xFFFFFFFFu, v[h][2], from), w3 = __shfl_sync(0xFFFFFFFFu, v[h][3], from);
+                    const float w = j < 8u ? (j & 1u ? w1 : w0) : (j & 1u ? w3 : w2);
+                    if (pos + j < p_lo[h] || pos + j >= p_hi[h] || page == kNone) continue;
+#pragma unroll
+                    for (uint32_t n = 0; n < HD / 8; ++n) {
+                        const uint8_t* row = my_ring + (vs - ring_addr) + at<HD>(j, n) + t2 * 2u;
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(row));
+                        acc[n][2u * h] = fmaf(w, f.x, acc[n][2u * h]);
+                        acc[n][2u * h + 1u] = fmaf(w, f.y, acc[n][2u * h + 1u]);
+                    }
                 }
             }
         }
@@ -230,40 +280,49 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
     // the warps' sums, in warp order
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-    l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-    if ((lane & 3u) == 0u) {
-        wm[warp][g] = (m == -INFINITY ? 0.f : m) - kUp;
-        wl[warp][g] = p >= 0 ? l : 0.f;  // padding sees nothing
+#pragma unroll
+    for (uint32_t h = 0; h < kMine; ++h) {
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
+        if ((lane & 3u) == 0u) {
+            wm[warp][g + 8u * h] = (m[h] == -INFINITY ? 0.f : m[h]) - kUp;
+            wl[warp][g + 8u * h] = row_pos[g + 8u * h] >= 0 ? l[h] : 0.f;  // padding sees nothing
+        }
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(ring);  // [warp][row][HD + 4]
     constexpr uint32_t kPitch = HD + 4u;
 #pragma unroll
-    for (uint32_t n = 0; n < HD / 8; ++n)
-        *reinterpret_cast<float2*>(part + (warp * kFewRows + g) * kPitch + n * 8u + t2) =
-            make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+    for (uint32_t n = 0; n < HD / 8; ++n) {
+        float* to = part + (warp * ROWS + g) * kPitch + n * 8u + t2;
+        if constexpr (kMine == 1u) {
+            *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+        } else {
+            *reinterpret_cast<float2*>(to) = make_float2(acc[n][0], acc[n][1]);
+            *reinterpret_cast<float2*>(to + 8u * kPitch) = make_float2(acc[n][2], acc[n][3]);
+        }
+    }
     __syncthreads();
-    few_finish<kWarps>(a, c, row_tok, row_head, row_pos, wm, wl, part, kPitch);
+    few_finish<kWarps, ROWS>(a, c, row_tok, row_head, row_pos, wm, wl, part, kPitch);
 }
 
-template <uint32_t HD>
+template <uint32_t HD, uint32_t ROWS>
 __global__ void __launch_bounds__(kThreads, 2) attention_few_kernel(const __grid_constant__ AttnArgs a) {
-    attention_few<HD>(a);
+    attention_few<HD, ROWS>(a);
     end_after_previous(a);
 }
 
-template <uint32_t HD>
+template <uint32_t HD, uint32_t ROWS>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    return launch_items(a, attention_few_kernel<HD>, items, kThreads, Few<HD>::kSmem, stream, a);
+    return launch_items(a, attention_few_kernel<HD, ROWS>, items, kThreads, Few<HD>::kSmem, stream, a);
 }
 
 }  // namespace
 
-cudaError_t launch_attention_few(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    if (a.kv.head_dim <= 64u) return launch<64>(a, items, stream);
-    if (a.kv.head_dim <= 128u) return launch<128>(a, items, stream);
-    return launch<256>(a, items, stream);
+cudaError_t launch_attention_few(const AttnArgs& a, uint32_t rows, uint64_t items, cudaStream_t stream) {
+    if (a.kv.head_dim > 128u) return launch<256, 8>(a, items, stream);
+    if (a.kv.head_dim <= 64u) return rows <= 8u ? launch<64, 8>(a, items, stream) : launch<64, 16>(a, items, stream);
+    return rows <= 8u ? launch<128, 8>(a, items, stream) : launch<128, 16>(a, items, stream);
 }
 
 }  // namespace nedo_gpu

@@ -73,7 +73,7 @@ __device__ __forceinline__ void attention_few32(const AttnArgs& a) {
     __shared__ uint32_t list[kMaxPicks];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     FewItem it;
-    if (!few_setup(a, row_tok, row_head, row_pos, list, &it)) return;
+    if (!few_setup<kFewRows>(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t kb = it.kb, ke = it.ke, kh = it.kh;
     // this warp's tiles: tile i starts at key j0 + 8 (4 i + warp); lane i holds the pages of
     // tiles i and i + 32 and the positions of their first keys
@@ -265,7 +265,7 @@ __device__ __forceinline__ void attention_few32(const AttnArgs& a) {
 #pragma unroll
         for (uint32_t d = 0; d < kD; ++d) part[(warp * kFewRows + r) * kPitch + dim_of<HD>(lane, d)] = acc[r][d];
     __syncthreads();
-    few_finish<kWarps>(a, it.c, row_tok, row_head, row_pos, wm, wl, part, kPitch);
+    few_finish<kWarps, kFewRows>(a, it.c, row_tok, row_head, row_pos, wm, wl, part, kPitch);
 }
 
 template <uint32_t HD, uint32_t R>
