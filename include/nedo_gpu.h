@@ -368,8 +368,10 @@ NEDO_GPU_API void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d);
  *
  * All of them are asynchronous on `stream`, allocate nothing and keep nothing
  * between calls, so they can be captured in CUDA graphs and may run at the same
- * time on several streams (each call with a workspace of its own).  Buffers are
- * 16-byte aligned device memory.  Results repeat bit for bit.
+ * time on several streams (each call with a workspace of its own; captured graphs
+ * that may overlap too).  The library's first call on a device allocates its state
+ * there: make it outside a capture.  Buffers are 16-byte aligned memory of the
+ * current device.  Results repeat bit for bit.
  *
  * Token row t of sequence s (q_start[s] <= t < q_start[s+1]) stands at position
  * kv_len[s] - (q_start[s+1] - t).  A row whose position is negative -- its
@@ -388,7 +390,7 @@ typedef struct {
     uint32_t kv_heads;
     uint32_t head_dim;   /* a multiple of 8, at most 256                                 */
     uint32_t page_size;  /* tokens per page: 16, 32, 64, 128 or 256                      */
-    uint64_t num_pages;
+    uint64_t num_pages;  /* num_pages * kv_heads below 2^31                              */
     void* k;             /* [num_pages][kv_heads][page_size][head_dim]                   */
     void* v;             /* [num_pages][kv_heads][page_size][head_dim]                   */
     void* bounds;        /* [num_pages][kv_heads][2][head_dim], in `type`: the smallest and
@@ -399,11 +401,13 @@ typedef struct {
 typedef struct {
     uint32_t seqs;               /* sequences                                            */
     uint32_t tokens;             /* rows of the q, qkv and output buffers                */
-    uint32_t max_q_len;          /* no sequence has more rows (a bound; shapes the launch) */
+    uint32_t max_q_len;          /* no sequence has more rows (a bound, at least 1; shapes the
+                                    launch)                                               */
     uint32_t max_kv_len;         /* no sequence has more cached tokens (a bound)          */
     uint32_t max_pages;          /* row length of page_table                             */
     uint32_t shared_pages;       /* paged attention: the first shared_pages entries of every
-                                    row of page_table are the same pages (0: none shared) */
+                                    row of page_table are the same pages (0: none shared);
+                                    they are read from the first row, used or not         */
     const uint32_t* q_start;     /* device, [seqs + 1]: first token row of each sequence  */
     const uint32_t* kv_len;      /* device, [seqs]: cached tokens, this call's included   */
     const uint32_t* page_table;  /* device, [seqs][max_pages]; entries behind a sequence's
@@ -433,7 +437,8 @@ NEDO_GPU_API int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cac
  *   out = sum_j softmax_j(scale * q.k_j) v_j,  max(0, p - window + 1) <= j <= p
  * for a row at position p (window 0: all).  With shared_pages > 0 the keys of the
  * shared prefix are read once for the whole batch.  Sums and softmax statistics
- * are kept in 32 bits. */
+ * are kept in 32 bits.  On the tensor cores a row's query channels keep 22 bits, or
+ * 2^-38 of the row's largest, whichever is coarser. */
 NEDO_GPU_API int nedo_gpu_paged_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
                                               uint32_t heads, const float* q_dev, float* out_dev, float scale,
                                               uint32_t window, void* workspace_dev, uint64_t workspace_bytes,
