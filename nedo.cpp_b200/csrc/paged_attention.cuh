@@ -58,39 +58,38 @@ __device__ __forceinline__ uint32_t first_tile_above(const AttnArgs& a, const Pa
 // not in steps), so that the launch does not end with one of them.
 __device__ __forceinline__ uint32_t find_tile(const AttnArgs& a, uint32_t want, uint32_t tile_rows, uint32_t* tile) {
     const uint32_t lane = threadIdx.x & 31u;
-    uint32_t before = 0, loaded = kNone;
-    PagedSeq sq{0u, 0u, 0u};
-    for (uint32_t step = a.depth != 0u ? 8u : 1u; step-- > 0u;) {
-        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-            uint32_t cnt = 0, first = 0;
-            if (s0 + lane < a.b.seqs) {
-                if (loaded != s0) sq = load_seq(a.b, s0 + lane, a.st);
-                loaded = s0;
-                const uint32_t rows = sq.n * a.group;
-                if (rows >= a.rows_from && rows <= a.rows_to) {
-                    cnt = (rows + tile_rows - 1u) / tile_rows;
-                    if (a.depth != 0u) {
-                        if (step != 0u) first = first_tile_above(a, sq, cnt, tile_rows, step * a.depth);
-                        const uint32_t end = step != 7u ? first_tile_above(a, sq, cnt, tile_rows, (step + 1u) * a.depth) : cnt;
-                        cnt = end - first;
-                    }
+    // a lane per sequence and step
+    const uint32_t steps = a.depth != 0u ? 8u : 1u, all = steps * a.b.seqs;
+    uint32_t before = 0;
+    for (uint32_t e0 = 0; e0 < all; e0 += 32u) {
+        const uint32_t turn = (e0 + lane) / a.b.seqs, s = e0 + lane - turn * a.b.seqs, step = steps - 1u - turn;
+        uint32_t cnt = 0, first = 0;
+        if (e0 + lane < all) {
+            const PagedSeq sq = load_seq(a.b, s, a.st);
+            const uint32_t rows = sq.n * a.group;
+            if (rows >= a.rows_from && rows <= a.rows_to) {
+                cnt = (rows + tile_rows - 1u) / tile_rows;
+                if (a.depth != 0u) {
+                    if (step != 0u) first = first_tile_above(a, sq, cnt, tile_rows, step * a.depth);
+                    const uint32_t end = step != 7u ? first_tile_above(a, sq, cnt, tile_rows, (step + 1u) * a.depth) : cnt;
+                    cnt = end - first;
                 }
             }
-            uint32_t inc = cnt;
-            for (uint32_t o = 1; o < 32u; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                if (lane >= o) inc += v;
-            }
-            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > want);
-            if (hit != 0u) {
-                const uint32_t w = __ffs(hit) - 1u;
-                // within a sequence the last tile first
-                const uint32_t at = want - before - __shfl_sync(0xFFFFFFFFu, inc - cnt, w);
-                *tile = __shfl_sync(0xFFFFFFFFu, first + cnt, w) - 1u - at;
-                return s0 + w;
-            }
-            before += __shfl_sync(0xFFFFFFFFu, inc, 31);
         }
+        uint32_t inc = cnt;
+        for (uint32_t o = 1; o < 32u; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > want);
+        if (hit != 0u) {
+            const uint32_t w = __ffs(hit) - 1u;
+            // within a sequence the last tile first
+            const uint32_t at = want - before - __shfl_sync(0xFFFFFFFFu, inc - cnt, w);
+            *tile = __shfl_sync(0xFFFFFFFFu, first + cnt, w) - 1u - at;
+            return __shfl_sync(0xFFFFFFFFu, s, w);
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
     *tile = 0;
     return kNone;

@@ -316,10 +316,17 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     ok = warp_wait(&cut, cuts & 1u, a.st, 62u);
                     ++cuts;
                     if (!ok) return;
-                    for (uint32_t x = lane; x < kKeys * 8u * T::kBlocks; x += 32u) {
-                        const uint32_t r = x / (8u * T::kBlocks), ch = x % (8u * T::kBlocks);
-                        if (j + r < kb || j + r >= ke || !(there >> (r >> box_shift) & 1u))
-                            *reinterpret_cast<uint4*>(sm + (dst - s0) + at(r, ch)) = make_uint4(0u, 0u, 0u, 0u);
+                    constexpr uint32_t kChunks = 8u * T::kBlocks;  // of 16 bytes in a row
+                    auto clear = [&](uint32_t from, uint32_t to) {
+#pragma unroll 4
+                        for (uint32_t x = from * kChunks + lane; x < to * kChunks; x += 32u)
+                            *reinterpret_cast<uint4*>(sm + (dst - s0) + at(x / kChunks, x % kChunks)) = make_uint4(0u, 0u, 0u, 0u);
+                    };
+                    if (kb > j) clear(0u, kb - j);
+                    if (ke < j + kKeys) clear(ke - j, kKeys);
+                    for (uint32_t gone = want & ~there; gone != 0u; gone &= gone - 1u) {
+                        const uint32_t b = __ffs(gone) - 1u;
+                        clear(b * box_rows, (b + 1u) * box_rows);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
