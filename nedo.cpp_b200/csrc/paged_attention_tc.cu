@@ -166,7 +166,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
+    __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
     __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
     __shared__ uint32_t found[2], tmem_slot, gaps[8];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
@@ -432,41 +432,41 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             constexpr uint32_t kC = kKeys / 32u;  // 16-key pieces of a side
             float unscale;
             {
-                // queries: a row per four threads, scaled, split, stored
-                constexpr uint32_t kPart = HD / 4u;  // channels of a thread
-                const uint32_t part = warp >> 2;
-                const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd + part * kPart;
-                float4 x[kPart / 4u];
-                float big = 0.f;
+                // queries: a row by HD / 4 lanes next to each other, scaled, split, stored (with a row
+                // per thread each load would be 32 cache lines, 4096 cycles of them in all)
+                constexpr uint32_t kLanes = HD / 4u, kAtOnce = 32u / kLanes, kTurns = kRows / (kSoftmax / 32u * kAtOnce);
+                const uint32_t ch = lane % kLanes * 4u;
+                const uint32_t lanes = kLanes == 32u ? 0xFFFFFFFFu : ((1u << (kLanes & 31u)) - 1u) << (lane & ~(kLanes - 1u));
+                auto row_of = [&](uint32_t i) { return (i * (kSoftmax / 32u) + warp) * kAtOnce + lane / kLanes; };
+                float4 x[kTurns];
 #pragma unroll
-                for (uint32_t e = 0; e < kPart / 4u; ++e) {
-                    x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (p >= 0 && part * kPart + 4u * e < hd) x[e] = *reinterpret_cast<const float4*>(q + 4u * e);
-                    x[e] = make_float4(x[e].x * a.scale_log2, x[e].y * a.scale_log2, x[e].z * a.scale_log2, x[e].w * a.scale_log2);
-                    big = fmaxf(big, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
-                }
-                side_max[0][part][r] = big;
-                named_barrier_sync(3, kSoftmax);
-                big = fmaxf(fmaxf(side_max[0][0][r], side_max[0][1][r]), fmaxf(side_max[0][2][r], side_max[0][3][r]));
-                const int e2 = up_exponent(big);
-                const float up = power_of_two(e2);
-                unscale = power_of_two(-e2);
-                uint32_t hi[kPart / 2u], lo[kPart / 2u];
-#pragma unroll
-                for (uint32_t e = 0; e < kPart / 4u; ++e) {
-                    split(x[e].x * up, x[e].y * up, &hi[2u * e], &lo[2u * e]);
-                    split(x[e].z * up, x[e].w * up, &hi[2u * e + 1u], &lo[2u * e + 1u]);
+                for (uint32_t i = 0; i < kTurns; ++i) {
+                    const uint32_t rq = row_of(i);
+                    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (row_pos[rq] >= 0 && ch < hd)
+                        x[i] = *reinterpret_cast<const float4*>(a.q + (static_cast<size_t>(row_tok[rq]) * a.heads + row_head[rq]) * hd + ch);
                 }
 #pragma unroll
-                for (uint32_t e = 0; e < kPart / 8u; ++e) {
-                    const uint32_t ch = part * (kPart / 8u) + e;
-                    *reinterpret_cast<uint4*>(sm + at(r, ch)) = make_uint4(hi[4u * e], hi[4u * e + 1u], hi[4u * e + 2u], hi[4u * e + 3u]);
-                    *reinterpret_cast<uint4*>(sm + T::kTile + at(r, ch)) =
-                        make_uint4(lo[4u * e], lo[4u * e + 1u], lo[4u * e + 2u], lo[4u * e + 3u]);
+                for (uint32_t i = 0; i < kTurns; ++i) {
+                    const uint32_t rq = row_of(i);
+                    float4 v = make_float4(x[i].x * a.scale_log2, x[i].y * a.scale_log2, x[i].z * a.scale_log2, x[i].w * a.scale_log2);
+                    // (magnitudes order like their bits)
+                    const float big = __uint_as_float(__reduce_max_sync(
+                        lanes, __float_as_uint(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))))));
+                    const int e2 = up_exponent(big);
+                    const float up = power_of_two(e2);
+                    if (ch == 0u) row_unscale[rq] = power_of_two(-e2);
+                    uint32_t hi[2], lo[2];
+                    split(v.x * up, v.y * up, &hi[0], &lo[0]);
+                    split(v.z * up, v.w * up, &hi[1], &lo[1]);
+                    uint8_t* const to = sm + at(rq, ch >> 3) + (ch & 4u) * 2u;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(to + T::kTile) = make_uint2(lo[0], lo[1]);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 warp_arrive(&q_full);
-                named_barrier_sync(3, kSoftmax);  // the maxima have been read: their place serves the tiles
+                named_barrier_sync(3, kSoftmax);
+                unscale = row_unscale[r];
             }
             float m = -INFINITY, l = 0.f;
             for (uint32_t i = half; i < ntiles; i += 2u) {
@@ -635,14 +635,16 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     make_float2(ref - kUp, sum);
             named_barrier_sync(5, kSums);
             if (ok) {
-                const uint32_t hd4 = hd / 4u;
-                for (uint32_t x = tid - kSoftmax; x < kRows * hd4; x += kSums) {
-                    const uint32_t rr = x / hd4, d = (x - rr * hd4) * 4u;
-                    if (row_pos[rr] == -2) continue;
-                    const size_t row = static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr];
-                    float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
-                    *reinterpret_cast<float4*>(o + d) = *reinterpret_cast<const float4*>(sums + rr * kPitch + d);
-                }
+                // rows by lanes next to each other
+                constexpr uint32_t kLanes = HD / 4u, kAtOnce = kSums / kLanes;
+                const uint32_t d = (tid - kSoftmax) % kLanes * 4u, row0 = (tid - kSoftmax) / kLanes;
+                float* const to = a.direct ? a.out : a.part_o + (a.slot0 + c) * rows_all * hd;
+                if (d < hd)
+#pragma unroll 8
+                    for (uint32_t rr = row0; rr < kRows; rr += kAtOnce)
+                        if (row_pos[rr] != -2)
+                            *reinterpret_cast<float4*>(to + (static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr]) * hd + d) =
+                                *reinterpret_cast<const float4*>(sums + rr * kPitch + d);
             }
         }
     }
