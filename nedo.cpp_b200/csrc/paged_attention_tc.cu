@@ -180,6 +180,22 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
 
     // what follows on the stream may come up where there is room (it waits for this kernel)
     if (tid == 0u) asm volatile("griddepcontrol.launch_dependents;");
+    if (tid == 32u * kLoadWarp) {
+        for (uint32_t i = 0; i < kSlots; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        mbar_init(&cut, 1);
+        for (uint32_t i = 0; i < kBuffers; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 8);
+        }
+        mbar_init(&o_full, 1);
+        mbar_init(&o_empty, kSums / 32u);
+        mbar_init(&q_full, kSoftmax / 32u);
+        mbar_init(&done, 1);
+        fence_barrier_init();
+    }
     // ---- the item: rows and keys
     uint32_t s = 0, r0 = 0, nrows, t0 = 0;
     PagedSeq sq{0u, 0u, 0u};
@@ -215,20 +231,29 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         row_head[tid] = head;
         row_pos[tid] = p;
     }
-    __syncthreads();
     uint32_t kb = kNone, ke = 0;
     {
-        uint32_t lo = kNone, hi = 0;
-#pragma unroll
-        for (uint32_t u = 0; u < kRows / 32u; ++u) {
-            const int p = row_pos[lane + 32u * u];
-            if (p >= 0) {
-                lo = min(lo, first_key(p, a.window));
-                hi = max(hi, static_cast<uint32_t>(p) + 1u);
+        if (a.part == kPartOwn) {
+            // the rows' positions ascend
+            const int p0 = sq.pos(r0 / a.group), p1 = sq.pos((r0 + nrows - 1u) / a.group);
+            if (p1 >= 0) {
+                kb = first_key(max(p0, 0), a.window);
+                ke = static_cast<uint32_t>(p1) + 1u;
             }
+        } else {
+            __syncthreads();
+            uint32_t lo = kNone, hi = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < kRows / 32u; ++u) {
+                const int p = row_pos[lane + 32u * u];
+                if (p >= 0) {
+                    lo = min(lo, first_key(p, a.window));
+                    hi = max(hi, static_cast<uint32_t>(p) + 1u);
+                }
+            }
+            kb = __reduce_min_sync(0xFFFFFFFFu, lo);
+            ke = __reduce_max_sync(0xFFFFFFFFu, hi);
         }
-        kb = __reduce_min_sync(0xFFFFFFFFu, lo);
-        ke = __reduce_max_sync(0xFFFFFFFFu, hi);
         uint32_t base = 0;
         if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
         else ke = min(ke, a.shared_len);
@@ -240,26 +265,30 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     const uint32_t j0 = kb & ~(kKeys - 1u), ntiles = kb < ke ? (ke - j0 + kKeys - 1u) / kKeys : 0u;
 
     // ---- barriers, TMEM, queries
-    if (tid == 0u) {
-        for (uint32_t i = 0; i < kSlots; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
-        mbar_init(&cut, 1);
-        for (uint32_t i = 0; i < kBuffers; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 8);
-        }
-        mbar_init(&o_full, 1);
-        mbar_init(&o_empty, kSums / 32u);
-        mbar_init(&q_full, kSoftmax / 32u);
-        mbar_init(&done, 1);
-        fence_barrier_init();
-    }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
                      "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
+    // lane b: page of box b of a tile (kNone: no keys of the item there, or no page), looked up
+    // and, when it is needed, checked; those of the first tiles before the rest is ready
+    auto wanted = [&](uint32_t i) {
+        const uint32_t j = j0 + i * kKeys + lane * box_rows;
+        return lane < boxes && i < ntiles && j < ke && j + box_rows > kb;
+    };
+    auto look_up = [&](uint32_t i) {
+        return wanted(i) ? a.b.table[static_cast<size_t>(s) * a.b.max_pages + ((j0 + i * kKeys + lane * box_rows) >> a.kv.page_shift)] : kNone;
+    };
+    auto checked = [&](uint32_t i, uint32_t page) {
+        if (page < a.kv.num_pages) return page;
+        if (wanted(i)) flag_argument(a.st);
+        return kNone;
+    };
+    uint32_t page0 = kNone, page1 = kNone;
+    if (warp == kLoadWarp) {
+        page0 = look_up(0);
+        page1 = look_up(1);
     }
     __syncwarp();
     tc_fence_before();
@@ -276,14 +305,6 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == kLoadWarp) {
             // ---- loads
-            const uint32_t box_rows = 1u << box_shift, boxes = kKeys >> box_shift, box_bytes = box_rows * 128u;
-            // lane b: page of box b of a tile (kNone: no keys of the item there, or no page)
-            auto look_up = [&](uint32_t i) {
-                const uint32_t j = j0 + i * kKeys + lane * box_rows;
-                return lane < boxes && i < ntiles && j < ke && j + box_rows > kb
-                           ? load_page(a.b, a.kv, s, j >> a.kv.page_shift, a.st)
-                           : kNone;
-            };
             bool ok = true;
             uint32_t issued = 0, cuts = 0;
             auto load = [&](uint32_t n, uint32_t i, uint32_t pages, bool values) {
@@ -335,14 +356,14 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 issued = n + 1u;
             };
             // pages of the tiles whose keys are in and whose values are not yet
-            uint32_t pages[4] = {look_up(0), kNone, kNone, kNone}, next = look_up(1);
+            uint32_t pages[4] = {checked(0, page0), kNone, kNone, kNone}, next = page1;
             for (uint32_t i = 0; i < ntiles + kBuffers - 1u && ok; ++i) {
                 const uint32_t after = look_up(i + 2u);
                 if (i < ntiles) load(k_at(i), i, pages[0], false);
                 if (i >= kBuffers - 1u && ok) load(v_at(i - (kBuffers - 1u)), i - (kBuffers - 1u), pages[kBuffers - 1u], true);
 #pragma unroll
                 for (uint32_t u = 3; u > 0u; --u) pages[u] = pages[u - 1u];
-                pages[0] = next;
+                pages[0] = checked(i + 1u, next);
                 next = after;
             }
             // the last copies into every slot have landed before the CTA ends

@@ -57,7 +57,7 @@ __device__ __forceinline__ bool not_finite(uint32_t two_halves) {
 // The power of two that takes a row's largest magnitude to [2^13, 2^14), where the low
 // half of its fp16 split is a normal number (0 for zero, infinite and NaN rows).
 __device__ __forceinline__ int up_exponent(float big) {
-    return big > 0.f && big < INFINITY ? min(126, 13 - static_cast<int>(ilogbf(big))) : 0;
+    return big > 0.f && big < INFINITY ? min(126, 13 + 127 - static_cast<int>(__float_as_uint(big) >> 23)) : 0;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((127 + e) << 23); }  // -126 <= e <= 127
 
