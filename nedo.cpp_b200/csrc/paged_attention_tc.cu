@@ -20,14 +20,15 @@
 //     of the channels, rescaling both to the larger of the maxima they go by (the even and the
 //     odd tiles keep maxima of their own, so neither half waits for the other).
 // TMEM, 512 columns: three S/P tiles and one O tile.  Two of them with the queries' halves in TMEM
-// as well (and six ring slots) took 130 us where this takes 126.
+// as well (and six ring slots) took 130 us where this took 126.
 // Registers: 56 for the softmax, 112 for the sums, 56 for the others.
 //
 // What bounds it: 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two
-// sequences over 4096 and 2550 keys, window 2048: 126 us, 688 TFLOP/s of fp16 MMAs (two for each
-// product of the formula), a tile about 3100 cycles of which the MMAs run 2050.  The rest is the round trip of
-// a tile: the softmax of its half, some 3300 cycles of exponentials, splits and TMEM traffic in
-// each of the two halves, and the waits on barriers between the roles.
+// sequences over 4096 and 2550 keys, window 2048: 105 us, 820 TFLOP/s of fp16 MMAs (two for each
+// product of the formula).  An item of 17 tiles is 70,000 cycles: 5,000 until its rows and keys
+// are known, 4,500 until the queries are in shared memory, 9,500 until the first tile's sums (the
+// softmax of both halves at once), then 2,850 a tile, of which the MMAs run 2,050, and 5,000 for
+// the results; and 372 items on 148 SMs leave 17 % of the cycles at the end.
 #include <algorithm>
 
 #include "paged_attention.cuh"
