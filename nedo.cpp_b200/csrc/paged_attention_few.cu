@@ -48,6 +48,12 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return r * Few<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
 }
 
+// up_exponent in other words: with the exponent taken from the number's bits the compiler orders
+// the loop over the keys worse (16 rows, the case above: 90.5 us instead of 86.6).
+__device__ __forceinline__ int row_exponent(float big) {
+    return big > 0.f && big < INFINITY ? min(126, 13 - static_cast<int>(ilogbf(big))) : 0;
+}
+
 template <uint32_t HD, uint32_t ROWS>
 __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     using F = Few<HD>;
@@ -133,7 +139,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
         }
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        const int e = up_exponent(big);
+        const int e = row_exponent(big);
         const float up = power_of_two(e);
         unscale[h] = power_of_two(-e);
 #pragma unroll
