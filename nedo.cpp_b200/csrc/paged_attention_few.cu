@@ -67,6 +67,19 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     FewItem it;
     if (!few_setup<ROWS>(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t c = it.c, kh = it.kh, s = it.s, kb = it.kb, ke = it.ke, all_b = it.all_b, all_e = it.all_e;
+    // the queries, on their way while the pages are looked up
+    const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u;
+    float2 qx[kMine][HD / 8];
+#pragma unroll
+    for (uint32_t h = 0; h < kMine; ++h) {
+        const uint32_t r = g + 8u * h;
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 8; ++i) {
+            qx[h][i] = make_float2(0.f, 0.f);
+            if (row_pos[r] >= 0 && i * 8u < hd) qx[h][i] = *reinterpret_cast<const float2*>(q + i * 8u + t2);
+        }
+    }
     // this warp's tiles: tile i starts at key j0 + 16 (4 i + warp); lane i holds its page and
     // the position of its first key
     const uint32_t j0 = kb & ~(kKeys - 1u);
@@ -118,7 +131,6 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     for (uint32_t i = 0; i + 1u < F::kStages; ++i) fetch(i);
 
     // this thread's query rows: g (and g + 8), channels 2t, 2t + 1, 2t + 8, 2t + 9 of every 16
-    const uint32_t g = lane >> 2, t2 = (lane & 3u) * 2u;
     uint32_t qf[kMine][HD / 16][4];  // 8 rows: both halves in one operand; 16: the high and the low halves
     float unscale[kMine], m[kMine], l[kMine];
     uint32_t p_lo[kMine], p_hi[kMine];
@@ -126,13 +138,10 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     for (uint32_t h = 0; h < kMine; ++h) {
         const uint32_t r = g + 8u * h;
         const int p = row_pos[r];
-        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
-        float2 x[HD / 8];
+        float2* const x = qx[h];
         float big = 0.f;
 #pragma unroll
         for (uint32_t i = 0; i < HD / 8; ++i) {
-            x[i] = make_float2(0.f, 0.f);
-            if (p >= 0 && i * 8u < hd) x[i] = *reinterpret_cast<const float2*>(q + i * 8u + t2);
             x[i].x *= a.scale_log2;
             x[i].y *= a.scale_log2;
             big = fmaxf(big, fmaxf(fabsf(x[i].x), fabsf(x[i].y)));

@@ -178,6 +178,20 @@ def test_windows_wider_than_any_sequence(lib, cuda, type_, q):
         assert cuda.equal(d.attention(window), whole), window
 
 
+@pytest.mark.parametrize("type_,hd,page", [(F16, 64, 16), (F16, 128, 256), (F32, 64, 32), (F16, 136, 64)])
+@pytest.mark.parametrize("seqs", [33, 64, 70])
+def test_many_sequences_of_many_lengths(lib, cuda, type_, hd, page, seqs):
+    """Row tiles found among many sequences, in order of their keys and not."""
+    r = np.random.default_rng(seqs)
+    q = r.integers(0, 24, seqs)
+    q[3] = 0
+    kv = q + r.integers(-3, 200, seqs).clip(-q)
+    d = dev(lib, cuda, type_, 6, 2, hd, page, q=[int(x) for x in q], kv=[int(x) for x in kv], tail=2, seed=34)
+    for window in (0, 50):
+        check_attention(d.s, d.attention(window), d.s.attention(window))
+    lib.status()
+
+
 @pytest.mark.parametrize("type_", [F16, F32])
 @pytest.mark.parametrize("q", [1, 40])
 def test_nothing_cached_anywhere(lib, cuda, type_, q):
