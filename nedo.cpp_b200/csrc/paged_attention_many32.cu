@@ -11,7 +11,7 @@
 // tile's scale a number keeps 2^-38 of the tile's largest: less than its own 22 bits where it is
 // below 2^-16 of that.  A tile in which some key or value is that much smaller than another as
 // a whole (a row must not lose its digits to one that it may not even see) is done in fp32, key
-// by key; so is one with values that are not finite and rows that do not see all of it.
+// by key; so is one with numbers that are not finite.
 //
 // Work.  A CTA of one warp for 16 rows (128 rows, 64 for heads above 128) takes its rows through
 // their keys in tiles of 64 (32).  The next tile's keys and values are on their way (cp.async)
@@ -41,16 +41,11 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return r * Many32<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
 }
 
-__device__ __forceinline__ float finite_size(float x) {
-    const float s = fabsf(x);
-    return s < INFINITY ? s : 0.f;
-}
-// Two values as halves {hi, lo}; an infinity or NaN is all in the high half.
-__device__ __forceinline__ void split_any(float x, float y, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    *hi = pack(h);
-    *lo = pack(__floats2half2_rn(fabsf(f.x) < INFINITY ? x - f.x : 0.f, fabsf(f.y) < INFINITY ? y - f.y : 0.f));
+// The largest magnitude of four numbers, as its bits (which order magnitudes; NaN last).
+__device__ __forceinline__ uint32_t size_bits(const float4& v) {
+    const uint32_t x = __float_as_uint(v.x) & 0x7FFFFFFFu, y = __float_as_uint(v.y) & 0x7FFFFFFFu;
+    const uint32_t z = __float_as_uint(v.z) & 0x7FFFFFFFu, w = __float_as_uint(v.w) & 0x7FFFFFFFu;
+    return max(max(x, y), max(z, w));
 }
 
 template <uint32_t HD>
@@ -60,8 +55,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
-    __shared__ float row_unscale[kRows], size[2][M::kWarps], least[2][M::kWarps];
-    __shared__ uint32_t found[2], odd_warp[M::kWarps];
+    __shared__ float row_unscale[kRows];
+    __shared__ uint32_t found[2], size[2][M::kWarps], least[2][M::kWarps];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t kh = blockIdx.x % a.kv.kv_heads;
     uint32_t rest = blockIdx.x / a.kv.kv_heads;
@@ -241,62 +236,61 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         const uint32_t have = there, j = j0 + i * kKeys;
         cp_wait<0>();
         // the tile as halves: every thread its own pieces (the ones it copied), first their sizes
-        float big[2] = {0.f, 0.f}, small[2] = {INFINITY, INFINITY};
-        bool odd = false;
+        uint32_t big[2] = {0u, 0u}, small[2] = {0x7F800000u, 0x7F800000u};
         constexpr uint32_t kLanes = HD / 4u < 32u ? HD / 4u : 32u;  // lanes that hold a key's (or half a key's) channels
-        const uint32_t lanes = kLanes == 32u ? 0xFFFFFFFFu : ((1u << kLanes) - 1u) << (lane & ~(kLanes - 1u));
-#pragma unroll 4
+        constexpr bool kHold = HD <= 128u;  // in registers from the one pass to the other
+        const uint32_t lanes = kLanes == 32u ? 0xFFFFFFFFu : ((1u << (kLanes & 31u)) - 1u) << (lane & ~(kLanes - 1u));
+        float4 held[kHold ? kPieces : 1u][2];
+#pragma unroll
         for (uint32_t x = 0; x < kPieces; ++x) {
             const uint32_t piece = (piece_row + x * kAtOnce) * (HD / 4u) + piece_ch;
 #pragma unroll
             for (uint32_t kv = 0; kv < 2u; ++kv) {
                 const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
-                const float most = fmaxf(fmaxf(finite_size(v.x), finite_size(v.y)), fmaxf(finite_size(v.z), finite_size(v.w)));
-                // (magnitudes order like their bits)
-                const float row = __uint_as_float(__reduce_max_sync(lanes, __float_as_uint(most)));
-                big[kv] = fmaxf(big[kv], row);
-                if (row != 0.f) small[kv] = fminf(small[kv], row);
-                if (kv == 1u) odd |= !(fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))) < INFINITY) ||
-                                     v.x != v.x || v.y != v.y || v.z != v.z || v.w != v.w;
+                if constexpr (kHold) held[x][kv] = v;
+                const uint32_t row = __reduce_max_sync(lanes, size_bits(v));
+                big[kv] = max(big[kv], row);
+                if (row != 0u) small[kv] = min(small[kv], row);
             }
         }
 #pragma unroll
         for (uint32_t kv = 0; kv < 2u; ++kv) {
             if constexpr (kLanes < 32u) {
-                big[kv] = fmaxf(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], 16));
-                small[kv] = fminf(small[kv], __shfl_xor_sync(0xFFFFFFFFu, small[kv], 16));
+                big[kv] = max(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], 16));
+                small[kv] = min(small[kv], __shfl_xor_sync(0xFFFFFFFFu, small[kv], 16));
             }
             if (lane == 0u) {
                 size[kv][warp] = big[kv];
                 least[kv][warp] = small[kv];
             }
         }
-        odd = __any_sync(0xFFFFFFFFu, odd);
-        if (lane == 0u) odd_warp[warp] = odd;
         __syncthreads();  // also: all warps are done with the halves of the tile before
-        odd = false;
 #pragma unroll
         for (uint32_t w = 0; w < M::kWarps; ++w) {
 #pragma unroll
             for (uint32_t kv = 0; kv < 2u; ++kv) {
-                big[kv] = fmaxf(big[kv], size[kv][w]);
-                small[kv] = fminf(small[kv], least[kv][w]);
+                big[kv] = max(big[kv], size[kv][w]);
+                small[kv] = min(small[kv], least[kv][w]);
             }
-            odd |= odd_warp[w] != 0u;
         }
-        const bool wild = big[0] > small[0] * 65536.f || big[1] > small[1] * 65536.f;
-        const int ek = up_exponent(big[0]), ev = up_exponent(big[1]);
+        const float k_big = __uint_as_float(big[0]), v_big = __uint_as_float(big[1]);
+        const bool slow = max(big[0], big[1]) >= 0x7F800000u || k_big > __uint_as_float(small[0]) * 65536.f ||
+                          v_big > __uint_as_float(small[1]) * 65536.f;
+        const int ek = up_exponent(k_big), ev = up_exponent(v_big);
         const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek), v_down = power_of_two(-ev);
-#pragma unroll 4
+#pragma unroll
         for (uint32_t x = 0; x < kPieces; ++x) {
             const uint32_t r = piece_row + x * kAtOnce, piece = r * (HD / 4u) + piece_ch;
 #pragma unroll
             for (uint32_t kv = 0; kv < 2u; ++kv) {
-                const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
+                float4 v;
+                if constexpr (kHold) v = held[x][kv];
+                else v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
                 const float up = kv ? v_up : k_up;
+                const float2 up2 = make_float2(up, up);
                 uint32_t hi[2], lo[2];
-                split_any(v.x * up, v.y * up, &hi[0], &lo[0]);
-                split_any(v.z * up, v.w * up, &hi[1], &lo[1]);
+                split(__fmul2_rn(make_float2(v.x, v.y), up2), &hi[0], &lo[0]);
+                split(__fmul2_rn(make_float2(v.z, v.w), up2), &hi[1], &lo[1]);
                 uint8_t* dst = halves + kv * 2u * M::kHalfBytes + at<HD>(r, piece_ch >> 1) + (piece_ch & 1u) * 8u;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(dst + M::kHalfBytes) = make_uint2(lo[0], lo[1]);
@@ -307,7 +301,6 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         __syncthreads();
         if (j < we && j + kKeys > wb) {
             const bool whole = have == (1u << kGroups) - 1u && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
-            const bool slow = wild || (odd && !whole);
             float sc[kCols][4];
 #pragma unroll
             for (uint32_t n = 0; n < kCols; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
