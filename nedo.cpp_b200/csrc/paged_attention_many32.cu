@@ -328,21 +328,33 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                         }
                 }
             } else {
+                float low[kCols][4];  // lo hi + hi lo: a part of its own, so that every half is loaded once
 #pragma unroll
-            for (uint32_t turn = 0; turn < 3u; ++turn) {  // lo hi, hi lo, hi hi
+                for (uint32_t n = 0; n < kCols; ++n) low[n][0] = low[n][1] = low[n][2] = low[n][3] = 0.f;
 #pragma unroll
                 for (uint32_t k = 0; k < HD / 16; ++k) {
-                    uint32_t qf[4];
-                    ldsm4(qf, q_addr + (turn == 0u ? M::kQBytes : 0u) + at<HD>(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1)));
+                    uint32_t qhi[4], qlo[4];
+                    const uint32_t q_at = q_addr + at<HD>(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1));
+                    ldsm4(qhi, q_at);
+                    ldsm4(qlo, q_at + M::kQBytes);
 #pragma unroll
                     for (uint32_t n = 0; n < kGroups; ++n) {
-                        uint32_t b[4];
-                        ldsm4(b, k_addr + (turn == 1u ? M::kHalfBytes : 0u) + at<HD>(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
-                        mma(sc[2 * n], qf, b[0], b[1]);
-                        mma(sc[2 * n + 1], qf, b[2], b[3]);
+                        uint32_t bhi[4], blo[4];
+                        const uint32_t k_at = k_addr + at<HD>(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u));
+                        ldsm4(bhi, k_at);
+                        ldsm4(blo, k_at + M::kHalfBytes);
+                        mma(low[2 * n], qlo, bhi[0], bhi[1]);
+                        mma(low[2 * n + 1], qlo, bhi[2], bhi[3]);
+                        mma(sc[2 * n], qhi, bhi[0], bhi[1]);
+                        mma(sc[2 * n + 1], qhi, bhi[2], bhi[3]);
+                        mma(low[2 * n], qhi, blo[0], blo[1]);
+                        mma(low[2 * n + 1], qhi, blo[2], blo[3]);
                     }
                 }
-            }
+#pragma unroll
+                for (uint32_t n = 0; n < kCols; ++n)
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) sc[n][e] += low[n][e];
             }
             const float k_one = slow ? 1.f : k_down;
             if (!whole) {
