@@ -224,21 +224,29 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
             float sc[kCols][4];
 #pragma unroll
             for (uint32_t n = 0; n < kCols; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+            float low[kCols][4];  // from the low halves: a part of its own, so that the keys are loaded once
 #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {  // low halves first
+            for (uint32_t n = 0; n < kCols; ++n) low[n][0] = low[n][1] = low[n][2] = low[n][3] = 0.f;
 #pragma unroll
-                for (uint32_t k = 0; k < HD / 16; ++k) {
-                    uint32_t qf[4];
-                    ldsm4(qf, q_addr + (half ? 0u : kQBytes) + at(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1)));
+            for (uint32_t k = 0; k < HD / 16; ++k) {
+                uint32_t qhi[4], qlo[4];
+                const uint32_t q_at = q_addr + at(warp * 16u + (mi & 1u) * 8u + mr, 2u * k + (mi >> 1));
+                ldsm4(qhi, q_at);
+                ldsm4(qlo, q_at + kQBytes);
 #pragma unroll
-                    for (uint32_t n = 0; n < kGroups; ++n) {
-                        uint32_t b[4];
-                        ldsm4(b, ks + at(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
-                        mma(sc[2 * n], qf, b[0], b[1]);
-                        mma(sc[2 * n + 1], qf, b[2], b[3]);
-                    }
+                for (uint32_t n = 0; n < kGroups; ++n) {
+                    uint32_t b[4];
+                    ldsm4(b, ks + at(n * 16u + (mi >> 1) * 8u + mr, 2u * k + (mi & 1u)));
+                    mma(low[2 * n], qlo, b[0], b[1]);
+                    mma(low[2 * n + 1], qlo, b[2], b[3]);
+                    mma(sc[2 * n], qhi, b[0], b[1]);
+                    mma(sc[2 * n + 1], qhi, b[2], b[3]);
                 }
             }
+#pragma unroll
+            for (uint32_t n = 0; n < kCols; ++n)
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) sc[n][e] += low[n][e];
             const bool gap = tile_gap[i % kStages] != 0u;
             const bool whole = !gap && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
             if (!whole) {
