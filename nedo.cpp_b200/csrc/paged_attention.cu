@@ -157,7 +157,7 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {k == Kernel::kFew ? kFewRows : 2u * kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
-        case Kernel::kMany:  // 64 rows of a head above 128 through the tensor cores, an item to an SM
+        case Kernel::kMany:  // 128 rows of a head above 128 through the tensor cores, an item to an SM
             return {kManyRows, 148u, 0u, 34.0, 5000.0, 1.0};
         case Kernel::kTc:  // 128 rows through 32 MMAs per 128 keys, an item to an SM; 24,000 cycles around its tiles
             return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 12000.0, 1.0};

@@ -1,4 +1,4 @@
-// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 64 query rows of
+// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 128 query rows of
 // heads above 128 channels (prompts, and the tokens of a whole batch over their shared
 // prefix): bound by the tensor cores.  (Up to 128 channels a tile's sums fit into the other
 // kernel's half of TMEM.)
@@ -9,18 +9,22 @@
 // tile's weighted values are therefore summed from zero in 4 steps and added to the
 // running sums in fp32 with the rescaling by 2^(m_old - m_new)).
 //
-// Work.  A CTA of four warps, 16 rows each, takes the 64 rows through its keys in tiles of
+// Work.  A CTA of eight warps, 16 rows each, takes the 128 rows through its keys in tiles of
 // 32; the tiles of keys and values are shared by the warps, brought in by cp.async two
 // tiles deep.  Tiles that none of a warp's rows sees are skipped by it, and only tiles
-// seen in part are masked.  8 query and 2 KV heads of 256 channels, 900 and 529 new tokens of two
-// sequences over 1600 and 1147 keys: 209 us, 118 TFLOP/s of MMAs (two for each product).
+// seen in part are masked.
+//
+// 12 query and 4 KV heads of 256 channels, 2048 and 1840 new tokens of two sequences over 4096 and
+// 2550 keys: 814 us, 280 TFLOP/s of MMAs (two for each product); a CTA of four warps for 64 rows
+// took 1084.  8 query and 2 KV heads, 900 and 529 tokens over 1600 and 1147 keys: 202 us, where 64
+// rows took 169, because 90 items leave SMs without one.
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
 namespace nedo_gpu {
 namespace {
 
-constexpr uint32_t kWarps = 4;
+constexpr uint32_t kWarps = kManyRows / 16u;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kStages = 2;
 constexpr uint32_t HD = 256;                             // channels of a row in shared memory
@@ -85,15 +89,17 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     // keys [kb, ke) of the tile and [wb, we) of this warp; [all_b, all_e): seen by all its rows
     uint32_t kb = kNone, ke = 0, wb = kNone, we = 0, all_b = 0, all_e = kNone;
     {
-        uint32_t lo[2], hi[2];
+        uint32_t lo = kNone, hi = 0;
 #pragma unroll
-        for (uint32_t u = 0; u < 2; ++u) {
+        for (uint32_t u = 0; u < kManyRows / 32u; ++u) {
             const int p = row_pos[lane + 32u * u];
-            lo[u] = p >= 0 ? first_key(p, a.window) : kNone;
-            hi[u] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
+            if (p >= 0) {
+                lo = min(lo, first_key(p, a.window));
+                hi = max(hi, static_cast<uint32_t>(p) + 1u);
+            }
         }
-        kb = __reduce_min_sync(0xFFFFFFFFu, min(lo[0], lo[1]));
-        ke = __reduce_max_sync(0xFFFFFFFFu, max(hi[0], hi[1]));
+        kb = __reduce_min_sync(0xFFFFFFFFu, lo);
+        ke = __reduce_max_sync(0xFFFFFFFFu, hi);
         const int p = row_pos[warp * 16u + (lane & 15u)];
         const uint32_t l1 = p >= 0 ? first_key(p, a.window) : kNone, h1 = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
         wb = __reduce_min_sync(0xFFFFFFFFu, l1);

