@@ -438,7 +438,14 @@ NEDO_GPU_API int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cac
  * for a row at position p (window 0: all).  With shared_pages > 0 the keys of the
  * shared prefix are read once for the whole batch.  Sums and softmax statistics
  * are kept in 32 bits.  On the tensor cores a row's query channels keep 22 bits, or
- * 2^-38 of the row's largest, whichever is coarser. */
+ * 2^-38 of the row's largest, whichever is coarser.
+ *
+ * Infinities (an F16 cache holds what is above 65504 as one) count as they do in the
+ * formula: a key whose score is -infinity has no weight, one whose score is +infinity
+ * makes its rows NaN, and an infinite value gives that infinity to its channel of every
+ * row that sees it, or NaN where its weight is below 2^-126 of the row's largest.  Rows
+ * whose sums are not finite are formed twice on F16 caches, the second time key by key:
+ * right, but slow. */
 NEDO_GPU_API int nedo_gpu_paged_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
                                               uint32_t heads, const float* q_dev, float* out_dev, float scale,
                                               uint32_t window, void* workspace_dev, uint64_t workspace_bytes,

@@ -126,6 +126,65 @@ __device__ __forceinline__ void checked_list(const uint32_t* __restrict__ l, uin
     }
 }
 
+// A query row's sums over F16 keys, formed by one warp key by key in fp32.  The tensor-core kernels
+// multiply with factors split in two halves, and an infinite key or value times halves of
+// different sign, or one that is zero, is NaN where the whole factor gives infinity (or, for a
+// score of -infinity, no weight at all).  A value that is not finite also reaches the rows of its
+// tile that do not see it, as 0 * inf.  Either stays in the running sums, so the kernels look
+// at a row's sums once, when they are complete, and take those that are not finite from here.
+// Sums go by 2^(s - m); lane i has channels i, i + 32, ...
+struct RowSums {
+    float m, l, o[8];
+};
+// Keys `from`, from + 1, ... below `to` in steps of 16 that are `stride` apart (from a multiple of
+// 16 where stride is not 16): positions, or places in the page list (`list`).
+static __device__ __noinline__ void row_key_by_key(const AttnArgs& a, uint32_t s, uint32_t kh, const uint32_t* list, uint32_t tok,
+                                            uint32_t head, int p, uint32_t from, uint32_t to, uint32_t stride, RowSums* r) {
+    const uint32_t lane = threadIdx.x & 31u, hd = a.kv.head_dim, in_page = a.kv.page_size - 1u;
+    const float* q = a.q + (static_cast<size_t>(tok) * a.heads + head) * hd;
+    float x[8], odd = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) {
+        x[i] = lane + 32u * i < hd ? q[lane + 32u * i] * a.scale_log2 : 0.f;
+        odd = fmaf(x[i], 0.f, odd);
+        r->o[i] = 0.f;
+    }
+    r->m = -INFINITY;
+    r->l = 0.f;
+    if (__any_sync(0xFFFFFFFFu, odd != 0.f)) {  // such a query has no number for an answer
+        r->m = 0.f;
+        r->l = NAN;
+        return;
+    }
+    const uint32_t lo = first_key(p, a.window), hi = static_cast<uint32_t>(p) + 1u;
+    for (uint32_t j = from & ~15u; j < to; j += stride) {
+        const uint32_t lp = list != nullptr ? list[j >> a.kv.page_shift] : j >> a.kv.page_shift;
+        if (lp == kNone) continue;
+        const uint32_t pos = (lp << a.kv.page_shift) + (j & in_page);
+        if (pos >= hi || pos + 16u <= lo) continue;
+        const uint32_t page = load_page(a.b, a.kv, s, lp, a.st);
+        if (page == kNone) continue;
+        for (uint32_t e = 0; e < 16u; ++e) {
+            if (pos + e < lo || pos + e >= hi || j + e < from || j + e >= to) continue;
+            const size_t at = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size + ((pos + e) & in_page)) * hd + lane;
+            const __half *k = static_cast<const __half*>(a.kv.k) + at, *v = static_cast<const __half*>(a.kv.v) + at;
+            float sum = 0.f;
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (lane + 32u * i < hd) sum = fmaf(x[i], __half2float(k[32u * i]), sum);
+            sum = warp_sum(sum);
+            const float m = fmaxf(r->m, sum), ref = m == -INFINITY ? 0.f : m;
+            const float alpha = exp2f(r->m - ref), w = exp2f(sum - ref);
+            r->l = fmaf(r->l, alpha, w);
+#pragma unroll
+            for (uint32_t i = 0; i < 8u; ++i)
+                if (lane + 32u * i < hd) r->o[i] = fmaf(r->o[i], alpha, w * __half2float(v[32u * i]));
+            r->m = m;
+        }
+    }
+    if (r->m == -INFINITY) r->m = 0.f;
+}
+
 constexpr uint32_t kFewRows = 8;
 constexpr uint32_t kFewMax = 16;     // rows of a sequence that still go to the few-rows kernels, in tiles of 8 or 16
 constexpr uint32_t kMaxCluster = 8;  // chunks that a cluster can hold

@@ -235,58 +235,26 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             for (uint32_t k = 0; k < 2u; ++k)
                 split(v[h][2u * k], v[h][2u * k + 1u], &pf[0][2u * k + h], kMine == 1u ? &pf[0][2u * k + 1u] : &pf[kMine - 1u][2u * k + h]);
         }
-        // a value that is not finite must not reach the rows that do not see it (0 * inf):
-        // only tiles that some row sees in part can hold one, and those are few
-        bool odd = false;
-        if (!whole) {
 #pragma unroll
-            for (uint32_t n = 0; n < HD / 16; ++n) {
-                uint32_t b[4];
-                ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
-                odd |= not_finite(b[0]) || not_finite(b[1]) || not_finite(b[2]) || not_finite(b[3]);
-            }
-            odd = __any_sync(0xFFFFFFFFu, odd);
-        }
-        if (!odd) {
+        for (uint32_t n = 0; n < HD / 16; ++n) {
+            uint32_t b[4];
+            ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+            if constexpr (kMine == 1u) {
+                mma(acc[2 * n], pf[0], b[0], b[1]);
+                mma(acc[2 * n + 1], pf[0], b[2], b[3]);
+            } else {
+                // from zero, and added in fp32: the tensor core would cut the running sums twice a tile
+                float o[2][4];
 #pragma unroll
-            for (uint32_t n = 0; n < HD / 16; ++n) {
-                uint32_t b[4];
-                ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
-                if constexpr (kMine == 1u) {
-                    mma(acc[2 * n], pf[0], b[0], b[1]);
-                    mma(acc[2 * n + 1], pf[0], b[2], b[3]);
-                } else {
-                    // from zero, and added in fp32: the tensor core would cut the running sums twice a tile
-                    float o[2][4];
+                for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+                mma(o[0], pf[kMine - 1u], b[0], b[1]);
+                mma(o[1], pf[kMine - 1u], b[2], b[3]);
+                mma(o[0], pf[0], b[0], b[1]);
+                mma(o[1], pf[0], b[2], b[3]);
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
-                    mma(o[0], pf[kMine - 1u], b[0], b[1]);
-                    mma(o[1], pf[kMine - 1u], b[2], b[3]);
-                    mma(o[0], pf[0], b[0], b[1]);
-                    mma(o[1], pf[0], b[2], b[3]);
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        acc[2 * n][e] += o[0][e];
-                        acc[2 * n + 1][e] += o[1][e];
-                    }
-                }
-            }
-        } else {
-            for (uint32_t j = 0; j < kKeys; ++j) {
-                const uint32_t from = (lane & ~3u) | ((j & 7u) >> 1);
-#pragma unroll
-                for (uint32_t h = 0; h < kMine; ++h) {
-                    const float w0 = __shfl_sync(0xFFFFFFFFu, v[h][0], from), w1 = __shfl_sync(0xFFFFFFFFu, v[h][1], from);
-                    const float w2 = __shfl_sync(0xFFFFFFFFu, v[h][2], from), w3 = __shfl_sync(0xFFFFFFFFu, v[h][3], from);
-                    const float w = j < 8u ? (j & 1u ? w1 : w0) : (j & 1u ? w3 : w2);
-                    if (pos + j < p_lo[h] || pos + j >= p_hi[h] || page == kNone) continue;
-#pragma unroll
-                    for (uint32_t n = 0; n < HD / 8; ++n) {
-                        const uint8_t* row = my_ring + (vs - ring_addr) + at<HD>(j, n) + t2 * 2u;
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(row));
-                        acc[n][2u * h] = fmaf(w, f.x, acc[n][2u * h]);
-                        acc[n][2u * h + 1u] = fmaf(w, f.y, acc[n][2u * h + 1u]);
-                    }
+                for (uint32_t e = 0; e < 4; ++e) {
+                    acc[2 * n][e] += o[0][e];
+                    acc[2 * n + 1][e] += o[1][e];
                 }
             }
         }
@@ -295,6 +263,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
     // the warps' sums, in warp order
+    uint32_t again[kMine];  // four bits to a row whose sums are not finite
 #pragma unroll
     for (uint32_t h = 0; h < kMine; ++h) {
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
@@ -303,6 +272,13 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             wm[warp][g + 8u * h] = (m[h] == -INFINITY ? 0.f : m[h]) - kUp;
             wl[warp][g + 8u * h] = row_pos[g + 8u * h] >= 0 ? l[h] : 0.f;  // padding sees nothing
         }
+        float odd = l[h] * 0.f;
+#pragma unroll
+        for (uint32_t n = 0; n < HD / 8; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 4u; ++e)
+                if (kMine == 1u || e >> 1 == h) odd = fmaf(acc[n][e], 0.f, odd);
+        again[h] = __ballot_sync(0xFFFFFFFFu, odd != 0.f && row_pos[g + 8u * h] >= 0);
     }
     __syncthreads();
     float* part = reinterpret_cast<float*>(ring);  // [warp][row][HD + 4]
@@ -315,6 +291,22 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
         } else {
             *reinterpret_cast<float2*>(to) = make_float2(acc[n][0], acc[n][1]);
             *reinterpret_cast<float2*>(to + 8u * kPitch) = make_float2(acc[n][2], acc[n][3]);
+        }
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < kMine; ++h) {
+        if (again[h] == 0u) continue;
+        __syncwarp();
+        for (uint32_t r = 8u * h; r < 8u * h + 8u; ++r) {
+            if ((again[h] >> (4u * (r & 7u)) & 15u) == 0u) continue;
+            RowSums x;
+            row_key_by_key(a, s, kh, a.part == kPartBlocks ? list : nullptr, row_tok[r], row_head[r], row_pos[r],
+                           j0 + kKeys * warp, ke, kKeys * kWarps, &x);
+            for (uint32_t i = 0; lane + 32u * i < hd; ++i) part[(warp * ROWS + r) * kPitch + lane + 32u * i] = x.o[i];
+            if (lane == 0u) {
+                wm[warp][r] = x.m;
+                wl[warp][r] = x.l;
+            }
         }
     }
     __syncthreads();

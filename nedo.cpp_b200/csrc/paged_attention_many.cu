@@ -300,72 +300,29 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
                 split(sc[n][0], sc[n][1], &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
                 split(sc[n][2], sc[n][3], &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
             }
-            bool odd = false;
-            if (!whole) {
-                // a value that is not finite must not reach the rows that do not see it (0 * inf)
-                for (uint32_t x = lane; x < kKeys * (HD / 8u); x += 32u) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(sm + (vs - q_addr) + x * 16u);
-                    odd |= not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w);
+#pragma unroll
+            for (uint32_t n = 0; n < HD / 16; ++n) {
+                float o[2][4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+                uint32_t b[kGroups][4];
+#pragma unroll
+                for (uint32_t k = 0; k < kGroups; ++k)
+                    ldsm4t(b[k], vs + at(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+#pragma unroll
+                for (uint32_t k = 0; k < kGroups; ++k) {
+                    mma(o[0], plo[k], b[k][0], b[k][1]);
+                    mma(o[1], plo[k], b[k][2], b[k][3]);
                 }
-                odd = __any_sync(0xFFFFFFFFu, odd);
-            }
-            if (!odd) {
 #pragma unroll
-                for (uint32_t n = 0; n < HD / 16; ++n) {
-                    float o[2][4];
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
-                    uint32_t b[kGroups][4];
-#pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k)
-                        ldsm4t(b[k], vs + at(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
-#pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k) {
-                        mma(o[0], plo[k], b[k][0], b[k][1]);
-                        mma(o[1], plo[k], b[k][2], b[k][3]);
-                    }
-#pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k) {
-                        mma(o[0], phi[k], b[k][0], b[k][1]);
-                        mma(o[1], phi[k], b[k][2], b[k][3]);
-                    }
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) {
-                        acc[2 * n][e] = fmaf(acc[2 * n][e], alpha[e >> 1], o[0][e]);
-                        acc[2 * n + 1][e] = fmaf(acc[2 * n + 1][e], alpha[e >> 1], o[1][e]);
-                    }
+                for (uint32_t k = 0; k < kGroups; ++k) {
+                    mma(o[0], phi[k], b[k][0], b[k][1]);
+                    mma(o[1], phi[k], b[k][2], b[k][3]);
                 }
-            } else {
 #pragma unroll
-                for (uint32_t n = 0; n < HD / 8; ++n)
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) acc[n][e] *= alpha[e >> 1];
-#pragma unroll
-                for (uint32_t n8 = 0; n8 < kCols; ++n8) {
-                    for (uint32_t jj = 0; jj < 8; ++jj) {
-                        const uint32_t from = (lane & ~3u) | (jj >> 1), key = j + n8 * 8u + jj;
-                        float w[2];
-#pragma unroll
-                        for (uint32_t h = 0; h < 2; ++h) {
-                            const float w0 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h], from);
-                            const float w1 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h + 1], from);
-                            w[h] = jj & 1u ? w1 : w0;
-                        }
-                        const bool see0 = key >= lo_key[0] && key < hi_key[0], see1 = key >= lo_key[1] && key < hi_key[1];
-#pragma unroll
-                        for (uint32_t n = 0; n < HD / 8; ++n) {
-                            const uint8_t* at_v = sm + (vs - q_addr) + at(n8 * 8u + jj, n) + t2 * 2u;
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(at_v));
-                            if (see0) {
-                                acc[n][0] = fmaf(w[0], f.x, acc[n][0]);
-                                acc[n][1] = fmaf(w[0], f.y, acc[n][1]);
-                            }
-                            if (see1) {
-                                acc[n][2] = fmaf(w[1], f.x, acc[n][2]);
-                                acc[n][3] = fmaf(w[1], f.y, acc[n][3]);
-                            }
-                        }
-                    }
+                for (uint32_t e = 0; e < 4; ++e) {
+                    acc[2 * n][e] = fmaf(acc[2 * n][e], alpha[e >> 1], o[0][e]);
+                    acc[2 * n + 1][e] = fmaf(acc[2 * n + 1][e], alpha[e >> 1], o[1][e]);
                 }
             }
         }
@@ -374,13 +331,18 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");
     const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
+    uint32_t again[2];  // four bits to a row whose sums are not finite
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 2);
         const uint32_t r = warp * 16u + g + 8u * h;
         const int p = row_pos[r];
-        if (p == -2) continue;
+        float odd = l[h] * 0.f;
+#pragma unroll
+        for (uint32_t n = 0; n < HD / 8; ++n) odd = fmaf(acc[n][2 * h], 0.f, fmaf(acc[n][2 * h + 1], 0.f, odd));
+        again[h] = __ballot_sync(0xFFFFFFFFu, odd != 0.f && p >= 0);
+        if (p == -2 || (again[h] >> (lane & ~3u) & 15u)) continue;
         if (p < 0) l[h] = 0.f;  // padding sees nothing
         const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
         float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
@@ -394,6 +356,21 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         }
         if (!a.direct && (lane & 3u) == 0u)
             a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2((m[h] == -INFINITY ? 0.f : m[h]) - kUp, l[h]);
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < 2; ++h) {
+        if (again[h] == 0u) continue;
+        for (uint32_t u = 0; u < 8u; ++u) {
+            if ((again[h] >> (4u * u) & 15u) == 0u) continue;
+            const uint32_t r = warp * 16u + 8u * h + u;
+            RowSums x;
+            row_key_by_key(a, s, kh, nullptr, row_tok[r], row_head[r], row_pos[r], kb, ke, 16u, &x);
+            const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
+            float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
+            const float f = !a.direct ? 1.f : x.l == 0.f ? 0.f : 1.f / x.l;
+            for (uint32_t i = 0; lane + 32u * i < hd; ++i) o[lane + 32u * i] = x.o[i] * f;
+            if (!a.direct && lane == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(x.m, x.l);
+        }
     }
 }
 

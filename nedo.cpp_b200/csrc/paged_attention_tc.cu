@@ -169,7 +169,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     __shared__ int row_pos[kRows];
     __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
     __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
-    __shared__ uint32_t found[2], tmem_slot, gaps[8];
+    __shared__ uint32_t found[2], tmem_slot, gaps[8], again[kRows / 32u];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
     uint8_t* const sm = sm_raw + (s0 - smem_addr(sm_raw));
     const uint32_t ring = s0 + 2u * T::kTile;
@@ -187,6 +187,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             mbar_init(&empty[i], 1);
         }
         mbar_init(&cut, 1);
+        for (uint32_t i = 0; i < kRows / 32u; ++i) again[i] = 0u;
         for (uint32_t i = 0; i < kBuffers; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 8);
@@ -575,63 +576,26 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 if (!ok) break;
                 tc_fence_after();
                 if (j < we && j + kKeys > wb) {
-                    const uint32_t gap = *reinterpret_cast<volatile uint32_t*>(&gaps[i & 7u]);
-                    const bool whole = gap == 0u && j >= all_b && j + kKeys <= all_e;
                     // the tile's weights go by its half's maximum, the sums by the largest so far
                     const float ref = tile_ref[i % (2u * kBuffers)][r], most = fmaxf(top, ref);
                     const float alpha = most == -INFINITY ? 1.f : exp2_fast(top - most);
                     const float beta = ref == -INFINITY ? 0.f : exp2_fast(ref - most);
                     top = most;
-                    uint32_t x[16];
-                    bool odd = false;
-                    if (!whole) {
-                        // a value that is not finite must not reach the rows that do not see it, yet
-                        // 0 * inf is in their sums: then the tile is done key by key
-                        float t = 0.f;
-#pragma unroll 1
-                        for (uint32_t k = 0; k < kD / 16u; ++k) {
-                            tmem_load(o_addr + 16u * k, x);
-                            tmem_ready(x);
-#pragma unroll
-                            for (uint32_t e = 0; e < 16u; ++e) t = fmaf(__uint_as_float(x[e]), 0.f, t);
-                        }
-                        odd = p >= 0 && t != 0.f;
-                    }
                     const float2 alpha2 = make_float2(alpha, alpha), beta2 = make_float2(beta, beta);
-                    if (!__any_sync(0xFFFFFFFFu, odd)) {
 #pragma unroll
-                        for (uint32_t k = 0; k < kD / 16u; k += 2u) {
-                            uint32_t y[2][16];
-                            tmem_load(o_addr + 16u * k, y[0]);
-                            tmem_load(o_addr + 16u * (k + 1u), y[1]);
-                            tmem_ready(y[0]);
-                            tmem_ready(y[1]);
+                    for (uint32_t k = 0; k < kD / 16u; k += 2u) {
+                        uint32_t y[2][16];
+                        tmem_load(o_addr + 16u * k, y[0]);
+                        tmem_load(o_addr + 16u * (k + 1u), y[1]);
+                        tmem_ready(y[0]);
+                        tmem_ready(y[1]);
 #pragma unroll
-                            for (uint32_t e = 0; e < 32u; e += 2u) {
-                                const float2 o = make_float2(__uint_as_float(y[e >> 4][e & 15u]), __uint_as_float(y[e >> 4][(e & 15u) + 1u]));
-                                const float2 z = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), alpha2, __fmul2_rn(o, beta2));
-                                acc[16u * k + e] = z.x;
-                                acc[16u * k + e + 1u] = z.y;
-                            }
+                        for (uint32_t e = 0; e < 32u; e += 2u) {
+                            const float2 o = make_float2(__uint_as_float(y[e >> 4][e & 15u]), __uint_as_float(y[e >> 4][(e & 15u) + 1u]));
+                            const float2 z = ffma2(make_float2(acc[16u * k + e], acc[16u * k + e + 1u]), alpha2, __fmul2_rn(o, beta2));
+                            acc[16u * k + e] = z.x;
+                            acc[16u * k + e + 1u] = z.y;
                         }
-                    } else {
-#pragma unroll
-                        for (uint32_t d = 0; d < kD; ++d) acc[d] *= alpha;
-                        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
-                        for (uint32_t key = max(row_b, j); key < min(row_e, j + kKeys); ++key) {
-                            if (!(seen(j, gap, (key - j) >> 4) >> ((key - j) & 15u) & 1u)) continue;
-                            const uint32_t page = a.b.table[static_cast<size_t>(s) * a.b.max_pages + (key >> a.kv.page_shift)];
-                            const size_t off = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size +
-                                                (key & (a.kv.page_size - 1u))) * hd;
-                            const __half *kr = static_cast<const __half*>(a.kv.k) + off, *vr = static_cast<const __half*>(a.kv.v) + off;
-                            float sum = 0.f;
-                            for (uint32_t d = 0; d < hd; ++d) sum = fmaf(q[d] * a.scale_log2, __half2float(kr[d]), sum);
-                            const float w = exp2_fast(sum - (most - kUp));
-#pragma unroll
-                            for (uint32_t d = 0; d < kD; ++d)
-                                if (side * kD + d < hd) acc[d] = fmaf(w, __half2float(vr[side * kD + d]), acc[d]);
-                        }
-                        __syncwarp();
                     }
                 }
                 tc_fence_before();
@@ -646,6 +610,10 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             const float ref = top == -INFINITY ? 0.f : top;
             const float sum = (l0 == 0.f ? 0.f : l0 * exp2_fast(sum_m[0][r] - ref)) + (l1 == 0.f ? 0.f : l1 * exp2_fast(sum_m[1][r] - ref));
             const float scale = a.direct ? 1.f / sum : 1.f;
+            float odd = sum * 0.f;
+#pragma unroll
+            for (uint32_t d = 0; d < kD; ++d) odd = fmaf(acc[d], 0.f, odd);
+            if (odd != 0.f && p >= 0) atomicOr(&again[r >> 5], 1u << (r & 31u));
 #pragma unroll
             for (uint32_t d = 0; d < kD; d += 4u)
                 *reinterpret_cast<float4*>(sums + r * kPitch + side * kD + d) =
@@ -656,6 +624,19 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]] =
                     make_float2(ref - kUp, sum);
             named_barrier_sync(5, kSums);
+            if ((again[0] | again[1] | again[2] | again[3]) != 0u) {  // rows whose sums are not finite
+                for (uint32_t rr = warp - kSumWarp; rr < kRows; rr += kSums / 32u) {
+                    if (!(again[rr >> 5] >> (rr & 31u) & 1u) || !ok) continue;
+                    RowSums x;
+                    row_key_by_key(a, s, kh, nullptr, row_tok[rr], row_head[rr], row_pos[rr], kb, ke, 16u, &x);
+                    const float f = !a.direct ? 1.f : x.l == 0.f ? 0.f : 1.f / x.l;
+                    for (uint32_t i = 0; lane + 32u * i < hd; ++i) sums[rr * kPitch + lane + 32u * i] = x.o[i] * f;
+                    if (!a.direct && lane == 0u)
+                        a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr]] =
+                            make_float2(x.m, x.l);
+                }
+                named_barrier_sync(5, kSums);
+            }
             if (ok) {
                 // rows by lanes next to each other
                 constexpr uint32_t kLanes = HD / 4u, kAtOnce = kSums / kLanes;

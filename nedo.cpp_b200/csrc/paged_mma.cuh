@@ -50,9 +50,6 @@ __device__ __forceinline__ void split(float2 x, uint32_t* hi, uint32_t* lo) {
     *hi = pack(h);
     *lo = pack(__float22half2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y))));
 }
-__device__ __forceinline__ bool not_finite(uint32_t two_halves) {
-    return (two_halves & 0x7C00u) == 0x7C00u || (two_halves & 0x7C000000u) == 0x7C000000u;
-}
 
 // The power of two that takes a row's largest magnitude to [2^13, 2^14), where the low
 // half of its fp16 split is a normal number (0 for zero, infinite and NaN rows).

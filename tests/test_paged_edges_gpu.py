@@ -1,0 +1,101 @@
+"""GPU: the paged KV-cache operators at the edges of their types and sizes, against the 64-bit
+reference (paged_ref.py)."""
+import numpy as np
+import pytest
+
+from paged_ref import F16, F32, Device, Setup
+
+pytestmark = pytest.mark.gpu
+
+
+class Without(Setup):
+    """A Setup whose reference leaves out the keys (sequence, position) in `out` for KV head 0."""
+
+    out = frozenset()
+
+    def keys(self, s, kh, positions):
+        if kh == 0:
+            positions = np.array([p for p in positions if (s, int(p)) not in self.out], np.int64)
+        return super().keys(s, kh, positions)
+
+
+def place(s, seq, pos):
+    return int(s.table[seq, pos // s.page]), pos % s.page
+
+
+def check(got, want, tol, inside):
+    """Infinities and NaN where the definition has them, the others within the tolerance."""
+    got = got.cpu().numpy().astype(np.float64)
+    assert (got[~inside] == 777.0).all()
+    got, want, tol = got[inside], want[inside], tol[inside]
+    assert np.array_equal(np.isnan(got), np.isnan(want)), "NaN elsewhere"
+    odd = np.isinf(want)
+    assert np.array_equal(got[odd], want[odd]), "infinities elsewhere"
+    fine = np.isfinite(want)
+    err = np.abs(got[fine] - want[fine])
+    assert (err <= tol[fine]).all(), f"worst {np.max(err / np.maximum(tol[fine], 1e-300)):.2f} x tolerance"
+
+
+def every_page(s):
+    """A list of all pages of every row's sequence, for block attention."""
+    n = s.max_pages
+    out = np.full((s.tokens, s.kv_heads, n), 0xFFFFFFFF, np.uint32)
+    for t, _, p in s.rows():
+        if p >= 0:
+            out[t, :, :p // s.page + 1] = np.arange(p // s.page + 1)
+    return out
+
+
+# heads, KV heads, channels: tiles of up to 8 and of 16 rows, of 128 rows up to and above 128 channels
+KINDS = [(12, 4, 128), (12, 1, 64), (11, 1, 128), (4, 2, 256), (6, 2, 40)]
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,kv_heads,hd", KINDS)
+@pytest.mark.parametrize("shared", [0, 8])
+def test_infinite_values(lib, cuda, type_, heads, kv_heads, hd, shared):
+    """An infinite value gives its channel of every row that sees it that infinity, two of
+    different signs NaN, wherever its tile lies; no other channel and no other row is touched."""
+    q, kv = [1, 70, 9, 1], [3000, 700, 300, 513]
+    s = Setup(type_, heads, kv_heads, hd, 32, q=q, kv=kv, shared=shared, tail=2, seed=40)
+    for seq, pos, ch, x in ((0, 37, 5, np.inf), (0, 2990, 6, -np.inf), (0, 1500, 5, np.inf), (1, 300, 0, -np.inf),
+                            (1, 660, 7, np.inf), (1, 650, 7, -np.inf), (1, 699, 9, np.inf), (2, 299, 3, -np.inf),
+                            (3, 512, 2, np.inf), (3, 260, 33, -np.inf), (3, 400, 33, np.inf)):
+        page, slot = place(s, seq, pos)
+        s.v[page, 0, slot, ch] = x
+    d = Device(lib, cuda, s)
+    with np.errstate(invalid="ignore"):
+        want = s.attention()
+    assert np.isinf(want[0]).any() and np.isnan(want[0]).any()
+    check(d.attention(), *want)
+    d.out.fill_(777.0)
+    check(d.block_attention(every_page(s)), *want)
+    lib.status()
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,kv_heads,hd", KINDS)
+@pytest.mark.parametrize("shared", [0, 8])
+def test_infinite_keys(lib, cuda, type_, heads, kv_heads, hd, shared):
+    """A key whose score is -infinity has no weight; one whose score is +infinity makes the row
+    NaN."""
+    q, kv = [1, 70, 9, 1], [3000, 700, 300, 513]
+    s = Without(type_, heads, kv_heads, hd, 32, q=q, kv=kv, shared=shared, tail=2, seed=41)
+    s.out = frozenset([(0, 37), (0, 2990), (1, 300), (1, 660), (2, 299), (3, 260), (3, 400)])
+    if shared:  # the first sequence's key lies in the prefix of all
+        s.out |= {(1, 37), (2, 37), (3, 37)}
+    s.queries[:, :, 1] = np.abs(s.queries[:, :, 1]) + 0.1  # their scores are -infinity in every row
+    s.queries[5:9, 0, 1] *= -1.0                           # but in these: +infinity
+    for seq, pos in s.out:
+        page, slot = place(s, seq, pos)
+        s.k[page, 0, slot, 1] = -np.inf
+    d = Device(lib, cuda, s)
+    want, tol, inside = s.attention()
+    for t, seq, p in s.rows():
+        if 5 <= t < 9 and any(x[0] == seq and x[1] <= p for x in s.out):
+            want[t, 0] = np.nan
+    assert np.isnan(want).any()
+    check(d.attention(), want, tol, inside)
+    d.out.fill_(777.0)
+    check(d.block_attention(every_page(s)), want, tol, inside)
+    lib.status()
