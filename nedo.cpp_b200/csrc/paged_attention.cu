@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
         for (uint32_t i0 = 0; i0 < n; i0 += kCombineThreads) {
             const uint32_t cnt = min(kCombineThreads, n - i0);
             __syncthreads();
-            float w = 0.f;
+            float w = -1.f;  // nothing seen there
             if (tid < cnt) {
                 const float2 x = ml[slot(i0 + tid) * rows_all];
                 if (x.y != 0.f) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
                 for (uint32_t i = grp; i < cnt; i += groups) {
                     const float f = wt[i];
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (f != 0.f)
+                    if (f != -1.f)  // (also where the weight is nothing: an infinite value is not passed over)
                         x = *reinterpret_cast<const float4*>(a.part_o + (slot(i0 + i) * rows_all + row) * hd + 4u * d);
                     acc.x = fmaf(x.x, f, acc.x);
                     acc.y = fmaf(x.y, f, acc.y);

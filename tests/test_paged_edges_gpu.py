@@ -99,3 +99,28 @@ def test_infinite_keys(lib, cuda, type_, heads, kv_heads, hd, shared):
     d.out.fill_(777.0)
     check(d.block_attention(every_page(s)), want, tol, inside)
     lib.status()
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,kv_heads,hd", KINDS)
+@pytest.mark.parametrize("shared", [0, 8])
+def test_infinite_values_of_no_weight(lib, cuda, type_, heads, kv_heads, hd, shared):
+    """An infinite value whose weight is below the smallest number still makes its channel no number."""
+    q, kv = [1, 70, 9], [3000, 700, 300]
+    s = Setup(type_, heads, kv_heads, hd, 32, q=q, kv=kv, shared=shared, seed=48)
+    s.queries[..., 0] = 40.0
+    s.scale = 1.0
+    for seq in range(3):  # the newest key and the first one: scores of 400 above all others
+        for pos, x in [(p, 0.0) for p in range(kv[seq] - q[seq], kv[seq])] + [(0, 10.0)]:
+            page, slot = place(s, seq, pos)
+            s.k[page, :, slot, 0] = x
+    for seq, pos in ((0, 2000), (1, 500), (2, 280)):
+        page, slot = place(s, seq, pos)
+        s.k[page, 0, slot, 0] = -10.0
+        s.v[page, 0, slot, 3] = np.inf
+    d = Device(lib, cuda, s)
+    for got in (d.attention().cpu().numpy(), d.block_attention(every_page(s)).cpu().numpy()):
+        g = heads // kv_heads
+        assert not np.isfinite(got[:, :g, 3]).any()
+        got[:, :g, 3] = 0
+        assert np.isfinite(got).all()
