@@ -360,9 +360,10 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
     };
 
     const uint32_t want = picks - 1u;
-    // what a score can be off, rounded up (nothing where all of them are zero)
+    // what a score can be off, rounded up (nothing where all of them are zero, not only too small for 32 bits)
     const float most = size * __uint_as_float(top_bits) * 1.01f;
-    const float off = most == 0.f ? 0.f : (PIECES * P::kCount + group + 13u) * 6.0e-8f * most + 1e-37f;
+    const bool zero = most == 0.f && (size == 0.f || top_bits == 0u);
+    const float off = zero ? 0.f : (PIECES * P::kCount + group + 13u) * 6.0e-8f * most + 1e-37f;
     // a thread's share of the pages, in order
     const uint32_t run = (others + kThreads - 1u) / kThreads, a0 = min(others, tid * run), a1 = min(others, a0 + run);
     uint32_t total;
@@ -433,7 +434,7 @@ __global__ void __launch_bounds__(kThreads) block_select_kernel(PagedKv kv, Page
             }
         }
     }
-    if (most == 0.f && all_bits == any_bits) {  // all scores are zero: the first pages
+    if (zero && all_bits == any_bits) {  // all scores are zero: the first pages
         for (uint32_t i = tid; i < picks; i += kThreads) out[i] = i < want ? i : n - 1u;
         return;
     }

@@ -124,3 +124,14 @@ def test_infinite_values_of_no_weight(lib, cuda, type_, heads, kv_heads, hd, sha
         assert not np.isfinite(got[:, :g, 3]).any()
         got[:, :g, 3] = 0
         assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("picks", [2, 5, 20])
+@pytest.mark.parametrize("query,bound", [(1e-26, 1e-22), (1e-38, 1e-30), (1e-44, 1e-38), (1e-30, 1e-10)])
+def test_select_tiny_scores(lib, cuda, picks, query, bound):
+    """Scores that are nothing in 32 bits are still told apart in 64."""
+    s = Setup(F32, 6, 2, 64, 16, q=[1, 2], kv=[700, 500], seed=42)
+    s.queries = (s.queries * query).astype(np.float32)
+    s.bounds = (s.bounds * np.float64(bound)).astype(np.float32)
+    d = Device(lib, cuda, s)
+    assert np.array_equal(d.select(picks).cpu().numpy().view(np.uint32), s.select(picks))
