@@ -487,9 +487,14 @@ cudaError_t launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const
                    uint32_t* blocks, DeviceStatus* st, cudaStream_t stream) {
     const uint32_t pages = (b.max_kv_len + kv.page_size - 1u) >> kv.page_shift;
     const uint32_t key_words = (pages + 3u) & ~3u;
-    const size_t smem = std::max(key_words * sizeof(uint64_t), key_words * sizeof(uint32_t) + kWarps * kStages * kGroup * PIECES * 512u);
+    auto bytes = [](uint32_t words) {
+        return std::max(words * sizeof(uint64_t), words * sizeof(uint32_t) + kWarps * kStages * kGroup * PIECES * 512u);
+    };
+    const size_t smem = bytes(key_words);
+    // the limit is the process's: the same for every call, or one host thread's call could lower it
+    // between another's limit and launch
     cudaError_t e = cudaFuncSetAttribute(block_select_kernel<T, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(smem));
+                                         static_cast<int>(bytes(kMaxSelectPages)));
     if (e != cudaSuccess) return e;
     // CTAs per token and KV head: as many as run at once on 148 SMs, with pages for every warp
     const uint64_t units = static_cast<uint64_t>(b.tokens) * kv.kv_heads;

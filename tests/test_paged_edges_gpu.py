@@ -1,5 +1,7 @@
 """GPU: the paged KV-cache operators at the edges of their types and sizes, against the 64-bit
 reference (paged_ref.py)."""
+import threading
+
 import numpy as np
 import pytest
 
@@ -135,3 +137,35 @@ def test_select_tiny_scores(lib, cuda, picks, query, bound):
     s.bounds = (s.bounds * np.float64(bound)).astype(np.float32)
     d = Device(lib, cuda, s)
     assert np.array_equal(d.select(picks).cpu().numpy().view(np.uint32), s.select(picks))
+
+
+def test_select_from_two_host_threads(lib, cuda):
+    """Calls with short and with long sequences from two threads, each on a stream of its own."""
+    sets = [Setup(F16, 2, 1, 64, 16, q=[1], kv=[100], seed=43), Setup(F16, 2, 1, 64, 16, q=[1], kv=[100], seed=44)]
+    sets[1].kv, sets[1].max_pages = [16384 * 16], 16384
+    sets[1].table = sets[1].table[:, np.arange(16384) % 6]
+    ds = [Device(lib, cuda, s) for s in sets]
+    want = [s.select(4) for s in sets]
+    streams = [cuda.cuda.Stream() for _ in ds]
+    outs = [cuda.zeros((1, 1, 4), dtype=cuda.int32, device="cuda") for _ in ds]
+    cuda.cuda.synchronize()
+    errors, go = [], threading.Barrier(2)
+
+    def work(i):
+        try:
+            go.wait(10)
+            for _ in range(3000):
+                lib.block_select_dev(ds[i].cache, ds[i].batch, 2, ds[i].q.data_ptr(), 4, outs[i].data_ptr(),
+                                     streams[i].cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    cuda.cuda.synchronize()
+    assert not errors, errors[0]
+    for o, w in zip(outs, want):
+        assert np.array_equal(o.cpu().numpy().view(np.uint32), w)
