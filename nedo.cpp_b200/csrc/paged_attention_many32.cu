@@ -28,6 +28,8 @@
 namespace nedo_gpu {
 namespace {
 
+constexpr float kDown = 1.f / 16384.f;  // 2^-kUp
+
 template <uint32_t HD>
 struct Many32 {
     static constexpr uint32_t kRows = HD <= 128u ? 128u : 64u;
@@ -282,7 +284,10 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         const bool slow = max(big[0], big[1]) >= 0x7F800000u || k_big > __uint_as_float(small[0]) * 65536.f ||
                           v_big > __uint_as_float(small[1]) * 65536.f;
         const int ek = up_exponent(k_big), ev = up_exponent(v_big);
-        const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek), v_down = power_of_two(-ev);
+        const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek);
+        // takes the tile's scale back, and the weights': the running sums hold weights of at most 1, or
+        // values near fp32's largest would leave it
+        const float v_down = power_of_two(-ev) * kDown;
 #pragma unroll
         for (uint32_t x = 0; x < kPieces; ++x) {
             const uint32_t r = piece_row + x * kAtOnce, piece = r * (HD / 4u) + piece_ch;
@@ -447,7 +452,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                         for (uint32_t h = 0; h < 2; ++h) {
                             const float w0 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h], from);
                             const float w1 = __shfl_sync(0xFFFFFFFFu, sc[n8][2 * h + 1], from);
-                            w[h] = jj & 1u ? w1 : w0;
+                            w[h] = (jj & 1u ? w1 : w0) * kDown;
                         }
                         if (!in_tile(key)) continue;
                         const bool see0 = key >= lo_key[0] && key < hi_key[0], see1 = key >= lo_key[1] && key < hi_key[1];
@@ -480,7 +485,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         const uint32_t r = warp * 16u + g + 8u * h;
         const int p = row_pos[r];
         if (p == -2) continue;
-        if (p < 0) l[h] = 0.f;  // padding sees nothing
+        l[h] = p < 0 ? 0.f : l[h] * kDown;  // padding sees nothing
         const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
         float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
         const bool none = l[h] == 0.f;
@@ -492,7 +497,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                 none ? make_float2(0.f, 0.f) : make_float2(acc[n][2 * h] / f, acc[n][2 * h + 1] / f);
         }
         if (!a.direct && (lane & 3u) == 0u)
-            a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2((m[h] == -INFINITY ? 0.f : m[h]) - kUp, l[h]);
+            a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(m[h] == -INFINITY ? 0.f : m[h], l[h]);
     }
 }
 

@@ -169,3 +169,16 @@ def test_select_from_two_host_threads(lib, cuda):
     assert not errors, errors[0]
     for o, w in zip(outs, want):
         assert np.array_equal(o.cpu().numpy().view(np.uint32), w)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("q", [1, 60])
+def test_largest_values(lib, cuda, hd, q):
+    """Weighted sums that fp32 holds do not leave it on the way."""
+    s = Setup(F32, 4, 2, hd, 16, q=[q, 1], kv=[120, 90], seed=47)
+    for seq in range(2):
+        for pos in range(s.kv[seq]):
+            page, slot = place(s, seq, pos)
+            s.v[page, :, slot] = np.clip(s.v[page, :, slot], -3, 3) * np.float32(5e35)
+    d = Device(lib, cuda, s)
+    check(d.attention(), *s.attention())
