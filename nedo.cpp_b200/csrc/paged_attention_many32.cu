@@ -3,15 +3,15 @@
 // cores.
 //
 // Mathematics.  Both factors of each product are fp32 here, so both are split in two fp16
-// halves (22 bits) and three of the four products are formed, the small ones first:
-// lo hi + hi lo + hi hi; what is left out is 2^-22 of the product.  Queries are scaled by a
-// power of two per row, keys and values by one per tile, to where the low halves are normal
-// numbers; the weights as in the other kernels.  A tile's weighted values are summed from zero
-// and added to the running sums in fp32, which also takes the tile's scale back.  Under the
-// tile's scale a number keeps 2^-38 of the tile's largest: less than its own 22 bits where it is
-// below 2^-16 of that.  A tile in which some key or value is that much smaller than another as
-// a whole (a row must not lose its digits to one that it may not even see) is done in fp32, key
-// by key; so is one with numbers that are not finite.
+// halves (22 bits), x = hi + 2^-11 lo, and three of the four products are formed: hi hi, and in
+// sums of their own lo hi + hi lo; what is left out is 2^-22 of the product.  Queries are scaled by a
+// power of two per row, keys and values by one per tile, weights by 2^14.  A tile's weighted values
+// are summed from zero and added to the running sums in fp32, which also takes the scales back.
+// With the low halves taken up by 2^11 a number keeps its 22 bits down to 2^-27 of the tile's
+// largest, and 2^-49 of that below.  A tile in which numbers are below 2^-27 together -- four
+// neighbouring channels of a key, or a channel of the keys that a thread looks at -- is done in fp32,
+// key by key: a row must not lose its digits to a key that it does not see, nor a channel to its
+// neighbours.  So is a tile with numbers that are not finite.
 //
 // Work.  A CTA of one warp for 16 rows (128 rows, 64 for heads above 128) takes its rows through
 // their keys in tiles of 64 (32).  The next tile's keys and values are on their way (cp.async)
@@ -19,7 +19,7 @@
 // magnitudes found, and its halves written next to it for ldmatrix, once for all warps.
 //
 // 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two sequences over 4096 and
-// 2550 keys, window 2048: 556 us, 234 TFLOP/s of MMAs (three for each product).  With two warps to
+// 2550 keys, window 2048: 563 us, 231 TFLOP/s of MMAs (three for each product).  With two warps to
 // a scheduler the tensor pipe is busy for half of the time; the rest is the halves' making and
 // the latency of what stands between the MMAs.
 #include "paged_attention.cuh"
@@ -29,6 +29,16 @@ namespace nedo_gpu {
 namespace {
 
 constexpr float kDown = 1.f / 16384.f;  // 2^-kUp
+constexpr float kLowUp = 2048.f, kLowDown = 1.f / 2048.f;
+constexpr float kRange = 134217728.f;   // 2^27: numbers of 2^14 and 2^-14 under one scale
+
+// x, y as two fp16 halves each, x = hi + 2^-11 lo.
+__device__ __forceinline__ void split_up(float2 x, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __float22half2_rn(x);
+    const float2 f = __half22float2(h), up = make_float2(kLowUp, kLowUp);
+    *hi = pack(h);
+    *lo = pack(__float22half2_rn(__fmul2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y)), up)));
+}
 
 template <uint32_t HD>
 struct Many32 {
@@ -46,13 +56,6 @@ struct Many32 {
 template <uint32_t HD>
 __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return r * Many32<HD>::kRowBytes + ((c ^ (r & 7u)) << 4);
-}
-
-// The largest magnitude of four numbers, as its bits (which order magnitudes; NaN last).
-__device__ __forceinline__ uint32_t size_bits(const float4& v) {
-    const uint32_t x = __float_as_uint(v.x) & 0x7FFFFFFFu, y = __float_as_uint(v.y) & 0x7FFFFFFFu;
-    const uint32_t z = __float_as_uint(v.z) & 0x7FFFFFFFu, w = __float_as_uint(v.w) & 0x7FFFFFFFu;
-    return max(max(x, y), max(z, w));
 }
 
 template <uint32_t HD>
@@ -213,7 +216,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
             for (uint32_t e = 0; e < 4; ++e) {
                 float2 x = make_float2(0.f, 0.f);
                 if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
-                split(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up, &hi[e], &lo[e]);
+                split_up(make_float2(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up), &hi[e], &lo[e]);
             }
             *reinterpret_cast<uint4*>(sm + at<HD>(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(sm + M::kQBytes + at<HD>(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -243,10 +246,10 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
         const uint32_t have = there, j = j0 + i * kKeys;
         cp_wait<0>();
         // the tile as halves: every thread its own pieces (the ones it copied), first their sizes
-        uint32_t big[2] = {0u, 0u}, small[2] = {0x7F800000u, 0x7F800000u};
-        constexpr uint32_t kLanes = HD / 4u < 32u ? HD / 4u : 32u;  // lanes that hold a key's (or half a key's) channels
+        // (twice their bits, without the sign; for the smallest less one, which leaves zero out): the
+        // largest of all, the smallest of the largest of four channels and of the thread's keys
+        uint32_t big[2] = {0u, 0u}, small[2] = {~0u, ~0u}, top[2][4] = {};
         constexpr bool kHold = HD <= 128u;  // in registers from the one pass to the other
-        const uint32_t lanes = kLanes == 32u ? 0xFFFFFFFFu : ((1u << (kLanes & 31u)) - 1u) << (lane & ~(kLanes - 1u));
         float4 held[kHold ? kPieces : 1u][2];
 #pragma unroll
         for (uint32_t x = 0; x < kPieces; ++x) {
@@ -255,17 +258,22 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
             for (uint32_t kv = 0; kv < 2u; ++kv) {
                 const float4 v = *reinterpret_cast<const float4*>(raw + kv * M::kRawBytes + piece * 16u);
                 if constexpr (kHold) held[x][kv] = v;
-                const uint32_t row = __reduce_max_sync(lanes, size_bits(v));
-                big[kv] = max(big[kv], row);
-                if (row != 0u) small[kv] = min(small[kv], row);
+                const uint32_t e[4] = {__float_as_uint(v.x) << 1, __float_as_uint(v.y) << 1, __float_as_uint(v.z) << 1,
+                                       __float_as_uint(v.w) << 1};
+                small[kv] = min(small[kv], max(max(e[0], e[1]), max(e[2], e[3])) - 1u);
+#pragma unroll
+                for (uint32_t u = 0; u < 4u; ++u) top[kv][u] = max(top[kv][u], e[u]);
             }
         }
 #pragma unroll
         for (uint32_t kv = 0; kv < 2u; ++kv) {
-            if constexpr (kLanes < 32u) {
-                big[kv] = max(big[kv], __shfl_xor_sync(0xFFFFFFFFu, big[kv], 16));
-                small[kv] = min(small[kv], __shfl_xor_sync(0xFFFFFFFFu, small[kv], 16));
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u) {
+                big[kv] = max(big[kv], top[kv][u]);
+                small[kv] = min(small[kv], top[kv][u] - 1u);
             }
+            big[kv] = __reduce_max_sync(0xFFFFFFFFu, big[kv]);
+            small[kv] = __reduce_min_sync(0xFFFFFFFFu, small[kv]);
             if (lane == 0u) {
                 size[kv][warp] = big[kv];
                 least[kv][warp] = small[kv];
@@ -280,9 +288,10 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                 small[kv] = min(small[kv], least[kv][w]);
             }
         }
-        const float k_big = __uint_as_float(big[0]), v_big = __uint_as_float(big[1]);
-        const bool slow = max(big[0], big[1]) >= 0x7F800000u || k_big > __uint_as_float(small[0]) * 65536.f ||
-                          v_big > __uint_as_float(small[1]) * 65536.f;
+        const float k_big = __uint_as_float(big[0] >> 1), v_big = __uint_as_float(big[1] >> 1);
+        auto least_of = [](uint32_t x) { return __uint_as_float((x + 1u) >> 1); };
+        const bool slow = max(big[0], big[1]) >= 0xFF000000u || (big[0] != 0u && k_big > least_of(small[0]) * kRange) ||
+                          (big[1] != 0u && v_big > least_of(small[1]) * kRange);
         const int ek = up_exponent(k_big), ev = up_exponent(v_big);
         const float k_up = power_of_two(ek), v_up = power_of_two(ev), k_down = power_of_two(-ek);
         // takes the tile's scale back, and the weights': the running sums hold weights of at most 1, or
@@ -299,8 +308,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                 const float up = kv ? v_up : k_up;
                 const float2 up2 = make_float2(up, up);
                 uint32_t hi[2], lo[2];
-                split(__fmul2_rn(make_float2(v.x, v.y), up2), &hi[0], &lo[0]);
-                split(__fmul2_rn(make_float2(v.z, v.w), up2), &hi[1], &lo[1]);
+                split_up(__fmul2_rn(make_float2(v.x, v.y), up2), &hi[0], &lo[0]);
+                split_up(__fmul2_rn(make_float2(v.z, v.w), up2), &hi[1], &lo[1]);
                 uint8_t* dst = halves + kv * 2u * M::kHalfBytes + at<HD>(r, piece_ch >> 1) + (piece_ch & 1u) * 8u;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(dst + M::kHalfBytes) = make_uint2(lo[0], lo[1]);
@@ -338,7 +347,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                         }
                 }
             } else {
-                float low[kCols][4];  // lo hi + hi lo: a part of its own, so that every half is loaded once
+                float low[kCols][4];  // lo hi + hi lo
 #pragma unroll
                 for (uint32_t n = 0; n < kCols; ++n) low[n][0] = low[n][1] = low[n][2] = low[n][3] = 0.f;
 #pragma unroll
@@ -364,7 +373,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
 #pragma unroll
                 for (uint32_t n = 0; n < kCols; ++n)
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; ++e) sc[n][e] += low[n][e];
+                    for (uint32_t e = 0; e < 4; ++e) sc[n][e] = fmaf(low[n][e], kLowDown, sc[n][e]);
             }
             const float k_one = slow ? 1.f : k_down;
             if (!whole) {
@@ -401,8 +410,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                     sc[n][e] = exp2_fast(fmaf(sc[n][e] * down[e >> 1], k_one, -ref[e >> 1]));
                     l[e >> 1] += sc[n][e];
                 }
-                split(sc[n][0], sc[n][1], &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
-                split(sc[n][2], sc[n][3], &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
+                split_up(make_float2(sc[n][0], sc[n][1]), &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
+                split_up(make_float2(sc[n][2], sc[n][3]), &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
             }
             if (!slow) {
 #pragma unroll
@@ -410,27 +419,55 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                     float o[2][4];
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
-                    uint32_t b[kGroups][4];
+                    const uint32_t v_at = v_addr + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1));  // 16 keys: 16 rows on
+                    if constexpr (HD <= 128u) {
+                        // hi hi on top of lo hi + hi lo: fewer registers (sums of their own took 575 us for the case above)
+                        uint32_t b[kGroups][4];
 #pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k)
-                        ldsm4t(b[k], v_addr + M::kHalfBytes + at<HD>(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+                        for (uint32_t k = 0; k < kGroups; ++k) ldsm4t(b[k], v_at + k * 16u * M::kRowBytes + M::kHalfBytes);
 #pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k) {
-                        mma(o[0], phi[k], b[k][0], b[k][1]);
-                        mma(o[1], phi[k], b[k][2], b[k][3]);
-                    }
+                        for (uint32_t k = 0; k < kGroups; ++k) {
+                            mma(o[0], phi[k], b[k][0], b[k][1]);
+                            mma(o[1], phi[k], b[k][2], b[k][3]);
+                        }
 #pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k)
-                        ldsm4t(b[k], v_addr + at<HD>(k * 16u + (mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
+                        for (uint32_t k = 0; k < kGroups; ++k) ldsm4t(b[k], v_at + k * 16u * M::kRowBytes);
 #pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k) {
-                        mma(o[0], plo[k], b[k][0], b[k][1]);
-                        mma(o[1], plo[k], b[k][2], b[k][3]);
-                    }
+                        for (uint32_t k = 0; k < kGroups; ++k) {
+                            mma(o[0], plo[k], b[k][0], b[k][1]);
+                            mma(o[1], plo[k], b[k][2], b[k][3]);
+                        }
 #pragma unroll
-                    for (uint32_t k = 0; k < kGroups; ++k) {
-                        mma(o[0], phi[k], b[k][0], b[k][1]);
-                        mma(o[1], phi[k], b[k][2], b[k][3]);
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            o[0][e] *= kLowDown;
+                            o[1][e] *= kLowDown;
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < kGroups; ++k) {
+                            mma(o[0], phi[k], b[k][0], b[k][1]);
+                            mma(o[1], phi[k], b[k][2], b[k][3]);
+                        }
+                    } else {
+                        float low[2][4];  // (392 us for a prompt of 1429 tokens; as above 413)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) low[0][e] = low[1][e] = 0.f;
+#pragma unroll
+                        for (uint32_t k = 0; k < kGroups; ++k) {
+                            uint32_t bhi[4], blo[4];
+                            ldsm4t(bhi, v_at + k * 16u * M::kRowBytes);
+                            ldsm4t(blo, v_at + k * 16u * M::kRowBytes + M::kHalfBytes);
+                            mma(low[0], plo[k], bhi[0], bhi[1]);
+                            mma(low[1], plo[k], bhi[2], bhi[3]);
+                            mma(o[0], phi[k], bhi[0], bhi[1]);
+                            mma(o[1], phi[k], bhi[2], bhi[3]);
+                            mma(low[0], phi[k], blo[0], blo[1]);
+                            mma(low[1], phi[k], blo[2], blo[3]);
+                        }
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) {
+                            o[0][e] = fmaf(low[0][e], kLowDown, o[0][e]);
+                            o[1][e] = fmaf(low[1][e], kLowDown, o[1][e]);
+                        }
                     }
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) {

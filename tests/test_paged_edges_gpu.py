@@ -182,3 +182,27 @@ def test_largest_values(lib, cuda, hd, q):
             s.v[page, :, slot] = np.clip(s.v[page, :, slot], -3, 3) * np.float32(5e35)
     d = Device(lib, cuda, s)
     check(d.attention(), *s.attention())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 200])
+@pytest.mark.parametrize("size", [1e-4, 1e-7, 1e-10, 1e-13, 1e-25])
+def test_value_channels_of_different_size(lib, cuda, hd, size):
+    """Channels far smaller than their neighbours keep their digits (F32 caches, tiles of many rows)."""
+    s = Setup(F32, 4, 2, hd, 32, q=[70, 1, 90], kv=[500, 90, 91], shared=1, seed=45)
+    s.v[..., 3] *= np.float32(size)
+    s.v[..., 17::8] *= np.float32(size)
+    d = Device(lib, cuda, s)
+    check(d.attention(), *s.attention())
+    check(d.attention(60), *s.attention(60))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 200])
+@pytest.mark.parametrize("size", [1e4, 1e7, 1e10, 1e13, 1e25])
+def test_key_channels_of_different_size(lib, cuda, hd, size):
+    """A key channel far larger than its neighbours, of queries that are zero there, takes no digits
+    from the others."""
+    s = Setup(F32, 4, 2, hd, 32, q=[70, 1, 90], kv=[500, 90, 91], shared=1, seed=46)
+    s.k[..., 5] *= np.float32(size)
+    s.queries[..., 5] = 0
+    d = Device(lib, cuda, s)
+    check(d.attention(), *s.attention())
