@@ -263,7 +263,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");  // the combining kernel may come up
     // the warps' sums, in warp order
-    uint32_t again[kMine];  // four bits to a row whose sums are not finite
+    uint32_t again = 0;  // rows whose sums are not finite
 #pragma unroll
     for (uint32_t h = 0; h < kMine; ++h) {
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
@@ -278,8 +278,9 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
 #pragma unroll
             for (uint32_t e = 0; e < 4u; ++e)
                 if (kMine == 1u || e >> 1 == h) odd = fmaf(acc[n][e], 0.f, odd);
-        again[h] = __ballot_sync(0xFFFFFFFFu, odd != 0.f && row_pos[g + 8u * h] >= 0);
+        if (odd != 0.f && row_pos[g + 8u * h] >= 0) again |= 1u << (g + 8u * h);
     }
+    again = __reduce_or_sync(0xFFFFFFFFu, again);
     __syncthreads();
     float* part = reinterpret_cast<float*>(ring);  // [warp][row][HD + 4]
     constexpr uint32_t kPitch = HD + 4u;
@@ -293,19 +294,20 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             *reinterpret_cast<float2*>(to + 8u * kPitch) = make_float2(acc[n][2], acc[n][3]);
         }
     }
-#pragma unroll
-    for (uint32_t h = 0; h < kMine; ++h) {
-        if (again[h] == 0u) continue;
+    if (again != 0u) {
         __syncwarp();
-        for (uint32_t r = 8u * h; r < 8u * h + 8u; ++r) {
-            if ((again[h] >> (4u * (r & 7u)) & 15u) == 0u) continue;
+        while (again != 0u) {
+            uint32_t n, rows = take_rows(&again, &n);
             RowSums x;
-            row_key_by_key(a, s, kh, a.part == kPartBlocks ? list : nullptr, row_tok[r], row_head[r], row_pos[r],
-                           j0 + kKeys * warp, ke, kKeys * kWarps, &x);
-            for (uint32_t i = 0; lane + 32u * i < hd; ++i) part[(warp * ROWS + r) * kPitch + lane + 32u * i] = x.o[i];
-            if (lane == 0u) {
-                wm[warp][r] = x.m;
-                wl[warp][r] = x.l;
+            rows_key_by_key(a, s, kh, a.part == kPartBlocks ? list : nullptr, {row_tok, row_head, row_pos}, 0u, rows,
+                            j0 + kKeys * warp, ke, kKeys * kWarps, &x);
+            for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
+                const uint32_t r = rows & 255u;
+                for (uint32_t i = 0; lane + 32u * i < hd; ++i) part[(warp * ROWS + r) * kPitch + lane + 32u * i] = x.o[u][i];
+                if (lane == 0u) {
+                    wm[warp][r] = x.m[u];
+                    wl[warp][r] = x.l[u];
+                }
             }
         }
     }

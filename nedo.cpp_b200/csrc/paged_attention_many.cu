@@ -331,7 +331,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");
     const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
-    uint32_t again[2];  // four bits to a row whose sums are not finite
+    uint32_t again = 0;  // rows of the warp whose sums are not finite
 #pragma unroll
     for (uint32_t h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], 1);
@@ -341,8 +341,9 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         float odd = l[h] * 0.f;
 #pragma unroll
         for (uint32_t n = 0; n < HD / 8; ++n) odd = fmaf(acc[n][2 * h], 0.f, fmaf(acc[n][2 * h + 1], 0.f, odd));
-        again[h] = __ballot_sync(0xFFFFFFFFu, odd != 0.f && p >= 0);
-        if (p == -2 || (again[h] >> (lane & ~3u) & 15u)) continue;
+        const bool redo = __ballot_sync(0xFFFFFFFFu, odd != 0.f && p >= 0) >> (lane & ~3u) & 15u;
+        if (redo) again |= 1u << (g + 8u * h);
+        if (p == -2 || redo) continue;
         if (p < 0) l[h] = 0.f;  // padding sees nothing
         const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
         float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
@@ -357,19 +358,18 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         if (!a.direct && (lane & 3u) == 0u)
             a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2((m[h] == -INFINITY ? 0.f : m[h]) - kUp, l[h]);
     }
-#pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {
-        if (again[h] == 0u) continue;
-        for (uint32_t u = 0; u < 8u; ++u) {
-            if ((again[h] >> (4u * u) & 15u) == 0u) continue;
-            const uint32_t r = warp * 16u + 8u * h + u;
-            RowSums x;
-            row_key_by_key(a, s, kh, nullptr, row_tok[r], row_head[r], row_pos[r], kb, ke, 16u, &x);
+    again = __reduce_or_sync(0xFFFFFFFFu, again);
+    while (again != 0u) {
+        uint32_t n, rows = take_rows(&again, &n);
+        RowSums x;
+        rows_key_by_key(a, s, kh, nullptr, {row_tok, row_head, row_pos}, warp * 16u, rows, kb, ke, 16u, &x);
+        for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
+            const uint32_t r = warp * 16u + (rows & 255u);
             const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
             float* o = a.direct ? a.out + row * hd : a.part_o + ((a.slot0 + c) * rows_all + row) * hd;
-            const float f = !a.direct ? 1.f : x.l == 0.f ? 0.f : 1.f / x.l;
-            for (uint32_t i = 0; lane + 32u * i < hd; ++i) o[lane + 32u * i] = x.o[i] * f;
-            if (!a.direct && lane == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(x.m, x.l);
+            const float f = !a.direct ? 1.f : x.l[u] == 0.f ? 0.f : 1.f / x.l[u];
+            for (uint32_t i = 0; lane + 32u * i < hd; ++i) o[lane + 32u * i] = x.o[u][i] * f;
+            if (!a.direct && lane == 0u) a.part_ml[(a.slot0 + c) * rows_all + row] = make_float2(x.m[u], x.l[u]);
         }
     }
 }

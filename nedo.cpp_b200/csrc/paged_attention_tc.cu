@@ -625,15 +625,21 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                     make_float2(ref - kUp, sum);
             named_barrier_sync(5, kSums);
             if ((again[0] | again[1] | again[2] | again[3]) != 0u) {  // rows whose sums are not finite
-                for (uint32_t rr = warp - kSumWarp; rr < kRows; rr += kSums / 32u) {
-                    if (!(again[rr >> 5] >> (rr & 31u) & 1u) || !ok) continue;
+                // 16 rows to a warp
+                const uint32_t first = (warp - kSumWarp) * 16u;
+                uint32_t set = ok ? again[first >> 5] >> (first & 31u) & 0xFFFFu : 0u;
+                while (set != 0u) {
+                    uint32_t n, rows = take_rows(&set, &n);
                     RowSums x;
-                    row_key_by_key(a, s, kh, nullptr, row_tok[rr], row_head[rr], row_pos[rr], kb, ke, 16u, &x);
-                    const float f = !a.direct ? 1.f : x.l == 0.f ? 0.f : 1.f / x.l;
-                    for (uint32_t i = 0; lane + 32u * i < hd; ++i) sums[rr * kPitch + lane + 32u * i] = x.o[i] * f;
-                    if (!a.direct && lane == 0u)
-                        a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr]] =
-                            make_float2(x.m, x.l);
+                    rows_key_by_key(a, s, kh, nullptr, {row_tok, row_head, row_pos}, first, rows, kb, ke, 16u, &x);
+                    for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
+                        const uint32_t rr = first + (rows & 255u);
+                        const float f = !a.direct ? 1.f : x.l[u] == 0.f ? 0.f : 1.f / x.l[u];
+                        for (uint32_t i = 0; lane + 32u * i < hd; ++i) sums[rr * kPitch + lane + 32u * i] = x.o[u][i] * f;
+                        if (!a.direct && lane == 0u)
+                            a.part_ml[(a.slot0 + c) * rows_all + static_cast<size_t>(row_tok[rr]) * a.heads + row_head[rr]] =
+                                make_float2(x.m[u], x.l[u]);
+                    }
                 }
                 named_barrier_sync(5, kSums);
             }
