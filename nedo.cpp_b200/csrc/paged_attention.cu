@@ -277,7 +277,7 @@ bool plan_paged_attention(PagedAttention* a) {
     a->own_chunks = chunks(a->own_chunk);
     a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
-    if (!takes_few(own) && a->b.seqs > 1u) {
+    if (!takes_few(own) && a->b.seqs > 1u && group <= kFewMax) {  // (a larger group has more rows with every token)
         const Cost few = cost_of(few_kernel(*a), a->kv);
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / few.rows);
         a->few_chunk = chunk_keys(keys, u, sums, a->kv, few, alone);
