@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kFew16, kFew32, kMany, kMany32, kTc };
+enum class Kernel { kFew, kFew16, kFew32, kMany, kMany64, kMany32, kTc };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -157,8 +157,12 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {k == Kernel::kFew ? kFewRows : 2u * kFewRows, slots, 2048u, 4.0 * hd * slots / 6500.0, 4000.0, 0.45};
         }
-        case Kernel::kMany:  // 128 rows of a head above 128 through the tensor cores, an item to an SM
-            return {kManyRows, 148u, 0u, 34.0, 5000.0, 1.0};
+        // 128 or 64 rows of a head above 128 through the tensor cores, an item to an SM (148 items of 128
+        // rows: 79, 134, 242 and 463 us over 500, 1000, 2000 and 4000 keys; of 64: 51, 90, 163 and 310)
+        case Kernel::kMany:
+            return {128u, 148u, 0u, 110.0, 24000.0, 1.0};
+        case Kernel::kMany64:
+            return {64u, 148u, 0u, 74.0, 14000.0, 1.0};
         case Kernel::kTc:  // 128 rows through 32 MMAs per 128 keys, an item to an SM; 24,000 cycles around its tiles
             return {kTcRows, 148u, 0u, hd <= 64u ? 8.0 : 12.0, 12000.0, 1.0};
         case Kernel::kFew32: {
@@ -175,9 +179,17 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
 // item and the bytes of the chunks' sums counted.
 // `cluster`: up to kMaxCluster chunks of a row tile can be added within a cluster, without the
 // combining kernel.
-uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c, bool cluster) {
+// `causal`: share of its keys by which a sequence's first rows see fewer than its last.  Where
+// items are of equal length (0) they run in whole rounds; where they are not, the long ones come
+// first and the short ones even them out.
+struct Chunks {
+    uint32_t keys;
+    double ns;  // estimated time
+};
+Chunks chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c, bool cluster,
+                  double causal = 0.0) {
     const uint64_t step = std::max(64u, kv.page_size);
-    if (keys <= step) return static_cast<uint32_t>(step);
+    keys = std::max<uint64_t>(keys, 1u);
     auto rounded = [&](uint64_t n) { return ((keys + n - 1u) / n + step - 1u) / step * step; };
     uint64_t best = 0;
     double best_ns = 0.0;
@@ -189,7 +201,9 @@ uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const Pag
         // a chunk's sums are written once and read once at about half the copy rate
         // few items do not share the memory's rate, but one alone has only its own copies in flight
         const double busy = std::min(1.0, static_cast<double>(units * n) / c.slots);
-        const double ns = rounds * (static_cast<double>(chunk) * c.ns_per_key * std::max(busy, c.least) + c.ns_fixed) +
+        const double item = static_cast<double>(chunk) * c.ns_per_key * std::max(busy, c.least) + c.ns_fixed;
+        const double all = units * (static_cast<double>(keys) * (1.0 - 0.5 * causal) * c.ns_per_key + n * c.ns_fixed);
+        const double ns = (1.0 - causal) * rounds * item + causal * std::max(item, all / c.slots) +
                           (n == 1u                          ? 0.0
                            : cluster && n <= kMaxCluster ? 1000.0
                                                          : 4000.0 + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0);
@@ -203,7 +217,7 @@ uint32_t chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const Pag
         const uint64_t n = rounds * c.slots / units;
         if (n > 1u) consider(std::min<uint64_t>(n, (keys + step - 1u) / step));
     }
-    return static_cast<uint32_t>(best);
+    return {static_cast<uint32_t>(best), best_ns};
 }
 
 uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1u) / b; }
@@ -221,12 +235,13 @@ Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
     if (rows <= kFewMax) return Kernel::kFew16;
     return kv.head_dim <= 128u ? Kernel::kTc : Kernel::kMany;
 }
+Kernel low_or_not(Kernel k, bool low) { return k == Kernel::kMany && low ? Kernel::kMany64 : k; }
 Kernel prefix_kernel(const PagedAttention& a) {
-    return kernel_for(a.kv, static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads));
+    return low_or_not(kernel_for(a.kv, static_cast<uint64_t>(a.b.tokens) * (a.heads / a.kv.kv_heads)), a.prefix_low);
 }
 Kernel own_kernel(const PagedAttention& a) {
     const uint32_t group = a.heads / a.kv.kv_heads;
-    return kernel_for(a.kv, a.picks ? std::min(group, kFewMax) : static_cast<uint64_t>(a.b.max_q_len) * group);
+    return low_or_not(kernel_for(a.kv, a.picks ? std::min(group, kFewMax) : static_cast<uint64_t>(a.b.max_q_len) * group), a.own_low);
 }
 // The kernel of the sequences with few rows among others with many: mostly single tokens.
 Kernel few_kernel(const PagedAttention& a) { return kernel_for(a.kv, std::min(a.heads / a.kv.kv_heads, kFewMax)); }
@@ -239,7 +254,8 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
         case Kernel::kFew: return launch_attention_few(a, kFewRows, items, stream);
         case Kernel::kFew16: return launch_attention_few(a, 2u * kFewRows, items, stream);
         case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
-        case Kernel::kMany: return launch_attention_many(a, tiles, stream);
+        case Kernel::kMany: return launch_attention_many(a, 128u, tiles, stream);
+        case Kernel::kMany64: return launch_attention_many(a, 64u, tiles, stream);
         case Kernel::kTc: return launch_attention_tc(a, tiles, stream);
         default: return launch_attention_many32(a, tiles, stream);
     }
@@ -248,15 +264,29 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
 }  // namespace
 
 bool plan_paged_attention(PagedAttention* a) {
+    // a part's plan with tiles of 64 rows or not, whichever should take less time
+    const bool choice = a->kv.type == kF16 && a->kv.head_dim > 128u;
+    auto faster = [choice](bool* low, auto plan) {
+        Chunks best = plan();
+        if (!choice) return best;
+        *low = true;
+        const Chunks at64 = plan();
+        if (at64.ns < best.ns) return at64;
+        *low = false;
+        return plan();
+    };
     const uint64_t rows = static_cast<uint64_t>(a->b.tokens) * a->heads;
     const uint64_t group = a->heads / a->kv.kv_heads, all = a->b.tokens * group;
     const uint64_t sums = rows * (a->kv.head_dim * sizeof(float) + sizeof(float2));  // bytes of one chunk of every row
     const uint64_t shared = a->picks ? 0u : static_cast<uint64_t>(a->shared_pages) << a->kv.page_shift;
     uint64_t units = 0, prefix_units = 0;
     if (shared != 0u) {
-        const Cost c = cost_of(prefix_kernel(*a), a->kv);
-        prefix_units = ceil_div(all, c.rows) * a->kv.kv_heads;
-        a->prefix_chunk = chunk_keys(shared, prefix_units, sums, a->kv, c, false);
+        const Chunks best = faster(&a->prefix_low, [&] {
+            const Cost c = cost_of(prefix_kernel(*a), a->kv);
+            prefix_units = ceil_div(all, c.rows) * a->kv.kv_heads;
+            return chunk_keys(shared, prefix_units, sums, a->kv, c, false);
+        });
+        a->prefix_chunk = best.keys;
         a->prefix_chunks = static_cast<uint32_t>(ceil_div(shared, a->prefix_chunk));
     }
     const uint64_t most = a->picks ? static_cast<uint64_t>(a->picks) << a->kv.page_shift
@@ -266,21 +296,26 @@ bool plan_paged_attention(PagedAttention* a) {
     if (!a->picks && a->window != 0u)
         keys = std::min<uint64_t>(keys, static_cast<uint64_t>(a->window) + a->b.max_q_len - 1u + 63u);
     auto chunks = [&](uint64_t chunk) { return static_cast<uint32_t>(std::max<uint64_t>(ceil_div(keys, chunk), 1u)); };
-    const Kernel own = own_kernel(*a);
-    const Cost c = cost_of(own, a->kv);
-    units = (a->picks          ? a->b.tokens * ceil_div(group, c.rows)
-             : takes_few(own) ? a->b.seqs * ceil_div(a->b.max_q_len * group, c.rows)
-                              : own_tiles(*a, c.rows)) *
-            a->kv.kv_heads;
     const bool alone = shared == 0u;
-    a->own_chunk = chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(own));
+    const double causal = a->picks || a->window != 0u ? 0.0 : std::min(1.0, static_cast<double>(a->b.max_q_len) / std::max<uint64_t>(keys, 1u));
+    const Chunks best = faster(&a->own_low, [&] {
+        const Kernel k = own_kernel(*a);
+        const Cost c = cost_of(k, a->kv);
+        units = (a->picks        ? a->b.tokens * ceil_div(group, c.rows)
+                 : takes_few(k) ? a->b.seqs * ceil_div(a->b.max_q_len * group, c.rows)
+                                : own_tiles(*a, c.rows)) *
+                a->kv.kv_heads;
+        return chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(k), choice ? causal : 0.0);
+    });
+    const Kernel own = own_kernel(*a);
+    a->own_chunk = best.keys;
     a->own_chunks = chunks(a->own_chunk);
     a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
     if (!takes_few(own) && a->b.seqs > 1u && group <= kFewMax) {  // (a larger group has more rows with every token)
         const Cost few = cost_of(few_kernel(*a), a->kv);
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / few.rows);
-        a->few_chunk = chunk_keys(keys, u, sums, a->kv, few, alone);
+        a->few_chunk = chunk_keys(keys, u, sums, a->kv, few, alone).keys;
         a->few_chunks = chunks(a->few_chunk);
         a->few_cluster = alone && a->few_chunks > 1u && a->few_chunks <= kMaxCluster;
         grid = std::max(grid, u * a->few_chunks);

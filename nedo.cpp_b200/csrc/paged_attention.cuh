@@ -499,10 +499,9 @@ cudaError_t launch_items(const AttnArgs& a, void (*kernel)(Args...), uint64_t it
 // 8 (paged_attention_few32.cu).
 cudaError_t launch_attention_few(const AttnArgs& a, uint32_t rows, uint64_t items, cudaStream_t stream);
 cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_t items, cudaStream_t stream);
-// Tiles of kManyRows rows on the tensor cores (paged_attention_many.cu): F16 caches, heads
+// Tiles of `rows` 64 or 128 rows on the tensor cores (paged_attention_many.cu): F16 caches, heads
 // above 128.
-constexpr uint32_t kManyRows = 128;
-cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream);
+cudaError_t launch_attention_many(const AttnArgs& a, uint32_t rows, uint64_t tiles, cudaStream_t stream);
 // Tiles of many32_rows(head_dim) rows of F32 caches on the tensor cores
 // (paged_attention_many32.cu).
 uint32_t many32_rows(uint32_t head_dim);

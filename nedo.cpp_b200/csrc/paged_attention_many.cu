@@ -1,4 +1,4 @@
-// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 128 query rows of
+// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 128 or 64 query rows of
 // heads above 128 channels (prompts, and the tokens of a whole batch over their shared
 // prefix): bound by the tensor cores.  (Up to 128 channels a tile's sums fit into the other
 // kernel's half of TMEM.)
@@ -9,40 +9,45 @@
 // tile's weighted values are therefore summed from zero in 4 steps and added to the
 // running sums in fp32 with the rescaling by 2^(m_old - m_new)).
 //
-// Work.  A CTA of eight warps, 16 rows each, takes the 128 rows through its keys in tiles of
-// 32; the tiles of keys and values are shared by the warps, brought in by cp.async two
+// Work.  A CTA of a warp for 16 rows takes its rows through its keys in tiles of 32; the tiles of keys and values are shared by the warps, brought in by cp.async two
 // tiles deep.  Tiles that none of a warp's rows sees are skipped by it, and only tiles
 // seen in part are masked.
 //
 // 12 query and 4 KV heads of 256 channels, 2048 and 1840 new tokens of two sequences over 4096 and
-// 2550 keys: 814 us, 280 TFLOP/s of MMAs (two for each product); a CTA of four warps for 64 rows
-// took 1084.  8 query and 2 KV heads, 900 and 529 tokens over 1600 and 1147 keys: 202 us, where 64
-// rows took 169, because 90 items leave SMs without one.
+// 2550 keys: 847 us, 270 TFLOP/s of MMAs (two for each product), in tiles of 128 rows; 64 rows, which
+// read the keys twice as often, take 1072.  Where there are few tiles 64 rows reach more SMs: 8 query
+// and 2 KV heads, 300 tokens 26 us (128 rows: 30), 37 sequences of 32 tokens over 500 keys 51 us (68).
+// The plan takes the height that it expects to end first.
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
 namespace nedo_gpu {
 namespace {
 
-constexpr uint32_t kWarps = kManyRows / 16u;
-constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kStages = 2;
 constexpr uint32_t HD = 256;                             // channels of a row in shared memory
 constexpr uint32_t kKeys = 32;                           // keys per tile
 constexpr uint32_t kGroups = kKeys / 16u, kCols = kKeys / 8u;
 constexpr uint32_t kRowBytes = HD * 2u;
-constexpr uint32_t kQBytes = kManyRows * kRowBytes;      // one half of the queries
 constexpr uint32_t kTileBytes = kKeys * kRowBytes;       // keys or values of a tile
 constexpr uint32_t kStageBytes = 2u * kTileBytes;
-constexpr uint32_t kSmem = 2u * kQBytes + kStages * kStageBytes;
+
+template <uint32_t ROWS>
+struct Many {
+    static constexpr uint32_t kThreads = 2u * ROWS;          // a warp for 16 rows
+    static constexpr uint32_t kQBytes = ROWS * kRowBytes;    // one half of the queries
+    static constexpr uint32_t kSmem = 2u * kQBytes + kStages * kStageBytes;
+};
 
 __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) { return r * kRowBytes + ((c ^ (r & 7u)) << 4); }
 
+template <uint32_t ROWS>
 __device__ __forceinline__ void attention_many(const AttnArgs& a) {
+    constexpr uint32_t kThreads = Many<ROWS>::kThreads, kQBytes = Many<ROWS>::kQBytes, kSmem = Many<ROWS>::kSmem;
     extern __shared__ __align__(128) uint8_t sm[];
-    __shared__ uint32_t row_tok[kManyRows], row_head[kManyRows];
-    __shared__ int row_pos[kManyRows];
-    __shared__ float row_unscale[kManyRows];
+    __shared__ uint32_t row_tok[ROWS], row_head[ROWS];
+    __shared__ int row_pos[ROWS];
+    __shared__ float row_unscale[ROWS];
     __shared__ uint32_t found[2];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     const uint32_t kh = blockIdx.x % a.kv.kv_heads;
@@ -54,12 +59,12 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     uint32_t s = 0, r0 = 0, nrows, t0 = 0;
     PagedSeq sq{0u, 0u, 0u};
     if (a.part == kPartPrefix) {
-        r0 = rest * kManyRows;
-        nrows = min(kManyRows, a.b.tokens * a.group - r0);
+        r0 = rest * ROWS;
+        nrows = min(ROWS, a.b.tokens * a.group - r0);
     } else {
         if (warp == 0) {
             uint32_t tile;
-            const uint32_t seq = find_tile(a, rest, kManyRows, &tile);
+            const uint32_t seq = find_tile(a, rest, ROWS, &tile);
             if (lane == 0u) {
                 found[0] = seq;
                 found[1] = tile;
@@ -70,10 +75,10 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         if (s == kNone) return;
         sq = load_seq(a.b, s, a.st);
         t0 = sq.t0;
-        r0 = found[1] * kManyRows;
-        nrows = min(kManyRows, sq.n * a.group - r0);
+        r0 = found[1] * ROWS;
+        nrows = min(ROWS, sq.n * a.group - r0);
     }
-    if (tid < kManyRows) {
+    if (tid < ROWS) {
         int p = -2;
         uint32_t tok = 0, head = 0;
         if (tid < nrows) {
@@ -91,7 +96,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     {
         uint32_t lo = kNone, hi = 0;
 #pragma unroll
-        for (uint32_t u = 0; u < kManyRows / 32u; ++u) {
+        for (uint32_t u = 0; u < ROWS / 32u; ++u) {
             const int p = row_pos[lane + 32u * u];
             if (p >= 0) {
                 lo = min(lo, first_key(p, a.window));
@@ -374,15 +379,22 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     }
 }
 
-__global__ void __launch_bounds__(kThreads, 1) attention_many_kernel(const __grid_constant__ AttnArgs a) {
-    attention_many(a);
+template <uint32_t ROWS>
+__global__ void __launch_bounds__(Many<ROWS>::kThreads, 1) attention_many_kernel(const __grid_constant__ AttnArgs a) {
+    attention_many<ROWS>(a);
     end_after_previous(a);
+}
+
+template <uint32_t ROWS>
+cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
+    return launch_items(a, attention_many_kernel<ROWS>, items, Many<ROWS>::kThreads, Many<ROWS>::kSmem, stream, a);
 }
 
 }  // namespace
 
-cudaError_t launch_attention_many(const AttnArgs& a, uint64_t tiles, cudaStream_t stream) {
-    return launch_items(a, attention_many_kernel, tiles * a.kv.kv_heads * a.chunks, kThreads, kSmem, stream, a);
+cudaError_t launch_attention_many(const AttnArgs& a, uint32_t rows, uint64_t tiles, cudaStream_t stream) {
+    const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
+    return rows <= 64u ? launch<64>(a, items, stream) : launch<128>(a, items, stream);
 }
 
 }  // namespace nedo_gpu

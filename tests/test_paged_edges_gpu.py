@@ -206,3 +206,20 @@ def test_key_channels_of_different_size(lib, cuda, hd, size):
     s.queries[..., 5] = 0
     d = Device(lib, cuda, s)
     check(d.attention(), *s.attention())
+
+
+@pytest.mark.parametrize("hd,page", [(256, 32), (136, 64)])
+@pytest.mark.parametrize("seqs,q,kv", [(74, 32, 100), (37, 32, 130), (3, 50, 700)])
+def test_wide_heads_in_tiles_of_either_height(lib, cuda, hd, page, seqs, q, kv):
+    """Heads above 128: batches that the plan takes in tiles of 128 rows (the first) and of 64, whole
+    and cut by a window, with a padded row and an infinite value in one of them."""
+    r = np.random.default_rng(seqs)
+    lens = [int(kv - x) for x in r.integers(0, 30, seqs)]
+    s = Setup(F16, 8, 2, hd, page, q=[q] * (seqs - 1) + [q - 3], kv=lens[:-1] + [5], tail=2, seed=49)
+    page_id, slot = place(s, 1, lens[1] - 20)
+    s.v[page_id, 0, slot, 9] = np.inf
+    d = Device(lib, cuda, s)
+    check(d.attention(), *s.attention())
+    d.out.fill_(777.0)
+    check(d.attention(40), *s.attention(40))
+    lib.status()
