@@ -371,7 +371,7 @@ NEDO_GPU_API void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d);
  * time on several streams (each call with a workspace of its own; captured graphs
  * that may overlap too).  The library's first call on a device allocates its state
  * there: make it outside a capture.  Buffers are 16-byte aligned memory of the
- * current device.  Results repeat bit for bit.
+ * current device (lists of uint32: 4-byte).  Results repeat bit for bit.
  *
  * Token row t of sequence s (q_start[s] <= t < q_start[s+1]) stands at position
  * kv_len[s] - (q_start[s+1] - t).  A row whose position is negative -- its

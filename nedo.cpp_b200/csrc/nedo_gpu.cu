@@ -1650,6 +1650,8 @@ void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d) {
 // ---- paged KV cache: append, attention, page selection ----------------------
 namespace {
 
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
 // Checks the two descriptors (everything the host can see) and fills the kernels'
 // views.  Lengths and page ids live in device memory: the kernels check those.
 int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_batch* b, uint32_t heads, PagedKv* kv,
@@ -1677,6 +1679,8 @@ int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_
         return fail(NEDO_GPU_ERR_ARG, w + "shared_pages exceeds max_pages");
     if (b->seqs && b->tokens && (!b->q_start || !b->kv_len || (b->max_pages && !b->page_table)))
         return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
+    if (!aligned4(b->q_start) || !aligned4(b->kv_len) || !aligned4(b->page_table))
+        return fail(NEDO_GPU_ERR_ARG, w + "lists must be 4-byte aligned");
     if (b->seqs && b->tokens && !b->max_q_len) return fail(NEDO_GPU_ERR_ARG, w + "max_q_len must be positive");
     uint32_t shift = 0;
     while ((1u << shift) < c->page_size) ++shift;
@@ -1798,6 +1802,7 @@ int nedo_gpu_block_select_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_
     if (!b.seqs || !b.tokens) return 0;
     if (!q_dev || !blocks_dev) return fail(NEDO_GPU_ERR_ARG, "block_select: null pointer");
     if (!aligned16(q_dev)) return fail(NEDO_GPU_ERR_ARG, "block_select: q must be 16-byte aligned");
+    if (!aligned4(blocks_dev)) return fail(NEDO_GPU_ERR_ARG, "block_select: lists must be 4-byte aligned");
     if (static_cast<uint64_t>(b.tokens) * kv.kv_heads > 0x0FFFFFFFull)
         return fail(NEDO_GPU_ERR_ARG, "block_select: batch too large");
     DeviceState* s = nullptr;
@@ -1825,6 +1830,7 @@ int nedo_gpu_block_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_
     PagedAttention a;
     if (int rc = plan_attention("block_attention", cache, batch, heads, 0, blocks_dev, picks, &a)) return rc;
     if (a.b.seqs && a.b.tokens && !blocks_dev) return fail(NEDO_GPU_ERR_ARG, "block_attention: null pointer");
+    if (!aligned4(blocks_dev)) return fail(NEDO_GPU_ERR_ARG, "block_attention: lists must be 4-byte aligned");
     return run_attention("block_attention", a, q_dev, out_dev, scale, workspace_dev, workspace_bytes, stream);
 }
 
