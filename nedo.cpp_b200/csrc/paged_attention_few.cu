@@ -10,8 +10,8 @@
 // two halves ride in one m16n8k16 operand, rows 0-7 the high and rows 8-15 the low half
 // of the same eight query rows, so the split costs no extra instruction: both parts of a
 // row's sum land in the same thread, which adds them.  With more than eight rows the halves
-// are operands of their own, and every tile's weighted values are summed from zero and added
-// in fp32.
+// are operands of their own.  Every tile's weighted values are summed from zero and added in
+// fp32: the tensor core cuts its sums instead of rounding them, by up to a step every time.
 //
 // Work.  A CTA of four warps takes one row tile and one chunk of keys; each warp streams
 // every fourth 16-key tile through a ring of its own (cp.async, three stages), with its
@@ -239,23 +239,19 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
         for (uint32_t n = 0; n < HD / 16; ++n) {
             uint32_t b[4];
             ldsm4t(b, vs + at<HD>((mi & 1u) * 8u + mr, 2u * n + (mi >> 1)));
-            if constexpr (kMine == 1u) {
-                mma(acc[2 * n], pf[0], b[0], b[1]);
-                mma(acc[2 * n + 1], pf[0], b[2], b[3]);
-            } else {
-                // from zero, and added in fp32: the tensor core would cut the running sums twice a tile
-                float o[2][4];
+            float o[2][4];
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+            for (uint32_t e = 0; e < 4; ++e) o[0][e] = o[1][e] = 0.f;
+            if constexpr (kMine == 2u) {
                 mma(o[0], pf[kMine - 1u], b[0], b[1]);
                 mma(o[1], pf[kMine - 1u], b[2], b[3]);
-                mma(o[0], pf[0], b[0], b[1]);
-                mma(o[1], pf[0], b[2], b[3]);
+            }
+            mma(o[0], pf[0], b[0], b[1]);
+            mma(o[1], pf[0], b[2], b[3]);
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) {
-                    acc[2 * n][e] += o[0][e];
-                    acc[2 * n + 1][e] += o[1][e];
-                }
+            for (uint32_t e = 0; e < 4; ++e) {
+                acc[2 * n][e] += o[0][e];
+                acc[2 * n + 1][e] += o[1][e];
             }
         }
         __syncwarp();

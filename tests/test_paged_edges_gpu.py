@@ -5,7 +5,7 @@ import threading
 import numpy as np
 import pytest
 
-from paged_ref import F16, F32, Device, Setup
+from paged_ref import F16, F32, U, Device, Setup
 
 pytestmark = pytest.mark.gpu
 
@@ -223,3 +223,17 @@ def test_wide_heads_in_tiles_of_either_height(lib, cuda, hd, page, seqs, q, kv):
     d.out.fill_(777.0)
     check(d.attention(40), *s.attention(40))
     lib.status()
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", [(12, 4, 128), (12, 4, 64), (8, 2, 256), (12, 1, 128)])
+def test_long_sums_are_not_cut(lib, cuda, heads, kv_heads, hd):
+    """Single tokens over many keys, all values between 1 and 2.  A tile's sum may be cut by less than
+    a step, 2 u of it; what comes after is rounded to nearest, whose errors even out: the mean error
+    is above -2 u, however many tiles there are, and below what the weights' rounding leaves, u."""
+    s = Setup(F16, heads, kv_heads, hd, 64, q=[1] * 3, kv=[20000, 19000, 15017], seed=60)
+    r = np.random.default_rng(61)
+    s.v = (1 + r.random(s.v.shape)).astype(np.float16)
+    d = Device(lib, cuda, s)
+    want = s.attention()[0]
+    err = (d.attention().cpu().numpy() - want) / want
+    assert -2 * U < err.mean() < U, err.mean() / U
