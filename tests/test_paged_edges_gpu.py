@@ -5,6 +5,7 @@ import threading
 import numpy as np
 import pytest
 
+import nedo_gpu
 from paged_ref import F16, F32, U, Device, Setup
 
 pytestmark = pytest.mark.gpu
@@ -237,3 +238,34 @@ def test_long_sums_are_not_cut(lib, cuda, heads, kv_heads, hd):
     want = s.attention()[0]
     err = (d.attention().cpu().numpy() - want) / want
     assert -2 * U < err.mean() < U, err.mean() / U
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("what", ["order", "too many rows"])
+def test_rows_of_sequences_left_out_stay_as_they_were(lib, cuda, type_, what):
+    """Every row of a sequence whose lengths are out of range is left alone, by append and by every
+    attention; the others' rows come out right."""
+    s = Setup(type_, 6, 2, 64, 32, q=[2, 3, 2], kv=[50, 40, 30], seed=15)
+    d = Device(lib, cuda, s)
+    want, tol, inside = s.attention()
+    if what == "order":  # 5 rows, -3 and 5, of at most 3
+        d.start[1], d.start[2] = 5, 2
+        inside[:] = False
+    else:  # 2 rows, 4 and 1: the last row stands where it stood
+        d.start[2] = 6
+        inside[2:6] = False
+    k = d.k.clone()
+    for run in (d.attention, lambda: d.attention(7), lambda: d.block_attention(every_page(s)), lambda: d.append(1e4)):
+        d.out.fill_(777.0)
+        got = run()
+        with pytest.raises(nedo_gpu.NedoGpuError) as e:
+            lib.status(d.stream())
+        assert e.value.code == nedo_gpu.ERR_DEVICE
+        assert (got[cuda.from_numpy(~inside).cuda()] == 777.0).all()
+        if run == d.attention:
+            check(got, want, tol, inside)
+    # append has written the keys of the rows left, and no others
+    changed = (d.k != k).any(-1).any(1)
+    changed &= ~(cuda.isnan(d.k) & cuda.isnan(k)).any(-1).any(1)
+    rows = {place(s, sq, p) for t, sq, p in s.rows() if inside[t]}
+    assert {tuple(x) for x in changed.nonzero().tolist()} == rows
