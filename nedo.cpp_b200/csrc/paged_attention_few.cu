@@ -4,9 +4,9 @@
 //
 // Mathematics.  Queries and weights are fp32 and the cache is fp16, so every product
 // runs on the fp16 tensor cores with the fp32 side split in two halves,
-// x = hi + lo, that keep 22 bits of it: q is scaled by a power of two per row (its
-// largest channel to [2^13, 2^14), so that the low half stays a normal number), and the
-// weights p = 2^(s - m + 14) are taken up by the same factor in numerator and sum.  The
+// x = hi + 2^-11 lo, that keep 22 bits of it: q is scaled by a power of two per row (its
+// largest channel to [2^13, 2^14)), and the weights p = 2^(s - m + 14) are taken up by the same
+// factor in numerator and sum.  The
 // two halves ride in one m16n8k16 operand, rows 0-7 the high and rows 8-15 the low half
 // of the same eight query rows, so the split costs no extra instruction: both parts of a
 // row's sum land in the same thread, which adds them.  With more than eight rows the halves
@@ -199,7 +199,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             for (uint32_t j = 0; j < 4; ++j) {
                 const float high = sc[0][j >> 1][(j & 1u) + 2u * h];
                 const float low = kMine == 1u ? sc[0][j >> 1][(j & 1u) + 2u] : sc[kMine - 1u][j >> 1][(j & 1u) + 2u * h];
-                v[h][j] = (high + low) * unscale[h];
+                v[h][j] = fmaf(low, kLowDown, high) * unscale[h];
                 if (!whole) {
                     const uint32_t at_key = pos + t2 + (j & 1u) + (j >> 1) * 8u;
                     if (page == kNone || at_key < p_lo[h] || at_key >= p_hi[h]) v[h][j] = -INFINITY;
@@ -245,6 +245,8 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             if constexpr (kMine == 2u) {
                 mma(o[0], pf[kMine - 1u], b[0], b[1]);
                 mma(o[1], pf[kMine - 1u], b[2], b[3]);
+                low_down(o[0]);
+                low_down(o[1]);
             }
             mma(o[0], pf[0], b[0], b[1]);
             mma(o[1], pf[0], b[2], b[3]);
@@ -284,7 +286,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
     for (uint32_t n = 0; n < HD / 8; ++n) {
         float* to = part + (warp * ROWS + g) * kPitch + n * 8u + t2;
         if constexpr (kMine == 1u) {
-            *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+            *reinterpret_cast<float2*>(to) = make_float2(fmaf(acc[n][2], kLowDown, acc[n][0]), fmaf(acc[n][3], kLowDown, acc[n][1]));
         } else {
             *reinterpret_cast<float2*>(to) = make_float2(acc[n][0], acc[n][1]);
             *reinterpret_cast<float2*>(to + 8u * kPitch) = make_float2(acc[n][2], acc[n][3]);

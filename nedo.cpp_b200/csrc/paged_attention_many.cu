@@ -257,7 +257,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
 #pragma unroll
             for (uint32_t n = 0; n < kCols; ++n)
 #pragma unroll
-                for (uint32_t e = 0; e < 4; ++e) sc[n][e] += low[n][e];
+                for (uint32_t e = 0; e < 4; ++e) sc[n][e] = fmaf(low[n][e], kLowDown, sc[n][e]);
             const bool gap = tile_gap[i % kStages] != 0u;
             const bool whole = !gap && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
             if (!whole) {
@@ -319,6 +319,8 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
                     mma(o[0], plo[k], b[k][0], b[k][1]);
                     mma(o[1], plo[k], b[k][2], b[k][3]);
                 }
+                low_down(o[0]);
+                low_down(o[1]);
 #pragma unroll
                 for (uint32_t k = 0; k < kGroups; ++k) {
                     mma(o[0], phi[k], b[k][0], b[k][1]);

@@ -29,16 +29,7 @@ namespace nedo_gpu {
 namespace {
 
 constexpr float kDown = 1.f / 16384.f;  // 2^-kUp
-constexpr float kLowUp = 2048.f, kLowDown = 1.f / 2048.f;
 constexpr float kRange = 134217728.f;   // 2^27: numbers of 2^14 and 2^-14 under one scale
-
-// x, y as two fp16 halves each, x = hi + 2^-11 lo.
-__device__ __forceinline__ void split_up(float2 x, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __float22half2_rn(x);
-    const float2 f = __half22float2(h), up = make_float2(kLowUp, kLowUp);
-    *hi = pack(h);
-    *lo = pack(__float22half2_rn(__fmul2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y)), up)));
-}
 
 template <uint32_t HD>
 struct Many32 {
@@ -216,7 +207,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
             for (uint32_t e = 0; e < 4; ++e) {
                 float2 x = make_float2(0.f, 0.f);
                 if (p >= 0 && d < hd) x = *reinterpret_cast<const float2*>(q + d + 2u * e);
-                split_up(make_float2(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up), &hi[e], &lo[e]);
+                split(make_float2(x.x * a.scale_log2 * up, x.y * a.scale_log2 * up), &hi[e], &lo[e]);
             }
             *reinterpret_cast<uint4*>(sm + at<HD>(r, d >> 3)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             *reinterpret_cast<uint4*>(sm + M::kQBytes + at<HD>(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -308,8 +299,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                 const float up = kv ? v_up : k_up;
                 const float2 up2 = make_float2(up, up);
                 uint32_t hi[2], lo[2];
-                split_up(__fmul2_rn(make_float2(v.x, v.y), up2), &hi[0], &lo[0]);
-                split_up(__fmul2_rn(make_float2(v.z, v.w), up2), &hi[1], &lo[1]);
+                split(__fmul2_rn(make_float2(v.x, v.y), up2), &hi[0], &lo[0]);
+                split(__fmul2_rn(make_float2(v.z, v.w), up2), &hi[1], &lo[1]);
                 uint8_t* dst = halves + kv * 2u * M::kHalfBytes + at<HD>(r, piece_ch >> 1) + (piece_ch & 1u) * 8u;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(dst + M::kHalfBytes) = make_uint2(lo[0], lo[1]);
@@ -410,8 +401,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                     sc[n][e] = exp2_fast(fmaf(sc[n][e] * down[e >> 1], k_one, -ref[e >> 1]));
                     l[e >> 1] += sc[n][e];
                 }
-                split_up(make_float2(sc[n][0], sc[n][1]), &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
-                split_up(make_float2(sc[n][2], sc[n][3]), &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
+                split(make_float2(sc[n][0], sc[n][1]), &phi[n >> 1][(n & 1u) * 2u], &plo[n >> 1][(n & 1u) * 2u]);
+                split(make_float2(sc[n][2], sc[n][3]), &phi[n >> 1][(n & 1u) * 2u + 1u], &plo[n >> 1][(n & 1u) * 2u + 1u]);
             }
             if (!slow) {
 #pragma unroll
@@ -437,11 +428,8 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                             mma(o[0], plo[k], b[k][0], b[k][1]);
                             mma(o[1], plo[k], b[k][2], b[k][3]);
                         }
-#pragma unroll
-                        for (uint32_t e = 0; e < 4; ++e) {
-                            o[0][e] *= kLowDown;
-                            o[1][e] *= kLowDown;
-                        }
+                        low_down(o[0]);
+                        low_down(o[1]);
 #pragma unroll
                         for (uint32_t k = 0; k < kGroups; ++k) {
                             mma(o[0], phi[k], b[k][0], b[k][1]);

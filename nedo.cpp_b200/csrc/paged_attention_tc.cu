@@ -3,8 +3,8 @@
 // prefix, groups of more than eight rows), heads of up to 128 channels.
 //
 // Mathematics.  As in the other tensor-core kernels the fp32 factors are split in two fp16
-// halves, low halves first: S = q_lo K^T + q_hi K^T, O = p_lo V + p_hi V, so every 128 x 128
-// tile is 32 MMAs of 128 x 128 x 16.  The tensor core cuts its fp32 sums instead of rounding
+// halves, low halves first: S = 2^-11 q_lo K^T + q_hi K^T, O = 2^-11 p_lo V + p_hi V, so every
+// 128 x 128 tile is 32 MMAs of 128 x 128 x 16; the first with the high halves scales what is there.  The tensor core cuts its fp32 sums instead of rounding
 // them, so a tile's O starts from zero in TMEM and is added to the running sums in fp32
 // registers, together with the rescaling by 2^(m_old - m_new).
 //
@@ -77,21 +77,36 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 // D (TMEM) = A (TMEM) * B (shared memory, the low word of its descriptor and the high one) [+ D].
 // All operands are the same in the whole warp, so that they live in uniform registers: built
 // per lane, each MMA took some 110 cycles to issue, of which it runs 64.
-template <uint32_t HIGH, uint32_t IDESC>
+// SCALE: [+ 2^-SCALE D].
+template <uint32_t HIGH, uint32_t IDESC, uint32_t SCALE>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-        "r"(a), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
-        : "memory");
+    if constexpr (SCALE == 0u)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+            "r"(a), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p, %6;\n\t}" ::"r"(d),
+            "r"(a), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add)), "n"(SCALE)
+            : "memory");
 }
-template <uint32_t HIGH, uint32_t IDESC>
+template <uint32_t HIGH, uint32_t IDESC, uint32_t SCALE>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-        "r"(a_low), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
-        : "memory");
+    if constexpr (SCALE == 0u)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+            "r"(a_low), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add))
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p, %6;\n\t}" ::"r"(d),
+            "r"(a_low), "r"(b_low), "n"(HIGH), "n"(IDESC), "r"(static_cast<uint32_t>(add)), "n"(SCALE)
+            : "memory");
 }
 // 16 columns of this warp's 32 lanes, a row per thread: the load is under way until
 // tmem_ready, which takes the registers so that nothing reads them before it.
@@ -386,12 +401,14 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 tc_fence_after();
                 const uint32_t d = kTmem + buf * 128u, k0 = desc_low(ring + slot * T::kTile, 16u), q0 = desc_low(s0, 16u);
                 if (elect_one()) {
+                    // low halves first, taken down by the first product with the high ones
+                    auto at_k = [](uint32_t k) { return ((k >> 2) * kBlock + (k & 3u) * 32u) >> 4; };
 #pragma unroll
-                    for (uint32_t half = 0; half < 2u; ++half)  // low halves first
+                    for (uint32_t k = 0; k < HD / 16u; ++k)
+                        mma_ss<kDescHigh, kS, 0u>(d, q0 + (T::kTile >> 4) + at_k(k), k0 + at_k(k), k != 0u);
+                    mma_ss<kDescHigh, kS, kLowBits>(d, q0, k0, true);
 #pragma unroll
-                        for (uint32_t k = 0; k < HD / 16u; ++k)
-                            mma_ss<kDescHigh, kS>(d, q0 + (((half ? 0u : T::kTile) + (k >> 2) * kBlock + (k & 3u) * 32u) >> 4),
-                                                  k0 + (((k >> 2) * kBlock + (k & 3u) * 32u) >> 4), half + k != 0u);
+                    for (uint32_t k = 1; k < HD / 16u; ++k) mma_ss<kDescHigh, kS, 0u>(d, q0 + at_k(k), k0 + at_k(k), true);
                     tc_commit(&s_full[buf]);
                     tc_commit(&empty[slot]);
                 }
@@ -415,12 +432,14 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 tc_fence_after();
                 const uint32_t p = kTmem + buf * 128u, v0 = desc_low(ring + slot * T::kTile, kBlock);
                 if (elect_one()) {
+                    // 16 keys: 8 + 8 columns of weights, 2048 bytes of values
 #pragma unroll
-                    for (uint32_t half = 0; half < 2u; ++half)
+                    for (uint32_t k = 0; k < kKeys / 16u; ++k)
+                        mma_ts<kDescHigh, kO, 0u>(kTmem + kOColumn, p + k * 16u + 8u, v0 + k * (2048u >> 4), k != 0u);
+                    mma_ts<kDescHigh, kO, kLowBits>(kTmem + kOColumn, p, v0, true);
 #pragma unroll
-                        for (uint32_t k = 0; k < kKeys / 16u; ++k)  // 16 keys: 8 + 8 columns of weights, 2048 bytes of values
-                            mma_ts<kDescHigh, kO>(kTmem + kOColumn, p + k * 16u + (half ? 0u : 8u), v0 + k * (2048u >> 4),
-                                                  half + k != 0u);
+                    for (uint32_t k = 1; k < kKeys / 16u; ++k)
+                        mma_ts<kDescHigh, kO, 0u>(kTmem + kOColumn, p + k * 16u, v0 + k * (2048u >> 4), true);
                     tc_commit(&o_full);
                     tc_commit(&empty[slot]);
                 }

@@ -36,19 +36,26 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t pack(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// x, y as two fp16 halves each: {hi, lo}
-__device__ __forceinline__ void split(float x, float y, uint32_t* hi, uint32_t* lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    *hi = pack(h);
-    *lo = pack(__floats2half2_rn(x - f.x, y - f.y));
-}
-// the same for a pair in packed arithmetic
+// A pair of numbers as two fp16 halves each, x = hi + 2^-11 lo.  Below 2^15, as the kernels scale
+// them, they keep 22 bits down to 2^-14, and 2^-36 below (a low half that is not taken up would leave
+// 2^-25, which is what an unscaled softmax weight of 2^-39 is: not nothing next to a large value).
+constexpr int kLowBits = 11;
+constexpr float kLowDown = 1.f / (1 << kLowBits);
 __device__ __forceinline__ void split(float2 x, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __float22half2_rn(x);
-    const float2 f = __half22float2(h);
+    const float2 f = __half22float2(h), up = make_float2(1 << kLowBits, 1 << kLowBits);
     *hi = pack(h);
-    *lo = pack(__float22half2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y))));
+    *lo = pack(__float22half2_rn(__fmul2_rn(__fadd2_rn(x, make_float2(-f.x, -f.y)), up)));
+}
+__device__ __forceinline__ void split(float x, float y, uint32_t* hi, uint32_t* lo) { split(make_float2(x, y), hi, lo); }
+// Sums from low halves, on which those from high halves can go.
+__device__ __forceinline__ void low_down(float (&c)[4]) {
+    const float2 d = make_float2(kLowDown, kLowDown);
+    const float2 x = __fmul2_rn(make_float2(c[0], c[1]), d), y = __fmul2_rn(make_float2(c[2], c[3]), d);
+    c[0] = x.x;
+    c[1] = x.y;
+    c[2] = y.x;
+    c[3] = y.y;
 }
 
 // The power of two that takes a row's largest magnitude to [2^13, 2^14), where the low

@@ -269,3 +269,45 @@ def test_rows_of_sequences_left_out_stay_as_they_were(lib, cuda, type_, what):
     changed &= ~(cuda.isnan(d.k) & cuda.isnan(k)).any(-1).any(1)
     rows = {place(s, sq, p) for t, sq, p in s.rows() if inside[t]}
     assert {tuple(x) for x in changed.nonzero().tolist()} == rows
+
+
+@pytest.mark.parametrize("type_", [F16, F32])
+@pytest.mark.parametrize("heads,kv_heads,hd", KINDS)
+@pytest.mark.parametrize("nats", [12.0, 18.0, 22.0])
+def test_small_weights_of_large_values(lib, cuda, type_, heads, kv_heads, hd, nats):
+    """Keys of far lower score with far larger values: their small weights keep their digits."""
+    q, kv = [1, 70, 9, 1], [3000, 700, 300, 513]
+    s = Setup(type_, heads, kv_heads, hd, 32, q=q, kv=kv, shared=4, seed=50)
+    s.scale = 1.0
+    s.queries *= np.float32(0.05)
+    s.queries[..., 0] = 1.0
+    r = np.random.default_rng(51)
+    seen = set()
+    for seq in range(4):
+        for pos in range(kv[seq]):
+            page, slot = place(s, seq, pos)
+            if (page, slot) in seen:
+                continue
+            seen.add((page, slot))
+            far = r.random() < 0.3
+            s.k[page, :, slot, 0] = -nats if far else 0.0
+            s.v[page, :, slot] *= s.v.dtype.type(1e4 if far else 1e4 * np.exp(-nats))
+    d = Device(lib, cuda, s)
+    want = s.attention()
+    check(d.attention(), *want)
+    check(d.block_attention(every_page(s)), *want)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd", KINDS)
+@pytest.mark.parametrize("size", [1e-3, 1e-5, 1e-7])
+def test_small_query_channels_of_large_key_channels(lib, cuda, heads, kv_heads, hd, size):
+    """A query channel far smaller than its neighbours, which meets a key channel as much larger."""
+    q, kv = [1, 70, 9], [3000, 700, 300]
+    s = Setup(F16, heads, kv_heads, hd, 32, q=q, kv=kv, seed=52)
+    s.queries[..., 4] *= np.float32(size)
+    s.k[..., 4] *= np.float16(1e3)
+    s.k[..., :4] *= np.float16(1e3 * size)
+    s.k[..., 5:] *= np.float16(1e3 * size)
+    s.scale = 1.0 / (1e3 * size)
+    d = Device(lib, cuda, s)
+    check(d.attention(), *s.attention())
