@@ -363,8 +363,11 @@ NEDO_GPU_API void nedo_gpu_decoder_destroy(nedo_gpu_decoder* d);
  * matvec: q|k|v of a batch comes from one nedo_gpu_matvec_dev, goes through
  * nedo_gpu_kv_append_dev, and the attention output goes into the output
  * projection.  The arithmetic is that of src/model.cpp:218-247 and
- * src/kernels.cpp:93-105 per sequence; pages, ragged batches, shared prefixes and
- * page selection have no reference counterpart.
+ * src/kernels.cpp:93-105 per sequence, but for the rotation's angles: append forms
+ * them in 64 bits, the decode pass in 32 as the reference does, so at far positions
+ * p the keys differ by a turn of up to p * 2^-24 radians, and a cache is continued by
+ * the one that began it.  Pages, ragged batches, shared prefixes and page selection
+ * have no reference counterpart.
  *
  * All of them are asynchronous on `stream`, allocate nothing and keep nothing
  * between calls, so they can be captured in CUDA graphs and may run at the same
@@ -417,7 +420,8 @@ typedef struct {
 /* The new tokens of a batch: rotates queries and keys to their positions and
  * writes keys and values into the cache.  qkv_dev holds `tokens` rows of
  * heads * head_dim query, kv_heads * head_dim key and as many value elements (the
- * decoder's q|k|v layout); the rotated queries go to q_out_dev
+ * decoder's q|k|v layout; an F16 cache gets them rounded to nearest, above 65504 as
+ * infinities); the rotated queries go to q_out_dev
  * [tokens][heads][head_dim], which must not overlap qkv_dev.  Channels i and
  * i + head_dim/2 turn by position * rope_theta^(-2i/head_dim), the angle in 64
  * bits; rope_theta 0: no rotation.  With cache->bounds, the channel bounds of every
@@ -437,8 +441,12 @@ NEDO_GPU_API int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cac
  *   out = sum_j softmax_j(scale * q.k_j) v_j,  max(0, p - window + 1) <= j <= p
  * for a row at position p (window 0: all).  With shared_pages > 0 the keys of the
  * shared prefix are read once for the whole batch.  Sums and softmax statistics
- * are kept in 32 bits.  On the tensor cores a row's query channels keep 22 bits, or
- * 2^-38 of the row's largest, whichever is coarser.
+ * are kept in 32 bits.  The factors of the tensor cores' products -- queries and
+ * softmax weights, and the keys and values of an F32 cache where a sequence (or, over a
+ * shared prefix, the batch) has more than 16 rows, tokens times heads per KV head -- keep
+ * 22 bits down to 2^-27 of the largest number they share a scale with (a row's query
+ * channels; a row's weights; 32 or 64 neighbouring keys or values), and 2^-49 of that
+ * below.  Fewer rows on an F32 cache are computed in 32 bits throughout.
  *
  * Infinities (an F16 cache holds what is above 65504 as one) count as they do in the
  * formula: a key whose score is -infinity has no weight, one whose score is +infinity

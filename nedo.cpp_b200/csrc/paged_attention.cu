@@ -5,7 +5,8 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = scale * log2(e) * q.k_j
 //
-// in one pass over the keys with a running maximum m, in 32 bits throughout.  A
+// in one pass over the keys with a running maximum m.  Sums and statistics are in 32 bits; the
+// factors that the tensor cores multiply are split in two fp16 halves, 22 bits.  A
 // work item is a tile of query rows of one KV head (the heads of its group next
 // to each other, so a key is read once for all of them) times a chunk of keys.
 // With one chunk per row the item writes the output; otherwise it writes
@@ -35,8 +36,8 @@ struct CombineArgs {
     uint32_t blocks;  // the sparse call: every slot is written
 };
 
-// One CTA per token and head (per token where most rows are done already).  The maximum over the row's chunks first, then in blocks of
-// kCombineThreads chunks their weights 2^(m_i - m) into shared memory, and the weighted
+// One CTA per token and head (per token where most rows are done already).  The maximum over the
+// row's chunks first, then in blocks of kCombineThreads chunks their weights 2^(m_i - m) into shared memory, and the weighted
 // sum with head_dim / 4 threads to a chunk and as many chunks at once as the CTA holds,
 // four loads in flight each; the groups' sums meet in group order.  A chunk in which the
 // row sees nothing has weight sum 0 and may hold anything.  Launched so that it comes up

@@ -18,8 +18,8 @@
 // own running maximum and sums, so the warps meet only at the end.  A 16-key tile lies
 // within one page.  Two CTAs share an SM.
 //
-// 32 single tokens of 12 query and 4 KV heads of 128 channels over 8191 to 32768 keys: 214 us,
-// 6.6 TB/s.  32 query heads over 2 KV heads, 5000 to 20000 keys: 86 us in tiles of 16 rows, 5.0
+// 32 single tokens of 12 query and 4 KV heads of 128 channels over 8191 to 32768 keys: 215 us,
+// 6.6 TB/s.  32 query heads over 2 KV heads, 5000 to 20000 keys: 90 us in tiles of 16 rows, 4.8
 // TB/s (118 us in two tiles of 8, which both read the cache).  Heads above 128 keep to 8: the
 // queries and sums of 16 rows would not stay in registers.
 #include "paged_attention.cuh"

@@ -5,7 +5,7 @@
 //
 // Mathematics.  As in paged_attention_few.cu the fp32 factors are split in two fp16
 // halves; here each half is an operand of its own, the low one first, so that the sums
-// grow in few steps (the tensor core cuts its fp32 sums instead of rounding them; a
+// can be taken down before the high ones come and grow in few steps (the tensor core cuts its fp32 sums instead of rounding them; a
 // tile's weighted values are therefore summed from zero in 4 steps and added to the
 // running sums in fp32 with the rescaling by 2^(m_old - m_new)).
 //
@@ -13,8 +13,8 @@
 // tiles deep.  Tiles that none of a warp's rows sees are skipped by it, and only tiles
 // seen in part are masked.
 //
-// 12 query and 4 KV heads of 256 channels, 2048 and 1840 new tokens of two sequences over 4096 and
-// 2550 keys: 847 us, 270 TFLOP/s of MMAs (two for each product), in tiles of 128 rows; 64 rows, which
+// 12 query and 4 KV heads of 256 channels, 2048 and 1919 new tokens of two sequences over 4096 and
+// 2929 keys: 869 us, 285 TFLOP/s of MMAs (two for each product), in tiles of 128 rows; 64 rows, which
 // read the keys twice as often, take 1072.  Where there are few tiles 64 rows reach more SMs: 8 query
 // and 2 KV heads, 300 tokens 26 us (128 rows: 30), 37 sequences of 32 tokens over 500 keys 51 us (68).
 // The plan takes the height that it expects to end first.

@@ -19,7 +19,7 @@
 // magnitudes found, and its halves written next to it for ldmatrix, once for all warps.
 //
 // 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two sequences over 4096 and
-// 2550 keys, window 2048: 563 us, 231 TFLOP/s of MMAs (three for each product).  With two warps to
+// 2550 keys, window 2048: 567 us, 230 TFLOP/s of MMAs (three for each product).  With two warps to
 // a scheduler the tensor pipe is busy for half of the time; the rest is the halves' making and
 // the latency of what stands between the MMAs.
 #include "paged_attention.cuh"
@@ -436,7 +436,7 @@ __device__ __forceinline__ void attention_many32(const AttnArgs& a) {
                             mma(o[1], phi[k], b[k][2], b[k][3]);
                         }
                     } else {
-                        float low[2][4];  // (392 us for a prompt of 1429 tokens; as above 413)
+                        float low[2][4];  // (392 us for prompts of 900 and 671 tokens; as above 413)
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e) low[0][e] = low[1][e] = 0.f;
 #pragma unroll

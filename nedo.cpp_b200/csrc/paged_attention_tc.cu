@@ -1,6 +1,6 @@
 // paged_attention_tc.cu -- attention over a paged F16 cache for tiles of 128 query rows on
 // the 5th-generation tensor cores (prompts, the tokens of a whole batch over their shared
-// prefix, groups of more than eight rows), heads of up to 128 channels.
+// prefix, groups of more than 16 heads), heads of up to 128 channels.
 //
 // Mathematics.  As in the other tensor-core kernels the fp32 factors are split in two fp16
 // halves, low halves first: S = 2^-11 q_lo K^T + q_hi K^T, O = 2^-11 p_lo V + p_hi V, so every
@@ -24,7 +24,7 @@
 // Registers: 56 for the softmax, 112 for the sums, 56 for the others.
 //
 // What bounds it: 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two
-// sequences over 4096 and 2550 keys, window 2048: 105 us, 820 TFLOP/s of fp16 MMAs (two for each
+// sequences over 4096 and 2550 keys, window 2048: 104 us, 825 TFLOP/s of fp16 MMAs (two for each
 // product of the formula).  An item of 17 tiles is 70,000 cycles: 5,000 until its rows and keys
 // are known, 4,500 until the queries are in shared memory, 9,500 until the first tile's sums (the
 // softmax of both halves at once), then 2,850 a tile, of which the MMAs run 2,050, and 5,000 for
@@ -314,7 +314,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     // all 512 columns: they begin at 0
     constexpr uint32_t tmem = kTmem;
 
-    // Ring order: K0, K1, V0, K2, V1, ..., V(last): the order in which the MMAs use them.
+    // Ring order: K0, K1, K2, V0, K3, V1, ..., V(last): the order in which the MMAs use them.
     auto k_at = [&](uint32_t i) { return i + (i >= kBuffers ? i - kBuffers + 1u : 0u); };
     auto v_at = [&](uint32_t i) { return i + min(ntiles, i + kBuffers); };
 
