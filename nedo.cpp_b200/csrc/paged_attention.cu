@@ -37,8 +37,8 @@ struct CombineArgs {
 };
 
 // One CTA per token and head (per token where most rows are done already).  The maximum over the
-// row's chunks first, then in blocks of kCombineThreads chunks their weights 2^(m_i - m) into shared memory, and the weighted
-// sum with head_dim / 4 threads to a chunk and as many chunks at once as the CTA holds,
+// row's chunks first, then in blocks of kCombineThreads chunks their weights 2^(m_i - m) into
+// shared memory, and the weighted sum with head_dim / 4 threads to a chunk and as many chunks at once as the CTA holds,
 // four loads in flight each; the groups' sums meet in group order.  A chunk in which the
 // row sees nothing has weight sum 0 and may hold anything.  Launched so that it comes up
 // while the last work items run; it waits for their sums before it reads them.
@@ -306,7 +306,7 @@ bool plan_paged_attention(PagedAttention* a) {
                  : takes_few(k) ? a->b.seqs * ceil_div(a->b.max_q_len * group, c.rows)
                                 : own_tiles(*a, c.rows)) *
                 a->kv.kv_heads;
-        return chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(k), choice ? causal : 0.0);
+        return chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(k), choice && !takes_few(k) ? causal : 0.0);
     });
     const Kernel own = own_kernel(*a);
     a->own_chunk = best.keys;
