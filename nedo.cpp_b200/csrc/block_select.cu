@@ -521,8 +521,9 @@ cudaError_t launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const
 
 cudaError_t launch_block_select(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* q, uint32_t picks,
                                 uint32_t* blocks, DeviceStatus* st, cudaStream_t stream) {
-    const uint32_t pieces = 2u * kv.head_dim * (kv.type == kF16 ? 2u : 4u) / 16u;  // of a page's bounds
-    if (kv.type == kF16)
+    const bool halves = kv.type != kF32;  // (the bounds of Q4_0 pages are F16)
+    const uint32_t pieces = 2u * kv.head_dim * (halves ? 2u : 4u) / 16u;  // of a page's bounds
+    if (halves)
         return pieces <= 32u ? launch<__half, 1>(kv, b, heads, q, picks, blocks, st, stream)
                              : launch<__half, 2>(kv, b, heads, q, picks, blocks, st, stream);
     return pieces <= 32u   ? launch<float, 1>(kv, b, heads, q, picks, blocks, st, stream)

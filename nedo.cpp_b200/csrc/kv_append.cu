@@ -19,51 +19,11 @@
 //     writes and one KV head, because the minimum and maximum of the page's channels over the
 //     new tokens need them in one place (the tokens spread over the thread groups, one round of
 //     loads for a page of 64).  With one token per sequence they are pieces of its row.
-#include <algorithm>
-
-#include "paged.cuh"
+#include "kv_append.cuh"
 
 namespace nedo_gpu {
 namespace {
 
-constexpr uint32_t kMaxRows = 4;  // token rows of a query CTA
-
-struct AppendArgs {
-    PagedKv kv;
-    PagedBatch b;
-    const float* qkv;
-    float* q_out;
-    double log2_theta;
-    uint32_t heads, rotate;
-    uint32_t segs;      // pages that a sequence's new tokens can touch
-    uint32_t key_ctas;  // CTAs of the first kind
-    uint32_t rows;      // token rows of a CTA of the other kind
-    uint32_t pieces, blocks;  // 16-byte pieces (pairs) of a row, and CTAs that share them
-    uint32_t row_keys;  // the keys are pieces of their rows
-    DeviceStatus* st;
-};
-
-// Turns per position of channel pair i.
-__device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
-    return exp2(-2.0 * i / a.kv.head_dim * a.log2_theta) * 0.15915494309189535;  // 1 / (2 pi)
-}
-// Cosine and sine of position p's rotation.
-__device__ __forceinline__ float2 rotation(int p, double turns) {
-    double turn = static_cast<double>(p) * turns;
-    turn -= rint(turn);
-    // what the fraction loses in 32 bits turns the result by the rest of the angle
-    const float f = static_cast<float>(turn), rest = static_cast<float>((turn - f) * 6.283185307179586);
-    float c, s;
-    sincospif(2.f * f, &s, &c);
-    return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
-}
-__device__ __forceinline__ void rotate4(float4& x, float4& y, const float2* c) {
-    const float4 u = x, w = y;
-    x = make_float4(u.x * c[0].x - w.x * c[0].y, u.y * c[1].x - w.y * c[1].y, u.z * c[2].x - w.z * c[2].y,
-                    u.w * c[3].x - w.w * c[3].y);
-    y = make_float4(u.x * c[0].y + w.x * c[0].x, u.y * c[1].y + w.y * c[1].x, u.z * c[2].y + w.z * c[2].x,
-                    u.w * c[3].y + w.w * c[3].x);
-}
 // Four values into the cache, and what they are there.
 __device__ __forceinline__ void store4(float* dst, float4& x) { *reinterpret_cast<float4*>(dst) = x; }
 __device__ __forceinline__ void store4(__half* dst, float4& x) {
@@ -72,13 +32,6 @@ __device__ __forceinline__ void store4(__half* dst, float4& x) {
     const float2 lo = __half22float2(h[0]), hi = __half22float2(h[1]);
     x = make_float4(lo.x, lo.y, hi.x, hi.y);
 }
-__device__ __forceinline__ float4 min4(const float4& a, const float4& b) {
-    return make_float4(fminf(a.x, b.x), fminf(a.y, b.y), fminf(a.z, b.z), fminf(a.w, b.w));
-}
-__device__ __forceinline__ float4 max4(const float4& a, const float4& b) {
-    return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
-}
-
 // The keys of one page and KV head, and its bounds (fminf / fmaxf leave NaN out).  A page
 // whose first slot is written begins anew.
 template <typename T>
@@ -258,29 +211,12 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
 
 cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
                              float* q_out, DeviceStatus* st, cudaStream_t stream) {
-    AppendArgs a = {};
-    a.kv = kv;
-    a.b = b;
-    a.qkv = qkv;
-    a.q_out = q_out;
-    a.rotate = theta > 0.0;
-    a.log2_theta = a.rotate ? log2(theta) : 0.0;
-    a.heads = heads;
-    a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
-    a.rows = b.tokens >= 4u * 148u ? kMaxRows : 1u;  // four rows share their sines where there are CTAs enough
-    a.row_keys = b.max_q_len <= 1u;
-    const uint32_t quads = kv.head_dim / 8u;
-    a.pieces = (heads + (a.row_keys ? kv.kv_heads : 0u)) * quads + kv.kv_heads * kv.head_dim / 4u;
-    a.blocks = (a.pieces + 255u) / 256u;
-    // a thread for every piece, and for every channel pair
-    const uint32_t threads = (std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u) + 31u) / 32u * 32u;
-    a.st = st;
-    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
-    const uint64_t grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
-    if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
-    a.key_ctas = static_cast<uint32_t>(keys);
-    if (kv.type == kF16) kv_append_kernel<__half><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
-    else kv_append_kernel<float><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
+    if (kv.type == kQ4_0) return launch_kv_append4(kv, b, heads, qkv, theta, q_out, st, stream);
+    const AppendLaunch l = append_launch(kv, b, heads, qkv, theta, q_out, st, kv.kv_heads * (kv.head_dim / 8u), 0u);
+    if (l.grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    const uint32_t grid = static_cast<uint32_t>(l.grid);
+    if (kv.type == kF16) kv_append_kernel<__half><<<grid, l.threads, 0, stream>>>(l.a);
+    else kv_append_kernel<float><<<grid, l.threads, 0, stream>>>(l.a);
     return cudaGetLastError();
 }
 

@@ -1,0 +1,90 @@
+// kv_append.cuh -- what the append kernels share (kv_append.cu: F16 and F32 caches, kv_append4.cu:
+// Q4_0 caches): the launch's arguments and the rotation.
+#pragma once
+
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace nedo_gpu {
+
+constexpr uint32_t kMaxRows = 4;  // token rows of a query CTA
+
+struct AppendArgs {
+    PagedKv kv;
+    PagedBatch b;
+    const float* qkv;
+    float* q_out;
+    double log2_theta;
+    uint32_t heads, rotate;
+    uint32_t segs;      // pages that a sequence's new tokens can touch
+    uint32_t key_ctas;  // CTAs of the first kind
+    uint32_t rows;      // token rows of a CTA of the other kind
+    uint32_t pieces, blocks;  // 16-byte pieces (pairs) of a row, and CTAs that share them
+    uint32_t row_keys;  // the keys are pieces of their rows
+    DeviceStatus* st;
+};
+
+// Turns per position of channel pair i.
+__device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
+    return exp2(-2.0 * i / a.kv.head_dim * a.log2_theta) * 0.15915494309189535;  // 1 / (2 pi)
+}
+// Cosine and sine of position p's rotation.
+__device__ __forceinline__ float2 rotation(int p, double turns) {
+    double turn = static_cast<double>(p) * turns;
+    turn -= rint(turn);
+    // what the fraction loses in 32 bits turns the result by the rest of the angle
+    const float f = static_cast<float>(turn), rest = static_cast<float>((turn - f) * 6.283185307179586);
+    float c, s;
+    sincospif(2.f * f, &s, &c);
+    return make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
+}
+__device__ __forceinline__ void rotate4(float4& x, float4& y, const float2* c) {
+    const float4 u = x, w = y;
+    x = make_float4(u.x * c[0].x - w.x * c[0].y, u.y * c[1].x - w.y * c[1].y, u.z * c[2].x - w.z * c[2].y,
+                    u.w * c[3].x - w.w * c[3].y);
+    y = make_float4(u.x * c[0].y + w.x * c[0].x, u.y * c[1].y + w.y * c[1].x, u.z * c[2].y + w.z * c[2].x,
+                    u.w * c[3].y + w.w * c[3].x);
+}
+__device__ __forceinline__ float4 min4(const float4& a, const float4& b) {
+    return make_float4(fminf(a.x, b.x), fminf(a.y, b.y), fminf(a.z, b.z), fminf(a.w, b.w));
+}
+__device__ __forceinline__ float4 max4(const float4& a, const float4& b) {
+    return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
+}
+
+// The launch's shape, and its arguments: CTAs for a.key_ctas pages, and for the rows.  Pieces are of
+// 16 bytes (pairs half a head apart where they turn as pairs): `key_pieces` of a row's keys.
+struct AppendLaunch {
+    AppendArgs a;
+    uint64_t grid;
+    uint32_t threads;
+};
+inline AppendLaunch append_launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
+                                  float* q_out, DeviceStatus* st, uint32_t key_pieces, uint32_t pieces_between) {
+    AppendLaunch l = {};
+    AppendArgs& a = l.a;
+    a.kv = kv;
+    a.b = b;
+    a.qkv = qkv;
+    a.q_out = q_out;
+    a.rotate = theta > 0.0;
+    a.log2_theta = a.rotate ? log2(theta) : 0.0;
+    a.heads = heads;
+    a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
+    a.rows = b.tokens >= 4u * 148u ? kMaxRows : 1u;  // four rows share their sines where there are CTAs enough
+    a.row_keys = b.max_q_len <= 1u;
+    a.pieces = heads * (kv.head_dim / 8u) + pieces_between + (a.row_keys ? key_pieces : 0u) + kv.kv_heads * kv.head_dim / 4u;
+    a.blocks = (a.pieces + 255u) / 256u;
+    // a thread for every piece, and for every channel pair
+    l.threads = (std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u) + 31u) / 32u * 32u;
+    a.st = st;
+    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
+    l.grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
+    a.key_ctas = static_cast<uint32_t>(keys);
+    return l;
+}
+cudaError_t launch_kv_append4(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
+                              float* q_out, DeviceStatus* st, cudaStream_t stream);
+
+}  // namespace nedo_gpu

@@ -251,11 +251,11 @@ cudaError_t launch_advance(DecodeIo* io, const int64_t* pick, uint32_t* ids, uin
 cudaError_t launch_silu_mul(float* gu, uint32_t f, const float* route, const DecodeIo* io, uint32_t shared_w,
                             uint32_t root_w, uint32_t suffix_w, cudaStream_t stream, bool pdl);
 
-// ---- paged KV cache (kv_append.cu, paged_attention.cu, block_select.cu) ----
+// ---- paged KV cache (kv_append.cu, kv_append4.cu, paged_attention.cu, block_select.cu) ----
 // Kernel-side views of nedo_gpu_kv_cache and nedo_gpu_kv_batch, checked by the host.
 constexpr uint32_t kF32 = 0;
 struct PagedKv {
-    uint32_t type = 0;       // kF32 or kF16
+    uint32_t type = 0;       // kF32, kF16 or kQ4_0 (paged_q4.cuh)
     uint32_t kv_heads = 0, head_dim = 0;
     uint32_t page_size = 0, page_shift = 0;
     uint32_t num_pages = 0;
@@ -271,6 +271,9 @@ struct PagedBatch {
 };
 cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
                              float* q_out, DeviceStatus* st, cudaStream_t stream);
+
+// The batch's rows out of the cache, [tokens][kv_heads][head_dim] in 32 bits.
+cudaError_t launch_kv_read(const PagedKv& kv, const PagedBatch& b, float* k, float* v, DeviceStatus* st, cudaStream_t stream);
 
 // One attention call: the plan (sizes of its launches and of its workspace) and its run.
 struct PagedAttention {
@@ -297,6 +300,22 @@ constexpr uint32_t kMaxPicks = 1024;       // pages a selection holds
 constexpr uint32_t kMaxSelectPages = 16384;  // pages a sequence may have for a selection
 cudaError_t launch_block_select(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* q, uint32_t picks,
                                 uint32_t* blocks, DeviceStatus* st, cudaStream_t stream);
+
+// ---- drafted tokens (verify_drafts.cu) ----
+// Kernel-side view of nedo_gpu_drafts, checked by the host.
+constexpr uint32_t kVerifyMaxRows = 256;  // of a sequence
+struct VerifyDrafts {
+    uint32_t seqs = 0, rows = 0, max_rows = 0, vocab = 0;
+    const uint32_t* row_start = nullptr;  // [seqs + 1]
+    const float* logits = nullptr;        // [rows][vocab]
+    const uint32_t* draft_ids = nullptr;  // [rows]
+    const float* draft_probs = nullptr;   // [rows][vocab] or null
+    const float* accept_u = nullptr;      // [rows]
+    const float* sample_u = nullptr;      // [seqs]
+};
+uint64_t verify_drafts_workspace(const VerifyDrafts& v);
+cudaError_t launch_verify_drafts(const VerifyDrafts& v, float temperature, uint32_t* accepted, uint32_t* ids, void* workspace,
+                                 DeviceStatus* st, cudaStream_t stream);
 
 // cuTensorMapEncodeTiled reached through the runtime's driver entry point
 // (null when the driver does not provide it).

@@ -1658,11 +1658,13 @@ int check_paged(const char* what, const nedo_gpu_kv_cache* c, const nedo_gpu_kv_
                 PagedBatch* pb) {
     const std::string w = std::string(what) + ": ";
     if (!c || !b) return fail(NEDO_GPU_ERR_ARG, w + "null pointer");
-    if (c->type != kF32 && c->type != kF16) return fail(NEDO_GPU_ERR_TYPE, w + "KV cache type not supported");
+    if (c->type != kF32 && c->type != kF16 && c->type != kQ4_0)
+        return fail(NEDO_GPU_ERR_TYPE, w + "KV cache type not supported");
     if (!heads || !c->kv_heads || heads % c->kv_heads) return fail(NEDO_GPU_ERR_ARG, w + "invalid GQA dimensions");
     if (heads > 4096u) return fail(NEDO_GPU_ERR_ARG, w + "more than 4096 heads");
     if (c->head_dim == 0 || c->head_dim > 256u || c->head_dim % 8u)
         return fail(NEDO_GPU_ERR_ARG, w + "head_dim must be a multiple of 8 in 8..256");
+    if (c->type == kQ4_0 && c->head_dim % 32u) return fail(NEDO_GPU_ERR_ALIGN, w + "Q4_0 head_dim not block aligned");
     if (c->page_size < 16u || c->page_size > 256u || (c->page_size & (c->page_size - 1u)))
         return fail(NEDO_GPU_ERR_ARG, w + "page_size must be 16, 32, 64, 128 or 256");
     // (512 GiB of keys at least; below it, a page and head is a signed TMA coordinate)
@@ -1773,6 +1775,24 @@ int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_bat
     return 0;
 }
 
+int nedo_gpu_kv_read_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, float* k_out_dev, float* v_out_dev,
+                         void* stream) {
+    PagedKv kv;
+    PagedBatch b;
+    if (int rc = check_paged("kv_read", cache, batch, cache ? cache->kv_heads : 1u, &kv, &b)) return rc;
+    if (!b.seqs || !b.tokens) return 0;
+    if (!k_out_dev || !v_out_dev) return fail(NEDO_GPU_ERR_ARG, "kv_read: null pointer");
+    if (!aligned16(k_out_dev) || !aligned16(v_out_dev))
+        return fail(NEDO_GPU_ERR_ARG, "kv_read: buffers must be 16-byte aligned");
+    const uint64_t bytes = static_cast<uint64_t>(b.tokens) * kv.kv_heads * kv.head_dim * sizeof(float);
+    if (overlap(k_out_dev, bytes, v_out_dev, bytes)) return fail(NEDO_GPU_ERR_ARG, "kv_read: k_out and v_out overlap");
+    DeviceState* s = nullptr;
+    if (int rc = get_state(&s)) return rc;
+    cudaError_t e = launch_kv_read(kv, b, k_out_dev, v_out_dev, s->status, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "kv_read launch");
+    return 0;
+}
+
 int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, uint32_t heads,
                                        uint32_t window, uint64_t* bytes) {
     if (!bytes) return fail(NEDO_GPU_ERR_ARG, "paged_attention: null pointer");
@@ -1832,6 +1852,75 @@ int nedo_gpu_block_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_
     if (a.b.seqs && a.b.tokens && !blocks_dev) return fail(NEDO_GPU_ERR_ARG, "block_attention: null pointer");
     if (!aligned4(blocks_dev)) return fail(NEDO_GPU_ERR_ARG, "block_attention: lists must be 4-byte aligned");
     return run_attention("block_attention", a, q_dev, out_dev, scale, workspace_dev, workspace_bytes, stream);
+}
+
+}  // extern "C"
+
+// ---- drafted tokens ----------------------------------------------------------
+namespace {
+
+int check_drafts(const nedo_gpu_drafts* d, VerifyDrafts* v) {
+    if (!d) return fail(NEDO_GPU_ERR_ARG, "verify_drafts: null pointer");
+    if (d->seqs > 0xFFFFFFu || d->rows > 0x7FFFFFFFu) return fail(NEDO_GPU_ERR_ARG, "verify_drafts: batch too large");
+    if (d->vocab == 0 || d->vocab > 0x7FFFFFFFu) return fail(NEDO_GPU_ERR_ARG, "verify_drafts: vocab must be in 1..2^31-1");
+    if (d->max_rows == 0 || d->max_rows > kVerifyMaxRows)
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: max_rows must be in 1.." + std::to_string(kVerifyMaxRows));
+    v->seqs = d->seqs;
+    v->rows = d->rows;
+    v->max_rows = d->max_rows;
+    v->vocab = d->vocab;
+    v->row_start = d->row_start;
+    v->logits = d->logits;
+    v->draft_ids = d->draft_ids;
+    v->draft_probs = d->draft_probs;
+    v->accept_u = d->accept_u;
+    v->sample_u = d->sample_u;
+    // the launch's grid (parts of a row are at least 4096 logits)
+    if (static_cast<uint64_t>(v->rows) * ((v->vocab + 4095ull) / 4096ull) > 0x7FFFFFFFull)
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: batch too large");
+    return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nedo_gpu_verify_drafts_workspace(const nedo_gpu_drafts* drafts, uint64_t* bytes) {
+    if (!bytes) return fail(NEDO_GPU_ERR_ARG, "verify_drafts: null pointer");
+    VerifyDrafts v;
+    if (int rc = check_drafts(drafts, &v)) return rc;
+    *bytes = v.seqs && v.rows ? verify_drafts_workspace(v) : 0u;
+    return 0;
+}
+
+int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature, uint32_t* accepted_dev, uint32_t* ids_dev,
+                               void* workspace_dev, uint64_t workspace_bytes, void* stream) {
+    VerifyDrafts v;
+    if (int rc = check_drafts(drafts, &v)) return rc;
+    if (!(temperature == 0.f || (temperature >= 1e-6f && temperature <= 1e6f)))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: temperature must be 0 (greedy) or in 1e-6..1e6");
+    if (!v.seqs || !v.rows) return 0;
+    const bool drawn = temperature != 0.f, several = v.max_rows > 1u;
+    if (!v.row_start || !v.logits || !accepted_dev || !ids_dev || (several && !v.draft_ids) ||
+        (drawn && (!v.sample_u || (several && !v.accept_u))))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: null pointer");
+    if (!aligned16(v.logits) || !aligned16(v.draft_probs) || !aligned16(workspace_dev))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: buffers must be 16-byte aligned");
+    if (!aligned4(v.row_start) || !aligned4(v.draft_ids) || !aligned4(v.accept_u) || !aligned4(v.sample_u) ||
+        !aligned4(accepted_dev) || !aligned4(ids_dev))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: lists must be 4-byte aligned");
+    const uint64_t list = static_cast<uint64_t>(v.rows) * sizeof(uint32_t);
+    if (several && overlap(ids_dev, list, v.draft_ids, list))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: ids and draft_ids overlap");
+    const uint64_t need = verify_drafts_workspace(v);
+    if (!workspace_dev || workspace_bytes < need)
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: workspace smaller than " + std::to_string(need) + " bytes");
+    DeviceState* s = nullptr;
+    if (int rc = get_state(&s)) return rc;
+    cudaError_t e = launch_verify_drafts(v, temperature, accepted_dev, ids_dev, workspace_dev, s->status,
+                                         static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e, "verify_drafts launch");
+    return 0;
 }
 
 }  // extern "C"

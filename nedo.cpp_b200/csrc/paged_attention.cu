@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
 }
 
 // Which kernel takes a part, and what its work items cost (for the plan).
-enum class Kernel { kFew, kFew16, kFew32, kMany, kMany64, kMany32, kTc };
+enum class Kernel { kFew, kFew16, kFew32, kFew4, kFew4x8, kFew4x16, kMany, kMany64, kMany32, kTc };
 struct Cost {
     uint32_t rows;       // query rows per tile
     uint32_t slots;      // work items that run at once on 148 SMs
@@ -169,6 +169,13 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
         case Kernel::kFew32: {
             const uint32_t slots = 148u * (hd <= 64u ? 4u : hd <= 128u ? 2u : 1u);
             return {kFewRows, slots, 2048u, 8.0 * hd * slots / 6500.0, 4000.0, 0.45};
+        }
+        case Kernel::kFew4:
+        case Kernel::kFew4x8:
+        case Kernel::kFew4x16: {  // 1.125 hd bytes per key
+            const uint32_t rows = k == Kernel::kFew4 ? 4u : k == Kernel::kFew4x8 ? 8u : 16u;
+            const uint32_t slots = 148u * (hd <= 128u ? 4u : 2u);
+            return {rows, slots, 2048u, 1.125 * hd * slots / 4000.0, 4000.0, 0.45};
         }
         default:  // kMany32: three products each way
             return {many32_rows(hd), 148u, 0u, hd <= 64u ? 24.0 : 48.0, 5000.0, 1.0};
@@ -231,7 +238,9 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 
 // The kernel of a part whose row tiles have up to `rows` rows.
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
-    if (kv.type != kF16) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
+    if (kv.type == kQ4_0)
+        return rows <= 4u ? Kernel::kFew4 : rows <= 8u || kv.head_dim > 128u ? Kernel::kFew4x8 : Kernel::kFew4x16;
+    if (kv.type == kF32) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
     if (rows <= kFewRows || (rows <= kFewMax && kv.head_dim > 128u)) return Kernel::kFew;
     if (rows <= kFewMax) return Kernel::kFew16;
     return kv.head_dim <= 128u ? Kernel::kTc : Kernel::kMany;
@@ -246,7 +255,8 @@ Kernel own_kernel(const PagedAttention& a) {
 }
 // The kernel of the sequences with few rows among others with many: mostly single tokens.
 Kernel few_kernel(const PagedAttention& a) { return kernel_for(a.kv, std::min(a.heads / a.kv.kv_heads, kFewMax)); }
-bool takes_few(Kernel k) { return k == Kernel::kFew || k == Kernel::kFew16 || k == Kernel::kFew32; }
+bool takes_few4(Kernel k) { return k == Kernel::kFew4 || k == Kernel::kFew4x8 || k == Kernel::kFew4x16; }
+bool takes_few(Kernel k) { return k == Kernel::kFew || k == Kernel::kFew16 || k == Kernel::kFew32 || takes_few4(k); }
 
 // A part on its kernel: `tiles` row tiles of up to max_rows rows, times KV heads and chunks.
 cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t max_rows, cudaStream_t stream) {
@@ -255,6 +265,9 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
         case Kernel::kFew: return launch_attention_few(a, kFewRows, items, stream);
         case Kernel::kFew16: return launch_attention_few(a, 2u * kFewRows, items, stream);
         case Kernel::kFew32: return launch_attention_few32(a, static_cast<uint32_t>(std::min<uint64_t>(max_rows, kFewRows)), items, stream);
+        case Kernel::kFew4: return launch_attention_few4(a, 4u, items, stream);
+        case Kernel::kFew4x8: return launch_attention_few4(a, 8u, items, stream);
+        case Kernel::kFew4x16: return launch_attention_few4(a, 16u, items, stream);
         case Kernel::kMany: return launch_attention_many(a, 128u, tiles, stream);
         case Kernel::kMany64: return launch_attention_many(a, 64u, tiles, stream);
         case Kernel::kTc: return launch_attention_tc(a, tiles, stream);

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "paged.cuh"
+#include "paged_q4.cuh"
 
 namespace nedo_gpu {
 
@@ -126,7 +127,7 @@ __device__ __forceinline__ void checked_list(const uint32_t* __restrict__ l, uin
     }
 }
 
-// The sums of up to kAgain query rows over F16 keys, formed by one warp key by key in fp32.  The
+// The sums of up to kAgain query rows over F16 (Q4: Q4_0) keys, formed by one warp key by key in fp32.  The
 // tensor-core kernels multiply with factors split in two halves, and an infinite key or value times
 // halves of different sign, or one that is zero, is NaN where the whole factor gives infinity (or,
 // for a score of -infinity, no weight at all).  A value that is not finite also reaches the rows of
@@ -161,6 +162,7 @@ __device__ __forceinline__ uint32_t take_rows(uint32_t* set, uint32_t* n) {
 // Rows rows & 255, ... (+ `first`); keys `from`, from + 1, ... below `to` in steps of 16 that are
 // `stride` apart (from a multiple of 16 where stride is not 16): positions, or places in the page
 // list (`list`).
+template <bool Q4 = false>
 static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t s, uint32_t kh, const uint32_t* list,
                                                     const TileRows& tile, uint32_t first, uint32_t rows, uint32_t from,
                                                     uint32_t to, uint32_t stride, RowSums* sums) {
@@ -193,7 +195,9 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
                 const uint32_t page = load_page(a.b, a.kv, s, lp, a.st);
                 if (page != kNone) {
                     pos = x;
-                    at = ((static_cast<size_t>(page) * a.kv.kv_heads + kh) * a.kv.page_size + (j & in_page)) * hd;
+                    at = static_cast<size_t>(page) * a.kv.kv_heads + kh;
+                    if constexpr (Q4) at *= q4_head_bytes(a.kv);  // (of the page, in bytes)
+                    else at = (at * a.kv.page_size + (j & in_page)) * hd;
                 }
             }
         }
@@ -204,8 +208,16 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
         if (pos != kNone)
 #pragma unroll 2
             for (uint32_t d = 0; d < hd; d += 8u) {
-                const uint4 x = *reinterpret_cast<const uint4*>(k + at + d);
-                const __half2* h = reinterpret_cast<const __half2*>(&x);
+                __half2 h[4];
+                if constexpr (Q4) {
+                    const uint8_t* head = static_cast<const uint8_t*>(a.kv.k) + at;
+                    q4_pairs(*reinterpret_cast<const uint32_t*>(head + (j & in_page) * (hd / 2u) + (d >> 3) * 4u), h);
+                    const __half2 s = __half2half2(q4_scale(a.kv, head, j & in_page, d));
+#pragma unroll
+                    for (uint32_t e = 0; e < 4u; ++e) h[e] = __hmul2(h[e], s);
+                } else {
+                    *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(k + at + d);
+                }
 #pragma unroll
                 for (uint32_t u = 0; u < kAgain; ++u)
 #pragma unroll
@@ -235,10 +247,15 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
             float x[2][8];
 #pragma unroll
             for (uint32_t z = 0; z < 2u; ++z) {
-                const __half* row = v + __shfl_sync(0xFFFFFFFFu, static_cast<unsigned long long>(at), e + z) + lane;
+                const size_t from_at = __shfl_sync(0xFFFFFFFFu, static_cast<unsigned long long>(at), e + z);
+                const uint32_t slot = __shfl_sync(0xFFFFFFFFu, j, e + z) & in_page;
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i)
-                    x[z][i] = lane + 32u * i < hd && (any >> (e + z) & 1u) ? __half2float(row[32u * i]) : 0.f;
+                for (uint32_t i = 0; i < 8u; ++i) {
+                    x[z][i] = 0.f;
+                    if (lane + 32u * i >= hd || !(any >> (e + z) & 1u)) continue;
+                    if constexpr (Q4) x[z][i] = q4_value(a.kv, static_cast<const uint8_t*>(a.kv.v) + from_at, slot, lane + 32u * i);
+                    else x[z][i] = __half2float(v[from_at + lane + 32u * i]);
+                }
             }
 #pragma unroll
             for (uint32_t z = 0; z < 2u; ++z)
@@ -496,9 +513,11 @@ cudaError_t launch_items(const AttnArgs& a, void (*kernel)(Args...), uint64_t it
 
 // The few-rows kernels: F16 caches on the tensor cores, tiles of `rows` 8 or (heads of up to
 // 128 channels) 16 query rows (paged_attention_few.cu), F32 caches on the CUDA cores, tiles of
-// 8 (paged_attention_few32.cu).
+// 8 (paged_attention_few32.cu); Q4_0 caches on the tensor cores, tiles of 4, 8 or (heads of up to 128
+// channels) 16 (paged_attention_few4.cu).
 cudaError_t launch_attention_few(const AttnArgs& a, uint32_t rows, uint64_t items, cudaStream_t stream);
 cudaError_t launch_attention_few32(const AttnArgs& a, uint32_t max_rows, uint64_t items, cudaStream_t stream);
+cudaError_t launch_attention_few4(const AttnArgs& a, uint32_t rows, uint64_t items, cudaStream_t stream);
 // Tiles of `rows` 64 or 128 rows on the tensor cores (paged_attention_many.cu): F16 caches, heads
 // above 128.
 cudaError_t launch_attention_many(const AttnArgs& a, uint32_t rows, uint64_t tiles, cudaStream_t stream);

@@ -70,6 +70,9 @@ EXPORTS = (
     "nedo_gpu_block_select_dev",
     "nedo_gpu_block_attention_workspace",
     "nedo_gpu_block_attention_dev",
+    "nedo_gpu_kv_read_dev",
+    "nedo_gpu_verify_drafts_workspace",
+    "nedo_gpu_verify_drafts_dev",
 )
 
 
@@ -113,6 +116,13 @@ class KvBatch(ctypes.Structure):
                                                                     ("q_start", "kv_len", "page_table")]
 
 
+class Drafts(ctypes.Structure):
+    """nedo_gpu_drafts: logits, drafted tokens and random numbers of a batch (device addresses)."""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("seqs", "rows", "max_rows", "vocab")] + [
+        (n, ctypes.c_void_p) for n in ("row_start", "logits", "draft_ids", "draft_probs", "accept_u", "sample_u")]
+
+
+_draftsp = ctypes.POINTER(Drafts)
 _cachep, _batchp = ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch)
 
 _SIGNATURES = {
@@ -155,6 +165,9 @@ _SIGNATURES = {
     "nedo_gpu_block_attention_workspace": ([_cachep, _batchp, _u32, _u32, _u64p], _i32),
     "nedo_gpu_block_attention_dev": ([_cachep, _batchp, _u32, _vp, _vp, _u32, _vp, ctypes.c_float, _vp, _u64, _vp],
                                      _i32),
+    "nedo_gpu_kv_read_dev": ([_cachep, _batchp, _vp, _vp, _vp], _i32),
+    "nedo_gpu_verify_drafts_workspace": ([_draftsp, _u64p], _i32),
+    "nedo_gpu_verify_drafts_dev": ([_draftsp, ctypes.c_float, _vp, _vp, _vp, _u64, _vp], _i32),
 }
 
 
@@ -305,6 +318,10 @@ class Library:
         """Rotate the q|k|v rows of a batch to their positions; keys and values into the cache."""
         self._check(self.lib.nedo_gpu_kv_append_dev(cache, batch, heads, qkv_ptr, rope_theta, q_out_ptr, stream))
 
+    def kv_read_dev(self, cache: KvCache, batch: KvBatch, k_ptr, v_ptr, stream=0) -> None:
+        """The keys and values that the cache holds for a batch's token rows, as fp32."""
+        self._check(self.lib.nedo_gpu_kv_read_dev(cache, batch, k_ptr, v_ptr, stream))
+
     def paged_attention_workspace(self, cache: KvCache, batch: KvBatch, heads, window=0) -> int:
         """Bytes of device workspace that paged_attention_dev needs for these sizes."""
         n = _u64(0)
@@ -332,6 +349,19 @@ class Library:
         """Attention of every query row over the pages listed for it (block_select_dev's layout)."""
         self._check(self.lib.nedo_gpu_block_attention_dev(cache, batch, heads, q_ptr, blocks_ptr, picks, out_ptr,
                                                           scale, workspace_ptr, workspace_bytes, stream))
+
+    # ------------------------------------------------------ drafted tokens
+    def verify_drafts_workspace(self, drafts: Drafts) -> int:
+        """Bytes of device workspace that verify_drafts_dev needs for these sizes."""
+        n = _u64(0)
+        self._check(self.lib.nedo_gpu_verify_drafts_workspace(drafts, n))
+        return n.value
+
+    def verify_drafts_dev(self, drafts: Drafts, temperature, accepted_ptr, ids_ptr, workspace_ptr, workspace_bytes,
+                          stream=0) -> None:
+        """How many of every sequence's drafts stand, and they with the token that follows (temperature 0: greedy)."""
+        self._check(self.lib.nedo_gpu_verify_drafts_dev(drafts, temperature, accepted_ptr, ids_ptr, workspace_ptr,
+                                                        workspace_bytes, stream))
 
     def status(self, stream=0) -> None:
         self._check(self.lib.nedo_gpu_status(stream))
