@@ -238,7 +238,7 @@ uint64_t own_tiles(const PagedAttention& a, uint32_t rows) {
 
 // The kernel of a part whose row tiles have up to `rows` rows.
 Kernel kernel_for(const PagedKv& kv, uint64_t rows) {
-    if (kv.type == kQ4_0)
+    if (kv.type == kQ4_0 && rows <= kFewMax)
         return rows <= 4u ? Kernel::kFew4 : rows <= 8u || kv.head_dim > 128u ? Kernel::kFew4x8 : Kernel::kFew4x16;
     if (kv.type == kF32) return rows <= kFewMax ? Kernel::kFew32 : Kernel::kMany32;
     if (rows <= kFewRows || (rows <= kFewMax && kv.head_dim > 128u)) return Kernel::kFew;
@@ -279,7 +279,7 @@ cudaError_t launch_part(Kernel k, const AttnArgs& a, uint64_t tiles, uint64_t ma
 
 bool plan_paged_attention(PagedAttention* a) {
     // a part's plan with tiles of 64 rows or not, whichever should take less time
-    const bool choice = a->kv.type == kF16 && a->kv.head_dim > 128u;
+    const bool choice = a->kv.type != kF32 && a->kv.head_dim > 128u;
     auto faster = [choice](bool* low, auto plan) {
         Chunks best = plan();
         if (!choice) return best;

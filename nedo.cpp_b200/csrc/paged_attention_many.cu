@@ -1,4 +1,4 @@
-// paged_attention_many.cu -- attention over a paged F16 cache for tiles of 128 or 64 query rows of
+// paged_attention_many.cu -- attention over a paged F16 or Q4_0 cache for tiles of 128 or 64 query rows of
 // heads above 128 channels (prompts, and the tokens of a whole batch over their shared
 // prefix): bound by the tensor cores.  (Up to 128 channels a tile's sums fit into the other
 // kernel's half of TMEM.)
@@ -18,6 +18,9 @@
 // read the keys twice as often, take 1072.  Where there are few tiles 64 rows reach more SMs: 8 query
 // and 2 KV heads, 300 tokens 26 us (128 rows: 30), 37 sequences of 32 tokens over 500 keys 51 us (68).
 // The plan takes the height that it expects to end first.
+//
+// Of a Q4_0 cache (paged_q4.cuh) a thread copies the same blocks of 32 channels of every tile, and
+// makes fp16 numbers of its own copies before the barrier that the tile waits for anyway.
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
@@ -32,18 +35,25 @@ constexpr uint32_t kRowBytes = HD * 2u;
 constexpr uint32_t kTileBytes = kKeys * kRowBytes;       // keys or values of a tile
 constexpr uint32_t kStageBytes = 2u * kTileBytes;
 
-template <uint32_t ROWS>
+template <uint32_t ROWS, bool Q4>
 struct Many {
     static constexpr uint32_t kThreads = 2u * ROWS;          // a warp for 16 rows
     static constexpr uint32_t kQBytes = ROWS * kRowBytes;    // one half of the queries
-    static constexpr uint32_t kSmem = 2u * kQBytes + kStages * kStageBytes;
+    // Q4_0: a tile's blocks as they come, 16 bytes of numbers and two keys' scales each
+    static constexpr uint32_t kRawBlocks = 2u * kKeys * (HD / 32u), kRawBytes = kRawBlocks * 20u;
+    static constexpr uint32_t kSmem = 2u * kQBytes + kStages * (kStageBytes + (Q4 ? kRawBytes : 0u));
 };
+
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 
 __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) { return r * kRowBytes + ((c ^ (r & 7u)) << 4); }
 
-template <uint32_t ROWS>
+template <uint32_t ROWS, bool Q4>
 __device__ __forceinline__ void attention_many(const AttnArgs& a) {
-    constexpr uint32_t kThreads = Many<ROWS>::kThreads, kQBytes = Many<ROWS>::kQBytes, kSmem = Many<ROWS>::kSmem;
+    using M = Many<ROWS, Q4>;
+    constexpr uint32_t kThreads = M::kThreads, kQBytes = M::kQBytes, kSmem = M::kSmem;
     extern __shared__ __align__(128) uint8_t sm[];
     __shared__ uint32_t row_tok[ROWS], row_head[ROWS];
     __shared__ int row_pos[ROWS];
@@ -141,6 +151,14 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         }
     };
     __shared__ uint32_t tile_gap[kStages];  // a page of the tile is no page
+    // Q4_0: the thread's blocks x of a tile's keys, and of its values behind them
+    constexpr uint32_t kMine = M::kRawBlocks / 2u / kThreads;
+    auto raw_at = [&](uint32_t i, uint32_t x) { return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + (x * kThreads + tid) * 16u; };
+    auto raw_scale_at = [&](uint32_t i, uint32_t x) {
+        return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + M::kRawBlocks * 16u + (x * kThreads + tid) * 4u;
+    };
+    const uint32_t my_key = (tid & 7u) + 8u * ((tid >> 4) & 3u);
+    auto block_of = [&](uint32_t x) { return ((tid >> 3) & 1u) + 2u * ((x * kThreads + tid) >> 6); };
     auto fetch = [&](uint32_t i) {
         if (i < ntiles) {
             const uint32_t dst = ring + (i % kStages) * kStageBytes;
@@ -154,7 +172,23 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
                 gap |= pages[u] == kNone && j < ke && j + 16u > kb;
             }
             if (tid == 0) tile_gap[i % kStages] = gap;
-            if (ch < chunks16) {
+            if constexpr (Q4) {
+                const uint32_t j = j0 + i * kKeys + my_key;
+                uint32_t page = pages[0];
+#pragma unroll
+                for (uint32_t u = 1; u < kGroups; ++u) page = my_key >= 16u * u ? pages[u] : page;
+                const bool there = page != kNone && j >= kb && j < ke;
+                const uint32_t slot = there ? j & (a.kv.page_size - 1u) : 0u, bytes = there ? 16u : 0u;
+                const size_t o = ((there ? static_cast<size_t>(page) : 0u) * a.kv.kv_heads + kh) * q4_head_bytes(a.kv);
+#pragma unroll
+                for (uint32_t x = 0; x < 2u * kMine; ++x) {
+                    const uint32_t b = block_of(x % kMine);
+                    if (b * 32u >= hd) continue;
+                    const uint8_t* from = static_cast<const uint8_t*>(x < kMine ? a.kv.k : a.kv.v) + o;
+                    cp_async16(q_addr + raw_at(i, x), from + slot * (hd / 2u) + b * 16u, bytes);
+                    cp_async4(q_addr + raw_scale_at(i, x), from + q4_scales_at(a.kv) + (b * a.kv.page_size + (slot & ~1u)) * 2u, bytes / 4u);
+                }
+            } else if (ch < chunks16) {
 #pragma unroll
                 for (uint32_t x = 0; x < kPer; ++x) {
                     const uint32_t r = tid / (HD / 8u) + x * kRowsAtOnce;
@@ -228,6 +262,24 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         fetch(i + 1u);
         look_up(i + 2u);
         cp_wait<1>();
+        if constexpr (Q4) {  // the thread's own blocks (of keys that are not there: numbers and scales zero)
+#pragma unroll
+            for (uint32_t x = 0; x < 2u * kMine; ++x) {
+                const uint32_t b = block_of(x % kMine);
+                if (b * 32u >= hd) continue;
+                const uint4 w = *reinterpret_cast<const uint4*>(sm + raw_at(i, x));
+                const __half2 d = __half2half2(*reinterpret_cast<const __half*>(sm + raw_scale_at(i, x) + (my_key & 1u) * 2u));
+                uint8_t* const to = sm + 2u * kQBytes + (i % kStages) * kStageBytes + (x < kMine ? 0u : kTileBytes);
+                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (uint32_t u = 0; u < 4u; ++u) {
+                    __half2 h[4];
+                    q4_pairs(words[u], h);
+                    *reinterpret_cast<uint4*>(to + at(my_key, b * 4u + u)) =
+                        make_uint4(pack(__hmul2(h[0], d)), pack(__hmul2(h[1], d)), pack(__hmul2(h[2], d)), pack(__hmul2(h[3], d)));
+                }
+            }
+        }
         __syncthreads();
         const uint32_t j = j0 + i * kKeys;
         if (j < we && j + kKeys > wb) {
@@ -369,7 +421,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     while (again != 0u) {
         uint32_t n, rows = take_rows(&again, &n);
         RowSums x;
-        rows_key_by_key(a, s, kh, nullptr, {row_tok, row_head, row_pos}, warp * 16u, rows, kb, ke, 16u, &x);
+        rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, warp * 16u, rows, kb, ke, 16u, &x);
         for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
             const uint32_t r = warp * 16u + (rows & 255u);
             const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];
@@ -381,22 +433,23 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     }
 }
 
-template <uint32_t ROWS>
-__global__ void __launch_bounds__(Many<ROWS>::kThreads, 1) attention_many_kernel(const __grid_constant__ AttnArgs a) {
-    attention_many<ROWS>(a);
+template <uint32_t ROWS, bool Q4>
+__global__ void __launch_bounds__(Many<ROWS, Q4>::kThreads, 1) attention_many_kernel(const __grid_constant__ AttnArgs a) {
+    attention_many<ROWS, Q4>(a);
     end_after_previous(a);
 }
 
-template <uint32_t ROWS>
+template <uint32_t ROWS, bool Q4>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    return launch_items(a, attention_many_kernel<ROWS>, items, Many<ROWS>::kThreads, Many<ROWS>::kSmem, stream, a);
+    return launch_items(a, attention_many_kernel<ROWS, Q4>, items, Many<ROWS, Q4>::kThreads, Many<ROWS, Q4>::kSmem, stream, a);
 }
 
 }  // namespace
 
 cudaError_t launch_attention_many(const AttnArgs& a, uint32_t rows, uint64_t tiles, cudaStream_t stream) {
     const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
-    return rows <= 64u ? launch<64>(a, items, stream) : launch<128>(a, items, stream);
+    if (a.kv.type == kQ4_0) return rows <= 64u ? launch<64, true>(a, items, stream) : launch<128, true>(a, items, stream);
+    return rows <= 64u ? launch<64, false>(a, items, stream) : launch<128, false>(a, items, stream);
 }
 
 }  // namespace nedo_gpu

@@ -1,4 +1,4 @@
-// paged_attention_tc.cu -- attention over a paged F16 cache for tiles of 128 query rows on
+// paged_attention_tc.cu -- attention over a paged F16 or Q4_0 cache for tiles of 128 query rows on
 // the 5th-generation tensor cores (prompts, the tokens of a whole batch over their shared
 // prefix, groups of more than 16 heads), heads of up to 128 channels.
 //
@@ -22,6 +22,11 @@
 // TMEM, 512 columns: three S/P tiles and one O tile.  Two of them with the queries' halves in TMEM
 // as well (and six ring slots) took 130 us where this took 126.
 // Registers: 56 for the softmax, 112 for the sums, 56 for the others.
+//
+// Q4_0 caches (paged_q4.cuh).  Three warps make the fp16 tiles that TMA brings in otherwise: bulk copies,
+// two half tiles ahead, take the pages' numbers and scales as they are next to the ring (a box is one run of
+// numbers and one of scales for each block), and the warps write the products where the swizzled copy would have
+// put them, a block of 32 channels to a lane.
 //
 // What bounds it: 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two
 // sequences over 4096 and 2550 keys, window 2048: 104 us, 825 TFLOP/s of fp16 MMAs (two for each
@@ -49,11 +54,17 @@ constexpr uint32_t kTmem = 0u;          // where an allocation of the whole TMEM
 constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
 constexpr uint32_t kSumWarp = kSoftmax / 32u, kLoadWarp = kSumWarp + kSums / 32u, kMmaWarp = kLoadWarp + 1u;
 
-template <uint32_t HD>
+constexpr uint32_t kRawSlots = 2;       // Q4_0: half tiles as the pages hold them
+constexpr uint32_t kMakers = 3;         // warps that make fp16 tiles of them
+
+template <uint32_t HD, bool Q4>
 struct Tc {
     static constexpr uint32_t kBlocks = HD / 64u;
     static constexpr uint32_t kTile = kBlocks * kBlock;   // a ring slot
-    static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u;  // the queries' high and low halves, the ring
+    static constexpr uint32_t kRawScales = kKeys * HD / 2u;                   // where a raw slot's scales begin, [block][key]
+    static constexpr uint32_t kRaw = kRawScales + HD / 32u * kKeys * 2u;
+    // the queries' high and low halves, the ring
+    static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u + (Q4 ? kRawSlots * kRaw : 0u);
 };
 
 struct TcMaps {
@@ -176,15 +187,24 @@ __device__ __forceinline__ uint32_t at(uint32_t r, uint32_t c) {
     return (c >> 3) * kBlock + r * 128u + (((c & 7u) ^ (r & 7u)) << 4);
 }
 
-template <uint32_t HD>
+// A run of 16-byte pieces into shared memory, counted by `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+template <uint32_t HD, bool Q4>
 __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs& a, uint32_t box_shift) {
-    using T = Tc<HD>;
+    using T = Tc<HD, Q4>;
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
     __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
     __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
     __shared__ uint32_t found[2], tmem_slot, gaps[8], again[kRows / 32u];
+    __shared__ uint64_t raw_full[kRawSlots], raw_empty[kRawSlots];  // Q4_0
+    __shared__ uint32_t raw_there[kRawSlots];
     const uint32_t s0 = (smem_addr(sm_raw) + 1023u) & ~1023u;
     uint8_t* const sm = sm_raw + (s0 - smem_addr(sm_raw));
     const uint32_t ring = s0 + 2u * T::kTile;
@@ -198,9 +218,14 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     if (tid == 0u) asm volatile("griddepcontrol.launch_dependents;");
     if (tid == 32u * kLoadWarp) {
         for (uint32_t i = 0; i < kSlots; ++i) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], Q4 ? kMakers : 1u);
             mbar_init(&empty[i], 1);
         }
+        if constexpr (Q4)
+            for (uint32_t i = 0; i < kRawSlots; ++i) {
+                mbar_init(&raw_full[i], 1);
+                mbar_init(&raw_empty[i], kMakers);
+            }
         mbar_init(&cut, 1);
         for (uint32_t i = 0; i < kRows / 32u; ++i) again[i] = 0u;
         for (uint32_t i = 0; i < kBuffers; ++i) {
@@ -318,9 +343,102 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     auto k_at = [&](uint32_t i) { return i + (i >= kBuffers ? i - kBuffers + 1u : 0u); };
     auto v_at = [&](uint32_t i) { return i + min(ntiles, i + kBuffers); };
 
+    // Q4_0: the tiles in ring order, keys and values in turn, by three warps; the first of them also sends
+    // for the numbers and scales, kRawSlots half tiles ahead of the one that is being made.
+    auto make_tiles = [&]() {
+        const uint32_t me = warp == kLoadWarp ? 0u : warp - kMmaWarp;
+        const uint32_t raw = ring + kSlots * T::kTile, blocks = hd >> 5, all = 2u * ntiles;
+        const uint32_t head_bytes = q4_head_bytes(a.kv), scales_at = q4_scales_at(a.kv);
+        // the n-th half tile: the keys of the first tiles, then values and keys in turn, values at the end
+        auto tile_at = [&](uint32_t n, bool* values) -> uint32_t {
+            const uint32_t lead = min(kBuffers, ntiles);
+            if (n < lead) return *values = false, n;
+            const uint32_t x = n - lead, pairs = 2u * (ntiles - lead);
+            *values = x >= pairs || (x & 1u) == 0u;
+            return x >= pairs ? x - pairs + (ntiles - lead) : (x & 1u) == 0u ? x >> 1 : lead + (x >> 1);
+        };
+        bool ok = true;
+        uint32_t sent = 0, next = page0;
+        auto send = [&]() {
+            bool values;
+            const uint32_t n = sent, i = tile_at(n, &values), rs = n % kRawSlots;
+            const uint32_t pages = checked(i, next);
+            bool v;
+            next = n + 1u < all ? look_up(tile_at(n + 1u, &v)) : kNone;
+            if (ok && n >= kRawSlots) ok = warp_wait(&raw_empty[rs], ((n / kRawSlots) - 1u) & 1u, a.st, 73u);
+            if (!ok) return;
+            const uint32_t j = j0 + i * kKeys, there = __ballot_sync(0xFFFFFFFFu, pages != kNone);
+            const uint32_t want = __ballot_sync(0xFFFFFFFFu, wanted(i));
+            if (lane == 0u) {
+                if (!values) gaps[i & 7u] = want & ~there;
+                raw_there[rs] = there;
+                const uint32_t bytes = __popc(there) * box_rows * (hd / 2u + blocks * 2u);
+                if (bytes != 0u) mbar_arrive_expect_tx(&raw_full[rs], bytes);
+                else mbar_arrive(&raw_full[rs]);
+            }
+            __syncwarp();
+            if (pages != kNone) {
+                const uint32_t slot_row = (j + lane * box_rows) & (a.kv.page_size - 1u);
+                const uint8_t* head = static_cast<const uint8_t*>(values ? a.kv.v : a.kv.k) +
+                                      (static_cast<size_t>(pages) * a.kv.kv_heads + kh) * head_bytes;
+                const uint32_t dst = raw + rs * T::kRaw;
+                bulk_load(dst + lane * box_rows * (hd / 2u), head + slot_row * (hd / 2u), box_rows * (hd / 2u), &raw_full[rs]);
+                for (uint32_t b = 0; b < blocks; ++b)
+                    bulk_load(dst + T::kRawScales + (b * kKeys + lane * box_rows) * 2u,
+                              head + scales_at + (b * a.kv.page_size + slot_row) * 2u, box_rows * 2u, &raw_full[rs]);
+            }
+            sent = n + 1u;
+        };
+        if (me == 0u)
+            while (sent < min(kRawSlots, all) && ok) send();
+        // a lane: one block of one key of every 32 / kPer; eight neighbouring lanes write to different banks
+        constexpr uint32_t kPer = HD / 32u, kUnits = kKeys * kPer / 32u, kStepKeys = 32u / kPer;
+        const uint32_t block = HD == 128u ? ((lane >> 2) & 1u) + 2u * (lane >> 4) : (lane >> 2) & 1u;
+        const uint32_t key0 = HD == 128u ? (lane & 3u) + 4u * ((lane >> 3) & 1u) : (lane & 3u) + 4u * (lane >> 3);
+        for (uint32_t n = 0; n < all && ok; ++n) {
+            bool values;
+            const uint32_t i = tile_at(n, &values), slot = n % kSlots, rs = n % kRawSlots, j = j0 + i * kKeys;
+            ok = warp_wait(&raw_full[rs], (n / kRawSlots) & 1u, a.st, 74u) &&
+                 (n < kSlots || warp_wait(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u));
+            if (!ok) break;
+            const uint32_t there = *reinterpret_cast<volatile uint32_t*>(&raw_there[rs]);
+            const uint8_t* const from = sm + (raw - s0) + rs * T::kRaw;
+            uint8_t* const to = sm + (ring - s0) + slot * T::kTile;
+#pragma unroll 2
+            for (uint32_t u = (me + n) % kMakers; u < kUnits; u += kMakers) {
+                const uint32_t r = u * kStepKeys + key0;
+                const bool in = block < blocks && (there >> (r >> box_shift) & 1u) && j + r >= kb && j + r < ke;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                __half2 d = __half2half2(__ushort_as_half(0));
+                if (in) {
+                    w = *reinterpret_cast<const uint4*>(from + r * (hd / 2u) + block * 16u);
+                    d = __half2half2(*reinterpret_cast<const __half*>(from + T::kRawScales + (block * kKeys + r) * 2u));
+                }
+                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (uint32_t x = 0; x < 4u; ++x) {
+                    __half2 h[4];
+                    q4_pairs(words[x], h);
+                    *reinterpret_cast<uint4*>(to + at(r, block * 4u + x)) =
+                        make_uint4(pack(__hmul2(h[0], d)), pack(__hmul2(h[1], d)), pack(__hmul2(h[2], d)), pack(__hmul2(h[3], d)));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            warp_arrive(&raw_empty[rs]);
+            warp_arrive(&full[slot]);
+            if (me == 0u && sent < all) send();
+        }
+        // the last copies have landed before the CTA ends
+        if (me == 0u)
+            for (uint32_t n = sent > kRawSlots ? sent - kRawSlots : 0u; n < sent; ++n)
+                mbar_wait_bounded(&raw_full[n % kRawSlots], (n / kRawSlots) & 1u, a.st, 63u);
+    };
+
     if (warp >= kLoadWarp) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        if (warp == kLoadWarp) {
+        if (Q4 && warp != kMmaWarp) {
+            if constexpr (Q4) make_tiles();
+        } else if (warp == kLoadWarp) {
             // ---- loads
             bool ok = true;
             uint32_t issued = 0, cuts = 0;
@@ -650,7 +768,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 while (set != 0u) {
                     uint32_t n, rows = take_rows(&set, &n);
                     RowSums x;
-                    rows_key_by_key(a, s, kh, nullptr, {row_tok, row_head, row_pos}, first, rows, kb, ke, 16u, &x);
+                    rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, first, rows, kb, ke, 16u, &x);
                     for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
                         const uint32_t rr = first + (rows & 255u);
                         const float f = !a.direct ? 1.f : x.l[u] == 0.f ? 0.f : 1.f / x.l[u];
@@ -685,10 +803,10 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     }
 }
 
-template <uint32_t HD>
+template <uint32_t HD, bool Q4>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_shift) {
-    attention_tc<HD>(maps, a, box_shift);
+    attention_tc<HD, Q4>(maps, a, box_shift);
     end_after_previous(a);
 }
 
@@ -703,13 +821,13 @@ bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <uint32_t HD>
+template <uint32_t HD, bool Q4>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    TcMaps maps;
+    TcMaps maps = {};
     const uint32_t box_rows = std::min(a.kv.page_size, kKeys);
-    if (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows))
+    if (!Q4 && (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows)))
         return cudaErrorInvalidValue;
-    return launch_items(a, attention_tc_kernel<HD>, items, kThreads, Tc<HD>::kSmem, stream, maps, a,
+    return launch_items(a, attention_tc_kernel<HD, Q4>, items, kThreads, Tc<HD, Q4>::kSmem, stream, maps, a,
                         std::min(a.kv.page_shift, 7u));
 }
 
@@ -717,7 +835,8 @@ cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
 
 cudaError_t launch_attention_tc(const AttnArgs& a, uint64_t tiles, cudaStream_t stream) {
     const uint64_t items = tiles * a.kv.kv_heads * a.chunks;
-    return a.kv.head_dim <= 64u ? launch<64>(a, items, stream) : launch<128>(a, items, stream);
+    if (a.kv.type == kQ4_0) return a.kv.head_dim <= 64u ? launch<64, true>(a, items, stream) : launch<128, true>(a, items, stream);
+    return a.kv.head_dim <= 64u ? launch<64, false>(a, items, stream) : launch<128, false>(a, items, stream);
 }
 
 }  // namespace nedo_gpu
