@@ -44,22 +44,24 @@ namespace {
 
 constexpr uint32_t kRows = kTcRows;     // 128
 constexpr uint32_t kKeys = 128;         // keys per tile
-constexpr uint32_t kSlots = 4;          // ring slots: the keys or the values of one tile
 constexpr uint32_t kSoftmax = 512;      // softmax threads: two to a row, for the even and the odd tiles
 constexpr uint32_t kSums = 256;         // threads of the running sums: two to a row
-constexpr uint32_t kThreads = kSoftmax + kSums + 128;
 constexpr uint32_t kBuffers = 3;        // S/P tiles
 constexpr uint32_t kOColumn = kBuffers * 128u;  // TMEM columns of O
 constexpr uint32_t kTmem = 0u;          // where an allocation of the whole TMEM lies
 constexpr uint32_t kBlock = kRows * 128u;  // bytes of 64 channels of a tile: rows of 128 bytes
 constexpr uint32_t kSumWarp = kSoftmax / 32u, kLoadWarp = kSumWarp + kSums / 32u, kMmaWarp = kLoadWarp + 1u;
 
-constexpr uint32_t kRawSlots = 2;       // Q4_0: half tiles as the pages hold them
-constexpr uint32_t kMakers = 3;         // warps that make fp16 tiles of them
+// Q4_0: half tiles as the pages hold them, and warps that make fp16 tiles of them, in turn by two groups
+constexpr uint32_t kRawSlots = 4;
+constexpr uint32_t kMakers = 3, kMakerGroups = 2, kFirstMaker = kMmaWarp + 1u;
 
 template <uint32_t HD, bool Q4>
 struct Tc {
+    static constexpr uint32_t kThreads = kSoftmax + kSums + (Q4 ? 256u : 128u);
+    static constexpr uint32_t kSumRegs = Q4 ? 104u : 112u, kOtherRegs = Q4 ? 40u : 56u;
     static constexpr uint32_t kBlocks = HD / 64u;
+    static constexpr uint32_t kSlots = Q4 ? 3u : 4u;      // ring slots: the keys or the values of one tile
     static constexpr uint32_t kTile = kBlocks * kBlock;   // a ring slot
     static constexpr uint32_t kRawScales = kKeys * HD / 2u;                   // where a raw slot's scales begin, [block][key]
     static constexpr uint32_t kRaw = kRawScales + HD / 32u * kKeys * 2u;
@@ -197,11 +199,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <uint32_t HD, bool Q4>
 __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs& a, uint32_t box_shift) {
     using T = Tc<HD, Q4>;
+    constexpr uint32_t kSlots = T::kSlots;
     extern __shared__ uint8_t sm_raw[];
     __shared__ uint32_t row_tok[kRows], row_head[kRows];
     __shared__ int row_pos[kRows];
     __shared__ float row_unscale[kRows], side_max[2][4][kRows], tile_ref[2 * kBuffers][kRows], sum_l[4][kRows], sum_m[2][kRows];
-    __shared__ uint64_t full[kSlots], empty[kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
+    __shared__ uint64_t full[T::kSlots], empty[T::kSlots], cut, s_full[kBuffers], p_full[kBuffers], o_full, o_empty, q_full, done;
     __shared__ uint32_t found[2], tmem_slot, gaps[8], again[kRows / 32u];
     __shared__ uint64_t raw_full[kRawSlots], raw_empty[kRawSlots];  // Q4_0
     __shared__ uint32_t raw_there[kRawSlots];
@@ -343,32 +346,27 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
     auto k_at = [&](uint32_t i) { return i + (i >= kBuffers ? i - kBuffers + 1u : 0u); };
     auto v_at = [&](uint32_t i) { return i + min(ntiles, i + kBuffers); };
 
-    // Q4_0: the tiles in ring order, keys and values in turn, by three warps; the first of them also sends
-    // for the numbers and scales, kRawSlots half tiles ahead of the one that is being made.
-    auto make_tiles = [&]() {
-        const uint32_t me = warp == kLoadWarp ? 0u : warp - kMmaWarp;
-        const uint32_t raw = ring + kSlots * T::kTile, blocks = hd >> 5, all = 2u * ntiles;
+    // Q4_0: half tile n of the ring's order -- the keys of the first tiles, then values and keys in turn,
+    // values at the end.
+    auto tile_at = [&](uint32_t n, bool* values) -> uint32_t {
+        const uint32_t lead = min(kBuffers, ntiles);
+        if (n < lead) return *values = false, n;
+        const uint32_t x = n - lead, pairs = 2u * (ntiles - lead);
+        *values = x >= pairs || (x & 1u) == 0u;
+        return x >= pairs ? x - pairs + (ntiles - lead) : (x & 1u) == 0u ? x >> 1 : lead + (x >> 1);
+    };
+    const uint32_t raw = ring + kSlots * T::kTile, blocks = hd >> 5, halves = 2u * ntiles;
+    auto send_raw = [&]() {  // one warp
         const uint32_t head_bytes = q4_head_bytes(a.kv), scales_at = q4_scales_at(a.kv);
-        // the n-th half tile: the keys of the first tiles, then values and keys in turn, values at the end
-        auto tile_at = [&](uint32_t n, bool* values) -> uint32_t {
-            const uint32_t lead = min(kBuffers, ntiles);
-            if (n < lead) return *values = false, n;
-            const uint32_t x = n - lead, pairs = 2u * (ntiles - lead);
-            *values = x >= pairs || (x & 1u) == 0u;
-            return x >= pairs ? x - pairs + (ntiles - lead) : (x & 1u) == 0u ? x >> 1 : lead + (x >> 1);
-        };
-        bool ok = true;
         uint32_t sent = 0, next = page0;
-        auto send = [&]() {
-            bool values;
-            const uint32_t n = sent, i = tile_at(n, &values), rs = n % kRawSlots;
-            const uint32_t pages = checked(i, next);
-            bool v;
-            next = n + 1u < all ? look_up(tile_at(n + 1u, &v)) : kNone;
-            if (ok && n >= kRawSlots) ok = warp_wait(&raw_empty[rs], ((n / kRawSlots) - 1u) & 1u, a.st, 73u);
-            if (!ok) return;
-            const uint32_t j = j0 + i * kKeys, there = __ballot_sync(0xFFFFFFFFu, pages != kNone);
-            const uint32_t want = __ballot_sync(0xFFFFFFFFu, wanted(i));
+        bool ok = true;
+        for (uint32_t n = 0; n < halves; ++n) {
+            bool values, v;
+            const uint32_t i = tile_at(n, &values), rs = n % kRawSlots, j = j0 + i * kKeys, pages = checked(i, next);
+            next = n + 1u < halves ? look_up(tile_at(n + 1u, &v)) : kNone;
+            if (n >= kRawSlots) ok = warp_wait(&raw_empty[rs], ((n / kRawSlots) - 1u) & 1u, a.st, 73u);
+            if (!ok) break;
+            const uint32_t there = __ballot_sync(0xFFFFFFFFu, pages != kNone), want = __ballot_sync(0xFFFFFFFFu, wanted(i));
             if (lane == 0u) {
                 if (!values) gaps[i & 7u] = want & ~there;
                 raw_there[rs] = there;
@@ -388,56 +386,67 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                               head + scales_at + (b * a.kv.page_size + slot_row) * 2u, box_rows * 2u, &raw_full[rs]);
             }
             sent = n + 1u;
-        };
-        if (me == 0u)
-            while (sent < min(kRawSlots, all) && ok) send();
+        }
+        // the last copies have landed before the CTA ends
+        for (uint32_t n = sent > kRawSlots ? sent - kRawSlots : 0u; n < sent; ++n)
+            mbar_wait_bounded(&raw_full[n % kRawSlots], (n / kRawSlots) & 1u, a.st, 63u);
+    };
+    auto make_tiles = [&]() {
+        const uint32_t me = (warp - kFirstMaker) % kMakers;
         // a lane: one block of one key of every 32 / kPer; eight neighbouring lanes write to different banks
         constexpr uint32_t kPer = HD / 32u, kUnits = kKeys * kPer / 32u, kStepKeys = 32u / kPer;
         const uint32_t block = HD == 128u ? ((lane >> 2) & 1u) + 2u * (lane >> 4) : (lane >> 2) & 1u;
         const uint32_t key0 = HD == 128u ? (lane & 3u) + 4u * ((lane >> 3) & 1u) : (lane & 3u) + 4u * (lane >> 3);
-        for (uint32_t n = 0; n < all && ok; ++n) {
+        for (uint32_t n = (warp - kFirstMaker) / kMakers; n < halves; n += kMakerGroups) {
             bool values;
             const uint32_t i = tile_at(n, &values), slot = n % kSlots, rs = n % kRawSlots, j = j0 + i * kKeys;
-            ok = warp_wait(&raw_full[rs], (n / kRawSlots) & 1u, a.st, 74u) &&
-                 (n < kSlots || warp_wait(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u));
-            if (!ok) break;
+            if (!warp_wait(&raw_full[rs], (n / kRawSlots) & 1u, a.st, 74u)) break;
+            if (n >= kSlots && !warp_wait(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u)) break;
             const uint32_t there = *reinterpret_cast<volatile uint32_t*>(&raw_there[rs]);
             const uint8_t* const from = sm + (raw - s0) + rs * T::kRaw;
             uint8_t* const to = sm + (ring - s0) + slot * T::kTile;
-#pragma unroll 2
-            for (uint32_t u = (me + n) % kMakers; u < kUnits; u += kMakers) {
-                const uint32_t r = u * kStepKeys + key0;
-                const bool in = block < blocks && (there >> (r >> box_shift) & 1u) && j + r >= kb && j + r < ke;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                __half2 d = __half2half2(__ushort_as_half(0));
-                if (in) {
-                    w = *reinterpret_cast<const uint4*>(from + r * (hd / 2u) + block * 16u);
-                    d = __half2half2(*reinterpret_cast<const __half*>(from + T::kRawScales + (block * kKeys + r) * 2u));
-                }
-                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            // (the loads of kAtOnce units first: each takes some 300 cycles, behind the softmax's exponentials)
+            constexpr uint32_t kAtOnce = 2;
+#pragma unroll 1
+            for (uint32_t u0 = (me + n) % kMakers; u0 < kUnits; u0 += kAtOnce * kMakers) {
+                uint4 w[kAtOnce];
+                __half d[kAtOnce];
 #pragma unroll
-                for (uint32_t x = 0; x < 4u; ++x) {
-                    __half2 h[4];
-                    q4_pairs(words[x], h);
-                    *reinterpret_cast<uint4*>(to + at(r, block * 4u + x)) =
-                        make_uint4(pack(__hmul2(h[0], d)), pack(__hmul2(h[1], d)), pack(__hmul2(h[2], d)), pack(__hmul2(h[3], d)));
+                for (uint32_t v = 0; v < kAtOnce; ++v) {
+                    const uint32_t u = u0 + v * kMakers, r = (u < kUnits ? u : u0) * kStepKeys + key0, b = min(block, blocks - 1u);
+                    w[v] = *reinterpret_cast<const uint4*>(from + r * (hd / 2u) + b * 16u);
+                    d[v] = *reinterpret_cast<const __half*>(from + T::kRawScales + (b * kKeys + r) * 2u);
+                }
+#pragma unroll
+                for (uint32_t v = 0; v < kAtOnce; ++v) {
+                    const uint32_t u = u0 + v * kMakers;
+                    if (u >= kUnits) break;
+                    const uint32_t r = u * kStepKeys + key0;
+                    const bool in = block < blocks && (there >> (r >> box_shift) & 1u) && j + r >= kb && j + r < ke;
+                    const __half2 scale = __half2half2(in ? d[v] : __ushort_as_half(0));
+                    const uint32_t words[4] = {w[v].x, w[v].y, w[v].z, w[v].w};
+#pragma unroll
+                    for (uint32_t x = 0; x < 4u; ++x) {
+                        __half2 h[4];
+                        q4_pairs(words[x], h);
+                        *reinterpret_cast<uint4*>(to + at(r, block * 4u + x)) =
+                            make_uint4(pack(__hmul2(h[0], scale)), pack(__hmul2(h[1], scale)), pack(__hmul2(h[2], scale)), pack(__hmul2(h[3], scale)));
+                    }
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(&raw_empty[rs]);
             warp_arrive(&full[slot]);
-            if (me == 0u && sent < all) send();
         }
-        // the last copies have landed before the CTA ends
-        if (me == 0u)
-            for (uint32_t n = sent > kRawSlots ? sent - kRawSlots : 0u; n < sent; ++n)
-                mbar_wait_bounded(&raw_full[n % kRawSlots], (n / kRawSlots) & 1u, a.st, 63u);
     };
 
     if (warp >= kLoadWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(T::kOtherRegs));
         if (Q4 && warp != kMmaWarp) {
-            if constexpr (Q4) make_tiles();
+            if constexpr (Q4) {
+                if (warp == kLoadWarp) send_raw();
+                else make_tiles();
+            }
         } else if (warp == kLoadWarp) {
             // ---- loads
             bool ok = true;
@@ -701,7 +710,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             asm volatile("bar.arrive 4, %0;" ::"n"(kSoftmax + kSums) : "memory");
         } else {
             // ---- running sums: channels of this side
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(T::kSumRegs));
             constexpr uint32_t kD = HD / 2u;
             const uint32_t o_addr = lanes + kOColumn + side * kD;
             float acc[kD], top = -INFINITY;
@@ -804,7 +813,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
 }
 
 template <uint32_t HD, bool Q4>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Tc<HD, Q4>::kThreads, 1)
     attention_tc_kernel(const __grid_constant__ TcMaps maps, const __grid_constant__ AttnArgs a, uint32_t box_shift) {
     attention_tc<HD, Q4>(maps, a, box_shift);
     end_after_previous(a);
@@ -827,7 +836,7 @@ cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
     const uint32_t box_rows = std::min(a.kv.page_size, kKeys);
     if (!Q4 && (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows)))
         return cudaErrorInvalidValue;
-    return launch_items(a, attention_tc_kernel<HD, Q4>, items, kThreads, Tc<HD, Q4>::kSmem, stream, maps, a,
+    return launch_items(a, attention_tc_kernel<HD, Q4>, items, Tc<HD, Q4>::kThreads, Tc<HD, Q4>::kSmem, stream, maps, a,
                         std::min(a.kv.page_shift, 7u));
 }
 
