@@ -59,18 +59,20 @@ constexpr uint32_t kMakers = 3, kMakerGroups = 2, kFirstMaker = kMmaWarp + 1u;
 template <uint32_t HD, bool Q4>
 struct Tc {
     static constexpr uint32_t kThreads = kSoftmax + kSums + (Q4 ? 256u : 128u);
-    static constexpr uint32_t kSumRegs = Q4 ? 104u : 112u, kOtherRegs = Q4 ? 40u : 56u;
+    static constexpr uint32_t kSumRegs = Q4 ? 96u : 112u, kOtherRegs = Q4 ? 48u : 56u;
     static constexpr uint32_t kBlocks = HD / 64u;
     static constexpr uint32_t kSlots = Q4 ? 3u : 4u;      // ring slots: the keys or the values of one tile
     static constexpr uint32_t kTile = kBlocks * kBlock;   // a ring slot
-    static constexpr uint32_t kRawScales = kKeys * HD / 2u;                   // where a raw slot's scales begin, [block][key]
-    static constexpr uint32_t kRaw = kRawScales + HD / 32u * kKeys * 2u;
+    static constexpr uint32_t kRawScales = kKeys * HD / 2u;                   // where a raw slot's scales begin
+    static constexpr uint32_t kRaw = kRawScales + 1024u;
     // the queries' high and low halves, the ring
     static constexpr uint32_t kSmem = 2u * kTile + kSlots * kTile + 1024u + (Q4 ? kRawSlots * kRaw : 0u);
 };
 
+// [num_pages * kv_heads][page_size][head_dim], boxes of 64 channels x box_rows slots; Q4_0: the scales,
+// [num_pages * kv_heads][head_dim / 32][page_size], boxes of all blocks x box_rows slots.
 struct TcMaps {
-    CUtensorMap k, v;  // [num_pages * kv_heads][page_size][head_dim], boxes of 64 channels x box_rows slots
+    CUtensorMap k, v;
 };
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2,
@@ -356,8 +358,9 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         return x >= pairs ? x - pairs + (ntiles - lead) : (x & 1u) == 0u ? x >> 1 : lead + (x >> 1);
     };
     const uint32_t raw = ring + kSlots * T::kTile, blocks = hd >> 5, halves = 2u * ntiles;
+    const uint32_t scale_pitch = max(128u, HD / 32u * box_rows * 2u);  // a box's scales, [block][key]
     auto send_raw = [&]() {  // one warp
-        const uint32_t head_bytes = q4_head_bytes(a.kv), scales_at = q4_scales_at(a.kv);
+        const uint32_t head_bytes = q4_head_bytes(a.kv);
         uint32_t sent = 0, next = page0;
         bool ok = true;
         for (uint32_t n = 0; n < halves; ++n) {
@@ -376,14 +379,13 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
             }
             __syncwarp();
             if (pages != kNone) {
-                const uint32_t slot_row = (j + lane * box_rows) & (a.kv.page_size - 1u);
-                const uint8_t* head = static_cast<const uint8_t*>(values ? a.kv.v : a.kv.k) +
-                                      (static_cast<size_t>(pages) * a.kv.kv_heads + kh) * head_bytes;
+                const uint32_t slot_row = (j + lane * box_rows) & (a.kv.page_size - 1u), head = pages * a.kv.kv_heads + kh;
                 const uint32_t dst = raw + rs * T::kRaw;
-                bulk_load(dst + lane * box_rows * (hd / 2u), head + slot_row * (hd / 2u), box_rows * (hd / 2u), &raw_full[rs]);
-                for (uint32_t b = 0; b < blocks; ++b)
-                    bulk_load(dst + T::kRawScales + (b * kKeys + lane * box_rows) * 2u,
-                              head + scales_at + (b * a.kv.page_size + slot_row) * 2u, box_rows * 2u, &raw_full[rs]);
+                bulk_load(dst + lane * box_rows * (hd / 2u),
+                          static_cast<const uint8_t*>(values ? a.kv.v : a.kv.k) + static_cast<size_t>(head) * head_bytes + slot_row * (hd / 2u),
+                          box_rows * (hd / 2u), &raw_full[rs]);
+                tma_load_3d(dst + T::kRawScales + lane * scale_pitch, values ? &maps.v : &maps.k, static_cast<int32_t>(slot_row), 0,
+                            static_cast<int32_t>(head), &raw_full[rs]);
             }
             sent = n + 1u;
         }
@@ -400,8 +402,11 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
         for (uint32_t n = (warp - kFirstMaker) / kMakers; n < halves; n += kMakerGroups) {
             bool values;
             const uint32_t i = tile_at(n, &values), slot = n % kSlots, rs = n % kRawSlots, j = j0 + i * kKeys;
-            if (!warp_wait(&raw_full[rs], (n / kRawSlots) & 1u, a.st, 74u)) break;
-            if (n >= kSlots && !warp_wait(&empty[slot], ((n / kSlots) - 1u) & 1u, a.st, 61u)) break;
+            // (looked at together, as by the warp of the MMAs)
+            const uint32_t raw_turn = (n / kRawSlots) & 1u, turn = ((n / kSlots) - 1u) & 1u;
+            const uint32_t raw_there_now = is_complete(&raw_full[rs], raw_turn), free_now = n < kSlots ? 1u : is_complete(&empty[slot], turn);
+            if (!__all_sync(0xFFFFFFFFu, raw_there_now) && !warp_wait(&raw_full[rs], raw_turn, a.st, 74u)) break;
+            if (!__all_sync(0xFFFFFFFFu, free_now) && !warp_wait(&empty[slot], turn, a.st, 61u)) break;
             const uint32_t there = *reinterpret_cast<volatile uint32_t*>(&raw_there[rs]);
             const uint8_t* const from = sm + (raw - s0) + rs * T::kRaw;
             uint8_t* const to = sm + (ring - s0) + slot * T::kTile;
@@ -415,7 +420,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 for (uint32_t v = 0; v < kAtOnce; ++v) {
                     const uint32_t u = u0 + v * kMakers, r = (u < kUnits ? u : u0) * kStepKeys + key0, b = min(block, blocks - 1u);
                     w[v] = *reinterpret_cast<const uint4*>(from + r * (hd / 2u) + b * 16u);
-                    d[v] = *reinterpret_cast<const __half*>(from + T::kRawScales + (b * kKeys + r) * 2u);
+                    d[v] = *reinterpret_cast<const __half*>(from + T::kRawScales + (r >> box_shift) * scale_pitch + (b * box_rows + (r & (box_rows - 1u))) * 2u);
                 }
 #pragma unroll
                 for (uint32_t v = 0; v < kAtOnce; ++v) {
@@ -822,9 +827,18 @@ __global__ void __launch_bounds__(Tc<HD, Q4>::kThreads, 1)
 bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows) {
     EncodeTiled encode = encode_tiled_fn();
     if (!encode) return false;
-    const cuuint64_t dims[3] = {kv.head_dim, kv.page_size, static_cast<cuuint64_t>(kv.num_pages) * kv.kv_heads};
+    const cuuint64_t heads = static_cast<cuuint64_t>(kv.num_pages) * kv.kv_heads;
+    const cuuint32_t step[3] = {1u, 1u, 1u};
+    if (kv.type == kQ4_0) {
+        const cuuint64_t dims[3] = {kv.page_size, kv.head_dim / 32u, heads}, strides[2] = {kv.page_size * 2ull, q4_head_bytes(kv)};
+        const cuuint32_t box[3] = {box_rows, kv.head_dim / 32u, 1u};
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, static_cast<uint8_t*>(base) + q4_scales_at(kv), dims, strides, box, step,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    }
+    const cuuint64_t dims[3] = {kv.head_dim, kv.page_size, heads};
     const cuuint64_t strides[2] = {kv.head_dim * 2ull, static_cast<cuuint64_t>(kv.page_size) * kv.head_dim * 2ull};
-    const cuuint32_t box[3] = {64u, box_rows, 1u}, step[3] = {1u, 1u, 1u};
+    const cuuint32_t box[3] = {64u, box_rows, 1u};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -832,9 +846,9 @@ bool make_map(CUtensorMap* map, void* base, const PagedKv& kv, uint32_t box_rows
 
 template <uint32_t HD, bool Q4>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    TcMaps maps = {};
+    TcMaps maps;
     const uint32_t box_rows = std::min(a.kv.page_size, kKeys);
-    if (!Q4 && (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows)))
+    if (!make_map(&maps.k, a.kv.k, a.kv, box_rows) || !make_map(&maps.v, a.kv.v, a.kv, box_rows))
         return cudaErrorInvalidValue;
     return launch_items(a, attention_tc_kernel<HD, Q4>, items, Tc<HD, Q4>::kThreads, Tc<HD, Q4>::kSmem, stream, maps, a,
                         std::min(a.kv.page_shift, 7u));
