@@ -159,13 +159,13 @@ __device__ __forceinline__ uint32_t take_rows(uint32_t* set, uint32_t* n) {
     }
     return rows;
 }
-// Rows rows & 255, ... (+ `first`); keys `from`, from + 1, ... below `to` in steps of 16 that are
-// `stride` apart (from a multiple of 16 where stride is not 16): positions, or places in the page
-// list (`list`).
+// Rows rows & 255, ... (+ `first`); keys `from`, from + 1, ... below `to`, 16 of them and 16 that lie
+// `stride` further at a time, every `step` (from a multiple of 16 where stride is not 16): positions,
+// or places in the page list (`list`).
 template <bool Q4 = false>
 static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t s, uint32_t kh, const uint32_t* list,
                                                     const TileRows& tile, uint32_t first, uint32_t rows, uint32_t from,
-                                                    uint32_t to, uint32_t stride, RowSums* sums) {
+                                                    uint32_t to, uint32_t stride, uint32_t step, RowSums* sums) {
     const uint32_t lane = threadIdx.x & 31u, hd = a.kv.head_dim, in_page = a.kv.page_size - 1u;
     const __half *k = static_cast<const __half*>(a.kv.k), *v = static_cast<const __half*>(a.kv.v);
     const float* q[kAgain];
@@ -184,7 +184,7 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
 #pragma unroll
         for (uint32_t d = 0; d < 8u; ++d) r.o[u][d] = 0.f;
     }
-    for (uint32_t j0 = from & ~15u; j0 < to; j0 += 2u * stride) {
+    for (uint32_t j0 = from & ~15u; j0 < to; j0 += step) {
         const uint32_t j = j0 + (lane >> 4) * stride + (lane & 15u);
         size_t at = 0;
         uint32_t pos = kNone;  // a key that no row sees

@@ -298,7 +298,7 @@ __device__ __forceinline__ void attention_few(const AttnArgs& a) {
             uint32_t n, rows = take_rows(&again, &n);
             RowSums x;
             rows_key_by_key(a, s, kh, a.part == kPartBlocks ? list : nullptr, {row_tok, row_head, row_pos}, 0u, rows,
-                            j0 + kKeys * warp, ke, kKeys * kWarps, &x);
+                            j0 + kKeys * warp, ke, kKeys * kWarps, 2u * kKeys * kWarps, &x);
             for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
                 const uint32_t r = rows & 255u;
                 for (uint32_t i = 0; lane + 32u * i < hd; ++i) part[(warp * ROWS + r) * kPitch + lane + 32u * i] = x.o[u][i];

@@ -421,7 +421,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     while (again != 0u) {
         uint32_t n, rows = take_rows(&again, &n);
         RowSums x;
-        rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, warp * 16u, rows, kb, ke, 16u, &x);
+        rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, warp * 16u, rows, kb, ke, 16u, 32u, &x);
         for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
             const uint32_t r = warp * 16u + (rows & 255u);
             const size_t row = static_cast<size_t>(row_tok[r]) * a.heads + row_head[r];

@@ -782,7 +782,7 @@ __device__ __forceinline__ void attention_tc(const TcMaps& maps, const AttnArgs&
                 while (set != 0u) {
                     uint32_t n, rows = take_rows(&set, &n);
                     RowSums x;
-                    rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, first, rows, kb, ke, 16u, &x);
+                    rows_key_by_key<Q4>(a, s, kh, nullptr, {row_tok, row_head, row_pos}, first, rows, kb, ke, 16u, 32u, &x);
                     for (uint32_t u = 0; u < n; ++u, rows >>= 8) {
                         const uint32_t rr = first + (rows & 255u);
                         const float f = !a.direct ? 1.f : x.l[u] == 0.f ? 0.f : 1.f / x.l[u];
