@@ -36,9 +36,10 @@ struct Few4 {
     static constexpr uint32_t kTileBytes = kScales + kBlocks * kKeys * 2u;  // keys or values of one tile
     static constexpr uint32_t kStageBytes = 2u * kTileBytes;
     static constexpr uint32_t kPitch = HD + 4u;
+    static constexpr uint32_t kQueries = HD / 16u * (ROWS / 4u) * 32u * 8u;  // [product][four rows][lane]
     static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
     static constexpr uint32_t kEnd = (kWarps * ROWS * kPitch + ROWS * HD) * 4u;  // the warps' sums, and the chunk's
-    static constexpr uint32_t kSmem = kRing > kEnd ? kRing : kEnd;
+    static constexpr uint32_t kSmem = kQueries + (kRing > kEnd ? kRing : kEnd);
 };
 
 // Byte offsets of 16-byte chunk c (a block's numbers) of key r among a tile's keys and values.  What a
@@ -82,7 +83,9 @@ template <uint32_t HD, uint32_t ROWS>
 __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
     using F = Few4<HD, ROWS>;
     constexpr uint32_t kN = ROWS / 4u;  // columns of eight: four rows each
-    extern __shared__ __align__(128) uint8_t ring[];
+    extern __shared__ __align__(128) uint8_t sm[];
+    uint8_t* const ring = sm + F::kQueries;
+    __shared__ float row_unscale[ROWS];
     __shared__ uint32_t row_tok[ROWS], row_head[ROWS];
     __shared__ int row_pos[ROWS];
     __shared__ float wm[kWarps][ROWS], wl[kWarps][ROWS];
@@ -146,42 +149,54 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
 #pragma unroll
     for (uint32_t i = 0; i + 1u < F::kStages; ++i) fetch(i);
 
-    // queries as columns: column g of eight is the high (g even) or low half of row 4 n + g / 2; of
-    // product s a thread has four channels, of the block(s) that it takes of every key
+    // queries as columns, for all warps: column g of eight is the high (g even) or low half of row 4 n + g / 2;
+    // of product s lane t has four channels, of the block(s) that it takes of every key
     constexpr uint32_t kSteps = HD / 16u, kKeyWords = HD / 32u, kValueWords = HD / 64u;
-    auto channel_of = [&](uint32_t step) { return HD == 256u ? (step >> 3) * 128u + 32u * t + 4u * (step & 7u) : HD / 4u * t + 4u * step; };
-    uint32_t qf[kN][kSteps][2];
+    {
+        // 128 / ROWS neighbouring threads to a row, four channels at a time
+        constexpr uint32_t kLanes = kThreads / ROWS, kTurns4 = (HD / 4u + kLanes - 1u) / kLanes;
+        const uint32_t r = tid / kLanes;
+        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
+        float4 x[kTurns4];
+        float big = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < kTurns4; ++i) {
+            const uint32_t ch = 4u * (i * kLanes + tid % kLanes);
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (row_pos[r] >= 0 && ch < hd) x[i] = *reinterpret_cast<const float4*>(q + ch);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kTurns4; ++i) {
+            x[i] = make_float4(x[i].x * a.scale_log2, x[i].y * a.scale_log2, x[i].z * a.scale_log2, x[i].w * a.scale_log2);
+            big = fmaxf(big, fmaxf(fmaxf(fabsf(x[i].x), fabsf(x[i].y)), fmaxf(fabsf(x[i].z), fabsf(x[i].w))));
+        }
+#pragma unroll
+        for (uint32_t o = 1; o < kLanes; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+        const int e2 = up_exponent(big);
+        const float up = power_of_two(e2);
+        if (tid % kLanes == 0u) row_unscale[r] = power_of_two(-e2);
+#pragma unroll
+        for (uint32_t i = 0; i < kTurns4; ++i) {
+            const uint32_t ch = 4u * (i * kLanes + tid % kLanes);
+            // the channels' lane and product
+            const uint32_t to = HD == 64u ? ch >> 4 : (ch >> 5) & 3u;
+            const uint32_t step = HD == 64u ? (ch & 15u) >> 2 : (ch >> 7) * 8u + ((ch & 31u) >> 2);
+            if (ch >= HD) break;
+            uint32_t hi[2], lo[2];
+            split(x[i].x * up, x[i].y * up, &hi[0], &lo[0]);
+            split(x[i].z * up, x[i].w * up, &hi[1], &lo[1]);
+            uint2* const at = reinterpret_cast<uint2*>(sm) + (step * kN + (r >> 2)) * 32u + 8u * (r & 3u) + to;
+            at[0] = make_uint2(hi[0], hi[1]);
+            at[4] = make_uint2(lo[0], lo[1]);
+        }
+    }
+    __syncthreads();
+    const uint32_t q_addr = smem_addr(sm) + 8u * lane;
     float unscale[kN], m[kN], l[kN];  // of row 4 n + t, as the scores come
     uint32_t p_lo[kN], p_hi[kN];
 #pragma unroll
     for (uint32_t n = 0; n < kN; ++n) {
-        const uint32_t r = 4u * n + (g >> 1);
-        const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
-        float4 x[kSteps];
-        float big = 0.f;
-#pragma unroll
-        for (uint32_t e = 0; e < kSteps; ++e) {
-            x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (row_pos[r] >= 0 && channel_of(e) < hd) x[e] = *reinterpret_cast<const float4*>(q + channel_of(e));
-        }
-#pragma unroll
-        for (uint32_t e = 0; e < kSteps; ++e) {
-            x[e] = make_float4(x[e].x * a.scale_log2, x[e].y * a.scale_log2, x[e].z * a.scale_log2, x[e].w * a.scale_log2);
-            big = fmaxf(big, fmaxf(fmaxf(fabsf(x[e].x), fabsf(x[e].y)), fmaxf(fabsf(x[e].z), fabsf(x[e].w))));
-        }
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
-        const int e2 = up_exponent(big);
-        const float up = power_of_two(e2);
-#pragma unroll
-        for (uint32_t e = 0; e < kSteps; ++e) {
-            uint32_t hi[2], lo[2];
-            split(x[e].x * up, x[e].y * up, &hi[0], &lo[0]);
-            split(x[e].z * up, x[e].w * up, &hi[1], &lo[1]);
-            qf[n][e][0] = g & 1u ? lo[0] : hi[0];
-            qf[n][e][1] = g & 1u ? lo[1] : hi[1];
-        }
-        unscale[n] = power_of_two(-__shfl_sync(0xFFFFFFFFu, e2, 8u * t));
+        unscale[n] = row_unscale[4u * n + t];
         const int p = row_pos[4u * n + t];
         p_lo[n] = p >= 0 ? first_key(p, a.window) : kNone;
         p_hi[n] = p >= 0 ? static_cast<uint32_t>(p) + 1u : 0u;
@@ -239,37 +254,41 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
 #pragma unroll
         for (uint32_t far = 0; far < (HD == 256u ? 2u : 1u); ++far) {
             constexpr uint32_t kWords = HD == 256u ? 4u : kKeyWords;
+            uint32_t w[kGroups][2][kWords];
+            __half2 d[kGroups][2];
+            // (HD 256: the other block, at 64 bytes this or that way)
+            const uint32_t from = stage + (far ? key_off ^ 64u : key_off);
 #pragma unroll
-            for (uint32_t h = 0; h < kGroups; ++h) {
-                uint32_t w[2][kWords];
-                __half2 d[2];
+            for (uint32_t h = 0; h < kGroups; ++h)
 #pragma unroll
                 for (uint32_t u = 0; u < 2u; ++u) {
-                    // (HD 256: the other block, at 64 bytes this or that way)
-                    const uint32_t off = far ? key_off ^ 64u : key_off;
-                    load_words<kWords>(stage + off + (16u * h + 8u * u) * F::kRowBytes, w[u]);
-                    uint32_t x = load_scale(stage + key_scale + far * 128u + h * F::kBlocks * 32u + 16u * u) & (far ? far_mask : key_mask);
-                    d[u] = *reinterpret_cast<__half2*>(&x);
+                    load_words<kWords>(from + (16u * h + 8u * u) * F::kRowBytes, w[h][u]);
+                    const uint32_t x = load_scale(stage + key_scale + far * 128u + h * F::kBlocks * 32u + 16u * u) & (far ? far_mask : key_mask);
+                    d[h][u] = *reinterpret_cast<const __half2*>(&x);
                 }
 #pragma unroll
-                for (uint32_t y = 0; y < kWords; ++y) {
-                    __half2 k[2][4];
+            for (uint32_t y = 0; y < kWords; ++y) {
+                __half2 k[kGroups][2][4];
+#pragma unroll
+                for (uint32_t h = 0; h < kGroups; ++h)
 #pragma unroll
                     for (uint32_t u = 0; u < 2u; ++u) {
-                        q4_pairs(w[u][y], k[u]);
+                        q4_pairs(w[h][u][y], k[h][u]);
 #pragma unroll
-                        for (uint32_t e = 0; e < 4u; ++e) k[u][e] = __hmul2(k[u][e], d[u]);
+                        for (uint32_t e = 0; e < 4u; ++e) k[h][u][e] = __hmul2(k[h][u][e], d[h][u]);
                     }
 #pragma unroll
-                    for (uint32_t e = 0; e < 2u; ++e) {
-                        const uint32_t x[4] = {pack(k[0][2u * e]), pack(k[1][2u * e]), pack(k[0][2u * e + 1u]), pack(k[1][2u * e + 1u])};
+                for (uint32_t e = 0; e < 2u; ++e)
 #pragma unroll
-                        for (uint32_t n = 0; n < kN; ++n) {
-                            const uint32_t step = far * 8u + 2u * y + e;
-                            mma(sc[h][n], x, qf[n][step][0], qf[n][step][1]);
+                    for (uint32_t n = 0; n < kN; ++n) {
+                        uint32_t q[2];
+                        load_words<2>(q_addr + ((far * 8u + 2u * y + e) * kN + n) * 256u, q);
+#pragma unroll
+                        for (uint32_t h = 0; h < kGroups; ++h) {
+                            const uint32_t x[4] = {pack(k[h][0][2u * e]), pack(k[h][1][2u * e]), pack(k[h][0][2u * e + 1u]), pack(k[h][1][2u * e + 1u])};
+                            mma(sc[h][n], x, q[0], q[1]);
                         }
                     }
-                }
             }
         }
         float v[kN][2 * kGroups];
@@ -408,7 +427,7 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
 }
 
 template <uint32_t HD, uint32_t ROWS>
-__global__ void __launch_bounds__(kThreads, HD <= 128u ? (ROWS <= 4u ? 4 : ROWS <= 8u ? 3 : 2) : 2) attention_few4_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, HD <= 128u ? (ROWS <= 8u ? 4 : 3) : 2) attention_few4_kernel(const __grid_constant__ AttnArgs a) {
     attention_few4<HD, ROWS>(a);
     end_after_previous(a);
 }
