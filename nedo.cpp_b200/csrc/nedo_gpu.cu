@@ -1875,8 +1875,8 @@ int check_drafts(const nedo_gpu_drafts* d, VerifyDrafts* v) {
     v->draft_probs = d->draft_probs;
     v->accept_u = d->accept_u;
     v->sample_u = d->sample_u;
-    // the launch's grid (parts of a row are at least 4096 logits)
-    if (static_cast<uint64_t>(v->rows) * ((v->vocab + 4095ull) / 4096ull) > 0x7FFFFFFFull)
+    // the launch's grid (parts of a row are at least 2048 logits)
+    if (static_cast<uint64_t>(v->rows) * ((v->vocab + 2047ull) / 2048ull) > 0x7FFFFFFFull)
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: batch too large");
     return 0;
 }

@@ -28,7 +28,6 @@ namespace {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWarps = kThreads / 32u;
 constexpr uint32_t kMaxCtas = 8;       // of a cluster
-constexpr uint32_t kStep = kThreads * 16u;  // logits that a CTA has on their way at once
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
 // NaN counts as minus infinity, infinity as the largest number.
@@ -38,7 +37,7 @@ struct VerifyArgs {
     VerifyDrafts v;
     float rate;          // log2(e) / T
     double inv_t;
-    uint32_t chunk;      // logits per part, a multiple of kStep
+    uint32_t chunk;      // logits per part, a multiple of 1024
     uint32_t parts;      // of a row
     float2* stats;       // [rows][parts]: (largest, sum); T = 0: the largest's key
     uint32_t* accepted;
@@ -58,70 +57,100 @@ __device__ __forceinline__ uint64_t pick_key(float l, uint32_t i) {
     return static_cast<uint64_t>((u >> 31) ? ~u : (u | 0x80000000u)) << 32 | (~i);
 }
 
-// Four numbers of a row from its element 4 x - shift on (those before the row's first and behind its
-// last count as minus infinity): the row begins `shift` elements behind a 16-byte border.
-__device__ __forceinline__ float4 load_quad(const float* row, uint32_t shift, uint32_t x, uint32_t from, uint32_t to) {
-    const int64_t i = static_cast<int64_t>(4u) * x - shift;
-    if (i >= static_cast<int64_t>(from) && i + 4 <= static_cast<int64_t>(to)) return __ldg(reinterpret_cast<const float4*>(row + i));
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = -INFINITY;
-        if (i + e >= static_cast<int64_t>(from) && i + e < static_cast<int64_t>(to)) v[e] = __ldg(row + i + e);
+// A row, which begins `shift` elements behind a 16-byte border, as quads: quad x holds its elements
+// 4 x - shift and on.  Those in front of it, and behind its `n` elements, count as `none`.
+struct Row {
+    const float* first;
+    uint32_t shift, n, whole0, wholes;  // quads [whole0, whole0 + wholes) are the row's alone
+    __device__ __forceinline__ Row(const float* base, size_t at, uint32_t vocab)
+        : first(base + at), shift(static_cast<uint32_t>(at & 3u)), n(vocab) {
+        whole0 = shift != 0u;
+        const uint32_t end = (n + shift) / 4u;
+        wholes = end > whole0 ? end - whole0 : 0u;
     }
-    return make_float4(v[0], v[1], v[2], v[3]);
+    __device__ __forceinline__ uint32_t quads() const { return (n + shift + 3u) / 4u; }
+    __device__ __forceinline__ float4 load(uint32_t x, float none) const {
+        const float* at = first + (static_cast<int64_t>(x) * 4 - shift);
+        if (x - whole0 < wholes) return __ldg(reinterpret_cast<const float4*>(at));
+        float v[4];
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) {
+            v[e] = none;
+            if (4u * x + e >= shift && 4u * x + e - shift < n) v[e] = __ldg(at + e);
+        }
+        return make_float4(v[0], v[1], v[2], v[3]);
+    }
+};
+
+// 16 of them, kThreads quads apart, up to quad `end`.
+__device__ __forceinline__ void load_sixteen(const Row& row, uint32_t x, uint32_t end, float (&v)[16]) {
+    float4 q[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4u; ++u) {
+        q[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (x + u * kThreads < end) q[u] = row.load(x + u * kThreads, -INFINITY);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 4u; ++u) {
+        v[4 * u] = q[u].x;
+        v[4 * u + 1] = q[u].y;
+        v[4 * u + 2] = q[u].z;
+        v[4 * u + 3] = q[u].w;
+    }
 }
 
 template <bool GREEDY>
-__global__ void __launch_bounds__(kThreads) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     __shared__ float2 sums[kWarps];
     __shared__ uint64_t keys[kWarps];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     asm volatile("griddepcontrol.launch_dependents;");
-    const size_t at = static_cast<size_t>(r) * a.v.vocab;
-    const float* row = a.v.logits + at;
-    const uint32_t shift = static_cast<uint32_t>(at & 3u);
-    const uint32_t from = part * a.chunk, to = min(a.v.vocab, from + a.chunk);
-    // (the parts' borders are 16-byte borders but for the shift: both sides read the quad on it)
-    const uint32_t x0 = (from + shift) / 4u, x1 = (to + shift + 3u) / 4u;
+    const Row row(a.v.logits, static_cast<size_t>(r) * a.v.vocab, a.v.vocab);
+    // (quads, so that no part reads another's)
+    const uint32_t x0 = part * (a.chunk / 4u), x1 = part + 1u == a.parts ? row.quads() : x0 + a.chunk / 4u;
     float m = -INFINITY, s = 0.f;
     uint64_t key = 0;
+    auto add = [&](const float(&v)[16]) {
+        float top = v[0];
+#pragma unroll
+        for (uint32_t e = 1; e < 16u; ++e) top = fmaxf(top, v[e]);
+        if (top > m) {
+            s *= exp2_fast((m - top) * a.rate);
+            m = top;
+        }
+        if (m > -INFINITY)
+#pragma unroll
+            for (uint32_t e = 0; e < 16u; ++e) s += exp2_fast((v[e] - m) * a.rate);
+    };
     for (uint32_t x = x0 + tid; x < x1; x += 4u * kThreads) {
-        float4 q[4];
-#pragma unroll
-        for (uint32_t u = 0; u < 4u; ++u) {
-            q[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (x + u * kThreads < x1) q[u] = load_quad(row, shift, x + u * kThreads, from, to);
-        }
-        float v[16], top = -INFINITY;
-#pragma unroll
-        for (uint32_t u = 0; u < 4u; ++u) {
-            v[4 * u] = counted(q[u].x);
-            v[4 * u + 1] = counted(q[u].y);
-            v[4 * u + 2] = counted(q[u].z);
-            v[4 * u + 3] = counted(q[u].w);
-        }
+        float v[16];
+        load_sixteen(row, x, x1, v);
         if constexpr (GREEDY) {
+            float top = v[0];
 #pragma unroll
-            for (uint32_t e = 0; e < 16u; ++e) {
-                // (in ascending order: the first of equal ones stays)
-                const uint32_t i = 4u * (x + (e >> 2) * kThreads) + (e & 3u) - shift;
-                if (v[e] > m) {
-                    m = v[e];
-                    key = pick_key(v[e], i);
-                }
-            }
+            for (uint32_t e = 1; e < 16u; ++e) top = fmaxf(top, v[e]);
+            if (top > m)
+#pragma unroll
+                for (uint32_t e = 0; e < 16u; ++e)
+                    // (in ascending order: the first of equal ones stays)
+                    if (counted(v[e]) > m) {
+                        m = counted(v[e]);
+                        key = pick_key(m, 4u * (x + (e >> 2) * kThreads) + (e & 3u) - row.shift);
+                    }
         } else {
+            add(v);
+        }
+    }
+    if (!GREEDY && s != s) {  // NaN, or infinite logits: once more, with what they count as
+        m = -INFINITY;
+        s = 0.f;
+        for (uint32_t x = x0 + tid; x < x1; x += 4u * kThreads) {
+            float v[16];
+            load_sixteen(row, x, x1, v);
 #pragma unroll
-            for (uint32_t e = 0; e < 16u; ++e) top = fmaxf(top, v[e]);
-            if (top > m) {
-                s *= exp2_fast((m - top) * a.rate);
-                m = top;
-            }
-            if (m > -INFINITY)
-#pragma unroll
-                for (uint32_t e = 0; e < 16u; ++e) s += exp2_fast((v[e] - m) * a.rate);
+            for (uint32_t e = 0; e < 16u; ++e) v[e] = counted(v[e]);
+            add(v);
         }
     }
     if constexpr (GREEDY) {
@@ -164,7 +193,7 @@ __device__ __forceinline__ bool load_rows(const VerifyArgs& a, uint32_t s, uint3
     return true;
 }
 __device__ __forceinline__ void write_ids(const VerifyArgs& a, uint32_t s, uint32_t t0, uint32_t n, uint32_t taken, uint32_t next) {
-    for (uint32_t i = threadIdx.x; i < n; i += kThreads)
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
         a.ids[t0 + i] = i < taken ? a.v.draft_ids[t0 + i] : i == taken ? next : kNone;
     if (threadIdx.x == 0u) a.accepted[s] = taken;
 }
@@ -223,51 +252,126 @@ __device__ __forceinline__ double warp_sum64(double v) {
     return v;
 }
 
+// e^x for x <= 0, by table (Tang's method): x = (32 j + i + f) ln 2 / 32 with |f| <= 1/2, and e^x is 2^j times
+// 2^(i/32), from the table, times the Taylor series of e^(f ln 2 / 32), whose sixth power is below 3 10^-15.  Below
+// 2^-1018 nothing.
+__device__ __forceinline__ double exp64(double x, const double* table) {
+    const double y = x * 46.166241308446828384, up = y + 6755399441055744.0;  // 32 / ln 2; 1.5 2^52 rounds to a whole number
+    const double f = y - (up - 6755399441055744.0);
+    constexpr double c = 0.021660849392498290195;  // ln 2 / 32
+    double p = fma(f, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
+    p = fma(f, p, c * c * c / 6.0);
+    p = fma(f, p, c * c / 2.0);
+    p = fma(f, p, c);
+    p = fma(f, p, 1.0);
+    const int k = __double2loint(up);
+    const double e = p * table[k & 31];
+    return x > -705.0 ? __hiloint2double(__double2hiint(e) + ((k >> 5) << 20), __double2loint(e)) : 0.0;
+}
+
 // What the tokens of a row weigh, in 64 bits.
 struct Weights {
-    const float* logits;
-    const float* probs;  // null: nothing taken off, but from token `without`
-    uint32_t without;
+    const double* table;  // 2^(i/32), i < 32
+    Row logits, probs;    // probs, where `cut`: taken off
+    uint32_t without;     // a token without weight
+    bool cut;
     float m;
     double inv_t, inv_z;
-    __device__ __forceinline__ double operator()(uint32_t i) const {
-        const float l = counted(__ldg(logits + i));
-        double e = m > -INFINITY ? exp((static_cast<double>(l) - m) * inv_t) : 0.0;
-        if (probs != nullptr) e = fmax(e * inv_z - fmax(static_cast<double>(__ldg(probs + i)), 0.0), 0.0);
+    template <bool CUT>
+    __device__ __forceinline__ double of(float l, float q, uint32_t i) const {
+        double e = exp64((static_cast<double>(counted(l)) - m) * inv_t, table);
+        if constexpr (CUT) {
+            e = fma(e, inv_z, -static_cast<double>(fmaxf(q, 0.f)));
+            return e > 0.0 ? e : 0.0;
+        }
         return i == without ? 0.0 : e;
+    }
+    __device__ __forceinline__ double at(uint32_t i) const {
+        return cut ? of<true>(__ldg(logits.first + i), __ldg(probs.first + i), i) : of<false>(__ldg(logits.first + i), 0.f, i);
     }
 };
 
+// One warp: the sum over quads [x0, x1) of the row.
+template <bool CUT>
+__device__ __noinline__ double share_sum(const Weights& weights, uint32_t x0, uint32_t x1) {
+    constexpr uint32_t kAtOnce = CUT ? 2 : 4;  // quads on their way
+    const Weights w = weights;
+    const uint32_t lane = threadIdx.x & 31u;
+    double sum = 0.0;
+    for (uint32_t x = x0 + lane; x < x1; x += 32u * kAtOnce) {
+        float4 l[kAtOnce], q[kAtOnce];
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            l[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (x + 32u * u < x1) {
+                l[u] = w.logits.load(x + 32u * u, -INFINITY);
+                if (CUT) q[u] = w.probs.load(x + 32u * u, 0.f);
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAtOnce; ++u) {
+            const uint32_t i = 4u * (x + 32u * u) - w.logits.shift;
+            sum += (w.of<CUT>(l[u].x, q[u].x, i) + w.of<CUT>(l[u].y, q[u].y, i + 1u)) +
+                   (w.of<CUT>(l[u].z, q[u].z, i + 2u) + w.of<CUT>(l[u].w, q[u].w, i + 3u));
+        }
+    }
+    return warp_sum64(sum);
+}
+__device__ __forceinline__ double share_of(const Weights& w, uint32_t x0, uint32_t x1) {
+    return w.cut ? share_sum<true>(w, x0, x1) : share_sum<false>(w, x0, x1);
+}
+
+constexpr uint32_t kSampleThreads = 512, kSampleWarps = kSampleThreads / 32u;
 struct VerifyShared {
+    double table[32];
     float row_m[kVerifyMaxRows];
     double row_z[kVerifyMaxRows];
-    double totals[2][kWarps];  // of the warps' parts (two, taken in turns)
+    double totals[2][kSampleWarps];  // of the warps' parts (two, taken in turns)
+    double before;
     uint32_t stop;
 };
 
 // A row's sum, the same in every thread of the cluster, and what makes it up: lane k of every warp
-// has the shares of warps k and k + 32 of the cluster and the sums up to and with them.
+// has the shares of warps k, k + 32, ... of the cluster and the sums up to and with them.
+constexpr uint32_t kHeld = kMaxCtas * kSampleWarps / 32u;
 struct Total {
-    double all, share[2], upto[2];
+    double all, share[kHeld], upto[kHeld];
+    // Of warps' shares in order: the first whose running sum passes `border`, or the last with any weight,
+    // and the sum in front of it.
+    __device__ __forceinline__ uint32_t owner(double border, double* before) const {
+        uint32_t some = kNone, hit = kNone;
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h) {
+            const uint32_t any = __ballot_sync(0xFFFFFFFFu, share[h] > 0.0);
+            const uint32_t over = __ballot_sync(0xFFFFFFFFu, share[h] > 0.0 && upto[h] > border);
+            if (any != 0u) some = 32u * h + 31u - __clz(any);
+            if (hit == kNone && over != 0u) hit = 32u * h + __ffs(over) - 1u;
+        }
+        const uint32_t k = hit != kNone ? hit : some;
+        double up = 0.0;
+#pragma unroll
+        for (uint32_t h = 0; h < kHeld; ++h) {
+            const double x = __shfl_sync(0xFFFFFFFFu, upto[h], (k - 1u) & 31u);
+            if (k != 0u && (k - 1u) >> 5 == h) up = x;
+        }
+        *before = up;
+        return k;
+    }
 };
-// Every warp takes tokens [begin, end); `mine`: the CTA's warps' shares.
-__device__ __forceinline__ Total row_total(const Weights& w, uint32_t begin, uint32_t end, double* mine, uint32_t ctas) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    double sum = 0.0;
-#pragma unroll 4
-    for (uint32_t i = begin + lane; i < end; i += 32u) sum += w(i);
-    sum = warp_sum64(sum);
-    if (lane == 0u) mine[warp] = sum;
-    cluster_sync();
+// The shares of up to 32 kHeld warps, in `n` places each behind the other in the CTAs of a cluster (or in this
+// CTA alone).
+__device__ __forceinline__ Total running(const double* mine, uint32_t n, bool cluster) {
+    const uint32_t lane = threadIdx.x & 31u;
     Total t;
     t.all = 0.0;
 #pragma unroll
-    for (uint32_t h = 0; h < 2u; ++h) {
+    for (uint32_t h = 0; h < kHeld; ++h) {
         const uint32_t k = lane + 32u * h;
-        t.share[h] = k < ctas * kWarps ? load_cluster(mine + k % kWarps, k / kWarps) : 0.0;
+        t.share[h] = k >= n ? 0.0 : cluster ? load_cluster(mine + k % kSampleWarps, k / kSampleWarps) : mine[k];
     }
 #pragma unroll
-    for (uint32_t h = 0; h < 2u; ++h) {
+    for (uint32_t h = 0; h < kHeld; ++h) {
         double up = t.share[h];
 #pragma unroll
         for (uint32_t o = 1; o < 32u; o <<= 1) {
@@ -281,11 +385,12 @@ __device__ __forceinline__ Total row_total(const Weights& w, uint32_t begin, uin
 }
 
 // The whole cluster of a sequence.
-__global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_constant__ VerifyArgs a, uint32_t ctas) {
+__global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const __grid_constant__ VerifyArgs a, uint32_t ctas) {
     __shared__ VerifyShared sm;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, s = blockIdx.x / ctas, rank = cluster_rank();
     uint32_t t0, n;
     const bool ok = load_rows(a, s, &t0, &n);
+    if (warp == 0u) sm.table[lane] = exp2(lane / 32.0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!ok) return;
     if (n == 0u) {
@@ -293,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_co
         return;
     }
     // the rows' parts
-    for (uint32_t i = warp; i < n; i += kWarps) {
+    for (uint32_t i = warp; i < n; i += kSampleWarps) {
         const float2* part = a.stats + static_cast<size_t>(t0 + i) * a.parts;
         float m = -INFINITY;
         for (uint32_t c = lane; c < a.parts; c += 32u) m = fmaxf(m, part[c].x);
@@ -307,25 +412,31 @@ __global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_co
             sm.row_z[i] = z;
         }
     }
-    // this warp's tokens
-    const uint32_t share = (a.v.vocab + ctas * kWarps - 1u) / (ctas * kWarps);
-    const uint32_t begin = min(a.v.vocab, (rank * kWarps + warp) * share), end = min(a.v.vocab, begin + share);
+    auto weights_of = [&](uint32_t i) {
+        const size_t at = static_cast<size_t>(t0 + i) * a.v.vocab;
+        return Weights{sm.table, Row(a.v.logits, at, a.v.vocab), Row(a.v.draft_probs, at, a.v.vocab), kNone, false, sm.row_m[i], a.inv_t, 1.0};
+    };
+    // the quads of a row that warp k of all takes
+    auto begin_of = [&](const Weights& w, uint32_t k) {
+        const uint32_t quads = w.logits.quads(), each = (quads + ctas * kSampleWarps - 1u) / (ctas * kSampleWarps);
+        return min(quads, k * each);
+    };
     uint32_t turn = 0;
     auto total = [&](const Weights& w) {
         double* mine = sm.totals[turn];
         turn ^= 1u;
-        return row_total(w, begin, end, mine, ctas);
-    };
-    auto weights_of = [&](uint32_t i) {
-        const size_t at = static_cast<size_t>(t0 + i) * a.v.vocab;
-        return Weights{a.v.logits + at, nullptr, kNone, sm.row_m[i], a.inv_t, 1.0};
+        const uint32_t k = rank * kSampleWarps + warp;
+        const double sum = share_of(w, begin_of(w, k), begin_of(w, k + 1u));
+        if (lane == 0u) mine[warp] = sum;
+        cluster_sync();
+        return running(mine, ctas * kSampleWarps, true);
     };
     // the first draft that is not taken (n - 1: all are)
     uint32_t taken = 0;
     while (true) {
         if (tid == 0u) sm.stop = 2u * (n - 1u);
         __syncthreads();
-        for (uint32_t i = taken + tid; i + 1u < n; i += kThreads) {
+        for (uint32_t i = taken + tid; i + 1u < n; i += kSampleThreads) {
             const uint32_t x = a.v.draft_ids[t0 + i];
             uint32_t what = 2u * i + 1u;  // not taken
             if (x >= a.v.vocab) {
@@ -354,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_co
         const double z = total(w).all;
         const uint32_t x = a.v.draft_ids[t0 + taken];
         const double q = a.v.draft_probs != nullptr ? fmax(static_cast<double>(a.v.draft_probs[static_cast<size_t>(t0 + taken) * a.v.vocab + x]), 0.0) : 1.0;
-        if (!(static_cast<double>(a.v.accept_u[t0 + taken]) * q < w(x) / z)) break;
+        if (!(static_cast<double>(a.v.accept_u[t0 + taken]) * q < w.at(x) / z)) break;
         ++taken;
         if (taken == n - 1u) break;
     }
@@ -366,13 +477,13 @@ __global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_co
     if (cut && w.m > -INFINITY) {
         if (a.v.draft_probs != nullptr) {
             w.inv_z = 1.0 / total(w).all;
-            w.probs = a.v.draft_probs + static_cast<size_t>(t0 + taken) * a.v.vocab;
+            w.cut = true;
         } else {
             w.without = a.v.draft_ids[t0 + taken];
         }
         t = total(w);
         if (!(t.all > 0.0)) {  // nothing left: from p itself
-            w.probs = nullptr;
+            w.cut = false;
             w.without = kNone;
         }
     }
@@ -380,66 +491,70 @@ __global__ void __launch_bounds__(kThreads) verify_sample_kernel(const __grid_co
     uint32_t next = kNone;
     bool mine = rank == 0u;  // the CTA that writes
     if (t.all > 0.0) {
-        // the warp whose share holds the border: the first whose running sum passes it, or the last
-        // with any weight
+        // the warp whose share holds the border; its CTA goes through the share again, every warp a part of
+        // it, and then the warp whose part holds the border through that
         const double border = static_cast<double>(a.v.sample_u[s]) * t.all;
-        uint32_t some[2], hits[2];
+        double before;
+        const uint32_t owner = t.owner(border, &before);
+        mine = owner / kSampleWarps == rank;
+        if (mine) {
+            const uint32_t from = begin_of(w, owner), to = begin_of(w, owner + 1u), each = (to - from + kSampleWarps - 1u) / kSampleWarps;
+            auto part_of = [&](uint32_t k) { return min(to, from + k * each); };
+            const double sum = share_of(w, part_of(warp), part_of(warp + 1u));
+            double* parts = sm.totals[turn];  // (not the one that others may still read)
+            if (lane == 0u) parts[warp] = sum;
+            __syncthreads();
+            const Total u = running(parts, kSampleWarps, false);
+            double ahead;
+            const uint32_t k = u.owner(border - before, &ahead);
+            if (warp == k) {
+                uint32_t last = kNone;
+                double run = before + ahead;
+                for (uint32_t i0 = 4u * part_of(k); i0 < 4u * part_of(k + 1u); i0 += 32u) {
+                    // (a quad on the row's border has elements of no row)
+                    const uint32_t i = i0 + lane - w.logits.shift;
+                    const double e = i0 + lane >= w.logits.shift && i < a.v.vocab && i0 + lane < 4u * part_of(k + 1u) ? w.at(i) : 0.0;
+                    double pre = e;
 #pragma unroll
-        for (uint32_t h = 0; h < 2u; ++h) {
-            some[h] = __ballot_sync(0xFFFFFFFFu, t.share[h] > 0.0);
-            hits[h] = __ballot_sync(0xFFFFFFFFu, t.share[h] > 0.0 && t.upto[h] > border);
-        }
-        const bool passed = (hits[0] | hits[1]) != 0u;
-        const uint32_t owner = passed ? (hits[0] != 0u ? __ffs(hits[0]) - 1u : 31u + __ffs(hits[1]))
-                                      : (some[1] != 0u ? 63u - __clz(some[1]) : 31u - __clz(some[0]));
-        // the running sum in front of it
-        const uint32_t prev = owner == 0u ? 0u : owner - 1u;
-        const double upto = __shfl_sync(0xFFFFFFFFu, prev >= 32u ? t.upto[1] : t.upto[0], prev & 31u);
-        const double before = owner == 0u ? 0.0 : upto;
-        mine = owner / kWarps == rank;
-        if (owner == rank * kWarps + warp) {
-            uint32_t last = kNone;
-            double sum = before;
-            for (uint32_t i0 = begin; i0 < end; i0 += 32u) {
-                const double e = i0 + lane < end ? w(i0 + lane) : 0.0;
-                double pre = e;
-#pragma unroll
-                for (uint32_t o = 1; o < 32u; o <<= 1) {
-                    const double up = __shfl_up_sync(0xFFFFFFFFu, pre, o);
-                    if (lane >= o) pre += up;
+                    for (uint32_t o = 1; o < 32u; o <<= 1) {
+                        const double up = __shfl_up_sync(0xFFFFFFFFu, pre, o);
+                        if (lane >= o) pre += up;
+                    }
+                    const uint32_t some = __ballot_sync(0xFFFFFFFFu, e > 0.0);
+                    if (some != 0u) last = i0 - w.logits.shift + 31u - __clz(some);
+                    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, e > 0.0 && run + pre > border);
+                    if (hit != 0u) {
+                        last = i0 - w.logits.shift + __ffs(hit) - 1u;
+                        break;
+                    }
+                    run += __shfl_sync(0xFFFFFFFFu, pre, 31);
                 }
-                const uint32_t some = __ballot_sync(0xFFFFFFFFu, e > 0.0);
-                if (some != 0u) last = i0 + 31u - __clz(some);
-                const uint32_t hit = __ballot_sync(0xFFFFFFFFu, e > 0.0 && sum + pre > border);
-                if (passed && hit != 0u) {
-                    last = i0 + __ffs(hit) - 1u;
-                    break;
-                }
-                sum += __shfl_sync(0xFFFFFFFFu, pre, 31);
+                if (lane == 0u) sm.stop = last;
             }
-            if (lane == 0u) sm.stop = last;
+            __syncthreads();
+            next = sm.stop;
         }
-        __syncthreads();
-        next = sm.stop;
     }
     if (mine) write_ids(a, s, t0, n, taken, next);
     cluster_sync();  // no CTA leaves while another still reads its sums
 }
 
-// CTAs of a sequence's cluster.
+// CTAs of a sequence's cluster: all that run at once for few sequences, but no warp with less than four
+// loads of a lane.
 uint32_t sample_ctas(const VerifyDrafts& v) {
-    const uint32_t work = (v.vocab + 4095u) / 4096u;
+    const uint32_t work = (v.vocab + 8191u) / 8192u;
     uint32_t c = 1;
-    while (c < kMaxCtas && c < work && static_cast<uint64_t>(v.seqs) * c < 4u * 148u) c *= 2u;
+    while (c < kMaxCtas && c < work && static_cast<uint64_t>(v.seqs) * c < 148u) c *= 2u;
     return c;
 }
 
-// Parts of a row: as many CTAs as run at once, but no part smaller than what one has on its way.
+// Parts of a row: as many CTAs as run at once, but no part smaller than two loads of a thread.
 uint32_t parts_of(const VerifyDrafts& v, uint32_t* chunk) {
-    const uint64_t want = std::max<uint64_t>(1u, (8u * 148u + v.rows - 1u) / std::max(v.rows, 1u));
-    const uint64_t steps = (static_cast<uint64_t>(v.vocab) + kStep - 1u) / kStep;
-    const uint64_t per = (steps + want - 1u) / want;
-    *chunk = static_cast<uint32_t>(std::min<uint64_t>(per * kStep, 0x40000000u));
+    constexpr uint32_t kRound = 4u * kThreads;
+    const uint64_t most = (static_cast<uint64_t>(v.vocab) + 2u * kRound - 1u) / (2u * kRound);
+    const uint64_t want = std::min<uint64_t>(most, std::max<uint64_t>(1u, 8u * 148u / v.rows));
+    const uint64_t each = (v.vocab + want - 1u) / want;
+    *chunk = static_cast<uint32_t>((each + kRound - 1u) / kRound * kRound);
     return static_cast<uint32_t>((static_cast<uint64_t>(v.vocab) + *chunk - 1u) / *chunk);
 }
 
@@ -470,7 +585,7 @@ cudaError_t launch_verify_drafts(const VerifyDrafts& v, float temperature, uint3
     const uint32_t ctas = temperature > 0.f ? sample_ctas(v) : 1u;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(v.seqs * ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(temperature > 0.f ? kSampleThreads : kThreads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
