@@ -71,7 +71,7 @@ struct Row {
     __device__ __forceinline__ uint32_t quads() const { return (n + shift + 3u) / 4u; }
     __device__ __forceinline__ float4 load(uint32_t x, float none) const {
         const float* at = first + (static_cast<int64_t>(x) * 4 - shift);
-        if (x - whole0 < wholes) return __ldg(reinterpret_cast<const float4*>(at));
+        if (x - whole0 < wholes) return __ldcs(reinterpret_cast<const float4*>(at));
         float v[4];
 #pragma unroll
         for (uint32_t e = 0; e < 4u; ++e) {
@@ -239,25 +239,18 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ double load_cluster(const double* p, uint32_t rank) {
-    uint32_t addr;
-    double v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_addr(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
-    return v;
-}
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
     return v;
 }
 
-// e^x for x <= 0, by table (Tang's method): x = (32 j + i + f) ln 2 / 32 with |f| <= 1/2, and e^x is 2^j times
-// 2^(i/32), from the table, times the Taylor series of e^(f ln 2 / 32), whose sixth power is below 3 10^-15.  Below
-// 2^-1018 nothing.
-__device__ __forceinline__ double exp64(double x, const double* table) {
-    const double y = x * 46.166241308446828384, up = y + 6755399441055744.0;  // 32 / ln 2; 1.5 2^52 rounds to a whole number
-    const double f = y - (up - 6755399441055744.0);
+// 2^(d scale / 32) for d <= 0, by table (Tang's method): with d scale = 32 j + i + f, |f| <= 1/2, it is 2^j times
+// 2^(i/32), from the table, times the Taylor series of e^(f ln 2 / 32), whose sixth power is below 3 10^-15.
+// d scale no less than -32 * 1018.
+__device__ __forceinline__ double exp64(double d, double scale, const double* table) {
+    const double up = fma(d, scale, 6755399441055744.0);  // 1.5 2^52 rounds to a whole number
+    const double f = fma(d, scale, 6755399441055744.0 - up);
     constexpr double c = 0.021660849392498290195;  // ln 2 / 32
     double p = fma(f, c * c * c * c * c / 120.0, c * c * c * c / 24.0);
     p = fma(f, p, c * c * c / 6.0);
@@ -266,7 +259,7 @@ __device__ __forceinline__ double exp64(double x, const double* table) {
     p = fma(f, p, 1.0);
     const int k = __double2loint(up);
     const double e = p * table[k & 31];
-    return x > -705.0 ? __hiloint2double(__double2hiint(e) + ((k >> 5) << 20), __double2loint(e)) : 0.0;
+    return __hiloint2double(__double2hiint(e) + ((k & ~31) << 15), __double2loint(e));
 }
 
 // What the tokens of a row weigh, in 64 bits.
@@ -275,16 +268,15 @@ struct Weights {
     Row logits, probs;    // probs, where `cut`: taken off
     uint32_t without;     // a token without weight
     bool cut;
-    float m;
-    double inv_t, inv_z;
+    float least;          // logits below it, whose weight is under 2^-500 of the largest, count as without
+    float m;              // the largest
+    double scale, inv_z;  // scale: 32 log2(e) / T
     template <bool CUT>
     __device__ __forceinline__ double of(float l, float q, uint32_t i) const {
-        double e = exp64((static_cast<double>(counted(l)) - m) * inv_t, table);
-        if constexpr (CUT) {
-            e = fma(e, inv_z, -static_cast<double>(fmaxf(q, 0.f)));
-            return e > 0.0 ? e : 0.0;
-        }
-        return i == without ? 0.0 : e;
+        // (NaN becomes the least, infinity the largest)
+        double e = exp64(static_cast<double>(fminf(fmaxf(l, least), m)) - static_cast<double>(m), scale, table);
+        if constexpr (CUT) e = fma(e, inv_z, -static_cast<double>(fmaxf(q, 0.f)));
+        return l >= least && (CUT ? __double2hiint(e) > 0 : i != without) ? e : 0.0;
     }
     __device__ __forceinline__ double at(uint32_t i) const {
         return cut ? of<true>(__ldg(logits.first + i), __ldg(probs.first + i), i) : of<false>(__ldg(logits.first + i), 0.f, i);
@@ -327,61 +319,30 @@ struct VerifyShared {
     double table[32];
     float row_m[kVerifyMaxRows];
     double row_z[kVerifyMaxRows];
-    double totals[2][kSampleWarps];  // of the warps' parts (two, taken in turns)
-    double before;
-    uint32_t stop;
+    double warps[2][kSampleWarps], ctas[2][kMaxCtas];  // sums of the warps of this CTA, of all CTAs (two, taken in turns)
+    uint32_t stop, last;
 };
-
-// A row's sum, the same in every thread of the cluster, and what makes it up: lane k of every warp
-// has the shares of warps k, k + 32, ... of the cluster and the sums up to and with them.
-constexpr uint32_t kHeld = kMaxCtas * kSampleWarps / 32u;
-struct Total {
-    double all, share[kHeld], upto[kHeld];
-    // Of warps' shares in order: the first whose running sum passes `border`, or the last with any weight,
-    // and the sum in front of it.
-    __device__ __forceinline__ uint32_t owner(double border, double* before) const {
-        uint32_t some = kNone, hit = kNone;
-#pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h) {
-            const uint32_t any = __ballot_sync(0xFFFFFFFFu, share[h] > 0.0);
-            const uint32_t over = __ballot_sync(0xFFFFFFFFu, share[h] > 0.0 && upto[h] > border);
-            if (any != 0u) some = 32u * h + 31u - __clz(any);
-            if (hit == kNone && over != 0u) hit = 32u * h + __ffs(over) - 1u;
+// Into the same place of CTA `rank` of the cluster.
+__device__ __forceinline__ void store_cluster(double* p, uint32_t rank, double v) {
+    uint32_t addr;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(smem_addr(p)), "r"(rank));
+    asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+// Of n shares in order the first whose running sum passes `border`, or the last with any weight; `run`: the
+// sum in front of the first, then of the one found.
+__device__ __forceinline__ uint32_t owner_of(const double* shares, uint32_t n, double border, double* run) {
+    uint32_t k = kNone;
+    double up = *run;
+    for (uint32_t i = 0; i < n; ++i) {
+        const double x = shares[i];
+        if (x > 0.0) {
+            k = i;
+            *run = up;
+            if (up + x > border) break;
         }
-        const uint32_t k = hit != kNone ? hit : some;
-        double up = 0.0;
-#pragma unroll
-        for (uint32_t h = 0; h < kHeld; ++h) {
-            const double x = __shfl_sync(0xFFFFFFFFu, upto[h], (k - 1u) & 31u);
-            if (k != 0u && (k - 1u) >> 5 == h) up = x;
-        }
-        *before = up;
-        return k;
+        up += x;
     }
-};
-// The shares of up to 32 kHeld warps, in `n` places each behind the other in the CTAs of a cluster (or in this
-// CTA alone).
-__device__ __forceinline__ Total running(const double* mine, uint32_t n, bool cluster) {
-    const uint32_t lane = threadIdx.x & 31u;
-    Total t;
-    t.all = 0.0;
-#pragma unroll
-    for (uint32_t h = 0; h < kHeld; ++h) {
-        const uint32_t k = lane + 32u * h;
-        t.share[h] = k >= n ? 0.0 : cluster ? load_cluster(mine + k % kSampleWarps, k / kSampleWarps) : mine[k];
-    }
-#pragma unroll
-    for (uint32_t h = 0; h < kHeld; ++h) {
-        double up = t.share[h];
-#pragma unroll
-        for (uint32_t o = 1; o < 32u; o <<= 1) {
-            const double x = __shfl_up_sync(0xFFFFFFFFu, up, o);
-            if (lane >= o) up += x;
-        }
-        t.upto[h] = t.all + up;
-        t.all = __shfl_sync(0xFFFFFFFFu, t.upto[h], 31);
-    }
-    return t;
+    return k;
 }
 
 // The whole cluster of a sequence.
@@ -414,7 +375,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     }
     auto weights_of = [&](uint32_t i) {
         const size_t at = static_cast<size_t>(t0 + i) * a.v.vocab;
-        return Weights{sm.table, Row(a.v.logits, at, a.v.vocab), Row(a.v.draft_probs, at, a.v.vocab), kNone, false, sm.row_m[i], a.inv_t, 1.0};
+        const float m = sm.row_m[i];
+        return Weights{sm.table, Row(a.v.logits, at, a.v.vocab), Row(a.v.draft_probs, at, a.v.vocab), kNone, false,
+                       fmaxf(m - 500.f / a.rate, -3.402823466e38f), m, 32.0 * 1.4426950408889634074 * a.inv_t, 1.0};
     };
     // the quads of a row that warp k of all takes
     auto begin_of = [&](const Weights& w, uint32_t k) {
@@ -422,14 +385,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
         return min(quads, k * each);
     };
     uint32_t turn = 0;
+    // a row's sum, the same in every thread of the cluster: every CTA's goes to all of them
     auto total = [&](const Weights& w) {
-        double* mine = sm.totals[turn];
         turn ^= 1u;
         const uint32_t k = rank * kSampleWarps + warp;
         const double sum = share_of(w, begin_of(w, k), begin_of(w, k + 1u));
-        if (lane == 0u) mine[warp] = sum;
+        if (lane == 0u) sm.warps[turn][warp] = sum;
+        __syncthreads();
+        if (warp == 0u) {
+            const double all = warp_sum64(lane < kSampleWarps ? sm.warps[turn][lane] : 0.0);
+            if (lane < ctas) store_cluster(&sm.ctas[turn][rank], lane, all);
+        }
         cluster_sync();
-        return running(mine, ctas * kSampleWarps, true);
+        double all = 0.0;
+        for (uint32_t c = 0; c < ctas; ++c) all += sm.ctas[turn][c];
+        return all;
     };
     // the first draft that is not taken (n - 1: all are)
     uint32_t taken = 0;
@@ -462,7 +432,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
         if (taken == n - 1u || (stop & 1u)) break;
         // the row in 64 bits
         const Weights w = weights_of(taken);
-        const double z = total(w).all;
+        const double z = total(w);
         const uint32_t x = a.v.draft_ids[t0 + taken];
         const double q = a.v.draft_probs != nullptr ? fmax(static_cast<double>(a.v.draft_probs[static_cast<size_t>(t0 + taken) * a.v.vocab + x]), 0.0) : 1.0;
         if (!(static_cast<double>(a.v.accept_u[t0 + taken]) * q < w.at(x) / z)) break;
@@ -472,71 +442,73 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     // the next token
     const bool cut = taken + 1u < n;
     Weights w = weights_of(taken);
-    Total t;
-    t.all = 0.0;
-    if (cut && w.m > -INFINITY) {
+    double all = 0.0;
+    if (cut && sm.row_m[taken] > -INFINITY) {
         if (a.v.draft_probs != nullptr) {
-            w.inv_z = 1.0 / total(w).all;
+            w.inv_z = 1.0 / total(w);
             w.cut = true;
         } else {
             w.without = a.v.draft_ids[t0 + taken];
         }
-        t = total(w);
-        if (!(t.all > 0.0)) {  // nothing left: from p itself
+        all = total(w);
+        if (!(all > 0.0)) {  // nothing left: from p itself
             w.cut = false;
             w.without = kNone;
         }
     }
-    if (!(t.all > 0.0) && w.m > -INFINITY) t = total(w);
-    uint32_t next = kNone;
-    bool mine = rank == 0u;  // the CTA that writes
-    if (t.all > 0.0) {
-        // the warp whose share holds the border; its CTA goes through the share again, every warp a part of
-        // it, and then the warp whose part holds the border through that
-        const double border = static_cast<double>(a.v.sample_u[s]) * t.all;
-        double before;
-        const uint32_t owner = t.owner(border, &before);
-        mine = owner / kSampleWarps == rank;
-        if (mine) {
-            const uint32_t from = begin_of(w, owner), to = begin_of(w, owner + 1u), each = (to - from + kSampleWarps - 1u) / kSampleWarps;
-            auto part_of = [&](uint32_t k) { return min(to, from + k * each); };
-            const double sum = share_of(w, part_of(warp), part_of(warp + 1u));
-            double* parts = sm.totals[turn];  // (not the one that others may still read)
-            if (lane == 0u) parts[warp] = sum;
-            __syncthreads();
-            const Total u = running(parts, kSampleWarps, false);
-            double ahead;
-            const uint32_t k = u.owner(border - before, &ahead);
-            if (warp == k) {
-                uint32_t last = kNone;
-                double run = before + ahead;
-                for (uint32_t i0 = 4u * part_of(k); i0 < 4u * part_of(k + 1u); i0 += 32u) {
-                    // (a quad on the row's border has elements of no row)
-                    const uint32_t i = i0 + lane - w.logits.shift;
-                    const double e = i0 + lane >= w.logits.shift && i < a.v.vocab && i0 + lane < 4u * part_of(k + 1u) ? w.at(i) : 0.0;
-                    double pre = e;
+    if (!(all > 0.0) && sm.row_m[taken] > -INFINITY) all = total(w);
+    if (!(all > 0.0)) {
+        if (rank == 0u) write_ids(a, s, t0, n, taken, kNone);
+        return;
+    }
+    // the CTA and the warp whose share holds the border; the CTA goes through that once more, a run of
+    // tokens to a thread
+    const double border = static_cast<double>(a.v.sample_u[s]) * all;
+    double run = 0.0;
+    if (owner_of(sm.ctas[turn], ctas, border, &run) != rank) return;  // (nobody reads what is here any more)
+    const uint32_t owner = rank * kSampleWarps + owner_of(sm.warps[turn], kSampleWarps, border, &run);
+    const uint32_t shift = w.logits.shift, from = max(4u * begin_of(w, owner), shift) - shift;
+    const uint32_t to = min(4u * begin_of(w, owner + 1u) - shift, a.v.vocab), each = (to - from + kSampleThreads - 1u) / kSampleThreads;
+    const uint32_t i0 = min(to, from + tid * each), i1 = min(to, i0 + each);
+    if (tid == 0u) {
+        sm.stop = kNone;
+        sm.last = 0u;
+    }
+    double sum = 0.0;
+    uint32_t last = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+        const double e = w.at(i);
+        sum += e;
+        if (e > 0.0) last = i;
+    }
+    double pre = sum;
 #pragma unroll
-                    for (uint32_t o = 1; o < 32u; o <<= 1) {
-                        const double up = __shfl_up_sync(0xFFFFFFFFu, pre, o);
-                        if (lane >= o) pre += up;
-                    }
-                    const uint32_t some = __ballot_sync(0xFFFFFFFFu, e > 0.0);
-                    if (some != 0u) last = i0 - w.logits.shift + 31u - __clz(some);
-                    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, e > 0.0 && run + pre > border);
-                    if (hit != 0u) {
-                        last = i0 - w.logits.shift + __ffs(hit) - 1u;
-                        break;
-                    }
-                    run += __shfl_sync(0xFFFFFFFFu, pre, 31);
+    for (uint32_t o = 1; o < 32u; o <<= 1) {
+        const double up = __shfl_up_sync(0xFFFFFFFFu, pre, o);
+        if (lane >= o) pre += up;
+    }
+    turn ^= 1u;
+    if (lane == 31u) sm.warps[turn][warp] = pre;
+    __syncthreads();
+    for (uint32_t k = 0; k < warp; ++k) run += sm.warps[turn][k];
+    if (sum > 0.0) {
+        atomicMax(&sm.last, last);
+        if (run + pre > border) {
+            run += pre - sum;
+            uint32_t hit = last;
+            for (uint32_t i = i0; i < i1; ++i) {
+                const double e = w.at(i);
+                run += e;
+                if (e > 0.0 && run > border) {
+                    hit = i;
+                    break;
                 }
-                if (lane == 0u) sm.stop = last;
             }
-            __syncthreads();
-            next = sm.stop;
+            atomicMin(&sm.stop, hit);
         }
     }
-    if (mine) write_ids(a, s, t0, n, taken, next);
-    cluster_sync();  // no CTA leaves while another still reads its sums
+    __syncthreads();
+    write_ids(a, s, t0, n, taken, sm.stop != kNone ? sm.stop : sm.last);
 }
 
 // CTAs of a sequence's cluster: all that run at once for few sequences, but no warp with less than four
