@@ -53,7 +53,7 @@ __device__ __forceinline__ float4 max4(const float4& a, const float4& b) {
     return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
 }
 
-// The launch's shape, and its arguments: CTAs for a.key_ctas pages, and for the rows.  Pieces are of
+// The launch's shape, and its arguments: a.key_ctas CTAs (page_ctas for a page and KV head), and those of the rows.  Pieces are of
 // 16 bytes (pairs half a head apart where they turn as pairs): `key_pieces` of a row's keys.
 struct AppendLaunch {
     AppendArgs a;
@@ -61,7 +61,8 @@ struct AppendLaunch {
     uint32_t threads;
 };
 inline AppendLaunch append_launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
-                                  float* q_out, DeviceStatus* st, uint32_t key_pieces, uint32_t pieces_between) {
+                                  float* q_out, DeviceStatus* st, uint32_t key_pieces, uint32_t pieces_between,
+                                  uint32_t page_ctas = 1u) {
     AppendLaunch l = {};
     AppendArgs& a = l.a;
     a.kv = kv;
@@ -79,7 +80,7 @@ inline AppendLaunch append_launch(const PagedKv& kv, const PagedBatch& b, uint32
     // a thread for every piece, and for every channel pair
     l.threads = (std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u) + 31u) / 32u * 32u;
     a.st = st;
-    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
+    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads * page_ctas;
     l.grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
     a.key_ctas = static_cast<uint32_t>(keys);
     return l;
