@@ -19,6 +19,8 @@
 //     writes and one KV head, because the minimum and maximum of the page's channels over the
 //     new tokens need them in one place (the tokens spread over the thread groups, one round of
 //     loads for a page of 64).  With one token per sequence they are pieces of its row.
+#include <algorithm>
+
 #include "kv_append.cuh"
 
 namespace nedo_gpu {
@@ -212,11 +214,29 @@ __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a) {
 cudaError_t launch_kv_append(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
                              float* q_out, DeviceStatus* st, cudaStream_t stream) {
     if (kv.type == kQ4_0) return launch_kv_append4(kv, b, heads, qkv, theta, q_out, st, stream);
-    const AppendLaunch l = append_launch(kv, b, heads, qkv, theta, q_out, st, kv.kv_heads * (kv.head_dim / 8u), 0u);
-    if (l.grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
-    const uint32_t grid = static_cast<uint32_t>(l.grid);
-    if (kv.type == kF16) kv_append_kernel<__half><<<grid, l.threads, 0, stream>>>(l.a);
-    else kv_append_kernel<float><<<grid, l.threads, 0, stream>>>(l.a);
+    AppendArgs a = {};
+    a.kv = kv;
+    a.b = b;
+    a.qkv = qkv;
+    a.q_out = q_out;
+    a.rotate = theta > 0.0;
+    a.log2_theta = a.rotate ? log2(theta) : 0.0;
+    a.heads = heads;
+    a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
+    a.rows = b.tokens >= 4u * 148u ? kMaxRows : 1u;  // four rows share their sines where there are CTAs enough
+    a.row_keys = b.max_q_len <= 1u;
+    const uint32_t quads = kv.head_dim / 8u;
+    a.pieces = (heads + (a.row_keys ? kv.kv_heads : 0u)) * quads + kv.kv_heads * kv.head_dim / 4u;
+    a.blocks = (a.pieces + 255u) / 256u;
+    // a thread for every piece, and for every channel pair
+    const uint32_t threads = (std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u) + 31u) / 32u * 32u;
+    a.st = st;
+    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads;
+    const uint64_t grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
+    if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
+    a.key_ctas = static_cast<uint32_t>(keys);
+    if (kv.type == kF16) kv_append_kernel<__half><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
+    else kv_append_kernel<float><<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
     return cudaGetLastError();
 }
 

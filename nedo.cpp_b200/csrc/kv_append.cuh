@@ -2,8 +2,6 @@
 // Q4_0 caches): the launch's arguments and the rotation.
 #pragma once
 
-#include <algorithm>
-
 #include "paged.cuh"
 
 namespace nedo_gpu {
@@ -53,38 +51,6 @@ __device__ __forceinline__ float4 max4(const float4& a, const float4& b) {
     return make_float4(fmaxf(a.x, b.x), fmaxf(a.y, b.y), fmaxf(a.z, b.z), fmaxf(a.w, b.w));
 }
 
-// The launch's shape, and its arguments: a.key_ctas CTAs (page_ctas for a page and KV head), and those of the rows.  Pieces are of
-// 16 bytes (pairs half a head apart where they turn as pairs): `key_pieces` of a row's keys.
-struct AppendLaunch {
-    AppendArgs a;
-    uint64_t grid;
-    uint32_t threads;
-};
-inline AppendLaunch append_launch(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
-                                  float* q_out, DeviceStatus* st, uint32_t key_pieces, uint32_t pieces_between,
-                                  uint32_t page_ctas = 1u) {
-    AppendLaunch l = {};
-    AppendArgs& a = l.a;
-    a.kv = kv;
-    a.b = b;
-    a.qkv = qkv;
-    a.q_out = q_out;
-    a.rotate = theta > 0.0;
-    a.log2_theta = a.rotate ? log2(theta) : 0.0;
-    a.heads = heads;
-    a.segs = (b.max_q_len + kv.page_size - 2u) / kv.page_size + 1u;
-    a.rows = b.tokens >= 4u * 148u ? kMaxRows : 1u;  // four rows share their sines where there are CTAs enough
-    a.row_keys = b.max_q_len <= 1u;
-    a.pieces = heads * (kv.head_dim / 8u) + pieces_between + (a.row_keys ? key_pieces : 0u) + kv.kv_heads * kv.head_dim / 4u;
-    a.blocks = (a.pieces + 255u) / 256u;
-    // a thread for every piece, and for every channel pair
-    l.threads = (std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u) + 31u) / 32u * 32u;
-    a.st = st;
-    const uint64_t keys = a.row_keys ? 0u : static_cast<uint64_t>(b.seqs) * a.segs * kv.kv_heads * page_ctas;
-    l.grid = keys + static_cast<uint64_t>((b.tokens + a.rows - 1u) / a.rows) * a.blocks;
-    a.key_ctas = static_cast<uint32_t>(keys);
-    return l;
-}
 cudaError_t launch_kv_append4(const PagedKv& kv, const PagedBatch& b, uint32_t heads, const float* qkv, double theta,
                               float* q_out, DeviceStatus* st, cudaStream_t stream);
 
