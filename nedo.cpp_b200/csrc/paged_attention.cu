@@ -176,7 +176,7 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
             const uint32_t rows = k == Kernel::kFew4 ? 4u : k == Kernel::kFew4x8 ? 8u : 16u;
             const uint32_t slots = 148u * (hd > 128u ? 2u : rows == 16u ? 3u : 4u);
             const double ns = rows == 16u ? 26.0 : rows == 8u ? 24.0 : 20.5;
-            return {rows, slots, 2048u, ns * hd / 128.0, rows == 16u ? 6000.0 : 4500.0, 0.45};
+            return {rows, slots, 2048u, ns * hd / 128.0, rows == 16u ? 6000.0 : 4500.0, 0.75};
         }
         default:  // kMany32: three products each way
             return {many32_rows(hd), 148u, 0u, hd <= 64u ? 24.0 : 48.0, 5000.0, 1.0};
