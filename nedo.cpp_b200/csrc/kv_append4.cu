@@ -291,20 +291,27 @@ __device__ __forceinline__ void append_keys4(const Append4Args& a, KeyShared& sm
             uint8_t* const at = static_cast<uint8_t*>(a.kv.k) + head * q4_head_bytes(a.kv);
             const float* src = a.qkv + static_cast<size_t>(a.heads + h) * hd + d;
             float4 lo = make_float4(INFINITY, INFINITY, INFINITY, INFINITY), hi = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            // (whole warps, for the shuffles: a thread beyond the last token goes along with it)
+            // (whole warps, for the shuffles: a thread beyond the last token goes along with it; the next token's
+            // channels are on their way.  A pair's other half is read only to turn with it: 0 times infinity is not 0)
+            float4 x, w;
+            auto load = [&](uint32_t jw) {
+                const float* row = src + static_cast<size_t>(sq.t0 + sq.n - (sq.kv - (first + min(jw + (g & 3u), b1 - 1u)))) * width;
+                x = __ldg(reinterpret_cast<const float4*>(row));
+                if (a.rotate) w = __ldg(reinterpret_cast<const float4*>(row + to));
+            };
+            w = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (b0 + 4u * warp < b1) load(b0 + 4u * warp);
 #pragma unroll 1
             for (uint32_t jw = b0 + 4u * warp; jw < b1; jw += groups) {
                 const uint32_t j = min(jw + (g & 3u), b1 - 1u);
                 const bool there = jw + (g & 3u) < b1;
-                const float* row = src + static_cast<size_t>(sq.t0 + sq.n - (sq.kv - (first + j))) * width;
-                const float4 x = __ldg(reinterpret_cast<const float4*>(row));
+                const float4 x0 = x, w0 = w;
+                if (jw + groups < b1) load(jw + groups);
                 Quad q;
                 if (a.rotate) {
-                    // (a pair's other half is read only to turn with it: 0 times infinity is not 0)
-                    const float4 w = __ldg(reinterpret_cast<const float4*>(row + to));
-                    q = quantise_key(x, w, second, sm.sines[j - b0] + c, second ? d - half : d, static_cast<int>(first + j), a.rate, there);
+                    q = quantise_key(x0, w0, second, sm.sines[j - b0] + c, second ? d - half : d, static_cast<int>(first + j), a.rate, there);
                 } else {
-                    const float u[4] = {x.x, x.y, x.z, x.w};
+                    const float u[4] = {x0.x, x0.y, x0.z, x0.w};
                     quantise<false>(u, u, q);
                 }
                 const float4 y = store_block(q, words_at(a.kv, at, j, d), scale_at(a.kv, at, j, d), there);
@@ -532,8 +539,10 @@ cudaError_t launch_kv_append4(const PagedKv& kv, const PagedBatch& b, uint32_t h
     const uint64_t grid = key_ctas + static_cast<uint64_t>((b.tokens + rows - 1u) / rows) * a.blocks;
     if (grid > 0x7FFFFFFFull) return cudaErrorInvalidConfiguration;
     a.key_ctas = static_cast<uint32_t>(key_ctas);
-    // a thread for every piece, and for every channel pair
-    const uint32_t threads = warps(std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u));
+    // a thread for every piece, and for every channel pair; more for the tokens of a page, the more where there are
+    // few pages (18 prompts of 35 to 106 tokens, 2 KV heads of 32 channels: 15 us; 26 with 64 threads)
+    const uint32_t least = keys ? 32u : key_ctas < 592u ? kMost : 128u;
+    const uint32_t threads = std::max(least, warps(std::max((a.pieces + a.blocks - 1u) / a.blocks, kv.head_dim / 2u)));
     void (*const kernel)(Append4Args) = keys ? (rows == 4u ? kv_append4_kernel<4, true> : kv_append4_kernel<1, true>)
                                              : (rows == 4u ? kv_append4_kernel<4, false> : kv_append4_kernel<1, false>);
     kernel<<<static_cast<uint32_t>(grid), threads, 0, stream>>>(a);
