@@ -287,6 +287,8 @@ struct PagedAttention {
     uint32_t own_chunk = 0, own_chunks = 0, prefix_chunk = 0, prefix_chunks = 0;
     uint32_t few_chunk = 0, few_chunks = 0;  // own part of sequences with few rows, where others have many
     bool own_cluster = false, few_cluster = false;  // a row tile's chunks are added within a cluster
+    uint32_t balance = 0;                           // the own part's chunks follow from the lengths: items at once
+    uint64_t balance_grid = 0;
     bool own_low = false, prefix_low = false;       // tiles of 64 rows where a kernel has 64 and 128
     uint64_t workspace = 0;          // bytes
 };

@@ -34,6 +34,7 @@ struct CombineArgs {
     uint32_t own_direct, few_direct;     // written out already
     uint32_t group, heads_per_cta;
     uint32_t blocks;  // the sparse call: every slot is written
+    const uint32_t* chunk_at;  // the own part's chunks follow from the lengths (null: own_chunk)
 };
 
 // One CTA per token and head (per token where most rows are done already).  The maximum over the
@@ -73,6 +74,11 @@ __global__ void __launch_bounds__(kCombineThreads) attention_combine_kernel(Comb
         }
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (a.chunk_at != nullptr && e1 != 0u) {
+        const uint32_t n = *a.chunk_at, begin = own_begin(sq, a.window, a.shared_len);
+        b1 = a.prefix_chunks + (max(first_key(p, a.window), begin) - begin) / n;
+        e1 = a.prefix_chunks + (static_cast<uint32_t>(p) - begin) / n + 1u;
+    }
     if (sq.n == 0u || (few ? a.few_direct : a.own_direct)) return;  // no row of any sequence, or done
     const uint32_t n0 = e0 - b0, n = n0 + (e1 - b1);
     for (uint32_t h = 0; h < a.heads_per_cta; ++h) {
@@ -327,6 +333,23 @@ bool plan_paged_attention(PagedAttention* a) {
     a->own_chunks = chunks(a->own_chunk);
     a->own_cluster = alone && takes_few(own) && a->own_chunks > 1u && a->own_chunks <= kMaxCluster;
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
+    // several chunks of few rows of several sequences: as long as their lengths make them, where that can save
+    // a round (16 sequences of 2005 to 16001 keys, 15 rows: 71 us, 85 with chunks for 16001 keys), not where
+    // chunks are short (7 of 421 keys behind a prefix: 33 us, 28) or there are many rounds (32 of up to
+    // 32768 keys: 121 us, 119)
+    a->balance = 0;
+    const uint64_t least = std::min<uint64_t>(std::max<uint64_t>((keys / 32u + 63u) / 64u * 64u, 256u), kBalanceMost);
+    const uint64_t each = units * keys / cost_of(own, a->kv).slots;  // keys for each of the items that run at once
+    if (takes_few4(own) && !a->picks && a->b.seqs > 1u && a->b.seqs <= 1024u && a->own_chunks > 1u && !a->own_cluster &&
+        keys > least && each >= 512u && each < 2u * kBalanceMost) {
+        a->balance = cost_of(own, a->kv).slots;
+        a->own_chunk = static_cast<uint32_t>(least);
+        a->own_chunks = chunks(a->own_chunk);
+        slots = a->own_chunks;
+        // (no more items than in whole rounds of the longest chunks, but for the last of every tile)
+        grid = (units * keys / kBalanceMost / a->balance + 1u) * a->balance + units;
+        a->balance_grid = grid;
+    }
     if (!takes_few(own) && a->b.seqs > 1u && group <= kFewMax) {  // (a larger group has more rows with every token)
         const Cost few = cost_of(few_kernel(*a), a->kv);
         const uint64_t u = static_cast<uint64_t>(a->b.seqs) * a->kv.kv_heads * (kFewMax / few.rows);
@@ -337,7 +360,7 @@ bool plan_paged_attention(PagedAttention* a) {
         if (!a->few_cluster) slots = std::max<uint64_t>(slots, a->few_chunks);
     }
     slots += a->prefix_chunks;
-    a->workspace = slots == 1u ? 0u : slots * sums;
+    a->workspace = slots == 1u ? 0u : slots * sums + (a->balance ? 16u : 0u);
     // the launches' grids
     return grid <= 0x7FFFFFFFull && prefix_units * a->prefix_chunks <= 0x7FFFFFFFull && rows <= 0x7FFFFFFFull;
 }
@@ -383,6 +406,8 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     a.slot0 = p.prefix_chunks;
     a.direct = own_direct;
     a.cluster = p.own_cluster;
+    a.balance = p.balance;
+    a.chunk_at = reinterpret_cast<uint32_t*>(a.part_ml + slots * rows);
     const Kernel k = own_kernel(p);
     const uint32_t tile = cost_of(k, p.kv).rows;
     if (p.picks) {
@@ -400,7 +425,8 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
         a.depth = p.b.seqs > 1u && p.b.seqs <= 64u ? static_cast<uint32_t>(ceil_div(most, 8u)) : 0u;
         a.rows_from = mixed ? kFewMax + 1u : 0u;
         a.row_blocks = takes_few(k) ? static_cast<uint32_t>(ceil_div(max_rows, tile)) : 1u;
-        e = launch_part(k, a, takes_few(k) ? static_cast<uint64_t>(p.b.seqs) * a.row_blocks : own_tiles(p, tile), max_rows, stream);
+        if (p.balance) e = launch_attention_few4(a, tile, p.balance_grid, stream);
+        else e = launch_part(k, a, takes_few(k) ? static_cast<uint64_t>(p.b.seqs) * a.row_blocks : own_tiles(p, tile), max_rows, stream);
         if (e == cudaSuccess && mixed) {
             a.rows_from = 0u;
             a.rows_to = kFewMax;
@@ -435,6 +461,7 @@ cudaError_t launch_paged_attention(const PagedAttention& p, const float* q, floa
     c.group = a.group;
     c.heads_per_cta = own_direct ? p.heads : 1u;
     c.blocks = p.picks != 0u;
+    c.chunk_at = p.balance ? a.chunk_at : nullptr;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<uint32_t>(rows / c.heads_per_cta));
     cfg.blockDim = dim3(kCombineThreads);

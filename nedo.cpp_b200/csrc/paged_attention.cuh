@@ -30,6 +30,10 @@ struct AttnArgs {
     uint32_t rows_from, rows_to;
     const uint32_t* blocks;
     uint32_t picks, row_blocks;
+    // few rows, Q4_0: items that run at once (0: chunks of a.chunk keys); the chunks' keys follow from the
+    // sequences' lengths, `chunk` at least, and are left at chunk_at
+    uint32_t balance;
+    uint32_t* chunk_at;
     DeviceStatus* st;
 };
 
@@ -274,6 +278,73 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
     *sums = r;
 }
 
+constexpr uint32_t kBalanceMost = 2048;  // keys of a few-rows item
+// One warp: the item of this CTA where the chunks follow from the lengths.  With chunks of the launch's
+// choice, by the batch's bounds, a batch of many lengths has items for one and a part of another
+// round of CTAs (16 sequences of 2005 to 16001 keys, 15 rows: 85 us).  Here every CTA adds up the
+// lengths, as a lane a sequence, and takes the least chunk of which there are no more than run at once (of as many
+// rounds as it takes chunks of kBalanceMost keys).  Items are those of the sequences in order, of a sequence's
+// tiles and KV heads, their chunks next to each other.
+struct BalancedItem {
+    uint32_t s, rest, c, chunk;  // rest: KV head and row tile
+};
+template <uint32_t ROWS>
+__device__ __forceinline__ bool balanced_item(const AttnArgs& a, BalancedItem* it) {
+    const uint32_t lane = threadIdx.x & 31u;
+    // tiles and KV heads of a sequence, and its keys
+    auto look = [&](uint32_t s, uint32_t* units, uint32_t* keys) {
+        *units = *keys = 0u;
+        if (s >= a.b.seqs) return;
+        const PagedSeq sq = load_seq(a.b, s, a.st);
+        if (sq.n == 0u || sq.n * a.group > a.rows_to) return;
+        const uint32_t base = own_begin(sq, a.window, a.shared_len);
+        *units = (sq.n * a.group + ROWS - 1u) / ROWS * a.kv.kv_heads;
+        *keys = sq.kv > base ? sq.kv - base : 0u;
+    };
+    uint64_t all = 0;
+    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
+        uint32_t units, keys;
+        look(s0 + lane, &units, &keys);
+        all += static_cast<uint64_t>(units) * keys;
+    }
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(all), o);
+    const uint64_t rounds = max(static_cast<uint64_t>(1), (all + static_cast<uint64_t>(a.balance) * kBalanceMost - 1u) / (static_cast<uint64_t>(a.balance) * kBalanceMost));
+    uint32_t chunk = static_cast<uint32_t>(min((all / (a.balance * rounds) + 64u) & ~static_cast<uint64_t>(63u), static_cast<uint64_t>(kBalanceMost)));
+    chunk = max(chunk, a.chunk);
+    while (chunk < kBalanceMost) {
+        uint32_t items = 0;
+        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
+            uint32_t units, keys;
+            look(s0 + lane, &units, &keys);
+            items += units * ((keys + chunk - 1u) / chunk);
+        }
+        if (__reduce_add_sync(0xFFFFFFFFu, items) <= a.balance * rounds) break;
+        chunk = min(chunk + max(64u, (chunk >> 4) & ~63u), kBalanceMost);
+    }
+    if (blockIdx.x == 0u && lane == 0u) *a.chunk_at = chunk;
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
+        uint32_t units, keys;
+        look(s0 + lane, &units, &keys);
+        const uint32_t chunks = (keys + chunk - 1u) / chunk;
+        uint32_t inc = units * chunks;
+        for (uint32_t o = 1; o < 32u; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > blockIdx.x);
+        if (hit != 0u) {
+            const uint32_t w = __ffs(hit) - 1u, n = __shfl_sync(0xFFFFFFFFu, chunks, w);
+            const uint32_t at = blockIdx.x - before - __shfl_sync(0xFFFFFFFFu, inc - units * chunks, w);
+            *it = BalancedItem{s0 + w, at / n, at % n, chunk};
+            return true;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, inc, 31);
+    }
+    it->s = kNone;
+    return false;
+}
+
 constexpr uint32_t kFewRows = 8;
 constexpr uint32_t kFewMax = 16;     // rows of a sequence that still go to the few-rows kernels, in tiles of 8 or 16
 constexpr uint32_t kMaxCluster = 8;  // chunks that a cluster can hold
@@ -285,12 +356,27 @@ struct FewItem {
     uint32_t all_b, all_e;   // positions seen by every row
 };
 // False: nothing to do.  All threads of the CTA.  ROWS: rows of a tile.
-template <uint32_t ROWS>
+template <uint32_t ROWS, bool BALANCED = false>
 __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, uint32_t* row_head, int* row_pos,
                                           uint32_t* list, FewItem* it) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5;
-    const uint32_t c = blockIdx.x % a.chunks;
-    uint32_t rest = blockIdx.x / a.chunks;
+    uint32_t c = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks, chunk = a.chunk, balanced_s = kNone;
+    if constexpr (BALANCED) {
+        __shared__ BalancedItem found;
+        if (a.balance != 0u) {
+            if (warp == 0u) {
+                BalancedItem item;
+                balanced_item<ROWS>(a, &item);
+                if ((tid & 31u) == 0u) found = item;
+            }
+            __syncthreads();
+            if (found.s == kNone) return false;
+            c = found.c;
+            rest = found.rest;
+            chunk = found.chunk;
+            balanced_s = found.s;
+        }
+    }
     const uint32_t kh = rest % a.kv.kv_heads;
     rest /= a.kv.kv_heads;
 
@@ -299,6 +385,7 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     PagedSeq sq{0u, 0u, 0u};
     r0 = rest % a.row_blocks * ROWS;
     rest /= a.row_blocks;
+    if (BALANCED && balanced_s != kNone) rest = balanced_s;
     if (a.part == kPartPrefix) {
         nrows = min(ROWS, a.b.tokens * a.group - r0);
     } else {
@@ -341,8 +428,8 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
         all_e = min(all_e, hi);
     }
     if (a.part == kPartBlocks) {
-        const uint32_t e0 = (c * a.chunk) >> a.kv.page_shift;
-        const uint32_t e1 = min(e0 + (a.chunk >> a.kv.page_shift), a.picks);
+        const uint32_t e0 = (c * chunk) >> a.kv.page_shift;
+        const uint32_t e1 = min(e0 + (chunk >> a.kv.page_shift), a.picks);
         if (warp == 0)
             checked_list(a.blocks + (static_cast<size_t>(t0) * a.kv.kv_heads + kh) * a.picks, e1, row_pos[0],
                          a.kv.page_shift, list);
@@ -353,9 +440,9 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
         uint32_t base = 0;
         if (a.part == kPartOwn) base = own_begin(sq, a.window, a.shared_len);
         else ke = min(ke, a.shared_len);
-        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * a.chunk;
+        const uint64_t cb = static_cast<uint64_t>(base) + static_cast<uint64_t>(c) * chunk;
         kb = cb > kb ? static_cast<uint32_t>(cb < kNone ? cb : kNone) : max(kb, base);
-        if (cb + a.chunk < ke) ke = static_cast<uint32_t>(cb + a.chunk);
+        if (cb + chunk < ke) ke = static_cast<uint32_t>(cb + chunk);
         if (kb >= ke && !a.direct) return false;  // no row of the tile sees a key of this chunk
     }
     *it = FewItem{s, kh, c, kb, ke, all_b, all_e};

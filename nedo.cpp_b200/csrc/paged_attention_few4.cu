@@ -92,7 +92,7 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
     __shared__ uint32_t list[kMaxPicks];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     FewItem it;
-    if (!few_setup<ROWS>(a, row_tok, row_head, row_pos, list, &it)) return;
+    if (!few_setup<ROWS, true>(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t c = it.c, kh = it.kh, s = it.s, kb = it.kb, ke = it.ke, all_b = it.all_b, all_e = it.all_e;
     const uint32_t g = lane >> 2, t = lane & 3u;
     // this warp's tiles: tile i starts at key j0 + 32 (4 i + warp); lane 2 i + h holds the page of its half h

@@ -54,7 +54,7 @@ def test_attention_workspaces(lib):
         for seqs, q, kv in ((1, 1, 640), (64, 1, 32768), (2, 2048, 4096)):
             b = batch(seqs=seqs, tokens=seqs * q, max_q_len=q, max_kv_len=kv, max_pages=-(-kv // 64))
             n = lib.paged_attention_workspace(cache(type=Q4_0, head_dim=hd), b, 12)
-            assert n % (seqs * q * 12 * (hd * 4 + 8)) == 0
+            assert n % (seqs * q * 12 * (hd * 4 + 8)) in (0, 16)  # chunks of every row, and their length
 
 
 # --------------------------------------------------------------------- drafts
