@@ -289,7 +289,7 @@ struct BalancedItem {
     uint32_t s, rest, c, chunk;  // rest: KV head and row tile
 };
 template <uint32_t ROWS>
-__device__ __forceinline__ bool balanced_item(const AttnArgs& a, BalancedItem* it) {
+__device__ __forceinline__ void balanced_item(const AttnArgs& a, BalancedItem* it) {
     const uint32_t lane = threadIdx.x & 31u;
     // tiles and KV heads of a sequence, and its keys
     auto look = [&](uint32_t s, uint32_t* units, uint32_t* keys) {
@@ -337,12 +337,11 @@ __device__ __forceinline__ bool balanced_item(const AttnArgs& a, BalancedItem* i
             const uint32_t w = __ffs(hit) - 1u, n = __shfl_sync(0xFFFFFFFFu, chunks, w);
             const uint32_t at = blockIdx.x - before - __shfl_sync(0xFFFFFFFFu, inc - units * chunks, w);
             *it = BalancedItem{s0 + w, at / n, at % n, chunk};
-            return true;
+            return;
         }
         before += __shfl_sync(0xFFFFFFFFu, inc, 31);
     }
     it->s = kNone;
-    return false;
 }
 
 constexpr uint32_t kFewRows = 8;
@@ -363,19 +362,17 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     uint32_t c = blockIdx.x % a.chunks, rest = blockIdx.x / a.chunks, chunk = a.chunk, balanced_s = kNone;
     if constexpr (BALANCED) {
         __shared__ BalancedItem found;
-        if (a.balance != 0u) {
-            if (warp == 0u) {
-                BalancedItem item;
-                balanced_item<ROWS>(a, &item);
-                if ((tid & 31u) == 0u) found = item;
-            }
-            __syncthreads();
-            if (found.s == kNone) return false;
-            c = found.c;
-            rest = found.rest;
-            chunk = found.chunk;
-            balanced_s = found.s;
+        if (warp == 0u) {
+            BalancedItem item;
+            balanced_item<ROWS>(a, &item);
+            if ((tid & 31u) == 0u) found = item;
         }
+        __syncthreads();
+        if (found.s == kNone) return false;
+        c = found.c;
+        rest = found.rest;
+        chunk = found.chunk;
+        balanced_s = found.s;
     }
     const uint32_t kh = rest % a.kv.kv_heads;
     rest /= a.kv.kv_heads;
@@ -385,7 +382,7 @@ __device__ __forceinline__ bool few_setup(const AttnArgs& a, uint32_t* row_tok, 
     PagedSeq sq{0u, 0u, 0u};
     r0 = rest % a.row_blocks * ROWS;
     rest /= a.row_blocks;
-    if (BALANCED && balanced_s != kNone) rest = balanced_s;
+    if constexpr (BALANCED) rest = balanced_s;
     if (a.part == kPartPrefix) {
         nrows = min(ROWS, a.b.tokens * a.group - r0);
     } else {

@@ -79,7 +79,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     return d;
 }
 
-template <uint32_t HD, uint32_t ROWS>
+template <uint32_t HD, uint32_t ROWS, bool BALANCED>
 __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
     using F = Few4<HD, ROWS>;
     constexpr uint32_t kN = ROWS / 4u;  // columns of eight: four rows each
@@ -92,7 +92,7 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
     __shared__ uint32_t list[kMaxPicks];
     const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
     FewItem it;
-    if (!few_setup<ROWS, true>(a, row_tok, row_head, row_pos, list, &it)) return;
+    if (!few_setup<ROWS, BALANCED>(a, row_tok, row_head, row_pos, list, &it)) return;
     const uint32_t c = it.c, kh = it.kh, s = it.s, kb = it.kb, ke = it.ke, all_b = it.all_b, all_e = it.all_e;
     const uint32_t g = lane >> 2, t = lane & 3u;
     // this warp's tiles: tile i starts at key j0 + 32 (4 i + warp); lane 2 i + h holds the page of its half h
@@ -426,15 +426,16 @@ __device__ __forceinline__ void attention_few4(const AttnArgs& a) {
     few_finish<kWarps, ROWS>(a, c, row_tok, row_head, row_pos, wm, wl, part, F::kPitch);
 }
 
-template <uint32_t HD, uint32_t ROWS>
+template <uint32_t HD, uint32_t ROWS, bool BALANCED>
 __global__ void __launch_bounds__(kThreads, HD <= 128u ? (ROWS <= 8u ? 4 : 3) : 2) attention_few4_kernel(const __grid_constant__ AttnArgs a) {
-    attention_few4<HD, ROWS>(a);
+    attention_few4<HD, ROWS, BALANCED>(a);
     end_after_previous(a);
 }
 
 template <uint32_t HD, uint32_t ROWS>
 cudaError_t launch(const AttnArgs& a, uint64_t items, cudaStream_t stream) {
-    return launch_items(a, attention_few4_kernel<HD, ROWS>, items, kThreads, Few4<HD, ROWS>::kSmem, stream, a);
+    return launch_items(a, a.balance ? attention_few4_kernel<HD, ROWS, true> : attention_few4_kernel<HD, ROWS, false>, items, kThreads,
+                        Few4<HD, ROWS>::kSmem, stream, a);
 }
 
 }  // namespace
