@@ -1909,9 +1909,11 @@ int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature,
     if (!aligned4(v.row_start) || !aligned4(v.draft_ids) || !aligned4(v.accept_u) || !aligned4(v.sample_u) ||
         !aligned4(accepted_dev) || !aligned4(ids_dev))
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: lists must be 4-byte aligned");
-    const uint64_t list = static_cast<uint64_t>(v.rows) * sizeof(uint32_t);
-    if (several && overlap(ids_dev, list, v.draft_ids, list))
-        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: ids and draft_ids overlap");
+    const uint64_t list = static_cast<uint64_t>(v.rows) * sizeof(uint32_t), counts = static_cast<uint64_t>(v.seqs) * sizeof(uint32_t);
+    if (several && (overlap(ids_dev, list, v.draft_ids, list) || overlap(accepted_dev, counts, v.draft_ids, list)))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: the results overlap draft_ids");
+    if (overlap(ids_dev, list, accepted_dev, counts))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: accepted and ids overlap");
     const uint64_t need = verify_drafts_workspace(v);
     if (!workspace_dev || workspace_bytes < need)
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: workspace smaller than " + std::to_string(need) + " bytes");

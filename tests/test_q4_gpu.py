@@ -95,6 +95,57 @@ def test_append_numbers_at_borders(lib, cuda, q):
         assert np.array_equal(bounds[page, 0].astype(np.float64), np.stack(seen))
 
 
+@pytest.mark.parametrize("q", [1, 2])
+def test_append_turned_keys_at_borders(lib, cuda, q):
+    """Keys whose turn leaves them where they are (position 0, and pairs of zeros), next to and on the borders of
+    scales and numbers: what 32 bits leave open has to come out as in 64."""
+    rng = np.random.default_rng(4)
+    x = []
+    for e in (-20, -17, -14, 0, 5):
+        for _ in range(8):
+            d = (128 + rng.integers(0, 128)) * 2.0 ** (e - 7)
+            y = d * (rng.integers(0, 16, 64) - 8.5)
+            y[[0, 32]] = -8 * d * np.array([1.0, 1.0 + rng.integers(0, 3) / 512])
+            y[5:10] = np.nextafter(y[5:10].astype(np.float32), np.float32(np.inf))
+            y[40:50] = np.nextafter(y[40:50].astype(np.float32), np.float32(-np.inf))
+            x += [y, -y, np.where(np.arange(64) < 32, y, 0.0)]
+    x = np.array(x).astype(np.float32)
+    n = len(x)
+    s = SetupQ4(2, 1, 64, 16, [q] * n, [q] * n, seed=6)
+    s.qkv[0::q, 128:192] = x
+    d = DeviceQ4(lib, cuda, s)
+    d.append(10000.0)
+    lib.status()
+    kn, kd = unpack(d.k.cpu().numpy(), 16, 64)
+    want = s.append(10000.0)[1]
+    for t, sq, p in s.rows():
+        wn, wd = quantise(want[t, 0])
+        page = int(s.table[sq, 0])
+        assert np.array_equal(kn[page, 0, p], wn) and np.array_equal(kd[page, 0, p].astype(np.float64), wd), (t, p)
+
+
+def test_append_turned_keys_of_any_size(lib, cuda):
+    """Keys up to the largest and down to the smallest numbers, infinities and NaN, turned."""
+    rng = np.random.default_rng(5)
+    x = rng.standard_normal((60, 64)) * np.exp2(rng.integers(-140, 127, (60, 1)))
+    x[10:20] = rng.choice([-3.4e38, 3.4e38, 1e38, 0.0, 1.0], (10, 64))
+    x[20:30, 40] = [np.inf, -np.inf, np.nan, np.inf, 3.4e38, -3.4e38, 1e37, 1.01e37, -0.0, 1e-45]
+    s = SetupQ4(2, 1, 64, 16, [60], [60], seed=7)
+    s.qkv[:, 128:192] = x
+    d = DeviceQ4(lib, cuda, s)
+    d.append(10000.0)
+    lib.status()
+    kn, kd = unpack(d.k.cpu().numpy(), 16, 64)
+    with np.errstate(invalid="ignore"):
+        want = s.append(10000.0)[1]
+    for t, sq, p in s.rows():
+        wn, wd = quantise(want[t, 0])
+        page, off = int(s.table[sq, p // 16]), p % 16
+        assert np.array_equal(kd[page, 0, off].astype(np.float64), wd, equal_nan=True), t
+        ok = np.repeat(np.isfinite(wd), 32)
+        assert np.array_equal(kn[page, 0, off][ok], wn[ok]), t
+
+
 def test_append_far_positions(lib, cuda):
     """A page of keys at positions near 2 10^6, turned as the definition turns each."""
     n = 2_000_064
