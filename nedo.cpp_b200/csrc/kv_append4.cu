@@ -187,9 +187,10 @@ __device__ __forceinline__ void store_bounds(__half* at, uint32_t hd, float4 lo,
 // back): u cos -+ w sin, as a pair.
 __device__ __forceinline__ Pair turned(float u, float w, bool second, double2 c) {
     const double t = second ? c.y : -c.y;
-    if (fmaxf(fabsf(u), fabsf(w)) > 1e37f) {  // (what leaves 32 bits has the largest scale, and counts as 3e38)
-        const double x = u * c.x + w * t;
-        return pair_of(fabs(x) < static_cast<double>(INFINITY) ? fmin(fmax(x, -3e38), 3e38) : x);
+    if (fmaxf(fabsf(u), fabsf(w)) > 1e35f) {
+        // what leaves 32 bits has the largest scale whatever it is: numbers above 10^36 come closer, in order
+        const double x = u * c.x + w * t, size = fabs(x);
+        return pair_of(size > 1e36 && size < static_cast<double>(INFINITY) ? copysign(1e36 + size * 0x1p-10, x) : x);
     }
     const Pair cos = pair_of(c.x), sin = pair_of(t);
     const float p = u * cos.hi, q = w * sin.hi;
