@@ -194,6 +194,7 @@ Cost cost_of(Kernel k, const PagedKv& kv) {
 // item and the bytes of the chunks' sums counted.
 // `cluster`: up to kMaxCluster chunks of a row tile can be added within a cluster, without the
 // combining kernel.
+// `joined`: a prefix makes the combining kernel necessary in any case.
 // `causal`: share of its keys by which a sequence's first rows see fewer than its last.  Where
 // items are of equal length (0) they run in whole rounds; where they are not, the long ones come
 // first and the short ones even them out.
@@ -202,7 +203,7 @@ struct Chunks {
     double ns;  // estimated time
 };
 Chunks chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const PagedKv& kv, const Cost& c, bool cluster,
-                  double causal = 0.0) {
+                  double causal = 0.0, bool joined = false) {
     const uint64_t step = std::max(64u, kv.page_size);
     keys = std::max<uint64_t>(keys, 1u);
     auto rounded = [&](uint64_t n) { return ((keys + n - 1u) / n + step - 1u) / step * step; };
@@ -221,7 +222,7 @@ Chunks chunk_keys(uint64_t keys, uint64_t units, uint64_t sum_bytes, const Paged
         const double ns = (1.0 - causal) * rounds * item + causal * std::max(item, all / c.slots) +
                           (n == 1u                          ? 0.0
                            : cluster && n <= kMaxCluster ? 1000.0
-                                                         : 4000.0 + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0);
+                                                         : (joined ? 0.0 : 4000.0) + static_cast<double>(n * sum_bytes) * 2.0 / 3000.0);
         if (best == 0u || ns < best_ns) {
             best = chunk;
             best_ns = ns;
@@ -326,7 +327,8 @@ bool plan_paged_attention(PagedAttention* a) {
                  : takes_few(k) ? a->b.seqs * ceil_div(a->b.max_q_len * group, c.rows)
                                 : own_tiles(*a, c.rows)) *
                 a->kv.kv_heads;
-        return chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(k), choice && !takes_few(k) ? causal : 0.0);
+        return chunk_keys(keys, units, sums, a->kv, c, alone && takes_few(k), choice && !takes_few(k) ? causal : 0.0,
+                          !alone && takes_few4(k));
     });
     const Kernel own = own_kernel(*a);
     a->own_chunk = best.keys;
