@@ -1910,8 +1910,13 @@ int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature,
         !aligned4(accepted_dev) || !aligned4(ids_dev))
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: lists must be 4-byte aligned");
     const uint64_t list = static_cast<uint64_t>(v.rows) * sizeof(uint32_t), counts = static_cast<uint64_t>(v.seqs) * sizeof(uint32_t);
-    if (several && (overlap(ids_dev, list, v.draft_ids, list) || overlap(accepted_dev, counts, v.draft_ids, list)))
-        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: the results overlap draft_ids");
+    const uint64_t all = list * v.vocab;
+    auto clash = [&](const void* in, uint64_t bytes) {
+        return in != nullptr && (overlap(ids_dev, list, in, bytes) || overlap(accepted_dev, counts, in, bytes));
+    };
+    if (clash(v.row_start, counts + sizeof(uint32_t)) || clash(v.logits, all) || (several && clash(v.draft_ids, list)) ||
+        (drawn && (clash(v.sample_u, counts) || (several && (clash(v.accept_u, list) || clash(v.draft_probs, all))))))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: the results overlap what is read");
     if (overlap(ids_dev, list, accepted_dev, counts))
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: accepted and ids overlap");
     const uint64_t need = verify_drafts_workspace(v);

@@ -235,9 +235,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ double warp_sum64(double v) {
 #pragma unroll
@@ -351,8 +353,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, s = blockIdx.x / ctas, rank = cluster_rank();
     uint32_t t0, n;
     const bool ok = load_rows(a, s, &t0, &n);
+    cluster_arrive();
     if (warp == 0u) sm.table[lane] = exp2(lane / 32.0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    cluster_wait();  // (no CTA writes into another before that one runs)
     if (!ok) return;
     if (n == 0u) {
         if (tid == 0u && rank == 0u) a.accepted[s] = 0u;

@@ -87,6 +87,19 @@ def test_bad_calls_refused(lib, kw, temperature, msg):
     assert e.value.code == nedo_gpu.ERR_ARG
 
 
+@pytest.mark.parametrize("name,size", [("row_start", 12), ("logits", 20000), ("draft_probs", 20000), ("accept_u", 20), ("sample_u", 8)])
+def test_results_over_inputs_refused(lib, name, size):
+    """What is read, up to its last element; not where the temperature leaves it unread."""
+    last = (1 << 21) - size + (16 if size > 20 else 4)  # its last elements under the first of ids
+    for at in (1 << 20, 1 << 21, last):
+        with pytest.raises(nedo_gpu.NedoGpuError, match="the results overlap") as e:
+            lib.verify_drafts_dev(drafts(**{name: at}), 1.0, 1 << 20, 1 << 21, A, 1 << 40)
+        assert e.value.code == nedo_gpu.ERR_ARG
+    for name in ("draft_probs", "accept_u", "sample_u"):
+        with pytest.raises(nedo_gpu.NedoGpuError, match="workspace"):
+            lib.verify_drafts_dev(drafts(**{name: 1 << 21}), 0.0, 1 << 20, 1 << 21, A, 0)
+
+
 def test_bad_outputs_refused(lib):
     need = lib.verify_drafts_workspace(drafts())
     assert need >= 5 * 8
