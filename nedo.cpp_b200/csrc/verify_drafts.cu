@@ -102,7 +102,7 @@ __device__ __forceinline__ void load_sixteen(const Row& row, uint32_t x, uint32_
 template <bool GREEDY>
 __global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_constant__ VerifyArgs a) {
     __shared__ float2 sums[kWarps];
-    __shared__ uint64_t keys[kWarps];
+    __shared__ uint32_t first;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t r = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
     asm volatile("griddepcontrol.launch_dependents;");
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_
     // (quads, so that no part reads another's)
     const uint32_t x0 = part * (a.chunk / 4u), x1 = part + 1u == a.parts ? row.quads() : x0 + a.chunk / 4u;
     float m = -INFINITY, s = 0.f;
-    uint64_t key = 0;
+    uint32_t at = x0;  // the first sixteen with m
     auto add = [&](const float(&v)[16]) {
         float top = v[0];
 #pragma unroll
@@ -130,14 +130,11 @@ __global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_
             float top = v[0];
 #pragma unroll
             for (uint32_t e = 1; e < 16u; ++e) top = fmaxf(top, v[e]);
-            if (top > m)
-#pragma unroll
-                for (uint32_t e = 0; e < 16u; ++e)
-                    // (in ascending order: the first of equal ones stays)
-                    if (counted(v[e]) > m) {
-                        m = counted(v[e]);
-                        key = pick_key(m, 4u * (x + (e >> 2) * kThreads) + (e & 3u) - row.shift);
-                    }
+            top = counted(top);
+            if (top > m) {
+                m = top;
+                at = x;
+            }
         } else {
             add(v);
         }
@@ -153,27 +150,28 @@ __global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_
             add(v);
         }
     }
-    if constexpr (GREEDY) {
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint64_t k = __shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(key), o);
-            key = k > key ? k : key;
-        }
-        if (lane == 0u) keys[warp] = key;
-    } else {
-        float top = m;
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        s = warp_sum(m > -INFINITY ? s * exp2_fast((m - top) * a.rate) : 0.f);
-        if (lane == 0u) sums[warp] = make_float2(top, s);
-    }
+    float top = m;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if constexpr (!GREEDY) s = warp_sum(m > -INFINITY ? s * exp2_fast((m - top) * a.rate) : 0.f);
+    if (lane == 0u) sums[warp] = make_float2(top, s);
+    if (GREEDY && tid == 0u) first = kNone;
     __syncthreads();
-    if (tid != 0u) return;
+    top = -INFINITY;
+    for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, sums[w].x);
     if constexpr (GREEDY) {
-        key = 0;
-        for (uint32_t w = 0; w < kWarps; ++w) key = keys[w] > key ? keys[w] : key;
-        reinterpret_cast<uint64_t*>(a.stats)[blockIdx.x] = key;
-    } else {
-        float top = -INFINITY;
-        for (uint32_t w = 0; w < kWarps; ++w) top = fmaxf(top, sums[w].x);
+        // who has the largest looks for it once more
+        if (m == top && m > -INFINITY) {
+            float v[16];
+            load_sixteen(row, at, x1, v);
+            uint32_t i = kNone;
+#pragma unroll
+            for (uint32_t e = 16; e-- > 0u;)
+                if (counted(v[e]) == m) i = 4u * (at + (e >> 2) * kThreads) + (e & 3u) - row.shift;
+            atomicMin(&first, i);
+        }
+        __syncthreads();
+        if (tid == 0u) reinterpret_cast<uint64_t*>(a.stats)[blockIdx.x] = first == kNone ? 0u : pick_key(top, first);
+    } else if (tid == 0u) {
         s = 0.f;
         for (uint32_t w = 0; w < kWarps; ++w)
             if (sums[w].x > -INFINITY) s += sums[w].y * exp2_fast((sums[w].x - top) * a.rate);
