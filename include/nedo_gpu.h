@@ -396,9 +396,9 @@ typedef struct {
     uint64_t num_pages;  /* num_pages * kv_heads below 2^31                              */
     void* k;             /* [num_pages][kv_heads][page_size][head_dim]                   */
     void* v;             /* [num_pages][kv_heads][page_size][head_dim]                   */
-    void* bounds;        /* [num_pages][kv_heads][2][head_dim], in `type` (Q4_0: in F16): the smallest and
-                            the largest value of each channel of the page's keys (NULL: not
-                            kept; nedo_gpu_block_select_dev needs it)                      */
+    void* bounds;        /* [num_pages][kv_heads][2][head_dim], in `type` (Q4_0: in F16): the
+                            smallest and the largest value of each channel of the page's keys
+                            (NULL: not kept; nedo_gpu_block_select_dev needs it)           */
 } nedo_gpu_kv_cache;
 
 typedef struct {
@@ -417,20 +417,21 @@ typedef struct {
                                     last page, or in front of its window, are not read    */
 } nedo_gpu_kv_batch;
 
-/* A cache of type NEDO_GPU_Q4_0 holds 4-bit numbers: 18 bytes for 32 channels of a token, as in a
- * GGUF tensor, with the same meaning, value = d * (n - 8) for n in 0..15 and an fp16 scale d, but
- * laid out by pages: k and v are [num_pages][kv_heads][page_size * head_dim / 32 * 18 bytes], of
- * which the first page_size * head_dim / 2 are the numbers, [page_size][head_dim / 8] words of 32 bits
- * (channel 8 w + j of a token: the four bits from bit 2 j on of word w for an even j, from bit
- * 14 + 2 j for an odd one), and the rest the scales, [head_dim / 32][page_size].  Append makes a block of 32
- * channels so, in 64 bits and without other rounding:
+/* A cache of type NEDO_GPU_Q4_0 holds 4-bit numbers: 18 bytes for 32 channels of a token,
+ * as in a GGUF tensor, with the same meaning, value = d * (n - 8) for n in 0..15 and an fp16
+ * scale d, but laid out by pages: k and v are
+ * [num_pages][kv_heads][page_size * head_dim / 32 * 18 bytes], of which the first
+ * page_size * head_dim / 2 are the numbers, [page_size][head_dim / 8] words of 32 bits
+ * (channel 8 w + j of a token: the four bits from bit 2 j on of word w for an even j, from
+ * bit 14 + 2 j for an odd one), and the rest the scales, [head_dim / 32][page_size].  Append
+ * makes a block of 32 channels so, in 64 bits and without other rounding:
  *   x: its number of largest magnitude (the negative one where both signs have it);
  *   d = -x / 8 to the nearest number of eight significant bits (equally near: the even one), in
  *       steps of no less than 2^-24, its magnitude at most 8160;
  *   n = floor(value / d + 8.5), at least 0 and at most 15; 8 where d is 0.
- * A block with a number that is not finite gets the scale NaN: all its values are NaN.  With such
- * scales every value is an F16 number; with others a caller may have put there (d as GGUF's
- * quantiser rounds it), it is the product rounded to F16. */
+ * A block with a number that is not finite gets the scale NaN: all its values are NaN.  With
+ * such scales every value is an F16 number; with others a caller may have put there (d as
+ * GGUF's quantiser rounds it), it is the product rounded to F16. */
 
 /* The new tokens of a batch: rotates queries and keys to their positions and
  * writes keys and values into the cache.  qkv_dev holds `tokens` rows of
@@ -446,10 +447,11 @@ NEDO_GPU_API int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const ne
                                         uint32_t heads, const float* qkv_dev, float rope_theta, float* q_out_dev,
                                         void* stream);
 
-/* The keys (rotated) and values that the cache holds for a batch's token rows, in 32 bits: k_out_dev and
- * v_out_dev [tokens][kv_heads][head_dim], not overlapping; for moving sequences to other pages or
- * another type of cache, and for looking at them.  Padding rows get zeros, and so do those on a page
- * id of num_pages or more. */
+/* The keys (rotated) and values that the cache holds for a batch's token rows, in 32 bits:
+ * k_out_dev and v_out_dev [tokens][kv_heads][head_dim], not overlapping; for moving sequences to
+ * other pages or another type of cache (kv_append with rope_theta 0 takes them), and for looking
+ * at them.  Padding rows get zeros, and so do those on a page id of num_pages or more; rows of no
+ * sequence are left as they were. */
 NEDO_GPU_API int nedo_gpu_kv_read_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, float* k_out_dev,
                                       float* v_out_dev, void* stream);
 
@@ -474,8 +476,8 @@ NEDO_GPU_API int nedo_gpu_paged_attention_workspace(const nedo_gpu_kv_cache* cac
  * formula: a key whose score is -infinity has no weight, one whose score is +infinity
  * makes its rows NaN, and an infinite value gives that infinity to its channel of every
  * row that sees it, or NaN where its weight is below 2^-126 of the row's largest.  Rows
- * whose sums are not finite are formed twice on F16 caches, the second time key by key:
- * right, but slow. */
+ * whose sums are not finite are formed twice on F16 and Q4_0 caches, the second time key by
+ * key: right, but slow. */
 NEDO_GPU_API int nedo_gpu_paged_attention_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
                                               uint32_t heads, const float* q_dev, float* out_dev, float scale,
                                               uint32_t window, void* workspace_dev, uint64_t workspace_bytes,
@@ -508,13 +510,14 @@ NEDO_GPU_API int nedo_gpu_block_attention_dev(const nedo_gpu_kv_cache* cache, co
 
 /* ---- Drafted tokens ------------------------------------------------------
  *
- * The sampling step of a batch whose sequences try several tokens at a time: somebody -- a smaller model,
- * a table of earlier text -- has drafted the next tokens of a sequence, one pass over the sequence's last
- * token and its drafts has given the target's logits behind each of them (paged attention takes the rows of a
- * sequence together), and this call says how many of the drafts stand and which token follows.  With
- * random numbers that are uniform and independent, the tokens are distributed as if each had been sampled
- * from the target.  Without drafts (one row per sequence) it samples a token for each.  The
- * reference samples one token of one sequence on the host (sample_token, src/model.cpp:31-53).
+ * The sampling step of a batch whose sequences try several tokens at a time: somebody -- a
+ * smaller model, a table of earlier text -- has drafted the next tokens of a sequence, one pass
+ * over the sequence's last token and its drafts has given the target's logits behind each of
+ * them (paged attention takes the rows of a sequence together), and this call says how many of
+ * the drafts stand and which token follows.  With random numbers that are uniform and
+ * independent, the tokens are distributed as if each had been sampled from the target.  Without
+ * drafts (one row per sequence) it samples a token for each.  The reference samples one token of
+ * one sequence on the host (sample_token, src/model.cpp:31-53).
  *
  * Row i of sequence s (row_start[s] + i, i below its n rows) has the target's logits behind the
  * sequence's i-th draft, row 0 those behind what was there before.  draft_ids[row] is the token drafted
@@ -542,18 +545,21 @@ NEDO_GPU_API int nedo_gpu_verify_drafts_workspace(const nedo_gpu_drafts* drafts,
  * probabilities (1 for a certain draft), a draft x of a row stands where all before it do and
  *   accept_u * q(x) < p(x),
  * and the following token is drawn from max(p - q, 0) of the row of the first draft that does
- * not stand (from p, where that leaves nothing), or from p of the last row: the first token at which the running sum passes
- * sample_u times the whole sum.  Temperature 0: a draft stands where it is the first of the largest
- * logits, which is also the token that follows.  Other temperatures: 1e-6 to 1e6.
+ * not stand (from p, where that leaves nothing), or from p of the last row: the first token at
+ * which the running sum passes sample_u times the whole sum.  Temperature 0: a draft stands where
+ * it is the first of the largest logits, which is also the token that follows.  Other
+ * temperatures: 1e-6 to 1e6.
  *
- * NaN logits count as minus infinity, infinite ones as the largest number; a row of nothing but minus infinity gives no
- * token (0xFFFFFFFF), and no draft stands on it.  NaN and negative draft probabilities count as 0.  The decisions
- * are those of 64-bit arithmetic: sums in 32 bits decide only where their error cannot.
+ * NaN logits count as minus infinity, infinite ones as the largest number; a row of nothing but
+ * minus infinity gives no token (0xFFFFFFFF), and no draft stands on it.  NaN and negative draft
+ * probabilities count as 0.  The decisions are those of 64-bit arithmetic, in which tokens below
+ * 2^-500 of a row's largest have no weight: sums in 32 bits decide only where their error cannot.
  *
- * A sequence whose rows are out of range (decreasing, beyond `rows`, more than max_rows) is left out, a draft that is
- * no token (vocab or more) does not stand, and either is reported by nedo_gpu_status.  Rows of no sequence are
- * left as they were.  Asynchronous on `stream`, without allocations; calls that overlap need
- * workspaces of their own.  logits, draft_probs and the workspace are 16-byte aligned. */
+ * A sequence whose rows are out of range (decreasing, beyond `rows`, more than max_rows) is left
+ * out, a draft that is no token (vocab or more) does not stand, and either is reported by
+ * nedo_gpu_status.  Rows of no sequence are left as they were.  Asynchronous on `stream`, without
+ * allocations; calls that overlap need workspaces of their own.  logits, draft_probs and the
+ * workspace are 16-byte aligned, and the results overlap nothing that is read. */
 NEDO_GPU_API int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature, uint32_t* accepted_dev,
                                             uint32_t* ids_dev, void* workspace_dev, uint64_t workspace_bytes,
                                             void* stream);

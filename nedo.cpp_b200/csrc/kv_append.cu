@@ -26,6 +26,27 @@
 namespace nedo_gpu {
 namespace {
 
+constexpr uint32_t kMaxRows = 4;  // token rows of a query CTA
+
+struct AppendArgs {
+    PagedKv kv;
+    PagedBatch b;
+    const float* qkv;
+    float* q_out;
+    double log2_theta;
+    uint32_t heads, rotate;
+    uint32_t segs;      // pages that a sequence's new tokens can touch
+    uint32_t key_ctas;  // CTAs of the first kind
+    uint32_t rows;      // token rows of a CTA of the other kind
+    uint32_t pieces, blocks;  // 16-byte pieces (pairs) of a row, and CTAs that share them
+    uint32_t row_keys;  // the keys are pieces of their rows
+    DeviceStatus* st;
+};
+
+// Turns per position of channel pair i.
+__device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
+    return exp2(-2.0 * i / a.kv.head_dim * a.log2_theta) * 0.15915494309189535;  // 1 / (2 pi)
+}
 // Four values into the cache, and what they are there.
 __device__ __forceinline__ void store4(float* dst, float4& x) { *reinterpret_cast<float4*>(dst) = x; }
 __device__ __forceinline__ void store4(__half* dst, float4& x) {
@@ -34,6 +55,7 @@ __device__ __forceinline__ void store4(__half* dst, float4& x) {
     const float2 lo = __half22float2(h[0]), hi = __half22float2(h[1]);
     x = make_float4(lo.x, lo.y, hi.x, hi.y);
 }
+
 // The keys of one page and KV head, and its bounds (fminf / fmaxf leave NaN out).  A page
 // whose first slot is written begins anew.
 template <typename T>

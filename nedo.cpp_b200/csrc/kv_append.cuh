@@ -1,32 +1,11 @@
 // kv_append.cuh -- what the append kernels share (kv_append.cu: F16 and F32 caches, kv_append4.cu:
-// Q4_0 caches): the launch's arguments and the rotation.
+// Q4_0 caches): the rotation in 32 bits.
 #pragma once
 
 #include "paged.cuh"
 
 namespace nedo_gpu {
 
-constexpr uint32_t kMaxRows = 4;  // token rows of a query CTA
-
-struct AppendArgs {
-    PagedKv kv;
-    PagedBatch b;
-    const float* qkv;
-    float* q_out;
-    double log2_theta;
-    uint32_t heads, rotate;
-    uint32_t segs;      // pages that a sequence's new tokens can touch
-    uint32_t key_ctas;  // CTAs of the first kind
-    uint32_t rows;      // token rows of a CTA of the other kind
-    uint32_t pieces, blocks;  // 16-byte pieces (pairs) of a row, and CTAs that share them
-    uint32_t row_keys;  // the keys are pieces of their rows
-    DeviceStatus* st;
-};
-
-// Turns per position of channel pair i.
-__device__ __forceinline__ double turns_of(const AppendArgs& a, uint32_t i) {
-    return exp2(-2.0 * i / a.kv.head_dim * a.log2_theta) * 0.15915494309189535;  // 1 / (2 pi)
-}
 // Cosine and sine of position p's rotation.
 __device__ __forceinline__ float2 rotation(int p, double turns) {
     double turn = static_cast<double>(p) * turns;
