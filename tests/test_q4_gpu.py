@@ -480,3 +480,42 @@ def test_results_repeat_and_graphs(lib, cuda):
         for a, b in zip((d.out, qo, ko, vo, d.k, d.v), want):
             assert cuda.equal(a, b)
     lib.status()
+
+
+@pytest.mark.parametrize("shape,q,kv,shared", [
+    ((4, 4, 64, 64), [1] * 6, [19001, 300, 12345, 18999, 1, 17000], 0), ((12, 12, 32, 16), [1] * 2, [16500, 6400], 0),
+    ((12, 4, 128, 64), [5, 1, 3, 5], [20000, 5, 6400, 17777], 0), ((8, 4, 160, 32), [1, 2, 1], [17000, 300, 16999], 0),
+    ((16, 8, 128, 64), [1] * 6, [9000, 1200, 8999, 1281, 5000, 6001], 18),
+])
+def test_chunks_from_the_lengths(lib, cuda, shape, q, kv, shared):
+    """Batches whose chunks the device makes as long as the lengths ask: with other lengths of the same limits, none
+    at all, and lengths out of range; eager and replayed."""
+    d = dev(lib, cuda, *shape, q=q, kv=kv, seed=35, shared=shared)
+    heads, hd = shape[0], shape[2]
+    need = lib.paged_attention_workspace(d.cache, d.batch, heads)
+    assert need % (d.s.tokens * heads * (hd * 4 + 8)) == 16  # the chunks' length is there
+    check_attention(d.s, d.attention(), d.s.attention())
+    window = 5000
+    check_attention(d.s, d.attention(window), d.s.attention(window))
+    ws, out = d.space(need), cuda.empty_like(d.out)
+
+    def step(into):
+        lib.paged_attention_dev(d.cache, d.batch, heads, d.q.data_ptr(), into.data_ptr(), d.s.scale, 0, ws.data_ptr(), need, d.stream())
+
+    step(out)
+    graph = cuda.cuda.CUDAGraph()
+    with cuda.cuda.graph(graph):
+        step(out)
+    first = shared * shape[3]
+    for lens in (kv, [first + (n - first) // 2 for n in kv], [min(n, first + 70) for n in kv], [first + n for n in q], [0] * len(kv), kv):
+        d.s.kv = list(lens)
+        d.len.copy_(cuda.tensor(lens, dtype=cuda.int32))
+        want = d.s.attention()
+        d.out.fill_(777.0)
+        out.fill_(777.0)
+        step(d.out)
+        check_attention(d.s, d.out, want)
+        ws.fill_(255)
+        graph.replay()
+        assert cuda.equal(out, d.out)
+    lib.status()
