@@ -198,18 +198,22 @@ __device__ __forceinline__ bool load_rows(const VerifyArgs& a, uint32_t s, uint3
     *n = e - b;
     return true;
 }
-__device__ __forceinline__ void write_ids(const VerifyArgs& a, uint32_t s, uint32_t t0, uint32_t n, uint32_t taken, uint32_t next) {
-    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x)
-        a.ids[t0 + i] = i < taken ? a.v.draft_ids[t0 + i] : i == taken ? next : kNone;
+__device__ __forceinline__ void write_ids(const VerifyArgs& a, uint32_t s, uint32_t t0, uint32_t n, const uint32_t* drafts,
+                                          uint32_t taken, uint32_t next) {
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) a.ids[t0 + i] = i < taken ? drafts[i] : i == taken ? next : kNone;
     if (threadIdx.x == 0u) a.accepted[s] = taken;
 }
 
 __global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const __grid_constant__ VerifyArgs a) {
-    __shared__ uint32_t pick[kVerifyMaxRows], end;
+    static_assert(kVerifyMaxRows <= kThreads, "a thread to a row");
+    __shared__ uint32_t pick[kVerifyMaxRows], drafts[kVerifyMaxRows], end;
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, s = blockIdx.x;
     uint32_t t0, n;
     const bool ok = load_rows(a, s, &t0, &n);
     if (tid == 0u) end = n - 1u;
+    const bool mine = ok && tid + 1u < n;  // (inputs, while the first kernel runs)
+    const uint32_t x = mine ? a.v.draft_ids[t0 + tid] : 0u;
+    if (mine) drafts[tid] = x;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!ok) return;
     if (n == 0u) {
@@ -227,13 +231,12 @@ __global__ void __launch_bounds__(kThreads) verify_greedy_kernel(const __grid_co
         if (lane == 0u) pick[i] = best == 0u ? kNone : ~static_cast<uint32_t>(best);
     }
     __syncthreads();
-    for (uint32_t i = tid; i + 1u < n; i += kThreads) {
-        const uint32_t x = a.v.draft_ids[t0 + i];
+    if (mine) {
         if (x >= a.v.vocab && a.st != nullptr) atomicOr(&a.st->flags, kErrArgument);
-        if (x >= a.v.vocab || pick[i] != x) atomicMin(&end, i);
+        if (x >= a.v.vocab || pick[tid] != x) atomicMin(&end, tid);
     }
     __syncthreads();
-    write_ids(a, s, t0, n, end, pick[end]);
+    write_ids(a, s, t0, n, drafts, end, pick[end]);
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -327,6 +330,7 @@ struct VerifyShared {
     double table[32];
     float row_m[kVerifyMaxRows];
     double row_z[kVerifyMaxRows];
+    uint32_t drafts[kVerifyMaxRows];
     double warps[2][kSampleWarps], ctas[2][kMaxCtas];  // sums of the warps of this CTA, of all CTAs (two, taken in turns)
     uint32_t stop, last;
 };
@@ -361,6 +365,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     const bool ok = load_rows(a, s, &t0, &n);
     cluster_arrive();
     if (warp == 0u) sm.table[lane] = exp2(lane / 32.0);
+    // what the inputs say of the thread's row's draft, while the first kernel runs
+    static_assert(kVerifyMaxRows <= kSampleThreads, "a thread to a row");
+    const bool mine = ok && tid + 1u < n;
+    const uint32_t x = mine ? a.v.draft_ids[t0 + tid] : 0u;
+    float logit = -INFINITY, u = 0.f, q = 1.f;
+    if (mine) {
+        sm.drafts[tid] = x;
+        u = a.v.accept_u[t0 + tid];
+        const size_t at = static_cast<size_t>(t0 + tid) * a.v.vocab + x;
+        if (x < a.v.vocab) {
+            logit = counted(a.v.logits[at]);
+            if (a.v.draft_probs != nullptr) q = fmaxf(a.v.draft_probs[at], 0.f);
+        }
+    }
+    const float sample_u = a.v.sample_u[s];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     cluster_wait();  // (no CTA writes into another before that one runs)
     if (!ok) return;
@@ -416,25 +435,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     while (true) {
         if (tid == 0u) sm.stop = 2u * (n - 1u);
         __syncthreads();
-        for (uint32_t i = taken + tid; i + 1u < n; i += kSampleThreads) {
-            const uint32_t x = a.v.draft_ids[t0 + i];
-            uint32_t what = 2u * i + 1u;  // not taken
+        if (mine && tid >= taken) {
+            uint32_t what = 2u * tid + 1u;  // not taken
             if (x >= a.v.vocab) {
                 if (a.st != nullptr) atomicOr(&a.st->flags, kErrArgument);
             } else {
-                const size_t at = static_cast<size_t>(t0 + i) * a.v.vocab + x;
-                const float m = sm.row_m[i], e = m > -INFINITY ? exp2_fast((counted(a.v.logits[at]) - m) * a.rate) : 0.f;
-                const float q = a.v.draft_probs != nullptr ? fmaxf(a.v.draft_probs[at], 0.f) : 1.f;
-                const double left = static_cast<double>(a.v.accept_u[t0 + i]) * q * sm.row_z[i], right = e;
+                const float m = sm.row_m[tid], e = m > -INFINITY ? exp2_fast((logit - m) * a.rate) : 0.f;
+                const double left = static_cast<double>(u) * q * sm.row_z[tid], right = e;
                 constexpr double kOff = 1.0 / 16384.0;
-                if (m == -INFINITY || left > right * (1.0 + kOff) + 1e-30) what = 2u * i + 1u;
+                if (m == -INFINITY || left > right * (1.0 + kOff) + 1e-30) what = 2u * tid + 1u;
                 else if (left < right * (1.0 - kOff) - 1e-30) what = kNone;
-                else what = 2u * i;  // open
+                else what = 2u * tid;  // open
             }
-            if (what != kNone) {
-                atomicMin(&sm.stop, what);
-                break;
-            }
+            if (what != kNone) atomicMin(&sm.stop, what);
         }
         __syncthreads();
         const uint32_t stop = sm.stop;
@@ -443,9 +456,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
         // the row in 64 bits
         const Weights w = weights_of(taken);
         const double z = total(w);
-        const uint32_t x = a.v.draft_ids[t0 + taken];
-        const double q = a.v.draft_probs != nullptr ? fmax(static_cast<double>(a.v.draft_probs[static_cast<size_t>(t0 + taken) * a.v.vocab + x]), 0.0) : 1.0;
-        if (!(static_cast<double>(a.v.accept_u[t0 + taken]) * q < w.at(x) / z)) break;
+        const uint32_t token = sm.drafts[taken];
+        const double p = a.v.draft_probs != nullptr ? fmax(static_cast<double>(a.v.draft_probs[static_cast<size_t>(t0 + taken) * a.v.vocab + token]), 0.0) : 1.0;
+        if (!(static_cast<double>(a.v.accept_u[t0 + taken]) * p < w.at(token) / z)) break;
         ++taken;
         if (taken == n - 1u) break;
     }
@@ -458,7 +471,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
             w.inv_z = 1.0 / total(w);
             w.cut = true;
         } else {
-            w.without = a.v.draft_ids[t0 + taken];
+            w.without = sm.drafts[taken];
         }
         all = total(w);
         if (!(all > 0.0)) {  // nothing left: from p itself
@@ -468,12 +481,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
     }
     if (!(all > 0.0) && sm.row_m[taken] > -INFINITY) all = total(w);
     if (!(all > 0.0)) {
-        if (rank == 0u) write_ids(a, s, t0, n, taken, kNone);
+        if (rank == 0u) write_ids(a, s, t0, n, sm.drafts, taken, kNone);
         return;
     }
     // the CTA and the warp whose share holds the border; the CTA goes through that once more, a run of
     // tokens to a thread
-    const double border = static_cast<double>(a.v.sample_u[s]) * all;
+    const double border = static_cast<double>(sample_u) * all;
     double run = 0.0;
     if (owner_of(sm.ctas[turn], ctas, border, &run) != rank) return;  // (nobody reads what is here any more)
     const uint32_t owner = rank * kSampleWarps + owner_of(sm.warps[turn], kSampleWarps, border, &run);
@@ -518,7 +531,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
         }
     }
     __syncthreads();
-    write_ids(a, s, t0, n, taken, sm.stop != kNone ? sm.stop : sm.last);
+    write_ids(a, s, t0, n, sm.drafts, taken, sm.stop != kNone ? sm.stop : sm.last);
 }
 
 // CTAs of a sequence's cluster: all that run at once for few sequences, but no warp with less than four
