@@ -19,9 +19,11 @@
 // and 2 KV heads, 300 tokens 26 us (128 rows: 30), 37 sequences of 32 tokens over 500 keys 51 us (68).
 // The plan takes the height that it expects to end first.
 //
-// Of a Q4_0 cache (paged_q4.cuh) a thread copies the same blocks of 32 channels of every tile, and
-// makes fp16 numbers of its own copies before the barrier that the tile waits for anyway: 887 us for
-// two prompts of 1919 and 2048 tokens over up to 4096 keys, 33 and 71 us for the two short ones above.
+// Of a Q4_0 cache (paged_q4.cuh) a thread copies the same blocks of 32 channels of every tile and makes
+// fp16 numbers of its own copies.  Under 64 rows, one warp to a scheduler, four more warps do so for
+// the tile ahead (300 tokens 30 us, 37 sequences 60; by the warps of the rows 33 and 70); under 128
+// those of the rows, before the barrier that the tile waits for anyway (prompts of 1919 and 2048
+// tokens over up to 4096 keys 888 us; a tile ahead, around the products of the one before, no faster).
 #include "paged_attention.cuh"
 #include "paged_mma.cuh"
 
@@ -38,7 +40,11 @@ constexpr uint32_t kStageBytes = 2u * kTileBytes;
 
 template <uint32_t ROWS, bool Q4>
 struct Many {
-    static constexpr uint32_t kThreads = 2u * ROWS;          // a warp for 16 rows
+    static constexpr uint32_t kRowThreads = 2u * ROWS;       // a warp for 16 rows
+    // Q4_0: those that make the tiles, the last ones (64 rows: warps of their own)
+    static constexpr bool kApart = Q4 && ROWS == 64u;
+    static constexpr uint32_t kMakers = 2u * ROWS;
+    static constexpr uint32_t kThreads = kApart ? kRowThreads + kMakers : kRowThreads;
     static constexpr uint32_t kQBytes = ROWS * kRowBytes;    // one half of the queries
     // Q4_0: a tile's blocks as they come, 16 bytes of numbers and two keys' scales each
     static constexpr uint32_t kRawBlocks = 2u * kKeys * (HD / 32u), kRawBytes = kRawBlocks * 20u;
@@ -60,7 +66,9 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     __shared__ int row_pos[ROWS];
     __shared__ float row_unscale[ROWS];
     __shared__ uint32_t found[2];
-    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
+    const uint32_t hd = a.kv.head_dim, tid = threadIdx.x, lane = tid & 31u;
+    const uint32_t warp = M::kApart ? (tid >> 5) % (ROWS / 16u) : tid >> 5;  // (of the rows; a maker's does not matter)
+    const bool of_rows = !M::kApart || tid < M::kRowThreads, maker = !M::kApart || tid >= M::kRowThreads;
     const uint32_t kh = blockIdx.x % a.kv.kv_heads;
     uint32_t rest = blockIdx.x / a.kv.kv_heads;
     const uint32_t c = rest % a.chunks;
@@ -73,7 +81,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         r0 = rest * ROWS;
         nrows = min(ROWS, a.b.tokens * a.group - r0);
     } else {
-        if (warp == 0) {
+        if (tid < 32u) {
             uint32_t tile;
             const uint32_t seq = find_tile(a, rest, ROWS, &tile);
             if (lane == 0u) {
@@ -151,15 +159,17 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
             pages[u] = i < ntiles && j < ke && j + 16u > kb ? load_page(a.b, a.kv, s, j >> a.kv.page_shift, a.st) : kNone;
         }
     };
-    __shared__ uint32_t tile_gap[kStages];  // a page of the tile is no page
+    constexpr uint32_t kGaps = M::kApart ? 2u * kStages : kStages;
+    __shared__ uint32_t tile_gap[kGaps];  // a page of the tile is no page
     // Q4_0: the thread's blocks x of a tile's keys, and of its values behind them
-    constexpr uint32_t kMine = M::kRawBlocks / 2u / kThreads;
-    auto raw_at = [&](uint32_t i, uint32_t x) { return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + (x * kThreads + tid) * 16u; };
+    constexpr uint32_t kMine = M::kRawBlocks / 2u / M::kMakers;
+    const uint32_t me = M::kApart ? tid - M::kRowThreads : tid;
+    auto raw_at = [&](uint32_t i, uint32_t x) { return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + (x * M::kMakers + me) * 16u; };
     auto raw_scale_at = [&](uint32_t i, uint32_t x) {
-        return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + M::kRawBlocks * 16u + (x * kThreads + tid) * 4u;
+        return 2u * kQBytes + kStages * kStageBytes + (i % kStages) * M::kRawBytes + M::kRawBlocks * 16u + (x * M::kMakers + me) * 4u;
     };
-    const uint32_t my_key = (tid & 7u) + 8u * ((tid >> 4) & 3u);
-    auto block_of = [&](uint32_t x) { return ((tid >> 3) & 1u) + 2u * ((x * kThreads + tid) >> 6); };
+    const uint32_t my_key = (me & 7u) + 8u * ((me >> 4) & 3u);
+    auto block_of = [&](uint32_t x) { return ((me >> 3) & 1u) + 2u * ((x * M::kMakers + me) >> 6); };
     auto fetch = [&](uint32_t i) {
         if (i < ntiles) {
             const uint32_t dst = ring + (i % kStages) * kStageBytes;
@@ -172,7 +182,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
                 const uint32_t j = j0 + i * kKeys + u * 16u;
                 gap |= pages[u] == kNone && j < ke && j + 16u > kb;
             }
-            if (tid == 0) tile_gap[i % kStages] = gap;
+            if (me == 0u) tile_gap[i % kGaps] = gap;
             if constexpr (Q4) {
                 const uint32_t j = j0 + i * kKeys + my_key;
                 uint32_t page = pages[0];
@@ -205,12 +215,35 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
         }
         cp_commit();
     };
-    look_up(0);
-    fetch(0);
-    look_up(1);
+    // Q4_0: tile i, once the thread's copies are there (of keys that are not: numbers and scales zero)
+    auto make = [&](uint32_t i) {
+        cp_wait<1>();
+        if (i >= ntiles) return;
+#pragma unroll
+        for (uint32_t x = 0; x < 2u * kMine; ++x) {
+            const uint32_t b = block_of(x % kMine);
+            if (b * 32u >= hd) continue;
+            const uint4 w = *reinterpret_cast<const uint4*>(sm + raw_at(i, x));
+            const __half2 d = __half2half2(*reinterpret_cast<const __half*>(sm + raw_scale_at(i, x) + (my_key & 1u) * 2u));
+            uint8_t* const to = sm + 2u * kQBytes + (i % kStages) * kStageBytes + (x < kMine ? 0u : kTileBytes);
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (uint32_t u = 0; u < 4u; ++u) {
+                __half2 h[4];
+                q4_pairs(words[u], h);
+                *reinterpret_cast<uint4*>(to + at(my_key, b * 4u + u)) =
+                    make_uint4(pack(__hmul2(h[0], d)), pack(__hmul2(h[1], d)), pack(__hmul2(h[2], d)), pack(__hmul2(h[3], d)));
+            }
+        }
+    };
+    if (maker) {
+        look_up(0);
+        fetch(0);
+        look_up(1);
+    }
 
     // queries: scaled, split and stored; a row per two threads
-    {
+    if (of_rows) {
         const uint32_t r = tid >> 1;
         const int p = row_pos[r];
         const float* q = a.q + (static_cast<size_t>(row_tok[r]) * a.heads + row_head[r]) * hd;
@@ -239,6 +272,11 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
             *reinterpret_cast<uint4*>(sm + kQBytes + at(r, d >> 3)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
+    if (M::kApart && maker) {
+        fetch(1);
+        look_up(2);
+        make(0);
+    }
     __syncthreads();
 
     // this thread's rows g and g + 8 of the warp's 16
@@ -260,30 +298,21 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     for (uint32_t n = 0; n < HD / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 
     for (uint32_t i = 0; i < ntiles; ++i) {
-        fetch(i + 1u);
-        look_up(i + 2u);
-        cp_wait<1>();
-        if constexpr (Q4) {  // the thread's own blocks (of keys that are not there: numbers and scales zero)
-#pragma unroll
-            for (uint32_t x = 0; x < 2u * kMine; ++x) {
-                const uint32_t b = block_of(x % kMine);
-                if (b * 32u >= hd) continue;
-                const uint4 w = *reinterpret_cast<const uint4*>(sm + raw_at(i, x));
-                const __half2 d = __half2half2(*reinterpret_cast<const __half*>(sm + raw_scale_at(i, x) + (my_key & 1u) * 2u));
-                uint8_t* const to = sm + 2u * kQBytes + (i % kStages) * kStageBytes + (x < kMine ? 0u : kTileBytes);
-                const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (uint32_t u = 0; u < 4u; ++u) {
-                    __half2 h[4];
-                    q4_pairs(words[u], h);
-                    *reinterpret_cast<uint4*>(to + at(my_key, b * 4u + u)) =
-                        make_uint4(pack(__hmul2(h[0], d)), pack(__hmul2(h[1], d)), pack(__hmul2(h[2], d)), pack(__hmul2(h[3], d)));
-                }
+        if constexpr (M::kApart) {  // the next tile is made meanwhile
+            if (maker) {
+                fetch(i + 2u);
+                look_up(i + 3u);
+                make(i + 1u);
             }
+        } else {
+            fetch(i + 1u);
+            look_up(i + 2u);
+            if constexpr (Q4) make(i);
+            else cp_wait<1>();
+            __syncthreads();
         }
-        __syncthreads();
         const uint32_t j = j0 + i * kKeys;
-        if (j < we && j + kKeys > wb) {
+        if (of_rows && j < we && j + kKeys > wb) {
             const uint32_t ks = ring + (i % kStages) * kStageBytes, vs = ks + kTileBytes;
             float sc[kCols][4];
 #pragma unroll
@@ -311,7 +340,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
             for (uint32_t n = 0; n < kCols; ++n)
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) sc[n][e] = fmaf(low[n][e], kLowDown, sc[n][e]);
-            const bool gap = tile_gap[i % kStages] != 0u;
+            const bool gap = tile_gap[i % kGaps] != 0u;
             const bool whole = !gap && j >= all_b && j + kKeys <= all_e && j >= kb && j + kKeys <= ke;
             if (!whole) {
                 uint32_t there = ~0u;  // groups of 16 keys whose page is a page
@@ -390,6 +419,7 @@ __device__ __forceinline__ void attention_many(const AttnArgs& a) {
     }
     cp_wait<0>();
     asm volatile("griddepcontrol.launch_dependents;");
+    if (!of_rows) return;
     const size_t rows_all = static_cast<size_t>(a.b.tokens) * a.heads;
     uint32_t again = 0;  // rows of the warp whose sums are not finite
 #pragma unroll
