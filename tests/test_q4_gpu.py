@@ -519,3 +519,45 @@ def test_chunks_from_the_lengths(lib, cuda, shape, q, kv, shared):
         graph.replay()
         assert cuda.equal(out, d.out)
     lib.status()
+
+
+def test_two_streams_at_once(lib, cuda):
+    """Two batches on two streams, each call with a workspace of its own, and two graphs replayed at once."""
+    ds = [dev(lib, cuda, 12, 4, 128, 64, q=[1] * 8, kv=[4000 + 31 * i for i in range(8)], seed=41),
+          dev(lib, cuda, 8, 2, 160, 32, q=[40, 1, 7], kv=[300, 900, 64], seed=42)]
+    want = [d.attention().clone() for d in ds]
+    need = [lib.paged_attention_workspace(d.cache, d.batch, d.s.heads) for d in ds]
+    ws = [d.space(n) for d, n in zip(ds, need)]
+    outs = [[cuda.empty_like(d.out) for _ in range(8)] for d in ds]
+    streams = [cuda.cuda.Stream() for _ in ds]
+
+    def call(i, out, stream):
+        d = ds[i]
+        lib.paged_attention_dev(d.cache, d.batch, d.s.heads, d.q.data_ptr(), out.data_ptr(), d.s.scale, 0, ws[i].data_ptr(), need[i],
+                                stream.cuda_stream)
+
+    def check_all():
+        cuda.cuda.synchronize()
+        for i in range(2):
+            for out in outs[i]:
+                inside = want[i] != 777.0
+                assert cuda.equal(out[inside], want[i][inside])
+
+    cuda.cuda.synchronize()
+    for n in range(8):
+        for i in range(2):
+            call(i, outs[i][n], streams[i])
+    check_all()
+    graphs = [cuda.cuda.CUDAGraph() for _ in ds]
+    for i in range(2):
+        with cuda.cuda.graph(graphs[i], stream=streams[i]):
+            for n in range(8):
+                call(i, outs[i][n], streams[i])
+    for x in outs[0] + outs[1]:
+        x.zero_()
+    cuda.cuda.synchronize()
+    for i in range(2):
+        with cuda.cuda.stream(streams[i]):
+            graphs[i].replay()
+    check_all()
+    lib.status()
