@@ -23,13 +23,14 @@
 // as well (and six ring slots) took 130 us where this took 126.
 // Registers: 56 for the softmax, 112 for the sums, 56 for the others.
 //
-// Q4_0 caches (paged_q4.cuh), 1024 threads.  The load warp brings in the pages' numbers and scales as they
-// are, four half tiles deep next to a ring of three: of each page piece one bulk copy and one TMA box with the
-// scales of all blocks (a copy for every block's, five in all, held the warp up: 137 us for the prompt below).  Two groups of
-// three warps in turn make the fp16 tiles of them, a block of 32 channels to a lane, where the swizzled copy would
-// have put them, and zeroes outside the item's keys (one group: 220 us).  Registers: 56 for the softmax, 96 for the sums, 48 for
-// the others.  The prompt below: 124 us; the makers are the seventh to tenth warp of every scheduler, whose issue
-// slots are taken for 62 % of the cycles (52 with F16 caches).
+// Q4_0 caches (paged_q4.cuh), 1024 threads.  The load warp brings in the pages' numbers and scales as
+// they are, four half tiles deep next to a ring of three: of each page piece one bulk copy and one TMA
+// box with the scales of all blocks (a copy for every block's, five in all, held the warp up: 137 us
+// for the prompt below).  Two groups of three warps in turn make the fp16 tiles of them, a block of 32
+// channels to a lane, where the swizzled copy would have put them, and zeroes outside the item's keys
+// (one group: 220 us).  Registers: 56 for the softmax, 96 for the sums, 48 for the others.  The prompt
+// below: 124 us; one or two of a scheduler's eight warps make tiles, and its issue slots are taken for
+// 62 % of the cycles (52 with F16 caches).
 //
 // What bounds it: 12 query and 4 KV heads of 128 channels, 2048 and 1840 new tokens of two
 // sequences over 4096 and 2550 keys, window 2048: 104 us, 825 TFLOP/s of fp16 MMAs (two for each
