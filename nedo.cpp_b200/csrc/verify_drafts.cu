@@ -12,10 +12,9 @@
 // largest logit and the sum of 2^((l - m) log2(e) / T), in 32 bits (T = 0: the largest one's place, which
 // a thread looks for at the end, among the 16 that it remembers: 19 us for 288 rows of 64000, 22 with a key
 // carried along).  The second, a cluster of CTAs per
-// sequence, adds the parts and decides: with the sums within 2^-14 (17 + 17 roundings of an exponent
-// of up to 17 that carries weight, those of up to 2^7 additions, 2^-22 of the exponential), a draft
-// whose two sides differ by more is decided, any other is looked at again with the row summed in 64
-// bits.  Then the one row that the next token comes from is read again, from L2, in 64 bits: a token
+// sequence, adds the parts and decides: a draft whose two sides differ by more than 2^-14, which is twice what they
+// can be off (kOff), is decided, any other is looked at again with the row summed in 64 bits.  Then
+// the one row that the next token comes from is read again, from L2, in 64 bits: a token
 // of a large vocabulary can be 10^-6 of the whole, and u falls on the border of two in 32 bits
 // every so often.  Every warp has a share of the tokens in order; the CTA of the warp whose share holds the
 // border goes through that once more, a run of tokens to a thread.
@@ -127,9 +126,16 @@ __global__ void __launch_bounds__(kThreads, 8) verify_stats_kernel(const __grid_
             s *= exp2_fast((m - top) * a.rate);
             m = top;
         }
-        if (m > -INFINITY)
+        if (m > -INFINITY) {  // the sixteen by halves: four roundings and one of the running sum
+            float w[16];
 #pragma unroll
-            for (uint32_t e = 0; e < 16u; ++e) s += exp2_fast((v[e] - m) * a.rate);
+            for (uint32_t e = 0; e < 16u; ++e) w[e] = exp2_fast((v[e] - m) * a.rate);
+#pragma unroll
+            for (uint32_t n = 8; n != 0u; n /= 2u)
+#pragma unroll
+                for (uint32_t e = 0; e < n; ++e) w[e] = w[2u * e] + w[2u * e + 1u];
+            s += w[0];
+        }
     };
     for (uint32_t x = x0 + tid; x < x1; x += 4u * kThreads) {
         float v[16];
@@ -393,10 +399,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
         float m = -INFINITY;
         for (uint32_t c = lane; c < a.parts; c += 32u) m = fmaxf(m, part[c].x);
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        float z = 0.f;
+        double z = 0.0;  // (a lane can have many)
         for (uint32_t c = lane; c < a.parts; c += 32u)
-            if (part[c].x > -INFINITY) z += part[c].y * exp2_fast((part[c].x - m) * a.rate);
-        z = warp_sum(z);
+            if (part[c].x > -INFINITY) z += static_cast<double>(part[c].y) * exp2_fast((part[c].x - m) * a.rate);
+        z = warp_sum64(z);
         if (lane == 0u) {
             sm.row_m[i] = m;
             sm.row_z[i] = z;
@@ -442,7 +448,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_sample_kernel(const 
             } else {
                 const float m = sm.row_m[tid], e = m > -INFINITY ? exp2_fast((logit - m) * a.rate) : 0.f;
                 const double left = static_cast<double>(u) * q * sm.row_z[tid], right = e;
-                constexpr double kOff = 1.0 / 16384.0;
+                // In units of 2^-24 the row's sum is off by no more than 298: a weight by 4 (the exponential) and its
+                // exponent's three roundings, 2.1 a bit, of which those that weigh have log2(vocab) in the mean, 31 at
+                // most; a thread's sum by 4 in the sixteen and 6 in each of up to kLongest / 4096 + 1 steps; a warp's by
+                // 10, a CTA's by 13, a row's by 4, each brought to the largest on the way.  The draft's weight, of up
+                // to 100 bits, is off by 212.
+                constexpr double kOff = 1024.0 / (1 << 24);
                 if (m == -INFINITY || left > right * (1.0 + kOff) + 1e-30) what = 2u * tid + 1u;
                 else if (left < right * (1.0 - kOff) - 1e-30) what = kNone;
                 else what = 2u * tid;  // open
@@ -543,13 +554,15 @@ uint32_t sample_ctas(const VerifyDrafts& v) {
     return c;
 }
 
-// Parts of a row: as many CTAs as run at once, but no part smaller than two loads of a thread.
+// Parts of a row: as many CTAs as run at once, but no part smaller than two loads of a thread, nor longer than the
+// bound on its sum allows for.
+constexpr uint32_t kLongest = 32u * 16u * kThreads;
 uint32_t parts_of(const VerifyDrafts& v, uint32_t* chunk) {
     constexpr uint32_t kRound = 4u * kThreads;
     const uint64_t most = (static_cast<uint64_t>(v.vocab) + 2u * kRound - 1u) / (2u * kRound);
     const uint64_t want = std::min<uint64_t>(most, std::max<uint64_t>(1u, 8u * 148u / v.rows));
     const uint64_t each = (v.vocab + want - 1u) / want;
-    *chunk = static_cast<uint32_t>((each + kRound - 1u) / kRound * kRound);
+    *chunk = static_cast<uint32_t>(std::min<uint64_t>((each + kRound - 1u) / kRound * kRound, kLongest));
     return static_cast<uint32_t>((static_cast<uint64_t>(v.vocab) + *chunk - 1u) / *chunk);
 }
 
