@@ -559,7 +559,8 @@ NEDO_GPU_API int nedo_gpu_verify_drafts_workspace(const nedo_gpu_drafts* drafts,
  * out, a draft that is no token (vocab or more) does not stand, and either is reported by
  * nedo_gpu_status.  Rows of no sequence are left as they were.  Asynchronous on `stream`, without
  * allocations; calls that overlap need workspaces of their own.  logits, draft_probs and the
- * workspace are 16-byte aligned, and the results overlap nothing that is read. */
+ * workspace are 16-byte aligned; the results and the workspace overlap neither each other nor anything
+ * that is read. */
 NEDO_GPU_API int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature, uint32_t* accepted_dev,
                                             uint32_t* ids_dev, void* workspace_dev, uint64_t workspace_bytes,
                                             void* stream);

@@ -1911,17 +1911,22 @@ int nedo_gpu_verify_drafts_dev(const nedo_gpu_drafts* drafts, float temperature,
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: lists must be 4-byte aligned");
     const uint64_t list = static_cast<uint64_t>(v.rows) * sizeof(uint32_t), counts = static_cast<uint64_t>(v.seqs) * sizeof(uint32_t);
     const uint64_t all = list * v.vocab;
-    auto clash = [&](const void* in, uint64_t bytes) {
-        return in != nullptr && (overlap(ids_dev, list, in, bytes) || overlap(accepted_dev, counts, in, bytes));
+    // whether what the call reads overlaps `at`
+    auto is_read = [&](const void* at, uint64_t bytes) {
+        auto over = [&](const void* in, uint64_t n) { return in != nullptr && overlap(at, bytes, in, n); };
+        return over(v.row_start, counts + sizeof(uint32_t)) || over(v.logits, all) || (several && over(v.draft_ids, list)) ||
+               (drawn && (over(v.sample_u, counts) || (several && (over(v.accept_u, list) || over(v.draft_probs, all)))));
     };
-    if (clash(v.row_start, counts + sizeof(uint32_t)) || clash(v.logits, all) || (several && clash(v.draft_ids, list)) ||
-        (drawn && (clash(v.sample_u, counts) || (several && (clash(v.accept_u, list) || clash(v.draft_probs, all))))))
+    if (is_read(ids_dev, list) || is_read(accepted_dev, counts))
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: the results overlap what is read");
     if (overlap(ids_dev, list, accepted_dev, counts))
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: accepted and ids overlap");
     const uint64_t need = verify_drafts_workspace(v);
     if (!workspace_dev || workspace_bytes < need)
         return fail(NEDO_GPU_ERR_ARG, "verify_drafts: workspace smaller than " + std::to_string(need) + " bytes");
+    if (is_read(workspace_dev, need) || overlap(workspace_dev, need, ids_dev, list) ||
+        overlap(workspace_dev, need, accepted_dev, counts))
+        return fail(NEDO_GPU_ERR_ARG, "verify_drafts: the workspace overlaps the results or what is read");
     DeviceState* s = nullptr;
     if (int rc = get_state(&s)) return rc;
     cudaError_t e = launch_verify_drafts(v, temperature, accepted_dev, ids_dev, workspace_dev, s->status,
