@@ -448,10 +448,10 @@ NEDO_GPU_API int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const ne
                                         void* stream);
 
 /* The keys (rotated) and values that the cache holds for a batch's token rows, in 32 bits:
- * k_out_dev and v_out_dev [tokens][kv_heads][head_dim], not overlapping; for moving sequences to
- * other pages or another type of cache (kv_append with rope_theta 0 takes them), and for looking
- * at them.  Padding rows get zeros, and so do those on a page id of num_pages or more; rows of no
- * sequence are left as they were. */
+ * k_out_dev and v_out_dev [tokens][kv_heads][head_dim], which overlap neither each other nor
+ * anything that is read; for moving sequences to other pages or another type of cache (kv_append
+ * with rope_theta 0 takes them), and for looking at them.  Padding rows get zeros, and so do those
+ * on a page id of num_pages or more; rows of no sequence are left as they were. */
 NEDO_GPU_API int nedo_gpu_kv_read_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch, float* k_out_dev,
                                       float* v_out_dev, void* stream);
 

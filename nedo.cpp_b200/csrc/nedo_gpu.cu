@@ -1786,6 +1786,14 @@ int nedo_gpu_kv_read_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch
         return fail(NEDO_GPU_ERR_ARG, "kv_read: buffers must be 16-byte aligned");
     const uint64_t bytes = static_cast<uint64_t>(b.tokens) * kv.kv_heads * kv.head_dim * sizeof(float);
     if (overlap(k_out_dev, bytes, v_out_dev, bytes)) return fail(NEDO_GPU_ERR_ARG, "kv_read: k_out and v_out overlap");
+    const uint64_t token = kv.type == kQ4_0 ? kv.head_dim / 32u * 18u : kv.head_dim * (kv.type == kF16 ? 2u : 4u);
+    const uint64_t pages = static_cast<uint64_t>(kv.num_pages) * kv.kv_heads * kv.page_size * token;
+    const uint64_t lens = static_cast<uint64_t>(b.seqs) * sizeof(uint32_t);
+    for (const float* at : {k_out_dev, v_out_dev})
+        if (overlap(at, bytes, kv.k, pages) || overlap(at, bytes, kv.v, pages) ||
+            overlap(at, bytes, b.q_start, lens + sizeof(uint32_t)) || overlap(at, bytes, b.kv_len, lens) ||
+            overlap(at, bytes, b.table, lens * b.max_pages))
+            return fail(NEDO_GPU_ERR_ARG, "kv_read: the outputs overlap what is read");
     DeviceState* s = nullptr;
     if (int rc = get_state(&s)) return rc;
     cudaError_t e = launch_kv_read(kv, b, k_out_dev, v_out_dev, s->status, static_cast<cudaStream_t>(stream));
