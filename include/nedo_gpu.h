@@ -397,8 +397,9 @@ typedef struct {
     void* k;             /* [num_pages][kv_heads][page_size][head_dim]                   */
     void* v;             /* [num_pages][kv_heads][page_size][head_dim]                   */
     void* bounds;        /* [num_pages][kv_heads][2][head_dim], in `type` (Q4_0: in F16): the
-                            smallest and the largest value of each channel of the page's keys
-                            (NULL: not kept; nedo_gpu_block_select_dev needs it)           */
+                            smallest and the largest value of each channel of the page's keys,
+                            as nedo_gpu_kv_append_dev keeps them (NULL: not kept;
+                            nedo_gpu_block_select_dev needs it)                            */
 } nedo_gpu_kv_cache;
 
 typedef struct {
@@ -442,7 +443,8 @@ typedef struct {
  * i + head_dim/2 turn by position * rope_theta^(-2i/head_dim), the angle in 64
  * bits; rope_theta 0: no rotation.  With cache->bounds, the channel bounds of every
  * page written are brought up to date: the range of the keys stored since the
- * page's first slot was last written (NaN keys left out). */
+ * page's first slot was last written (NaN keys left out), those included that have been
+ * written over since, as rejected drafts are, or that lie behind a length taken back. */
 NEDO_GPU_API int nedo_gpu_kv_append_dev(const nedo_gpu_kv_cache* cache, const nedo_gpu_kv_batch* batch,
                                         uint32_t heads, const float* qkv_dev, float rope_theta, float* q_out_dev,
                                         void* stream);
