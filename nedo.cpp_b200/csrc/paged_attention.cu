@@ -339,12 +339,15 @@ bool plan_paged_attention(PagedAttention* a) {
     uint64_t grid = units * a->own_chunks, slots = a->own_cluster ? 1u : a->own_chunks;
     // several chunks of few rows of several sequences: as long as their lengths make them, where that can save
     // a round (16 sequences of 2005 to 16001 keys, 15 rows: 71 us, 85 with chunks for 16001 keys), not where
-    // chunks are short (7 of 421 keys behind a prefix: 33 us, 28) or there are many rounds (32 of up to
-    // 32768 keys: 121 us, 119)
+    // chunks are short (7 of 421 keys behind a prefix: 33 us, 28), there are many rounds (32 of up to
+    // 32768 keys: 121 us, 119) or more sequences than a warp holds (700 of up to 3000 keys, looked through
+    // again for every length tried: 185 us, 104).  What the host cannot see is whether the lengths differ:
+    // 40 sequences of 2000 to 16000 keys take 52 us (71 otherwise), 12 of 3750 to 30000 33 (46), but 3
+    // that all have 30000 behind a prefix 49 (41), 32 of 8 KV heads and 375 to 3000 93 (79)
     a->balance = 0;
     const uint64_t least = std::min<uint64_t>(std::max<uint64_t>((keys / 32u + 63u) / 64u * 64u, 256u), kBalanceMost);
     const uint64_t each = units * keys / cost_of(own, a->kv).slots;  // keys for each of the items that run at once
-    if (takes_few4(own) && !a->picks && a->b.seqs > 1u && a->b.seqs <= 1024u && a->own_chunks > 1u && !a->own_cluster &&
+    if (takes_few4(own) && !a->picks && a->b.seqs > 1u && a->b.seqs <= kBalanceSeqs && a->own_chunks > 1u && !a->own_cluster &&
         keys > least && each >= 512u && each < 2u * kBalanceMost) {
         a->balance = cost_of(own, a->kv).slots;
         a->own_chunk = static_cast<uint32_t>(least);

@@ -279,33 +279,34 @@ static __device__ __noinline__ void rows_key_by_key(const AttnArgs& a, uint32_t 
 }
 
 constexpr uint32_t kBalanceMost = 2048;  // keys of a few-rows item
+constexpr uint32_t kBalanceSeqs = 64;    // sequences whose lengths a warp holds, two to a lane
 // One warp: the item of this CTA where the chunks follow from the lengths.  With chunks of the launch's
 // choice, by the batch's bounds, a batch of many lengths has items for one and a part of another
 // round of CTAs (16 sequences of 2005 to 16001 keys, 15 rows: 85 us).  Here every CTA adds up the
-// lengths, as a lane a sequence, and takes the least chunk of which there are no more than run at once (of as many
-// rounds as it takes chunks of kBalanceMost keys).  Items are those of the sequences in order, of a sequence's
-// tiles and KV heads, their chunks next to each other.
+// lengths and takes a chunk, the first in steps from the mean, of which there are no more than run at once (or in as
+// many rounds as it takes chunks of kBalanceMost keys), or kBalanceMost.  Items are those of the sequences in order, of a
+// sequence's tiles and KV heads, their chunks next to each other.
 struct BalancedItem {
     uint32_t s, rest, c, chunk;  // rest: KV head and row tile
 };
 template <uint32_t ROWS>
 __device__ __forceinline__ void balanced_item(const AttnArgs& a, BalancedItem* it) {
+    constexpr uint32_t kMine = kBalanceSeqs / 32u;
     const uint32_t lane = threadIdx.x & 31u;
-    // tiles and KV heads of a sequence, and its keys
-    auto look = [&](uint32_t s, uint32_t* units, uint32_t* keys) {
-        *units = *keys = 0u;
-        if (s >= a.b.seqs) return;
-        const PagedSeq sq = load_seq(a.b, s, a.st);
-        if (sq.n == 0u || sq.n * a.group > a.rows_to) return;
-        const uint32_t base = own_begin(sq, a.window, a.shared_len);
-        *units = (sq.n * a.group + ROWS - 1u) / ROWS * a.kv.kv_heads;
-        *keys = sq.kv > base ? sq.kv - base : 0u;
-    };
+    // tiles and KV heads of the lane's sequences, and their keys
+    uint32_t units[kMine], keys[kMine];
     uint64_t all = 0;
-    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-        uint32_t units, keys;
-        look(s0 + lane, &units, &keys);
-        all += static_cast<uint64_t>(units) * keys;
+#pragma unroll
+    for (uint32_t u = 0; u < kMine; ++u) {
+        const uint32_t s = u * 32u + lane;
+        units[u] = keys[u] = 0u;
+        if (s >= a.b.seqs) continue;
+        const PagedSeq sq = load_seq(a.b, s, a.st);
+        if (sq.n == 0u || sq.n * a.group > a.rows_to) continue;
+        const uint32_t base = own_begin(sq, a.window, a.shared_len);
+        units[u] = (sq.n * a.group + ROWS - 1u) / ROWS * a.kv.kv_heads;
+        keys[u] = sq.kv > base ? sq.kv - base : 0u;
+        all += static_cast<uint64_t>(units[u]) * keys[u];
     }
     for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xFFFFFFFFu, static_cast<unsigned long long>(all), o);
     const uint64_t rounds = max(static_cast<uint64_t>(1), (all + static_cast<uint64_t>(a.balance) * kBalanceMost - 1u) / (static_cast<uint64_t>(a.balance) * kBalanceMost));
@@ -313,21 +314,17 @@ __device__ __forceinline__ void balanced_item(const AttnArgs& a, BalancedItem* i
     chunk = max(chunk, a.chunk);
     while (chunk < kBalanceMost) {
         uint32_t items = 0;
-        for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-            uint32_t units, keys;
-            look(s0 + lane, &units, &keys);
-            items += units * ((keys + chunk - 1u) / chunk);
-        }
+#pragma unroll
+        for (uint32_t u = 0; u < kMine; ++u) items += units[u] * ((keys[u] + chunk - 1u) / chunk);
         if (__reduce_add_sync(0xFFFFFFFFu, items) <= a.balance * rounds) break;
         chunk = min(chunk + max(64u, (chunk >> 4) & ~63u), kBalanceMost);
     }
     if (blockIdx.x == 0u && lane == 0u) *a.chunk_at = chunk;
     uint32_t before = 0;
-    for (uint32_t s0 = 0; s0 < a.b.seqs; s0 += 32u) {
-        uint32_t units, keys;
-        look(s0 + lane, &units, &keys);
-        const uint32_t chunks = (keys + chunk - 1u) / chunk;
-        uint32_t inc = units * chunks;
+#pragma unroll
+    for (uint32_t u = 0; u < kMine; ++u) {
+        const uint32_t chunks = (keys[u] + chunk - 1u) / chunk;
+        uint32_t inc = units[u] * chunks;
         for (uint32_t o = 1; o < 32u; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
             if (lane >= o) inc += v;
@@ -335,8 +332,8 @@ __device__ __forceinline__ void balanced_item(const AttnArgs& a, BalancedItem* i
         const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + inc > blockIdx.x);
         if (hit != 0u) {
             const uint32_t w = __ffs(hit) - 1u, n = __shfl_sync(0xFFFFFFFFu, chunks, w);
-            const uint32_t at = blockIdx.x - before - __shfl_sync(0xFFFFFFFFu, inc - units * chunks, w);
-            *it = BalancedItem{s0 + w, at / n, at % n, chunk};
+            const uint32_t at = blockIdx.x - before - __shfl_sync(0xFFFFFFFFu, inc - units[u] * chunks, w);
+            *it = BalancedItem{u * 32u + w, at / n, at % n, chunk};
             return;
         }
         before += __shfl_sync(0xFFFFFFFFu, inc, 31);
