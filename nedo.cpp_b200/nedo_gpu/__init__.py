@@ -23,7 +23,7 @@ from . import blocks
 from .blocks import F16, Q4_0, Q8_0, row_bytes
 
 __all__ = ["F16", "Q4_0", "Q8_0", "row_bytes", "blocks", "Library", "load", "NedoGpuError", "LIB_PATH",
-           "KvCache", "KvBatch"]
+           "KvCache", "KvBatch", "Drafts"]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_DIR = os.path.join(os.path.dirname(HERE), "lib")
