@@ -21,9 +21,12 @@
 //
 // What bounds it: 32 sequences of four drafts with their probabilities over 128000 tokens 46 us, of which
 // the first launch 15 (82 MB: 13 at the rate of a copy); then 5.5 us for the row's sum, 10 for that of what
-// the draft's probabilities leave and 3 for the search, by the 64-bit arithmetic of two CTAs to most SMs (four
-// CTAs to a cluster: 61 us; a table for every lane, or the probabilities brought into L2 during the first sum:
-// the same).  One sequence over 64000 tokens 16 us: two launches, and some 25,000 cycles of the second.
+// the draft's probabilities leave and 3 for the search.  Those are latency: six warps to a scheduler, which issue in
+// 42 % of its cycles (the 64-bit pipe is busy for 20), wait for loads, for the result before and for
+// the cluster's other CTAs in about equal parts; the second sum has a row of probabilities to load from memory, with
+// two quads of a lane on their way, and forms the first one's exponentials again.  (Four CTAs to a cluster: 61 us; a
+// table for every lane, or the probabilities brought into L2 during the first sum: the same.)  One sequence over
+// 64000 tokens 16 us: two launches, and some 25,000 cycles of the second.
 #include <algorithm>
 
 #include "common.cuh"
